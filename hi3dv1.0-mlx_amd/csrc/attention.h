@@ -1,0 +1,219 @@
+// Shared parts of the attention kernels (attention.hip, attention_grad.hip): arguments,
+// the packed rows and their segments, LDS tiles and the two matrix products on them.
+//
+// Definitions. A segment is one sequence: lq queries and lk keys, hq query heads over hk
+// key heads, G = hq / hk query heads to each. All rows of a segment that read the same key
+// head, (query i, head hk * G + g), are packed rows r = i * G + g: one packed row is one
+// row of the score matrix of that key head, so shared key heads cost no second read of K
+// and V and their gradients sum inside one workgroup.
+//
+// Matrix layout. v_mfma_f32_32x32x16 with the streamed operand (a tile of 64 rows in LDS)
+// first and the owned operand (32 rows a wave keeps in registers) second: lane l then
+// holds, for owned row l % 32, the 16 streamed rows 8 g + 4 (l / 32) + e. That layout is
+// also the second operand of the product that follows (streamed^T times P), when the
+// streamed rows of a 16-row step are taken in the order 4 h + {0..3}, 8 + 4 h + {0..3}
+// for lane half h: the probabilities never leave the registers, and the first operand
+// comes from the same LDS tile through the transposing read ds_read_b64_tr_b16.
+//
+// LDS tiles are rows of DP values (DP = head size rounded up to 32), 16-byte chunk c of
+// row r at c ^ f(r): f spreads 8 consecutive rows over the banks for the row reads, and 4
+// consecutive rows over 32-byte pairs of chunks for the transposing reads.
+#pragma once
+
+#include "common.h"
+#include "conv_tile.h"
+
+namespace hi3d {
+
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kKT = 64;  // streamed rows of an LDS tile
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+struct AttnArgs {
+  const void *q, *k, *v;        // rows of heads: element (b, i, h, d) at b*_b + i*_n + h*_h + d
+  const void *o, *dout;         // backward: output and its gradient, [total_q, hq, d]
+  void *out, *dk, *dv;          // out: output, or dq; all [total, heads, d]
+  float *lse, *delta;           // [total_q, hq]
+  float *part, *part_ml;        // split forward: [split, total_q, hq, d], [split, total_q, hq, 2]
+  int64_t q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h;
+  const int32_t *cu_q, *cu_k;   // [batch + 1] offsets of packed segments, or null: b * len
+  const int32_t* lens_k;        // [batch] keys in use of each segment of len_k rows, or null
+  const uint8_t* mask;          // [total_k], 0 where a key is hidden, or null
+  int32_t batch, len_q, len_k;
+  int64_t total_q, total_k;
+  int32_t hq, hk, group, dim;
+  uint32_t group_magic;         // ceil(2^32 / group) for group > 1
+  float scale, scale2;          // scale, scale * log2(e)
+  int32_t causal, splits, slots, head_minor, reverse;
+};
+
+template <typename T>
+struct Vec8;
+template <>
+struct Vec8<_Float16> {
+  typedef f16x8 type;
+};
+template <>
+struct Vec8<__bf16> {
+  typedef bf16x8 type;
+};
+
+// 8 fp32 values rounded to nearest into one 16-byte operand. Probabilities and score
+// gradients take this one rounding before their product; sums stay in fp32.
+template <typename T>
+__device__ __forceinline__ u32x4 pack8(f32x8 v) {
+  return __builtin_bit_cast(u32x4, __builtin_convertvector(v, typename Vec8<T>::type));
+}
+
+template <int DP>
+__device__ __forceinline__ int row_xor(int row) {
+  if constexpr (DP % 64 == 0) return ((row & 3) << 1) | ((row >> 2) & 1);
+  else return (row & 2) | ((row >> 2) & 1);
+}
+
+// First operand of a score product: chunk 2 s + h of row `row` (a multiple of 32 plus l % 32).
+template <int DP>
+__device__ __forceinline__ u32x4 read_rows(const char* tile, int row, int s, int h) {
+  const int c = (2 * s + h) ^ row_xor<DP>(row);
+  return *reinterpret_cast<const u32x4*>(tile + row * (2 * DP) + c * 16);
+}
+
+// First operand of a product over streamed rows: columns 32 db + l % 32 of rows
+// row0 + {4 h + 0..3, 8 + 4 h + 0..3}. A 16-lane group reads 4 rows x 16 columns and gets
+// them transposed (lane i: column i).
+template <int DP>
+__device__ __forceinline__ u32x4 read_columns(const char* tile, int row0, int db, int lane) {
+  const int i = lane & 15, grp = (lane >> 4) & 1, h = lane >> 5;
+  const int row = 4 * h + (i >> 2);  // row0 is a multiple of 16: row_xor does not see it
+  const int c = (4 * db + 2 * grp + ((i & 3) >> 1)) ^ row_xor<DP>(row);
+  const char* p = tile + (row0 + row) * (2 * DP) + c * 16 + (i & 1) * 8;
+  typedef __attribute__((address_space(3))) s16x4* lds4;
+  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p));
+  const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 8 * 2 * DP));
+  const u32x2 x = __builtin_bit_cast(u32x2, a), y = __builtin_bit_cast(u32x2, b);
+  return u32x4{x[0], x[1], y[0], y[1]};
+}
+
+// The values of the two lanes (l, l ^ 32) that hold one owned row.
+__device__ __forceinline__ void both_halves(float x, float& lo, float& hi) {
+  const uint32_t a = __builtin_bit_cast(uint32_t, x);
+  const auto r = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+  const uint32_t r0 = r[0], r1 = r[1];  // a bit cast of r[1] itself would read r[0]
+  lo = __builtin_bit_cast(float, r0), hi = __builtin_bit_cast(float, r1);
+}
+__device__ __forceinline__ float half_max(float x) {
+  float lo, hi;
+  both_halves(x, lo, hi);
+  return fmaxf(lo, hi);
+}
+__device__ __forceinline__ float half_sum(float x) {
+  float lo, hi;
+  both_halves(x, lo, hi);
+  return lo + hi;
+}
+
+__device__ const uint4 kZeroChunk = {0, 0, 0, 0};
+
+struct Segment {
+  int b, tile;          // segment and the workgroup's tile of it
+  int lq, lk;
+  int64_t q0, k0;       // first row of the segment among all queries / keys
+};
+
+__device__ __forceinline__ int clamp_offset(int v, int64_t total) {
+  return v < 0 ? 0 : (v > total ? static_cast<int>(total) : v);
+}
+
+// Lengths and first rows of segment b. Offsets are clamped to the rows there are, so no
+// offset can lead outside the tensors.
+__device__ __forceinline__ void segment_rows(const AttnArgs& a, Segment& s) {
+  if (a.cu_q != nullptr) {
+    const int q0 = clamp_offset(a.cu_q[s.b], a.total_q), q1 = clamp_offset(a.cu_q[s.b + 1], a.total_q);
+    s.q0 = q0, s.lq = q1 > q0 ? q1 - q0 : 0;
+  } else {
+    s.q0 = static_cast<int64_t>(s.b) * a.len_q, s.lq = a.len_q;
+  }
+  if (a.cu_k != nullptr) {
+    const int k0 = clamp_offset(a.cu_k[s.b], a.total_k), k1 = clamp_offset(a.cu_k[s.b + 1], a.total_k);
+    s.k0 = k0, s.lk = k1 > k0 ? k1 - k0 : 0;
+  } else {
+    s.k0 = static_cast<int64_t>(s.b) * a.len_k, s.lk = a.len_k;
+    if (a.lens_k != nullptr) {
+      const int n = a.lens_k[s.b];
+      s.lk = n < 0 ? 0 : (n < s.lk ? n : s.lk);
+    }
+  }
+}
+
+// Which segment and tile slot `slot` is. Segment b owns the slots from
+// floor(cu[b] * rows / T) + b to that of b + 1: at least ceil(length * rows / T) of them and
+// at most one more, so the launch needs only the total, and nothing is built beforehand.
+// The segment is found by 64-way search, first around the place an even split gives.
+__device__ __forceinline__ void find_segment(const int32_t* cu, int len, int batch, int64_t total, int rows, int tile,
+                                             int slot, Segment& s) {
+  if (cu == nullptr) {
+    const int per = static_cast<int>((static_cast<int64_t>(len) * rows + tile - 1) / tile);
+    s.b = slot / per, s.tile = slot - s.b * per;
+    return;
+  }
+  const int lane = threadIdx.x & 63;
+  auto first = [&](int b) {
+    return static_cast<int>(static_cast<int64_t>(clamp_offset(cu[b], total)) * rows / tile) + b;
+  };
+  int lo = 0, hi = batch;  // first(lo) <= slot < first(hi), hi exclusive of the answer
+  if (batch > 64) {
+    const int64_t all = total * rows / tile + batch;
+    int at = static_cast<int>(static_cast<int64_t>(slot) * batch / (all > 0 ? all : 1)) - 32;
+    at = at < 0 ? 0 : (at > batch - 64 ? batch - 64 : at);
+    const uint64_t le = __ballot(first(at + lane) <= slot);
+    if (le == ~0ull) lo = at + 63;
+    else if (le == 0) hi = at;
+    else lo = at + 63 - __builtin_clzll(le), hi = lo + 1;
+  }
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 63) / 64;
+    const int at = lo + lane * step;
+    const uint64_t le = __ballot(at < hi && first(at < hi ? at : lo) <= slot);  // bit 0 is always set
+    lo += (63 - __builtin_clzll(le | 1)) * step;
+    hi = lo + step < hi ? lo + step : hi;
+  }
+  s.b = __builtin_amdgcn_readfirstlane(lo);
+  s.tile = slot - first(s.b);
+}
+
+__device__ __forceinline__ void split_row(const AttnArgs& a, int r, int& i, int& g) {
+  i = a.group == 1 ? r : static_cast<int>(__umulhi(static_cast<uint32_t>(r), a.group_magic));
+  g = r - i * a.group;
+}
+
+// Copies `rows` rows (the rest repeat the last one) from key `base` on into a tile pair,
+// straight to LDS. BITS: rows whose bit is clear and chunks past the head size read zeros,
+// so what a hidden key holds cannot reach a product.
+template <int DP, int NW, bool Z>
+__device__ __forceinline__ void load_pair(const char* x, int64_t x_n, const char* y, int64_t y_n, int rows,
+                                          uint64_t bits, int dim, char* tile, int wave, int lane) {
+  constexpr int CH = DP / 8, UNITS = 2 * CH * (kKT / 64);
+  static_assert(UNITS % NW == 0, "the waves share a tile's loads evenly");
+#pragma unroll
+  for (int i = 0; i < UNITS / NW; ++i) {
+    const int j = wave + i * NW;
+    const bool second = j >= CH;
+    const int u = (second ? j - CH : j) * 64 + lane;
+    const int row = u / CH, c = (u % CH) ^ row_xor<DP>(row);
+    const int from = row < rows ? row : rows - 1;
+    const char* base = second ? y : x;
+    const int stride = static_cast<int>(second ? y_n : x_n) * 2;
+    const char* src = base + (from * stride + c * 16);
+    if constexpr (Z) {
+      if (!((bits >> row) & 1) || c * 8 >= dim) src = reinterpret_cast<const char*>(&kZeroChunk);
+    }
+    lds_dma16(src, tile + (second ? kKT * DP * 2 : 0) + (second ? j - CH : j) * 1024);
+  }
+}
+
+}  // namespace hi3d

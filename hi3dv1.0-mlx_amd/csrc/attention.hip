@@ -1,0 +1,418 @@
+// Attention over packed segments: out = softmax(scale q k^T) v, with grouped heads, a
+// causal limit aligned to the last query and key, and a mask of keys.
+#include "attention.h"
+
+namespace hi3d {
+namespace {
+
+// A workgroup owns NW * QW * 32 packed rows of one key head (QW blocks of 32 per wave,
+// their queries in registers) and walks the keys in tiles of 64 held twice in LDS: the
+// next tile's loads go straight to LDS while the present one is computed, one barrier per
+// tile. Per 64 keys a wave forms S^T = K Q^T, keeps the running reference m and sum of
+// exp2(s - m) of its rows in fp32, and adds V^T P^T to the output it holds.
+//
+// m only moves when some row's maximum has grown by more than 2^8 over it (the first tile
+// included): any reference gives the same quotient, and between moves the probabilities
+// stay below 2^8, well inside fp16's and fp32's range, so the output is rescaled rarely.
+template <typename T, int DP, int NW, int QW, bool Z, bool SPLIT>
+__global__ __launch_bounds__(64 * NW, 2) void attend_kernel(AttnArgs a) {
+  constexpr int ROWS = NW * QW * 32, KS = DP / 16, DB = DP / 32, PAIR = 2 * kKT * DP * 2;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c32 = lane & 31, h = lane >> 5;
+
+  // task: (head, split, slot), neighbours on one XCD so that they share its L2
+  const int64_t id = xcd_remap(blockIdx.x, gridDim.x);
+  int head, split = 0, slot;
+  if (a.head_minor) {
+    head = static_cast<int>(id % a.hk), slot = static_cast<int>(id / a.hk);
+    if constexpr (SPLIT) split = slot % a.splits, slot /= a.splits;
+  } else {
+    slot = static_cast<int>(id % a.slots), head = static_cast<int>(id / a.slots);
+    if constexpr (SPLIT) split = head % a.splits, head /= a.splits;
+  }
+  if (a.reverse) slot = a.slots - 1 - slot;  // causal: the longest rows first
+  Segment s;
+  find_segment(a.cu_q, a.len_q, a.batch, a.total_q, a.group, ROWS, slot, s);
+  segment_rows(a, s);
+  const int rows = s.lq * a.group, row0 = s.tile * ROWS;
+  if (s.tile < 0 || row0 >= rows) return;
+
+  // this wave's rows and the keys they see
+  const int wrow = row0 + wave * (QW * 32);
+  const int off = s.lk - s.lq;
+  int qi[QW], qg[QW];
+  u32x4 qf[QW][KS];
+#pragma unroll
+  for (int b = 0; b < QW; ++b) {
+    const int r = wrow + b * 32 + c32;
+    split_row(a, r < rows ? r : rows - 1, qi[b], qg[b]);
+    const T* src = static_cast<const T*>(a.q) + s.b * a.q_b + (a.cu_q != nullptr ? s.q0 + qi[b] : qi[b]) * a.q_n +
+                   static_cast<int64_t>(head * a.group + qg[b]) * a.q_h;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      const int c = 16 * k + 8 * h;
+      u32x4 x = {0, 0, 0, 0};
+      if (c < a.dim) x = *reinterpret_cast<const u32x4*>(src + c);
+      qf[b][k] = x;
+    }
+  }
+  int kend = s.lk, wkend = wrow < rows ? s.lk : 0, wfull = s.lk;  // keys of the workgroup; of the wave; of all its rows
+  if (a.causal) {
+    int i, g;
+    split_row(a, min(rows, row0 + ROWS) - 1, i, g);
+    kend = min(kend, i + off + 1);
+    if (wrow < rows) {
+      split_row(a, min(rows, wrow + QW * 32) - 1, i, g);
+      wkend = min(wkend, i + off + 1);
+      split_row(a, wrow, i, g);
+      wfull = min(wfull, i + off + 1);
+    }
+  }
+  const int tiles = kend > 0 ? (kend + kKT - 1) / kKT : 0;
+  int t0 = 0, t1 = tiles;
+  if constexpr (SPLIT) {
+    const int per = (tiles + a.splits - 1) / a.splits;
+    t0 = min(tiles, split * per), t1 = min(tiles, t0 + per);
+  }
+
+  const char* kp = reinterpret_cast<const char*>(static_cast<const T*>(a.k) + s.b * a.k_b + head * a.k_h +
+                                                 (a.cu_k != nullptr ? s.k0 * a.k_n : 0));
+  const char* vp = reinterpret_cast<const char*>(static_cast<const T*>(a.v) + s.b * a.v_b + head * a.v_h +
+                                                 (a.cu_k != nullptr ? s.k0 * a.v_n : 0));
+  // bit j: key 64 t + j is in the segment and not hidden
+  auto key_bits = [&](int t) -> uint64_t {
+    const int key = t * kKT + lane;
+    bool on = key < s.lk;
+    if (Z && a.mask != nullptr) on = on && a.mask[s.k0 + (key < s.lk ? key : 0)] != 0;
+    return __ballot(on);
+  };
+  auto load = [&](int t, uint64_t bits, int buf) {
+    const int64_t at = static_cast<int64_t>(t) * kKT;
+    load_pair<DP, NW, Z>(kp + at * a.k_n * 2, a.k_n, vp + at * a.v_n * 2, a.v_n, min(kKT, s.lk - t * kKT), bits, a.dim,
+                         smem + buf * PAIR, wave, lane);
+  };
+
+  f32x16 acc[DB][QW] = {};
+  float m[QW], l[QW];
+#pragma unroll
+  for (int b = 0; b < QW; ++b) m[b] = -INFINITY, l[b] = 0.0f;
+
+  uint64_t bits = 0, next = 0;
+  if (t0 < t1) {
+    bits = key_bits(t0);
+    load(t0, bits, 0);
+    if (t0 + 1 < t1) next = key_bits(t0 + 1);
+  }
+  __syncthreads();
+  for (int t = t0, buf = 0; t < t1; ++t, buf ^= 1) {
+    if (t + 1 < t1) load(t + 1, next, buf ^ 1);
+    uint64_t after = 0;
+    if (t + 2 < t1) after = key_bits(t + 2);
+    if (t * kKT < wkend) {
+      const char* kt = smem + buf * PAIR;
+      const char* vt = kt + kKT * DP * 2;
+      f32x16 sc[2][QW] = {};
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const u32x4 x = read_rows<DP>(kt, 32 * n + c32, k, h);
+#pragma unroll
+          for (int b = 0; b < QW; ++b) Mfma<T>::run(x, qf[b][k], sc[n][b]);
+        }
+      // keys that are hidden from a row
+      if (bits != ~0ull || (t + 1) * kKT > wfull) {
+#pragma unroll
+        for (int b = 0; b < QW; ++b) {
+          uint64_t on = bits;
+          if (a.causal) {
+            const int n = qi[b] + off + 1 - t * kKT;  // keys of this tile that the row sees
+            on &= n >= 64 ? ~0ull : (n <= 0 ? 0ull : (1ull << n) - 1);
+          }
+          on >>= 4 * h;
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const uint32_t w = static_cast<uint32_t>(on >> (32 * n));
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              sc[n][b][e] = (w >> (8 * (e >> 2) + (e & 3))) & 1 ? sc[n][b][e] : -INFINITY;
+          }
+        }
+      }
+      float top[QW];
+      bool grow = false;
+#pragma unroll
+      for (int b = 0; b < QW; ++b) {
+        float x = fmaxf(sc[0][b][0], sc[1][b][0]);
+#pragma unroll
+        for (int e = 1; e < 16; ++e) x = fmaxf(x, fmaxf(sc[0][b][e], sc[1][b][e]));
+        top[b] = half_max(x) * a.scale2;
+        grow = grow || top[b] > m[b] + 8.0f;
+      }
+      if (__any(grow)) {
+#pragma unroll
+        for (int b = 0; b < QW; ++b) {
+          const float to = fmaxf(m[b], top[b]);
+          const float by = m[b] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[b] - to);
+          m[b] = to;
+          l[b] *= by;
+#pragma unroll
+          for (int d = 0; d < DB; ++d) acc[d][b] *= by;
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < QW; ++b) {
+        const float ref = m[b] == -INFINITY ? 0.0f : m[b];
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            sc[n][b][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][b][e], a.scale2, -ref));
+            l[b] += sc[n][b][e];
+          }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        u32x4 p[QW];
+#pragma unroll
+        for (int b = 0; b < QW; ++b) {
+          f32x8 x;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = sc[k >> 1][b][8 * (k & 1) + e];
+          p[b] = pack8<T>(x);
+        }
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+          const u32x4 x = read_columns<DP>(vt, 16 * k, d, lane);
+#pragma unroll
+          for (int b = 0; b < QW; ++b) Mfma<T>::run(x, p[b], acc[d][b]);
+        }
+      }
+    }
+    bits = next, next = after;
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int b = 0; b < QW; ++b) {
+    if (wrow + b * 32 + c32 >= rows) continue;
+    const float sum = half_sum(l[b]);
+    const int64_t at = (s.q0 + qi[b]) * a.hq + head * a.group + qg[b];
+    if constexpr (SPLIT) {
+      float* to = a.part + (static_cast<int64_t>(split) * a.total_q * a.hq + at) * a.dim;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int c = 32 * d + 8 * e + 4 * h;
+          if (c < a.dim)
+            *reinterpret_cast<f32x4*>(to + c) = f32x4{acc[d][b][4 * e], acc[d][b][4 * e + 1], acc[d][b][4 * e + 2],
+                                                       acc[d][b][4 * e + 3]};
+        }
+      if (h == 0) {
+        float* ml = a.part_ml + (static_cast<int64_t>(split) * a.total_q * a.hq + at) * 2;
+        ml[0] = m[b], ml[1] = sum;
+      }
+    } else {
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // no key seen: zeros
+      T* to = static_cast<T*>(a.out) + at * a.dim;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int c = 32 * d + 8 * e + 4 * h;
+          typedef T t4 __attribute__((ext_vector_type(4)));
+          t4 x;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[j] = static_cast<T>(acc[d][b][4 * e + j] * inv);
+          if (c < a.dim) *reinterpret_cast<t4*>(to + c) = x;
+        }
+      if (a.lse != nullptr && h == 0) a.lse[at] = sum == 0.0f ? -INFINITY : (m[b] + __builtin_amdgcn_logf(sum)) * kLn2;
+    }
+  }
+}
+
+// Joins the splits of a row: a wave per row, each part weighed by exp2(m - max m) in fp32.
+// Reads splits * (dim + 2) * 4 bytes a row.
+template <typename T>
+__global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a, int64_t rows) {
+  const int lane = threadIdx.x & 63;
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (r >= rows) return;
+  float top = -INFINITY;
+  for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, a.part_ml[(s * rows + r) * 2]);
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+  const float ref = top == -INFINITY ? 0.0f : top;
+  float sum = 0.0f;
+  for (int s = lane; s < a.splits; s += 64) {
+    const float* ml = a.part_ml + (s * rows + r) * 2;
+    sum += ml[1] * __builtin_amdgcn_exp2f(ml[0] - ref);
+  }
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  for (int c = lane; c < a.dim; c += 64) {
+    float x = 0.0f;
+    for (int s = 0; s < a.splits; ++s)
+      x += a.part[(s * rows + r) * a.dim + c] * __builtin_amdgcn_exp2f(a.part_ml[(s * rows + r) * 2] - ref);
+    static_cast<T*>(a.out)[r * a.dim + c] = static_cast<T>(x * inv);
+  }
+  if (a.lse != nullptr && lane == 0) a.lse[r] = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
+template <typename T, int DP, int NW, int QW>
+int launch_attend(AttnArgs a, hipStream_t stream) {
+  constexpr int rows = NW * QW * 32;
+  const bool z = a.mask != nullptr || a.dim < DP;
+  const int64_t per = a.cu_q != nullptr ? a.total_q * a.group / rows + a.batch
+                                        : ceil_div(static_cast<int64_t>(a.len_q) * a.group, rows) * a.batch;
+  const int64_t blocks = per * a.hk * a.splits;
+  HI3D_REQUIRE(blocks < (1ll << 31), "too many rows for one launch");
+  a.slots = static_cast<int>(per);
+  const size_t lds = 4 * kKT * DP * 2;
+  const dim3 grid(static_cast<unsigned>(blocks)), block(64 * NW);
+  if (a.splits > 1) {
+    if (z) hipLaunchKernelGGL((attend_kernel<T, DP, NW, QW, true, true>), grid, block, lds, stream, a);
+    else hipLaunchKernelGGL((attend_kernel<T, DP, NW, QW, false, true>), grid, block, lds, stream, a);
+    HI3D_LAUNCH_CHECK();
+    const int64_t n = a.total_q * a.hq;
+    hipLaunchKernelGGL(attend_join_kernel<T>, dim3(static_cast<unsigned>(ceil_div(n, 4))), dim3(256), 0, stream, a, n);
+  } else {
+    if (z) hipLaunchKernelGGL((attend_kernel<T, DP, NW, QW, true, false>), grid, block, lds, stream, a);
+    else hipLaunchKernelGGL((attend_kernel<T, DP, NW, QW, false, false>), grid, block, lds, stream, a);
+  }
+  HI3D_LAUNCH_CHECK();
+  return HI3D_OK;
+}
+
+// Rows of a workgroup: one wave where segments are short (a larger tile would be empty),
+// else four.
+int64_t segment_average(const AttnArgs& a) { return ceil_div(a.total_q * a.group, a.batch); }
+
+template <typename T, int DP>
+int launch_attend_dim(const AttnArgs& a, hipStream_t stream) {
+  const int64_t average = segment_average(a);
+  if (average <= 32) return launch_attend<T, DP, 1, 1>(a, stream);
+  if (average <= 64) return launch_attend<T, DP, 1, 2>(a, stream);
+  if constexpr (DP <= 64) return launch_attend<T, DP, 4, 2>(a, stream);
+  else return launch_attend<T, DP, 4, 1>(a, stream);
+}
+
+template <typename T>
+int launch_attend_type(const AttnArgs& a, hipStream_t stream) {
+  switch ((a.dim + 31) / 32) {
+    case 1: return launch_attend_dim<T, 32>(a, stream);
+    case 2: return launch_attend_dim<T, 64>(a, stream);
+    case 3: return launch_attend_dim<T, 96>(a, stream);
+    default: return launch_attend_dim<T, 128>(a, stream);
+  }
+}
+
+// Splits of the key axis: as many as fill the chip twice over, each of at least 4 tiles.
+int attend_splits(int64_t total_q, int64_t total_k, int batch, int hq, int hk, int cus) {
+  const int64_t rows = total_q * (hq / hk), average = ceil_div(rows, batch);
+  const int tile = average <= 32 ? 32 : (average <= 64 ? 64 : 256);
+  const int64_t blocks = (batch * ceil_div(average, tile)) * hk;
+  const int64_t tiles = ceil_div(ceil_div(total_k, batch), kKT);
+  const int64_t fill = static_cast<int64_t>(cus) * (tile <= 64 ? 8 : 2);
+  int64_t splits = fill / (blocks > 0 ? blocks : 1);
+  if (splits > tiles / 4) splits = tiles / 4;
+  if (splits > 256) splits = 256;
+  return splits < 1 ? 1 : static_cast<int>(splits);
+}
+
+}  // namespace
+
+int attention_args(const hi3d_attention_desc* d, AttnArgs& a) {
+  HI3D_REQUIRE(d != nullptr, "null descriptor");
+  HI3D_REQUIRE(d->dtype == HI3D_F16 || d->dtype == HI3D_BF16, "attention takes fp16 or bf16 (got type %d)", d->dtype);
+  HI3D_REQUIRE(d->dim >= 8 && d->dim <= 128 && d->dim % 8 == 0, "head size must be a multiple of 8 up to 128 (got %d)",
+               d->dim);
+  HI3D_REQUIRE(d->heads_k > 0 && d->heads_q > 0 && d->heads_q % d->heads_k == 0,
+               "%d query heads are no multiple of %d key heads", d->heads_q, d->heads_k);
+  HI3D_REQUIRE(d->batch >= 0 && d->total_q >= 0 && d->total_k >= 0, "bad sizes");
+  HI3D_REQUIRE(d->total_q < (1ll << 31) && d->total_k < (1ll << 31), "at most 2^31 - 1 rows");
+  HI3D_REQUIRE(d->scale > 0.0f && d->scale < INFINITY, "scale must be positive and finite");
+  const int group = d->heads_q / d->heads_k;
+  HI3D_REQUIRE(group <= 4096 && d->total_q * group < (1ll << 31) / group, "too many rows for this many heads to a key head");
+  HI3D_REQUIRE(d->cu_q != nullptr || (d->len_q >= 0 && d->total_q == static_cast<int64_t>(d->batch) * d->len_q),
+               "queries: %lld rows are not %d segments of %d", static_cast<long long>(d->total_q), d->batch, d->len_q);
+  HI3D_REQUIRE(d->cu_k != nullptr || (d->len_k >= 0 && d->total_k == static_cast<int64_t>(d->batch) * d->len_k),
+               "keys: %lld rows are not %d segments of %d", static_cast<long long>(d->total_k), d->batch, d->len_k);
+  HI3D_REQUIRE(d->lens_k == nullptr || d->cu_k == nullptr, "lens_k belongs to segments of equal room, not to offsets");
+  if (d->total_q > 0) HI3D_REQUIRE(d->q != nullptr, "null pointer argument");
+  if (d->total_k > 0) HI3D_REQUIRE(d->k != nullptr && d->v != nullptr, "null pointer argument");
+  const uintptr_t at = reinterpret_cast<uintptr_t>(d->q) | reinterpret_cast<uintptr_t>(d->k) | reinterpret_cast<uintptr_t>(d->v);
+  HI3D_REQUIRE(at % 16 == 0, "q, k and v must be 16-byte aligned");
+  for (int i = 0; i < 9; ++i) HI3D_REQUIRE(d->strides[i] % 8 == 0, "strides must be multiples of 8 elements");
+  // 64 rows of a tile are addressed with 32-bit byte offsets
+  for (int i : {1, 4, 7})
+    HI3D_REQUIRE(d->strides[i] >= 0 && d->strides[i] < (1ll << 23), "row strides must be below 2^23 elements");
+  a = AttnArgs{};
+  a.q = d->q, a.k = d->k, a.v = d->v;
+  a.q_b = d->strides[0], a.q_n = d->strides[1], a.q_h = d->strides[2];
+  a.k_b = d->strides[3], a.k_n = d->strides[4], a.k_h = d->strides[5];
+  a.v_b = d->strides[6], a.v_n = d->strides[7], a.v_h = d->strides[8];
+  if (d->cu_q != nullptr) a.q_b = 0;
+  if (d->cu_k != nullptr) a.k_b = a.v_b = 0;
+  a.cu_q = d->cu_q, a.cu_k = d->cu_k, a.lens_k = d->lens_k, a.mask = d->key_mask;
+  a.batch = d->batch, a.len_q = d->len_q, a.len_k = d->len_k, a.total_q = d->total_q, a.total_k = d->total_k;
+  a.hq = d->heads_q, a.hk = d->heads_k, a.group = group, a.dim = d->dim;
+  a.group_magic = group > 1 ? static_cast<uint32_t>(((1ull << 32) + group - 1) / group) : 0;
+  a.scale = d->scale, a.scale2 = d->scale * kLog2e;
+  a.causal = d->causal != 0, a.splits = 1;
+  // short segments: the heads of a row share its cache lines, so they run side by side
+  a.head_minor = d->batch > 0 && d->total_k / d->batch <= 512;
+  a.reverse = a.causal;
+  return HI3D_OK;
+}
+
+}  // namespace hi3d
+
+using namespace hi3d;
+
+extern "C" {
+
+int hi3d_attention_workspace(const hi3d_attention_desc* d, int64_t* bytes) {
+  AttnArgs a;
+  const int rc = attention_args(d, a);
+  if (rc != HI3D_OK) return rc;
+  HI3D_REQUIRE(bytes != nullptr, "null pointer argument");
+  *bytes = 0;
+  if (a.total_q == 0 || a.batch == 0) return HI3D_OK;
+  // without a device (a size query on a build host) the MI355X's 256 compute units
+  int cus = compute_units();
+  if (cus <= 0) cus = 256;
+  const int splits = attend_splits(a.total_q, a.total_k, a.batch, a.hq, a.hk, cus);
+  if (splits > 1) *bytes = static_cast<int64_t>(splits) * a.total_q * a.hq * (a.dim + 2) * 4 + 256;
+  return HI3D_OK;
+}
+
+int hi3d_attention_forward(const hi3d_attention_desc* d, void* out, float* lse, void* workspace,
+                           int64_t workspace_bytes, void* stream_) {
+  AttnArgs a;
+  const int rc = attention_args(d, a);
+  if (rc != HI3D_OK) return rc;
+  if (a.total_q == 0) return HI3D_OK;
+  HI3D_REQUIRE(a.batch > 0, "rows without a segment");
+  HI3D_REQUIRE(out != nullptr && reinterpret_cast<uintptr_t>(out) % 16 == 0, "out must be 16-byte aligned");
+  const int cus = compute_units();
+  HI3D_REQUIRE(cus > 0, "cannot query the compute unit count");
+  a.out = out, a.lse = lse;
+  int splits = attend_splits(a.total_q, a.total_k, a.batch, a.hq, a.hk, cus);
+  if (splits > 1) {
+    const int64_t row_bytes = a.total_q * a.hq * 4;
+    HI3D_REQUIRE(workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 &&
+                     workspace_bytes >= splits * row_bytes * (a.dim + 2),
+                 "workspace too small (%lld bytes)", static_cast<long long>(workspace_bytes));
+    a.splits = splits;
+    a.part = static_cast<float*>(workspace);
+    a.part_ml = a.part + static_cast<int64_t>(splits) * a.total_q * a.hq * a.dim;
+  }
+  hipStream_t stream = as_stream(stream_);
+  return d->dtype == HI3D_F16 ? launch_attend_type<_Float16>(a, stream) : launch_attend_type<__bf16>(a, stream);
+}
+
+}  // extern "C"

@@ -1,7 +1,8 @@
 /*
  * hi3d_amd — C ABI of the MI355X (gfx950) sparse-tensor hot path of the Hi3D refiner:
  * voxel-hash kernel maps, gather-MFMA sparse convolution (submanifold and 2x2x2/s2 with
- * its transpose), the W8A8 int8 linear and the LayerNorm+adaLN row kernel.
+ * its transpose), the W8A8 int8 linear and the LayerNorm+adaLN row kernel; and of the
+ * torso's token operators, rotary positions and attention with its gradients.
  *
  * Conventions
  *  - Every pointer argument named *_dev is device memory owned by the caller; host
@@ -602,6 +603,70 @@ int hi3d_adaln_projection(const float* w_dev, const float* b_dev, const float* c
 int hi3d_adaln_modulation(const void* w_dev, const void* b_dev, int32_t param_dtype, const void* cond_dev,
                           int32_t cond_dtype, int32_t batches, int32_t n_out, int32_t n_in, int32_t apply_silu,
                           void* scale1p_dev, void* shift_dev, void* stream);
+
+/* ------------------------------------------------------------ tokens: positions -- */
+
+/* Rotary positions of up to two tensors of token heads in one launch. Pair p of a token
+ * turns by t = sum_a positions[row][a] * freqs[a][p] (formed and reduced in fp64), p <
+ * rot / 2; a pair is (x[p], x[p + rot / 2]) (interleaved = 0) or (x[2p], x[2p + 1])
+ * (interleaved = 1):
+ *   y_first = scale * (x_first cos t - x_second sin t)
+ *   y_second = scale * (x_first sin t + x_second cos t)
+ * with -t in place of t when inverse = 1 (the gradient). Values from rot on are copied.
+ * Tensor i (0, 1; heads[i] = 0: absent) reads element (row, h, d) at row * x_strides[2i] +
+ * h * x_strides[2i+1] + d and writes y_dev[i] [n, heads[i], dim]; y_dev[i] may be x_dev[i]
+ * when that is contiguous. F32, F16 or BF16; fp32 arithmetic, one rounding. positions_dev is
+ * I32 or I64 with row and axis strides; freqs_dev fp64 [axes, rot / 2]. dim <= 1024,
+ * axes <= 4. */
+int hi3d_rotary(const void* const x_dev[2], void* const y_dev[2], const int32_t heads[2],
+                const int64_t x_strides[4], int32_t dtype, int64_t n, int32_t dim, int32_t rot,
+                const void* positions_dev, int32_t position_dtype, int64_t position_row, int64_t position_axis,
+                int32_t axes, const double* freqs_dev, int32_t interleaved, int32_t inverse, float scale,
+                void* stream);
+
+/* ------------------------------------------------------------ tokens: attention -- */
+
+/* One attention problem: `batch` segments, each with its own queries and keys.
+ * Element (segment b, row i, head h, d) of q lies at b * strides[0] + i * strides[1] +
+ * h * strides[2] + d, of k at strides[3..5], of v at strides[6..8]. With offsets cu_q / cu_k
+ * (int32 [batch + 1], ascending from 0 to the row count) the rows of all segments follow one
+ * another, row cu[b] + i, and the segment stride is not used; without, every segment has
+ * len_q / len_k rows, of which lens_k (int32 [batch], optional) keys are in use.
+ * heads_q is a multiple of heads_k; query head h reads key head h / (heads_q / heads_k).
+ * causal: query i sees keys j <= i + lk - lq. key_mask (uint8, one per key row; optional):
+ * keys with 0 are not seen, whatever they hold. A row that sees no key gives zeros and
+ * lse = -infinity. F16 or BF16, dim a multiple of 8 up to 128, 16-byte aligned pointers,
+ * strides multiples of 8, row strides below 2^23. */
+typedef struct hi3d_attention_desc {
+  const void* q;
+  const void* k;
+  const void* v;
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  const int32_t* lens_k;
+  const uint8_t* key_mask;
+  int64_t strides[9];
+  int64_t total_q;
+  int64_t total_k;
+  int32_t batch;
+  int32_t len_q;
+  int32_t len_k;
+  int32_t heads_q;
+  int32_t heads_k;
+  int32_t dim;
+  int32_t dtype;
+  int32_t causal;
+  float scale;
+} hi3d_attention_desc;
+
+/* Workspace bytes of hi3d_attention_forward (0 where the key axis is not split). */
+int hi3d_attention_workspace(const hi3d_attention_desc* desc_host, int64_t* bytes_host);
+
+/* out_dev [total_q, heads_q, dim] = softmax(scale q k^T) v, and lse_dev fp32 [total_q,
+ * heads_q] (optional) = log sum exp(scale q k^T). Scores, sums and the output accumulate in
+ * fp32; the probabilities are rounded once to the inputs' type for their product with v. */
+int hi3d_attention_forward(const hi3d_attention_desc* desc_host, void* out_dev, float* lse_dev,
+                           void* workspace_dev, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
