@@ -216,4 +216,12 @@ __device__ __forceinline__ void load_pair(const char* x, int64_t x_n, const char
   }
 }
 
+// Every wave's tile loads have landed and its reads of the other tile are done. The wait is
+// explicit: a wave that skips a tile runs none of the reads that the compiler waits before,
+// and a workgroup of one wave has no barrier at all.
+__device__ __forceinline__ void tile_barrier() {
+  wait_vmcnt<0>();
+  __syncthreads();
+}
+
 }  // namespace hi3d

@@ -104,7 +104,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_kernel(AttnArgs a) {
     load(t0, bits, 0);
     if (t0 + 1 < t1) next = key_bits(t0 + 1);
   }
-  __syncthreads();
+  tile_barrier();
   for (int t = t0, buf = 0; t < t1; ++t, buf ^= 1) {
     if (t + 1 < t1) load(t + 1, next, buf ^ 1);
     uint64_t after = 0;
@@ -191,7 +191,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_kernel(AttnArgs a) {
       }
     }
     bits = next, next = after;
-    __syncthreads();
+    tile_barrier();
   }
 
 #pragma unroll

@@ -151,7 +151,7 @@ int hi3d_rotary(const void* const x[2], void* const y[2], const int32_t heads[2]
   HI3D_REQUIRE(dtype == HI3D_F32 || dtype == HI3D_F16 || dtype == HI3D_BF16, "rotary takes fp32, fp16 or bf16 (got type %d)",
                dtype);
   HI3D_REQUIRE(position_dtype == HI3D_I32 || position_dtype == HI3D_I64, "positions must be int32 or int64");
-  HI3D_REQUIRE(n >= 0 && heads[0] >= 0 && heads[1] >= 0 && heads[0] <= 4096 && heads[1] <= 4096, "bad sizes");
+  HI3D_REQUIRE(n >= 0 && heads[0] >= 0 && heads[1] >= 0 && heads[0] <= 2048 && heads[1] <= 2048, "bad sizes");
   HI3D_REQUIRE(dim > 0 && dim <= 1024, "head size must be 1 to 1024 (got %d)", dim);
   HI3D_REQUIRE(rot >= 0 && rot % 2 == 0 && rot <= dim, "%d turned values of %d: must be even and at most the head size",
                rot, dim);
