@@ -37,8 +37,11 @@ constexpr float kLn2 = 0.6931471805599453f;
 struct AttnArgs {
   const void *q, *k, *v;        // rows of heads: element (b, i, h, d) at b*_b + i*_n + h*_h + d
   const void *o, *dout;         // backward: output and its gradient, [total_q, hq, d]
+  const float* dlse;            // gradient of lse [total_q, hq], or null
   void *out, *dk, *dv;          // out: output, or dq; all [total, heads, d]
   float *lse, *delta;           // [total_q, hq]
+  float* bound;                 // backward: [hk, dq_slots, dq_waves] bounds of dout's rows (fp16)
+  int32_t dq_rows, dq_waves, dq_slots;
   float *part, *part_ml;        // split forward: [split, total_q, hq, d], [split, total_q, hq, 2]
   int64_t q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h;
   const int32_t *cu_q, *cu_k;   // [batch + 1] offsets of packed segments, or null: b * len

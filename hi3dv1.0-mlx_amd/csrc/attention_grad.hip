@@ -1,0 +1,599 @@
+// Gradients of attention (attention.hip). With D_i = sum_d dout_id out_id - dlse_i and
+// p_ij = exp(scale q_i k_j - lse_i), recomputed from q, k and the forward's lse:
+//   dv_j = sum_i p_ij dout_i          dp_ij = dout_i v_j       ds_ij = p_ij (dp_ij - D_i)
+//   dq_i = scale sum_j ds_ij k_j      dk_j = scale sum_i ds_ij q_i
+// Two kernels, each of which owns what it sums, so nothing is added by atomics and the bits
+// are the same every time: dq by query rows (it also forms D), then dk and dv by key rows.
+// Scores and dp are formed in both: 7 products for 5, against fp32 atomics on dq.
+//
+// p and ds are rounded once to the inputs' type for their products. fp16 holds 2^-24 to
+// 2^16, and a loss's gradients over long rows (p near 1 / keys) would sink below that, so in
+// fp16 both are scaled by powers of two that come out again in fp32 at the end: p by 2^10,
+// ds so that 8 to 16 stands for the largest sum_d |dout_d| of the rows that are summed
+// (|ds| <= p (1 - p) 2 sum |dout| max |v|: it cannot overflow below |v| = 8190). bf16 has
+// fp32's range and takes no scale.
+#include <type_traits>
+
+#include "attention.h"
+
+namespace hi3d {
+
+int attention_args(const hi3d_attention_desc* d, AttnArgs& a);
+
+namespace {
+
+// 32 owned rows of a wave as second operands (lane l: row l % 32, chunks 2 k + l / 32).
+template <int DP>
+__device__ __forceinline__ void load_owned(const char* src, int dim, int h, bool on, u32x4 (&x)[DP / 16]) {
+#pragma unroll
+  for (int k = 0; k < DP / 16; ++k) {
+    const int c = 16 * k + 8 * h;
+    u32x4 v = {0, 0, 0, 0};
+    if (on && c < dim) v = *reinterpret_cast<const u32x4*>(src + c * 2);
+    x[k] = v;
+  }
+}
+
+template <typename T, int DP>
+__device__ __forceinline__ void store_owned(T* to, int dim, int h, const f32x16 (&acc)[DP / 32], float by, bool zero) {
+  typedef T t4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int c = 32 * d + 8 * e + 4 * h;
+      t4 x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = static_cast<T>(zero ? 0.0f : acc[d][4 * e + j] * by);
+      if (c < dim) *reinterpret_cast<t4*>(to + c) = x;
+    }
+}
+
+template <typename T>
+constexpr float kPLog2 = std::is_same_v<T, _Float16> ? 10.0f : 0.0f;
+
+// Exponent of the scale of ds for rows whose sum |dout| is at most `bound`.
+template <typename T>
+__device__ __forceinline__ int ds_exponent(float bound) {
+  if constexpr (!std::is_same_v<T, _Float16>) return 0;
+  if (!(bound > 0.0f && bound < INFINITY)) return 0;
+  const int e = 4 - __builtin_amdgcn_frexp_expf(bound);
+  return e < -64 ? -64 : (e > 64 ? 64 : e);
+}
+__device__ __forceinline__ float power_of_two(int e) { return __builtin_amdgcn_ldexpf(1.0f, e); }
+
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) x = fmaxf(x, __shfl_xor(x, d));
+  return x;
+}
+
+// dq and D. A workgroup owns NW * QW * 32 packed query rows of one key head (queries and
+// dout in registers) and walks the keys in tiles of 64 held twice in LDS, as the forward
+// does. Per 32 keys a wave forms S^T = K Q^T and dP^T = V dO^T, then dq += K^T dS^T with
+// the same K tile read transposed.
+template <typename T, int DP, int NW, int QW, bool Z>
+__global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
+  constexpr int ROWS = NW * QW * 32, KS = DP / 16, DB = DP / 32, PAIR = 2 * kKT * DP * 2;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c32 = lane & 31, h = lane >> 5;
+  const int64_t id = xcd_remap(blockIdx.x, gridDim.x);
+  int head, slot;
+  if (a.head_minor) head = static_cast<int>(id % a.hk), slot = static_cast<int>(id / a.hk);
+  else slot = static_cast<int>(id % a.slots), head = static_cast<int>(id / a.slots);
+  if (a.causal) slot = a.slots - 1 - slot;  // the longest rows first
+  Segment s;
+  find_segment(a.cu_q, a.len_q, a.batch, a.total_q, a.group, ROWS, slot, s);
+  segment_rows(a, s);
+  const int rows = s.lq * a.group, row0 = s.tile * ROWS;
+  const int wrow = row0 + wave * (QW * 32);
+  float* bound = a.bound + (static_cast<int64_t>(head) * a.slots + slot) * NW + wave;
+  if (s.tile < 0 || row0 >= rows) return;
+
+  const int off = s.lk - s.lq;
+  int qi[QW], qg[QW];
+  u32x4 qf[QW][KS], df[QW][KS];
+  float ref[QW], delta[QW], size[QW];  // log2 of the scaled p's divisor, D, sum |dout|
+#pragma unroll
+  for (int b = 0; b < QW; ++b) {
+    const int r = wrow + b * 32 + c32;
+    split_row(a, r < rows ? r : rows - 1, qi[b], qg[b]);
+    const int64_t at = (s.q0 + qi[b]) * a.hq + head * a.group + qg[b];
+    const T* src = static_cast<const T*>(a.q) + s.b * a.q_b + (a.cu_q != nullptr ? s.q0 + qi[b] : qi[b]) * a.q_n +
+                   static_cast<int64_t>(head * a.group + qg[b]) * a.q_h;
+    load_owned<DP>(reinterpret_cast<const char*>(src), a.dim, h, true, qf[b]);
+    load_owned<DP>(reinterpret_cast<const char*>(static_cast<const T*>(a.dout) + at * a.dim), a.dim, h, true, df[b]);
+    u32x4 of[KS];
+    load_owned<DP>(reinterpret_cast<const char*>(static_cast<const T*>(a.o) + at * a.dim), a.dim, h, true, of);
+    float x = 0.0f, y = 0.0f;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      const auto u = __builtin_bit_cast(typename Vec8<T>::type, df[b][k]), v = __builtin_bit_cast(typename Vec8<T>::type, of[k]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x = __builtin_fmaf(static_cast<float>(u[e]), static_cast<float>(v[e]), x);
+        y += __builtin_fabsf(static_cast<float>(u[e]));
+      }
+    }
+    delta[b] = half_sum(x), size[b] = half_sum(y);
+    if (a.dlse != nullptr) {
+      const float z = a.dlse[at];
+      delta[b] -= z, size[b] = fmaxf(size[b], __builtin_fabsf(z));
+    }
+    const float lse = a.lse[at];
+    ref[b] = (lse == -INFINITY ? 0.0f : lse * kLog2e) - kPLog2<T>;  // a row that sees no key: all its scores are hidden
+    if (h == 0 && r < rows) a.delta[at] = delta[b];
+  }
+  if constexpr (std::is_same_v<T, _Float16>) {  // (a row repeated past the end changes no maximum)
+    float x = size[0];
+#pragma unroll
+    for (int b = 1; b < QW; ++b) x = fmaxf(x, size[b]);
+    x = wave_max(x);
+    if (lane == 0) *bound = wrow < rows ? x : 0.0f;
+  }
+  if (a.out == nullptr) return;  // only D and the bounds are wanted
+  float by[QW];  // of dp - D: the scale of ds without that of p
+#pragma unroll
+  for (int b = 0; b < QW; ++b) {
+    const int e = ds_exponent<T>(size[b]);
+    by[b] = power_of_two(e - static_cast<int>(kPLog2<T>)), delta[b] *= by[b];
+    size[b] = a.scale * power_of_two(-e);  // takes the scale out of dq
+  }
+  int kend = s.lk, wkend = wrow < rows ? s.lk : 0, wfull = s.lk;  // keys of the workgroup; of the wave; of all its rows
+  if (a.causal) {
+    int i, g;
+    split_row(a, min(rows, row0 + ROWS) - 1, i, g);
+    kend = min(kend, i + off + 1);
+    if (wrow < rows) {
+      split_row(a, min(rows, wrow + QW * 32) - 1, i, g);
+      wkend = min(wkend, i + off + 1);
+      split_row(a, wrow, i, g);
+      wfull = min(wfull, i + off + 1);
+    }
+  }
+  const int tiles = kend > 0 ? (kend + kKT - 1) / kKT : 0;
+
+  const char* kp = reinterpret_cast<const char*>(static_cast<const T*>(a.k) + s.b * a.k_b + head * a.k_h +
+                                                 (a.cu_k != nullptr ? s.k0 * a.k_n : 0));
+  const char* vp = reinterpret_cast<const char*>(static_cast<const T*>(a.v) + s.b * a.v_b + head * a.v_h +
+                                                 (a.cu_k != nullptr ? s.k0 * a.v_n : 0));
+  auto key_bits = [&](int t) -> uint64_t {
+    const int key = t * kKT + lane;
+    bool on = key < s.lk;
+    if (Z && a.mask != nullptr) on = on && a.mask[s.k0 + (key < s.lk ? key : 0)] != 0;
+    return __ballot(on);
+  };
+  auto load = [&](int t, uint64_t bits, int buf) {
+    const int64_t at = static_cast<int64_t>(t) * kKT;
+    load_pair<DP, NW, Z>(kp + at * a.k_n * 2, a.k_n, vp + at * a.v_n * 2, a.v_n, min(kKT, s.lk - t * kKT), bits, a.dim,
+                         smem + buf * PAIR, wave, lane);
+  };
+
+  f32x16 acc[QW][DB] = {};
+  uint64_t bits = 0, next = 0;
+  if (tiles > 0) {
+    bits = key_bits(0);
+    load(0, bits, 0);
+    if (tiles > 1) next = key_bits(1);
+  }
+  tile_barrier();
+  for (int t = 0, buf = 0; t < tiles; ++t, buf ^= 1) {
+    if (t + 1 < tiles) load(t + 1, next, buf ^ 1);
+    uint64_t after = 0;
+    if (t + 2 < tiles) after = key_bits(t + 2);
+    if (t * kKT < wkend) {
+      const char* kt = smem + buf * PAIR;
+      const char* vt = kt + kKT * DP * 2;
+      const bool hide = bits != ~0ull || (t + 1) * kKT > wfull;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        f32x16 sc[QW] = {}, dp[QW] = {};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const u32x4 x = read_rows<DP>(kt, 32 * n + c32, k, h), y = read_rows<DP>(vt, 32 * n + c32, k, h);
+#pragma unroll
+          for (int b = 0; b < QW; ++b) Mfma<T>::run(x, qf[b][k], sc[b]), Mfma<T>::run(y, df[b][k], dp[b]);
+        }
+        if (hide) {
+#pragma unroll
+          for (int b = 0; b < QW; ++b) {
+            uint64_t on = bits;
+            if (a.causal) {
+              const int seen = qi[b] + off + 1 - t * kKT;  // keys of this tile that the row sees
+              on &= seen >= 64 ? ~0ull : (seen <= 0 ? 0ull : (1ull << seen) - 1);
+            }
+            const uint32_t w = static_cast<uint32_t>(on >> (32 * n)) >> (4 * h);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sc[b][e] = (w >> (8 * (e >> 2) + (e & 3))) & 1 ? sc[b][e] : -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < QW; ++b)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][e], a.scale2, -ref[b]));
+            dp[b][e] = p * __builtin_fmaf(dp[b][e], by[b], -delta[b]);
+          }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          u32x4 ds[QW];
+#pragma unroll
+          for (int b = 0; b < QW; ++b) {
+            f32x8 x;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = dp[b][8 * k + e];
+            ds[b] = pack8<T>(x);
+          }
+#pragma unroll
+          for (int d = 0; d < DB; ++d) {
+            const u32x4 x = read_columns<DP>(kt, 32 * n + 16 * k, d, lane);
+#pragma unroll
+            for (int b = 0; b < QW; ++b) Mfma<T>::run(x, ds[b], acc[b][d]);
+          }
+        }
+      }
+    }
+    bits = next, next = after;
+    tile_barrier();
+  }
+#pragma unroll
+  for (int b = 0; b < QW; ++b) {
+    if (wrow + b * 32 + c32 >= rows) continue;
+    const int64_t at = (s.q0 + qi[b]) * a.hq + head * a.group + qg[b];
+    store_owned<T, DP>(static_cast<T*>(a.out) + at * a.dim, a.dim, h, acc[b], size[b], false);
+  }
+}
+
+// dk and dv. A workgroup owns NW * QW * 32 keys of one key head (keys and values in
+// registers) and walks the packed query rows that read the head in tiles of 64 (queries and
+// dout, with lse and D of each row) held twice in LDS, so the query heads of a shared key
+// head sum in registers. Rows past the segment and rows that saw no key have lse = +infinity:
+// their probabilities are zero.
+template <typename T, int DP, int NW, int QW, bool Z, bool SPLIT>
+__global__ __launch_bounds__(64 * NW, 2) void attend_dkv_kernel(AttnArgs a) {
+  constexpr int KEYS = NW * QW * 32, KS = DP / 16, DB = DP / 32, PAIR = 2 * kKT * DP * 2, CH = DP / 8;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  float* stats = reinterpret_cast<float*>(smem + 2 * PAIR);  // [2][lse, D][64]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c32 = lane & 31, h = lane >> 5;
+  const int64_t id = xcd_remap(blockIdx.x, gridDim.x);
+  int head, split = 0, slot;
+  if (a.head_minor) {
+    head = static_cast<int>(id % a.hk), slot = static_cast<int>(id / a.hk);
+    if constexpr (SPLIT) split = slot % a.splits, slot /= a.splits;
+  } else {
+    slot = static_cast<int>(id % a.slots), head = static_cast<int>(id / a.slots);
+    if constexpr (SPLIT) split = head % a.splits, head /= a.splits;
+  }
+  Segment s;
+  find_segment(a.cu_k, a.len_k, a.batch, a.total_k, 1, KEYS, slot, s);
+  segment_rows(a, s);
+  const int room = a.cu_k != nullptr ? s.lk : a.len_k;  // keys past those in use get zeros
+  const int key0 = s.tile * KEYS;
+  if (s.tile < 0 || key0 >= room) return;
+
+  const int wkey = key0 + wave * (QW * 32);
+  const int off = s.lk - s.lq, rows = s.lq * a.group;
+  u32x4 kf[QW][KS], vf[QW][KS];
+  bool on[QW];
+#pragma unroll
+  for (int b = 0; b < QW; ++b) {
+    const int j = wkey + b * 32 + c32;
+    on[b] = j < s.lk;
+    if (Z && a.mask != nullptr) on[b] = on[b] && a.mask[s.k0 + (j < s.lk ? j : 0)] != 0;
+    const int64_t row = (a.cu_k != nullptr ? s.k0 : 0) + (j < s.lk ? j : 0);
+    load_owned<DP>(reinterpret_cast<const char*>(static_cast<const T*>(a.k) + s.b * a.k_b + row * a.k_n + head * a.k_h),
+                   a.dim, h, on[b], kf[b]);
+    load_owned<DP>(reinterpret_cast<const char*>(static_cast<const T*>(a.v) + s.b * a.v_b + row * a.v_n + head * a.v_h),
+                   a.dim, h, on[b], vf[b]);
+  }
+  // packed rows that see a key of the workgroup, of the wave, and all keys of the wave: i >= key - off
+  int first = 0, wfirst = wkey < s.lk ? 0 : rows, wfull = 0;
+  if (a.causal) {
+    first = min(s.lq, max(0, key0 - off)) * a.group;
+    if (wkey < s.lk) wfirst = min(s.lq, max(0, wkey - off)) * a.group;
+    wfull = min(s.lq, max(0, wkey + QW * 32 - 1 - off)) * a.group;
+  }
+  const int tiles = key0 < s.lk ? (rows + kKT - 1) / kKT : 0;
+  int t0 = first / kKT, t1 = tiles;
+  if constexpr (SPLIT) {
+    const int per = max(1, (tiles - t0 + a.splits - 1) / a.splits);
+    t0 = min(tiles, t0 + split * per), t1 = min(tiles, t0 + per);
+  }
+
+  const char* qp = reinterpret_cast<const char*>(static_cast<const T*>(a.q) + s.b * a.q_b +
+                                                 (a.cu_q != nullptr ? s.q0 * a.q_n : 0) +
+                                                 static_cast<int64_t>(head) * a.group * a.q_h);
+  const int64_t row_at = s.q0 * a.hq + head * a.group;  // of lse, D and dout
+  const char* dp_ = reinterpret_cast<const char*>(static_cast<const T*>(a.dout) + row_at * a.dim);
+  auto load = [&](int t, int buf) {
+#pragma unroll
+    for (int i = 0; i < CH / NW; ++i) {
+      const int u = (wave + i * NW) * 64 + lane;
+      const int row = u / CH, c = (u % CH) ^ row_xor<DP>(row);
+      int qi, qg;
+      split_row(a, min(t * kKT + row, rows - 1), qi, qg);
+      const char* x = qp + (qi * a.q_n + qg * a.q_h) * 2 + c * 16;
+      const char* y = dp_ + (static_cast<int64_t>(qi) * a.hq + qg) * a.dim * 2 + c * 16;
+      if constexpr (Z) {
+        if (c * 8 >= a.dim) x = y = reinterpret_cast<const char*>(&kZeroChunk);
+      }
+      char* to = smem + buf * PAIR + (wave + i * NW) * 1024;
+      lds_dma16(x, to);
+      lds_dma16(y, to + kKT * DP * 2);
+    }
+  };
+  // the scale of ds of this segment and head, from the bounds that the dq kernel's waves left
+  float by = 1.0f, dk_by = a.scale, dv_by = 1.0f;
+  if constexpr (std::is_same_v<T, _Float16>) {
+    const int64_t slot0 = a.cu_q != nullptr
+                              ? static_cast<int64_t>(clamp_offset(a.cu_q[s.b], a.total_q)) * a.group / a.dq_rows + s.b
+                              : s.b * ((static_cast<int64_t>(a.len_q) * a.group + a.dq_rows - 1) / a.dq_rows);
+    const float* bounds = a.bound + (static_cast<int64_t>(head) * a.dq_slots + slot0) * a.dq_waves;
+    const int count = (rows + a.dq_rows - 1) / a.dq_rows * a.dq_waves;
+    float x = 0.0f;
+    for (int j = lane; j < count; j += 64) x = fmaxf(x, bounds[j]);
+    const int e = ds_exponent<T>(wave_max(x));
+    by = power_of_two(e - static_cast<int>(kPLog2<T>)), dk_by *= power_of_two(-e);
+    dv_by = power_of_two(-static_cast<int>(kPLog2<T>));
+  }
+  float lse = 0.0f, delta = 0.0f;
+  auto load_stats = [&](int t) {  // by the first wave: row t * 64 + lane
+    const int r = t * kKT + lane;
+    int qi, qg;
+    split_row(a, min(r, rows - 1), qi, qg);
+    const int64_t at = row_at + static_cast<int64_t>(qi) * a.hq + qg;
+    lse = r < rows ? a.lse[at] : -INFINITY, delta = a.delta[at];
+  };
+  auto store_stats = [&](int buf) {  // used only here, so that the loads are not waited for before the tile's work
+    const bool none = lse == -INFINITY;
+    stats[buf * 128 + lane] = none ? INFINITY : lse * kLog2e - kPLog2<T>;
+    stats[buf * 128 + 64 + lane] = none ? 0.0f : delta * by;
+  };
+
+  f32x16 dk[QW][DB] = {}, dv[QW][DB] = {};
+  if (t0 < t1) {
+    load(t0, 0);
+    if (wave == 0) load_stats(t0), store_stats(0);
+  }
+  tile_barrier();
+  for (int t = t0, buf = 0; t < t1; ++t, buf ^= 1) {
+    if (t + 1 < t1) {
+      load(t + 1, buf ^ 1);
+      if (wave == 0) load_stats(t + 1);
+    }
+    if ((t + 1) * kKT > wfirst) {
+      const char* qt = smem + buf * PAIR;
+      const char* dt = qt + kKT * DP * 2;
+      const float* st = stats + buf * 128;
+      const bool hide = t * kKT < wfull;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        f32x16 sc[QW] = {}, dp[QW] = {};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const u32x4 x = read_rows<DP>(qt, 32 * n + c32, k, h), y = read_rows<DP>(dt, 32 * n + c32, k, h);
+#pragma unroll
+          for (int b = 0; b < QW; ++b) Mfma<T>::run(x, kf[b][k], sc[b]), Mfma<T>::run(y, vf[b][k], dp[b]);
+        }
+        if (hide) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            int qi, qg;
+            split_row(a, min(t * kKT + 32 * n + 8 * (e >> 2) + 4 * h + (e & 3), rows - 1), qi, qg);
+#pragma unroll
+            for (int b = 0; b < QW; ++b)
+              sc[b][e] = wkey + b * 32 + c32 <= qi + off ? sc[b][e] : -INFINITY;
+          }
+        }
+        u32x4 p[QW][2], ds[QW][2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          f32x8 ps[QW], dss[QW];
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const f32x4 l4 = *reinterpret_cast<const f32x4*>(st + 32 * n + 16 * k + 8 * g + 4 * h);
+            const f32x4 d4 = *reinterpret_cast<const f32x4*>(st + 64 + 32 * n + 16 * k + 8 * g + 4 * h);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+              for (int b = 0; b < QW; ++b) {
+                const int at = 8 * k + 4 * g + e;
+                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][at], a.scale2, -l4[e]));
+                ps[b][4 * g + e] = x, dss[b][4 * g + e] = x * __builtin_fmaf(dp[b][at], by, -d4[e]);
+              }
+          }
+#pragma unroll
+          for (int b = 0; b < QW; ++b) p[b][k] = pack8<T>(ps[b]), ds[b][k] = pack8<T>(dss[b]);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int d = 0; d < DB; ++d) {
+            const u32x4 x = read_columns<DP>(dt, 32 * n + 16 * k, d, lane), y = read_columns<DP>(qt, 32 * n + 16 * k, d, lane);
+#pragma unroll
+            for (int b = 0; b < QW; ++b) Mfma<T>::run(x, p[b][k], dv[b][d]), Mfma<T>::run(y, ds[b][k], dk[b][d]);
+          }
+      }
+    }
+    if (wave == 0 && t + 1 < t1) store_stats(buf ^ 1);
+    tile_barrier();
+  }
+#pragma unroll
+  for (int b = 0; b < QW; ++b) {
+    const int j = wkey + b * 32 + c32;
+    if (j >= room) continue;
+    const int64_t at = ((s.k0 + j) * a.hk + head) * a.dim;
+    if constexpr (SPLIT) {
+      const int64_t all = a.total_k * a.hk * a.dim;
+      store_owned<float, DP>(a.part + split * 2 * all + at, a.dim, h, dk[b], dk_by, !on[b]);
+      store_owned<float, DP>(a.part + (split * 2 + 1) * all + at, a.dim, h, dv[b], dv_by, !on[b]);
+    } else {
+      store_owned<T, DP>(static_cast<T*>(a.dk) + at, a.dim, h, dk[b], dk_by, !on[b]);
+      store_owned<T, DP>(static_cast<T*>(a.dv) + at, a.dim, h, dv[b], dv_by, !on[b]);
+    }
+  }
+}
+
+// Sums the splits of dk and dv in order; 4 values a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void attend_dkv_join_kernel(AttnArgs a, int64_t all) {
+  const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
+  if (i >= 2 * all) return;
+  f32x4 x = {0, 0, 0, 0};
+  for (int s = 0; s < a.splits; ++s) x += *reinterpret_cast<const f32x4*>(a.part + s * 2 * all + i);
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  T* to = i < all ? static_cast<T*>(a.dk) + i : static_cast<T*>(a.dv) + (i - all);
+  *reinterpret_cast<t4*>(to) = t4{static_cast<T>(x[0]), static_cast<T>(x[1]), static_cast<T>(x[2]), static_cast<T>(x[3])};
+}
+
+template <typename T, int DP, int NW, int QW>
+int launch_dq(AttnArgs a, hipStream_t stream) {
+  constexpr int rows = NW * QW * 32;
+  HI3D_REQUIRE(static_cast<int64_t>(a.dq_slots) * a.hk < (1ll << 31), "too many rows for one launch");
+  if (rows != a.dq_rows || NW != a.dq_waves) return fail(HI3D_ERR_INVALID, "the tile differs from the workspace's");
+  a.slots = a.dq_slots;
+  const dim3 grid(static_cast<unsigned>(a.slots * a.hk)), block(64 * NW);
+  const size_t lds = 4 * kKT * DP * 2;
+  if (a.mask != nullptr || a.dim < DP) hipLaunchKernelGGL((attend_dq_kernel<T, DP, NW, QW, true>), grid, block, lds, stream, a);
+  else hipLaunchKernelGGL((attend_dq_kernel<T, DP, NW, QW, false>), grid, block, lds, stream, a);
+  HI3D_LAUNCH_CHECK();
+  return HI3D_OK;
+}
+
+template <typename T, int DP, int NW, int QW, bool Z, bool SPLIT>
+int launch_dkv_variant(const AttnArgs& a, dim3 grid, size_t lds, hipStream_t stream) {
+  if (lds > 65536)
+    HI3D_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&attend_dkv_kernel<T, DP, NW, QW, Z, SPLIT>),
+                                       hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
+  hipLaunchKernelGGL((attend_dkv_kernel<T, DP, NW, QW, Z, SPLIT>), grid, dim3(64 * NW), lds, stream, a);
+  HI3D_LAUNCH_CHECK();
+  return HI3D_OK;
+}
+
+template <typename T, int DP, int NW, int QW>
+int launch_dkv(AttnArgs a, hipStream_t stream) {
+  constexpr int keys = NW * QW * 32;
+  const int64_t per = a.cu_k != nullptr ? a.total_k / keys + a.batch : ceil_div(a.len_k, keys) * a.batch;
+  const int64_t blocks = per * a.hk * a.splits;
+  HI3D_REQUIRE(blocks < (1ll << 31), "too many rows for one launch");
+  a.slots = static_cast<int>(per);
+  const dim3 grid(static_cast<unsigned>(blocks));
+  const size_t lds = 4 * kKT * DP * 2 + 1024;
+  const bool z = a.mask != nullptr || a.dim < DP;
+  if (a.splits == 1)
+    return z ? launch_dkv_variant<T, DP, NW, QW, true, false>(a, grid, lds, stream)
+             : launch_dkv_variant<T, DP, NW, QW, false, false>(a, grid, lds, stream);
+  const int rc = z ? launch_dkv_variant<T, DP, NW, QW, true, true>(a, grid, lds, stream)
+                   : launch_dkv_variant<T, DP, NW, QW, false, true>(a, grid, lds, stream);
+  if (rc != HI3D_OK) return rc;
+  const int64_t all = a.total_k * a.hk * a.dim;
+  hipLaunchKernelGGL(attend_dkv_join_kernel<T>, dim3(static_cast<unsigned>(ceil_div(2 * all, 1024))), dim3(256), 0, stream, a,
+                     all);
+  HI3D_LAUNCH_CHECK();
+  return HI3D_OK;
+}
+
+template <typename T, int DP>
+int launch_grad_dim(const AttnArgs& a, hipStream_t stream) {
+  if (a.total_q > 0) {
+    int rc = HI3D_OK;
+    if (a.dq_waves == 1) rc = launch_dq<T, DP, 1, 1>(a, stream);
+    else rc = launch_dq<T, DP, 4, 1>(a, stream);
+    if (rc != HI3D_OK) return rc;
+  }
+  if (a.total_k == 0 || a.dk == nullptr) return HI3D_OK;
+  if (ceil_div(a.total_k, a.batch) <= 32) return launch_dkv<T, DP, 1, 1>(a, stream);
+  return launch_dkv<T, DP, 4, 1>(a, stream);
+}
+
+template <typename T>
+int launch_grad_type(const AttnArgs& a, hipStream_t stream) {
+  switch ((a.dim + 31) / 32) {
+    case 1: return launch_grad_dim<T, 32>(a, stream);
+    case 2: return launch_grad_dim<T, 64>(a, stream);
+    case 3: return launch_grad_dim<T, 96>(a, stream);
+    default: return launch_grad_dim<T, 128>(a, stream);
+  }
+}
+
+// Splits of the query rows for dk and dv: as many as give every compute unit two workgroups,
+// each of at least 4 tiles of the average segment.
+int dkv_splits(const AttnArgs& a, int cus) {
+  const int64_t average = ceil_div(a.total_k, a.batch), tile = average <= 32 ? 32 : 128;
+  const int64_t blocks = a.batch * ceil_div(average, tile) * a.hk;
+  const int64_t tiles = ceil_div(ceil_div(a.total_q * a.group, a.batch), kKT);
+  int64_t splits = 2 * static_cast<int64_t>(cus) * (tile == 32 ? 4 : 1) / (blocks > 0 ? blocks : 1);
+  if (splits > tiles / 4) splits = tiles / 4;
+  if (splits > 64) splits = 64;
+  return splits < 1 ? 1 : static_cast<int>(splits);
+}
+
+// Query rows to a workgroup: segments of up to 32 rows on average get a wave each (a larger
+// tile would be empty).
+void dq_tiles(AttnArgs& a) {
+  a.dq_waves = ceil_div(a.total_q * a.group, a.batch) <= 32 ? 1 : 4;
+  a.dq_rows = 32 * a.dq_waves;
+  a.dq_slots = static_cast<int>(a.cu_q != nullptr ? a.total_q * a.group / a.dq_rows + a.batch
+                                                  : ceil_div(static_cast<int64_t>(a.len_q) * a.group, a.dq_rows) * a.batch);
+}
+
+// Workspace: D, the bounds of dout's rows, the parts of dk and dv.
+int64_t delta_bytes(const AttnArgs& a) { return align_up(a.total_q * a.hq * 4, 256); }
+int64_t bound_bytes(const AttnArgs& a) { return align_up(static_cast<int64_t>(a.hk) * a.dq_slots * a.dq_waves * 4, 256); }
+
+}  // namespace
+}  // namespace hi3d
+
+using namespace hi3d;
+
+extern "C" {
+
+int hi3d_attention_backward_workspace(const hi3d_attention_desc* d, int64_t* bytes) {
+  AttnArgs a;
+  const int rc = attention_args(d, a);
+  if (rc != HI3D_OK) return rc;
+  HI3D_REQUIRE(bytes != nullptr, "null pointer argument");
+  *bytes = 0;
+  if (a.batch == 0) return HI3D_OK;
+  int cus = compute_units();
+  if (cus <= 0) cus = 256;  // without a device: the MI355X's
+  const int splits = a.total_k > 0 ? dkv_splits(a, cus) : 1;
+  dq_tiles(a);
+  *bytes = delta_bytes(a) + bound_bytes(a) + (splits > 1 ? splits * 2 * a.total_k * a.hk * a.dim * 4 : 0);
+  return HI3D_OK;
+}
+
+int hi3d_attention_backward(const hi3d_attention_desc* d, const void* out, const float* lse, const void* dout,
+                            const float* dlse, void* dq, void* dk, void* dv, void* workspace, int64_t workspace_bytes,
+                            void* stream_) {
+  AttnArgs a;
+  int64_t need = 0;
+  int rc = attention_args(d, a);
+  if (rc == HI3D_OK) rc = hi3d_attention_backward_workspace(d, &need);
+  if (rc != HI3D_OK) return rc;
+  HI3D_REQUIRE((dk == nullptr) == (dv == nullptr), "dk and dv are formed together");
+  if ((a.total_q == 0 && a.total_k == 0) || (dq == nullptr && dk == nullptr)) return HI3D_OK;
+  HI3D_REQUIRE(a.batch > 0, "rows without a segment");
+  if (a.total_q > 0) HI3D_REQUIRE(out != nullptr && lse != nullptr && dout != nullptr, "null pointer argument");
+  const uintptr_t at = reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(dout) | reinterpret_cast<uintptr_t>(dq) |
+                       reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv) |
+                       reinterpret_cast<uintptr_t>(workspace);
+  HI3D_REQUIRE(at % 16 == 0, "out, dout, the gradients and the workspace must be 16-byte aligned");
+  HI3D_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), "workspace too small (%lld bytes, need %lld)",
+               static_cast<long long>(workspace_bytes), static_cast<long long>(need));
+  const int cus = compute_units();
+  HI3D_REQUIRE(cus > 0, "cannot query the compute unit count");
+  a.o = out, a.lse = const_cast<float*>(lse), a.dout = dout, a.dlse = dlse;
+  a.out = dq, a.dk = dk, a.dv = dv;
+  a.delta = static_cast<float*>(workspace);
+  dq_tiles(a);
+  a.bound = reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes(a));
+  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes(a) + bound_bytes(a));
+  a.splits = a.total_k > 0 ? dkv_splits(a, cus) : 1;
+  hipStream_t stream = as_stream(stream_);
+  return d->dtype == HI3D_F16 ? launch_grad_type<_Float16>(a, stream) : launch_grad_type<__bf16>(a, stream);
+}
+
+}  // extern "C"

@@ -101,6 +101,8 @@ _SIGNATURES = {
     "hi3d_rotary": [_p, _p, _p, _p, _i32, _i64, _i32, _i32, _p, _i32, _i64, _i64, _i32, _p, _i32, _i32, _f32, _p],
     "hi3d_attention_workspace": [_p, _p],
     "hi3d_attention_forward": [_p, _p, _p, _p, _i64, _p],
+    "hi3d_attention_backward_workspace": [_p, _p],
+    "hi3d_attention_backward": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _p],
 }
 _RESTYPES = {"hi3d_last_error": ctypes.c_char_p, "hi3d_version": ctypes.c_char_p, "hi3d_conv_tile_rows": _i32,
              "hi3d_gather_conv_group16": _i32, "hi3d_w8a8_gemm_kernel": _i32,

@@ -134,6 +134,49 @@ class _Problem:
         return out, lse
 
 
+    def backward(self, out, lse, dout, dlse, want_q: bool, want_kv: bool):
+        q, k = self.keep[:2]
+        self.dense = [x if x is None else _dense(x) for x in (out, lse, dout, dlse)]
+        out, lse, dout, dlse = self.dense
+        dq = torch.empty(q.shape, dtype=q.dtype, device=self.device) if want_q else None
+        dk = torch.empty(k.shape, dtype=k.dtype, device=self.device) if want_kv else None
+        dv = torch.empty(k.shape, dtype=k.dtype, device=self.device) if want_kv else None
+        need = _lib.query("hi3d_attention_backward_workspace", ctypes.byref(self.desc))
+        work = _lib.workspace(need, self.device) if need else None
+        _lib.call("hi3d_attention_backward", ctypes.byref(self.desc), out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
+                  _lib.ptr(dlse), _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), _lib.ptr(work), need, _lib.stream(self.device))
+        return dq, dk, dv
+
+
+def _dense(x: torch.Tensor) -> torch.Tensor:
+    x = x.contiguous()
+    return x.clone() if x.data_ptr() % 16 else x
+
+
+class _Attend(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, cu_q, cu_k, lens_k, scale, causal, key_mask):
+        p = _Problem(q, k, v, cu_q, cu_k, lens_k, scale, causal, key_mask)
+        out, lse = p.forward(True)
+        ctx.save_for_backward(q, k, v, cu_q, cu_k, lens_k, key_mask, out, lse)
+        ctx.how = (scale, causal)
+        ctx.set_materialize_grads(False)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, dlse):
+        q, k, v, cu_q, cu_k, lens_k, key_mask, out, lse = ctx.saved_tensors
+        want_q, want_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        if (dout is None and dlse is None) or not (want_q or want_kv):
+            return (None,) * 9
+        dout = torch.zeros_like(out) if dout is None else dout
+        p = _Problem(q, k, v, cu_q, cu_k, lens_k, *ctx.how, key_mask)
+        with torch.cuda.device(p.device):
+            dq, dk, dv = p.backward(out, lse, dout, dlse, want_q, want_kv)
+        return dq, dk, dv, None, None, None, None, None, None
+
+
 def attend(
     q: torch.Tensor,
     k: torch.Tensor,
@@ -153,13 +196,51 @@ def attend(
     ascending from 0 to ``Nq`` / ``Nk``; ``cu_k`` = ``cu_q`` by default; one segment without
     offsets), or ``[B, L, heads, dim]``, where ``lens_k [B]`` says how many keys of each are in
     use (a cache). Query head ``h`` reads key head ``h // (hq // hk)``. ``causal``: query ``i``
-    of ``lq`` sees the keys ``j <= i + lk - lq``. ``key_mask`` (bool, one per key): False keys
+    of ``lq`` sees the keys ``j <= i + lk - lq`` (a later key whose value is not finite can still
+    reach it: such keys belong in ``key_mask``). ``key_mask`` (bool, one per key): False keys
     are not seen, whatever they hold. A row that sees no key gives zeros. Views with other
     strides are read in place where their rows are 16-byte aligned.
 
     Returns ``[..., hq, dim]`` (and with ``return_lse`` the float32 ``log(sum(exp(scores)))``
-    per row and head, -inf for a row that sees no key)."""
+    per row and head, -inf for a row that sees no key). Differentiable once in ``q``, ``k`` and
+    ``v``, through both outputs; :func:`attend_grad` is the same without autograd."""
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        out, lse = _Attend.apply(q, k, v, cu_q, cu_k, lens_k, scale, causal, key_mask)
+        return (out, lse) if return_lse else out
     p = _Problem(q, k, v, cu_q, cu_k, lens_k, scale, causal, key_mask)
     with torch.cuda.device(p.device):
         out, lse = p.forward(return_lse)
     return (out, lse) if return_lse else out
+
+
+def attend_grad(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    out: torch.Tensor,
+    lse: torch.Tensor,
+    dout: torch.Tensor,
+    cu_q: torch.Tensor | None = None,
+    cu_k: torch.Tensor | None = None,
+    *,
+    dlse: torch.Tensor | None = None,
+    lens_k: torch.Tensor | None = None,
+    scale: float | None = None,
+    causal: bool = False,
+    key_mask: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``dq``, ``dk`` and ``dv`` of :func:`attend` from its arguments, its ``out`` and ``lse``, the
+    gradient ``dout`` of ``out`` and optionally ``dlse`` of ``lse``.
+
+    Sums run in a fixed order: the same bits every time. fp32 sums; probabilities and score
+    gradients are rounded once to the inputs' type for their products (in fp16 after a scaling
+    by powers of two, so that small gradients of long rows keep their digits). Launches only:
+    this is the form to capture into a graph, with no autograd node of another stream in it."""
+    p = _Problem(q, k, v, cu_q, cu_k, lens_k, scale, causal, key_mask)
+    for name, x, shape, dtype in (("out", out, q.shape, q.dtype), ("dout", dout, q.shape, q.dtype),
+                                  ("lse", lse, q.shape[:-1], torch.float32), ("dlse", dlse, q.shape[:-1], torch.float32)):
+        if x is not None and (x.shape != shape or x.dtype != dtype):
+            raise ValueError(f"{name} must be {list(shape)} of {dtype} (got {list(x.shape)} of {x.dtype})")
+    _lib.require_gpu(q, out, lse, dout, dlse)
+    with torch.cuda.device(p.device), torch.no_grad():
+        return p.backward(out, lse, dout, dlse, True, True)

@@ -668,6 +668,20 @@ int hi3d_attention_workspace(const hi3d_attention_desc* desc_host, int64_t* byte
 int hi3d_attention_forward(const hi3d_attention_desc* desc_host, void* out_dev, float* lse_dev,
                            void* workspace_dev, int64_t workspace_bytes, void* stream);
 
+/* Workspace bytes of hi3d_attention_backward. */
+int hi3d_attention_backward_workspace(const hi3d_attention_desc* desc_host, int64_t* bytes_host);
+
+/* Gradients of hi3d_attention_forward: dq_dev [total_q, heads_q, dim] and dk_dev, dv_dev
+ * [total_k, heads_k, dim] (dq, or dk and dv together, may be null), from the forward's
+ * out_dev and lse_dev, the gradient dout_dev [total_q, heads_q, dim] of out and optionally
+ * that of lse, dlse_dev fp32 [total_q, heads_q]. Probabilities are formed again from lse;
+ * they and the scores' gradients are rounded once to the inputs' type for their products,
+ * everything is summed in fp32 in a fixed order. Hidden keys and keys past those in use get
+ * zeros. */
+int hi3d_attention_backward(const hi3d_attention_desc* desc_host, const void* out_dev, const float* lse_dev,
+                            const void* dout_dev, const float* dlse_dev, void* dq_dev, void* dk_dev, void* dv_dev,
+                            void* workspace_dev, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

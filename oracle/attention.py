@@ -56,11 +56,11 @@ def forward(q, k, v, segments_q, segments_k, scale=None, causal=False, mask=None
 
 
 def backward(q, k, v, dout, segments_q, segments_k, scale=None, causal=False, mask=None, delta_error=None,
-             p_error=0.0, u=0.0, floor=0.0) -> dict:
+             p_error=0.0, u=0.0, floor=0.0, dlse=None) -> dict:
     """``dq``, ``dk``, ``dv`` and bounds ``dq_off``, ``dk_off``, ``dv_off`` of their errors when
     probabilities and score gradients are rounded to a relative ``u`` (absolute ``floor``)
     before their products, a row's ``sum(dout * out)`` is off by ``delta_error [Nq, hq]`` and
-    a probability by a relative ``p_error [Nq, hq]``."""
+    a probability by a relative ``p_error [Nq, hq]``. ``dlse [Nq, hq]``: the gradient of ``lse``."""
     q, k, v, dout = (np.asarray(x, np.float64) for x in (q, k, v, dout))
     hq, hk, d = q.shape[1], k.shape[1], q.shape[2]
     scale = d ** -0.5 if scale is None else scale
@@ -74,7 +74,10 @@ def backward(q, k, v, dout, segments_q, segments_k, scale=None, causal=False, ma
             qq, do = q[q0:q1, h], dout[q0:q1, h]
             kk, vv, p, out, _ = _head(qq, k[k0:k1, g], v[k0:k1, g], scale, seen)
             dp = do @ vv.T
-            inner = np.where(seen, dp - (do * out).sum(1)[:, None], 0.0)
+            inner = dp - (do * out).sum(1)[:, None]
+            if dlse is not None:
+                inner = inner + np.asarray(dlse, np.float64)[q0:q1, h][:, None]
+            inner = np.where(seen, inner, 0.0)
             ds = p * inner
             r["dq"][q0:q1, h] = scale * ds @ kk
             r["dk"][k0:k1, g] += scale * ds.T @ qq

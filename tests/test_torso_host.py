@@ -206,3 +206,47 @@ def test_attention_c_refusals():
         _lib.call("hi3d_attention_forward", ctypes.byref(_desc(batch=0, cu_q=64, cu_k=64)), 4096, None, None, 0, None)
     with pytest.raises(ValueError, match="out must be"):
         _lib.call("hi3d_attention_forward", ctypes.byref(_desc()), None, None, None, 0, None)
+
+
+def test_attention_oracle_gradient_of_lse():
+    rng = np.random.default_rng(2)
+    q, k, v = rng.standard_normal((5, 4, 8)), rng.standard_normal((7, 2, 8)), rng.standard_normal((7, 2, 8))
+    do, dl = rng.standard_normal((5, 4, 8)), rng.standard_normal((5, 4))
+    r = oattention.backward(q, k, v, do, [(0, 5)], [(0, 7)], dlse=dl)
+    tq, tk, tv = (torch.tensor(x, requires_grad=True) for x in (q, k, v))
+    s = torch.einsum("ihd,jhd->hij", tq, tk.repeat_interleave(2, 1)) * 8 ** -0.5
+    out = torch.einsum("hij,jhd->ihd", s.softmax(-1), tv.repeat_interleave(2, 1))
+    torch.autograd.backward((out, s.logsumexp(-1).T), (torch.tensor(do), torch.tensor(dl)))
+    for name, t in (("dq", tq), ("dk", tk), ("dv", tv)):
+        assert np.allclose(r[name], t.grad.numpy())
+
+
+def test_attention_grad_refusals():
+    from hi3d_amd import attention
+
+    q, k, v = _qkv()
+    with pytest.raises(ValueError, match="ROCm GPU only"):
+        attention.attend_grad(q, k, v, q, torch.zeros(4, 2), q)
+    with pytest.raises(ValueError, match="ROCm GPU only"):
+        attention.attend(q.requires_grad_(True), k, v)
+
+
+def test_attention_grad_c_refusals():
+    from hi3d_amd import _lib
+
+    def call(out=4096, lse=4096, dout=4096, dlse=None, dq=4096, dk=4096, dv=4096, work=4096, size=1 << 30, **kw):
+        _lib.call("hi3d_attention_backward", ctypes.byref(_desc(**kw)), out, lse, dout, dlse, dq, dk, dv, work, size, None)
+
+    call(dq=None, dk=None, dv=None)
+    call(total_q=0, len_q=0, total_k=0, len_k=0)
+    for match, kw in [("together", dict(dk=None)), ("together", dict(dv=None)), ("null", dict(out=None)),
+                      ("null", dict(lse=None)), ("null", dict(dout=None)), ("aligned", dict(dq=4100)),
+                      ("aligned", dict(work=4104)), ("too small", dict(size=8)), ("too small", dict(work=None)),
+                      ("type 0", dict(dtype=_lib.F32)), ("without a segment", dict(batch=0, cu_q=64, cu_k=64))]:
+        with pytest.raises(ValueError, match=match):
+            call(**kw)
+    query = lambda **kw: _lib.query("hi3d_attention_backward_workspace", ctypes.byref(_desc(**kw)))  # noqa: E731
+    assert query() == 512
+    assert query(total_q=4096, len_q=4096) > 4096 * 4 * 4 + 2 * 4 * 2 * 64 * 4
+    with pytest.raises(ValueError, match="null"):
+        _lib.query("hi3d_attention_backward_workspace", None)
