@@ -39,7 +39,8 @@ struct AttnArgs {
   const void *o, *dout;         // backward: output and its gradient, [total_q, hq, d]
   const float* dlse;            // gradient of lse [total_q, hq], or null
   void *out, *dk, *dv;          // out: output, or dq; all [total, heads, d]
-  float *lse, *delta;           // [total_q, hq]
+  float* lse;                   // [total_q, hq]
+  float *lse2, *delta;          // backward: log2(e) lse and D of the packed rows, [hk, total_q * group]
   float* bound;                 // backward: [hk, dq_slots, dq_waves] bounds of dout's rows (fp16)
   int32_t dq_rows, dq_waves, dq_slots;
   float *part, *part_ml;        // split forward: [split, total_q, hq, d], [split, total_q, hq, 2]
@@ -120,8 +121,6 @@ __device__ __forceinline__ float half_sum(float x) {
   return lo + hi;
 }
 
-__device__ const uint4 kZeroChunk = {0, 0, 0, 0};
-
 struct Segment {
   int b, tile;          // segment and the workgroup's tile of it
   int lq, lk;
@@ -194,29 +193,52 @@ __device__ __forceinline__ void split_row(const AttnArgs& a, int r, int& i, int&
   g = r - i * a.group;
 }
 
-// Copies `rows` rows (the rest repeat the last one) from key `base` on into a tile pair,
-// straight to LDS. BITS: rows whose bit is clear and chunks past the head size read zeros,
-// so what a hidden key holds cannot reach a product.
-template <int DP, int NW, bool Z>
-__device__ __forceinline__ void load_pair(const char* x, int64_t x_n, const char* y, int64_t y_n, int rows,
-                                          uint64_t bits, int dim, char* tile, int wave, int lane) {
-  constexpr int CH = DP / 8, UNITS = 2 * CH * (kKT / 64);
-  static_assert(UNITS % NW == 0, "the waves share a tile's loads evenly");
-#pragma unroll
-  for (int i = 0; i < UNITS / NW; ++i) {
-    const int j = wave + i * NW;
-    const bool second = j >= CH;
-    const int u = (second ? j - CH : j) * 64 + lane;
-    const int row = u / CH, c = (u % CH) ^ row_xor<DP>(row);
-    const int from = row < rows ? row : rows - 1;
-    const char* base = second ? y : x;
-    const int stride = static_cast<int>(second ? y_n : x_n) * 2;
-    const char* src = base + (from * stride + c * 16);
-    if constexpr (Z) {
-      if (!((bits >> row) & 1) || c * 8 >= dim) src = reinterpret_cast<const char*>(&kZeroChunk);
-    }
-    lds_dma16(src, tile + (second ? kKT * DP * 2 : 0) + (second ? j - CH : j) * 1024);
+// The lane, formed anew: what follows from it is not kept in registers across the tile loop,
+// where a spilled register's reload would also wait for the tile loads in flight.
+__device__ __forceinline__ int fresh_lane() {
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));
+  return lane;
+}
+
+// Chunk of an LDS tile that a lane loads in step i: row and (unswizzled) chunk. A wave's 64
+// lanes fill 1024 bytes of the tile in order.
+template <int DP, int NW>
+__device__ __forceinline__ void tile_chunk(int i, int wave, int lane, int& row, int& c) {
+  constexpr int CH = DP / 8, STEP = 64 * NW / CH;
+  if constexpr (64 * NW % CH == 0 && STEP % 8 == 0) {  // the same chunk of rows STEP apart
+    const int u = wave * 64 + lane;
+    row = u / CH, c = (u % CH) ^ row_xor<DP>(row);
+    row += i * STEP;
+  } else {
+    const int u = (wave + i * NW) * 64 + lane;
+    row = u / CH, c = (u % CH) ^ row_xor<DP>(row);
   }
+}
+
+// Copies a tile of 64 keys and their values from x and y on straight to LDS; row r comes from
+// row of(r). Chunks past the head size are left out (Z): they were zeroed once.
+template <int DP, int NW, bool Z, typename F>
+__device__ __forceinline__ void load_pair(const char* x, int64_t x_n, const char* y, int64_t y_n, int dim, char* tile,
+                                          int wave, int lane, F of) {
+  static_assert(DP / 8 % NW == 0, "the waves share a tile's loads evenly");
+  const uint32_t xs = static_cast<uint32_t>(x_n) * 2, ys = static_cast<uint32_t>(y_n) * 2;
+#pragma unroll
+  for (int i = 0; i < DP / 8 / NW; ++i) {
+    int row, c;
+    tile_chunk<DP, NW>(i, wave, lane, row, c);
+    if (Z && c * 8 >= dim) continue;
+    const uint32_t from = of(row);
+    char* to = tile + (wave + i * NW) * 1024;
+    lds_dma16(x + (from * xs + c * 16), to);
+    lds_dma16(y + (from * ys + c * 16), to + kKT * DP * 2);
+  }
+}
+
+// Zeroes LDS tiles, for heads that do not fill their rows. Ends with a barrier.
+__device__ __forceinline__ void clear_tiles(char* smem, int bytes) {
+  for (int i = threadIdx.x * 16; i < bytes; i += blockDim.x * 16) *reinterpret_cast<u32x4*>(smem + i) = u32x4{0, 0, 0, 0};
+  __syncthreads();
 }
 
 // Every wave's tile loads have landed and its reads of the other tile are done. The wait is

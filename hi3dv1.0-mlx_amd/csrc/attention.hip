@@ -87,10 +87,14 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_kernel(AttnArgs a) {
     if (Z && a.mask != nullptr) on = on && a.mask[s.k0 + (key < s.lk ? key : 0)] != 0;
     return __ballot(on);
   };
+  // rows past the segment repeat the last key, hidden ones the tile's first visible key: their
+  // probabilities are zero, and what a hidden key holds cannot reach a product
   auto load = [&](int t, uint64_t bits, int buf) {
+    if (Z && bits == 0) return;
     const int64_t at = static_cast<int64_t>(t) * kKT;
-    load_pair<DP, NW, Z>(kp + at * a.k_n * 2, a.k_n, vp + at * a.v_n * 2, a.v_n, min(kKT, s.lk - t * kKT), bits, a.dim,
-                         smem + buf * PAIR, wave, lane);
+    const int last = s.lk - t * kKT - 1, shown = Z ? __builtin_ctzll(bits) : 0;
+    load_pair<DP, NW, Z>(kp + at * a.k_n * 2, a.k_n, vp + at * a.v_n * 2, a.v_n, a.dim, smem + buf * PAIR, wave, lane,
+                         [&](int row) { return Z ? ((bits >> row) & 1 ? row : shown) : (row < last ? row : last); });
   };
 
   f32x16 acc[DB][QW] = {};
@@ -98,6 +102,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_kernel(AttnArgs a) {
 #pragma unroll
   for (int b = 0; b < QW; ++b) m[b] = -INFINITY, l[b] = 0.0f;
 
+  if (Z && a.dim < DP) clear_tiles(smem, 2 * PAIR);
   uint64_t bits = 0, next = 0;
   if (t0 < t1) {
     bits = key_bits(t0);
@@ -109,7 +114,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_kernel(AttnArgs a) {
     if (t + 1 < t1) load(t + 1, next, buf ^ 1);
     uint64_t after = 0;
     if (t + 2 < t1) after = key_bits(t + 2);
-    if (t * kKT < wkend) {
+    if (t * kKT < wkend && (!Z || bits != 0)) {
       const char* kt = smem + buf * PAIR;
       const char* vt = kt + kKT * DP * 2;
       f32x16 sc[2][QW] = {};

@@ -68,6 +68,13 @@ __device__ __forceinline__ float wave_max(float x) {
   return x;
 }
 
+// D from the forward's output carries that output's rounding (p's and its own), which for a
+// row of few keys is as large as the rounding of ds: sum_j ds_ij, which is zero, misses by
+// just that. Rows that see at most 4 tiles of keys take one walk more to find and mend it:
+// gradients of 16 to 128 causal keys come from 1.7-1.55 times the error of a single rounding
+// down to 1.42 (sqrt 2); above that many keys the miss is below a tenth of ds's rounding.
+constexpr int kExactTiles = 4;
+
 // dq and D. A workgroup owns NW * QW * 32 packed query rows of one key head (queries and
 // dout in registers) and walks the keys in tiles of 64 held twice in LDS, as the forward
 // does. Per 32 keys a wave forms S^T = K Q^T and dP^T = V dO^T, then dq += K^T dS^T with
@@ -92,16 +99,23 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
   if (s.tile < 0 || row0 >= rows) return;
 
   const int off = s.lk - s.lq;
-  int qi[QW], qg[QW];
+  // place of this lane's row of block b among [total_q, hq]
+  auto row_at = [&](int b) -> int64_t {
+    int i, g;
+    split_row(a, min(wrow + b * 32 + (fresh_lane() & 31), rows - 1), i, g);
+    return (s.q0 + i) * a.hq + head * a.group + g;
+  };
   u32x4 qf[QW][KS], df[QW][KS];
+  bool none[QW];
   float ref[QW], delta[QW], size[QW];  // log2 of the scaled p's divisor, D, sum |dout|
 #pragma unroll
   for (int b = 0; b < QW; ++b) {
     const int r = wrow + b * 32 + c32;
-    split_row(a, r < rows ? r : rows - 1, qi[b], qg[b]);
-    const int64_t at = (s.q0 + qi[b]) * a.hq + head * a.group + qg[b];
-    const T* src = static_cast<const T*>(a.q) + s.b * a.q_b + (a.cu_q != nullptr ? s.q0 + qi[b] : qi[b]) * a.q_n +
-                   static_cast<int64_t>(head * a.group + qg[b]) * a.q_h;
+    int i, g;
+    split_row(a, r < rows ? r : rows - 1, i, g);
+    const int64_t at = (s.q0 + i) * a.hq + head * a.group + g;
+    const T* src = static_cast<const T*>(a.q) + s.b * a.q_b + (a.cu_q != nullptr ? s.q0 + i : i) * a.q_n +
+                   static_cast<int64_t>(head * a.group + g) * a.q_h;
     load_owned<DP>(reinterpret_cast<const char*>(src), a.dim, h, true, qf[b]);
     load_owned<DP>(reinterpret_cast<const char*>(static_cast<const T*>(a.dout) + at * a.dim), a.dim, h, true, df[b]);
     u32x4 of[KS];
@@ -122,8 +136,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
       delta[b] -= z, size[b] = fmaxf(size[b], __builtin_fabsf(z));
     }
     const float lse = a.lse[at];
-    ref[b] = (lse == -INFINITY ? 0.0f : lse * kLog2e) - kPLog2<T>;  // a row that sees no key: all its scores are hidden
-    if (h == 0 && r < rows) a.delta[at] = delta[b];
+    none[b] = lse == -INFINITY;  // a row that sees no key: all its scores are hidden
+    ref[b] = (none[b] ? 0.0f : lse * kLog2e) - kPLog2<T>;
   }
   if constexpr (std::is_same_v<T, _Float16>) {  // (a row repeated past the end changes no maximum)
     float x = size[0];
@@ -132,7 +146,6 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
     x = wave_max(x);
     if (lane == 0) *bound = wrow < rows ? x : 0.0f;
   }
-  if (a.out == nullptr) return;  // only D and the bounds are wanted
   float by[QW];  // of dp - D: the scale of ds without that of p
 #pragma unroll
   for (int b = 0; b < QW; ++b) {
@@ -140,6 +153,14 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
     by[b] = power_of_two(e - static_cast<int>(kPLog2<T>)), delta[b] *= by[b];
     size[b] = a.scale * power_of_two(-e);  // takes the scale out of dq
   }
+  auto store_stats = [&]() {  // for the rows' part in dk and dv: lse in powers of two, and D
+#pragma unroll
+    for (int b = 0; b < QW; ++b) {
+      const int r = wrow + b * 32 + c32;
+      const int64_t at = (head * a.total_q + s.q0) * a.group + r;
+      if (h == 0 && r < rows) a.lse2[at] = none[b] ? INFINITY : ref[b], a.delta[at] = none[b] ? 0.0f : delta[b] / by[b];
+    }
+  };
   int kend = s.lk, wkend = wrow < rows ? s.lk : 0, wfull = s.lk;  // keys of the workgroup; of the wave; of all its rows
   if (a.causal) {
     int i, g;
@@ -153,6 +174,12 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
     }
   }
   const int tiles = kend > 0 ? (kend + kKT - 1) / kKT : 0;
+  // walks over the tiles: the first one corrects D where the rows see few keys; none where
+  // only D and the bounds are wanted
+  const int exact = tiles <= kExactTiles ? tiles : 0;
+  const int steps = exact + (a.out != nullptr ? tiles : 0);
+  if (exact == 0) store_stats();
+  float miss[QW] = {};
 
   const char* kp = reinterpret_cast<const char*>(static_cast<const T*>(a.k) + s.b * a.k_b + head * a.k_h +
                                                  (a.cu_k != nullptr ? s.k0 * a.k_n : 0));
@@ -164,86 +191,119 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
     if (Z && a.mask != nullptr) on = on && a.mask[s.k0 + (key < s.lk ? key : 0)] != 0;
     return __ballot(on);
   };
+  // rows past the segment repeat the last key, hidden ones the tile's first visible key: their
+  // probabilities are zero, and what a hidden key holds cannot reach a product
   auto load = [&](int t, uint64_t bits, int buf) {
+    if (Z && bits == 0) return;
     const int64_t at = static_cast<int64_t>(t) * kKT;
-    load_pair<DP, NW, Z>(kp + at * a.k_n * 2, a.k_n, vp + at * a.v_n * 2, a.v_n, min(kKT, s.lk - t * kKT), bits, a.dim,
-                         smem + buf * PAIR, wave, lane);
+    const int lane = fresh_lane(), last = s.lk - t * kKT - 1, shown = Z ? __builtin_ctzll(bits) : 0;
+    load_pair<DP, NW, Z>(kp + at * a.k_n * 2, a.k_n, vp + at * a.v_n * 2, a.v_n, a.dim, smem + buf * PAIR, wave, lane,
+                         [&](int row) { return Z ? ((bits >> row) & 1 ? row : shown) : (row < last ? row : last); });
   };
 
   f32x16 acc[QW][DB] = {};
-  uint64_t bits = 0, next = 0;
-  if (tiles > 0) {
-    bits = key_bits(0);
-    load(0, bits, 0);
-    if (tiles > 1) next = key_bits(1);
-  }
-  tile_barrier();
-  for (int t = 0, buf = 0; t < tiles; ++t, buf ^= 1) {
-    if (t + 1 < tiles) load(t + 1, next, buf ^ 1);
-    uint64_t after = 0;
-    if (t + 2 < tiles) after = key_bits(t + 2);
-    if (t * kKT < wkend) {
-      const char* kt = smem + buf * PAIR;
-      const char* vt = kt + kKT * DP * 2;
-      const bool hide = bits != ~0ull || (t + 1) * kKT > wfull;
+  // one tile; hide: some keys are hidden from some rows; exact_step: only sums ds
+  auto walk = [&](const char* kt, int t, uint64_t bits, bool hide, bool exact_step) {
+    const char* vt = kt + kKT * DP * 2;
+#pragma unroll 2
+    for (int n = 0; n < 2; ++n) {
+      f32x16 sc[QW] = {}, dp[QW] = {};
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        f32x16 sc[QW] = {}, dp[QW] = {};
+      for (int k = 0; k < KS; ++k) {
+        const u32x4 x = read_rows<DP>(kt, 32 * n + c32, k, h), y = read_rows<DP>(vt, 32 * n + c32, k, h);
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          const u32x4 x = read_rows<DP>(kt, 32 * n + c32, k, h), y = read_rows<DP>(vt, 32 * n + c32, k, h);
+        for (int b = 0; b < QW; ++b) Mfma<T>::run(x, qf[b][k], sc[b]), Mfma<T>::run(y, df[b][k], dp[b]);
+      }
+      if (hide) {
+        asm volatile("");  // a branch, not 16 selects for every tile
 #pragma unroll
-          for (int b = 0; b < QW; ++b) Mfma<T>::run(x, qf[b][k], sc[b]), Mfma<T>::run(y, df[b][k], dp[b]);
-        }
-        if (hide) {
-#pragma unroll
-          for (int b = 0; b < QW; ++b) {
-            uint64_t on = bits;
-            if (a.causal) {
-              const int seen = qi[b] + off + 1 - t * kKT;  // keys of this tile that the row sees
-              on &= seen >= 64 ? ~0ull : (seen <= 0 ? 0ull : (1ull << seen) - 1);
-            }
-            const uint32_t w = static_cast<uint32_t>(on >> (32 * n)) >> (4 * h);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) sc[b][e] = (w >> (8 * (e >> 2) + (e & 3))) & 1 ? sc[b][e] : -INFINITY;
+        for (int b = 0; b < QW; ++b) {
+          uint64_t on = bits;
+          if (a.causal) {
+            int i, g;
+            split_row(a, min(wrow + b * 32 + (fresh_lane() & 31), rows - 1), i, g);
+            const int seen = i + off + 1 - t * kKT;  // keys of this tile that the row sees
+            on &= seen >= 64 ? ~0ull : (seen <= 0 ? 0ull : (1ull << seen) - 1);
           }
+          const uint32_t w = static_cast<uint32_t>(on >> (32 * n)) >> (4 * h);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) sc[b][e] = (w >> (8 * (e >> 2) + (e & 3))) & 1 ? sc[b][e] : -INFINITY;
         }
+      }
+#pragma unroll
+      for (int b = 0; b < QW; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][e], a.scale2, -ref[b]));
+          dp[b][e] = p * __builtin_fmaf(dp[b][e], by[b], -delta[b]);
+        }
+      if (exact_step) {
+        asm volatile("");
 #pragma unroll
         for (int b = 0; b < QW; ++b)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][e], a.scale2, -ref[b]));
-            dp[b][e] = p * __builtin_fmaf(dp[b][e], by[b], -delta[b]);
-          }
+          for (int e = 0; e < 16; ++e) miss[b] += dp[b][e];
+      } else {
+        u32x4 pk[2][QW];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          u32x4 ds[QW];
+        for (int k = 0; k < 2; ++k)
 #pragma unroll
           for (int b = 0; b < QW; ++b) {
             f32x8 x;
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = dp[b][8 * k + e];
-            ds[b] = pack8<T>(x);
+            pk[k][b] = pack8<T>(x);
           }
+  #pragma unroll
+        for (int k = 0; k < 2; ++k) {
 #pragma unroll
           for (int d = 0; d < DB; ++d) {
             const u32x4 x = read_columns<DP>(kt, 32 * n + 16 * k, d, lane);
 #pragma unroll
-            for (int b = 0; b < QW; ++b) Mfma<T>::run(x, ds[b], acc[b][d]);
+            for (int b = 0; b < QW; ++b) Mfma<T>::run(x, pk[k][b], acc[b][d]);
           }
         }
+        }
+    }
+  };
+  if (Z && a.dim < DP) clear_tiles(smem, 2 * PAIR);
+  uint64_t bits = 0, next = 0;
+  auto tile_of = [&](int step) { return step < exact ? step : step - exact; };
+  if (steps > 0) {
+    bits = key_bits(0);
+    load(0, bits, 0);
+    if (steps > 1) next = key_bits(tile_of(1));
+  }
+  tile_barrier();
+  for (int step = 0, buf = 0; step < steps; ++step, buf ^= 1) {
+    const int t = tile_of(step);
+    if (step + 1 < steps) load(tile_of(step + 1), next, buf ^ 1);
+    uint64_t after = 0;
+    if (step + 2 < steps) after = key_bits(tile_of(step + 2));
+    if (t * kKT < wkend && (!Z || bits != 0)) {
+      const char* tile = smem + buf * PAIR;
+      walk(tile, t, bits, bits != ~0ull || (t + 1) * kKT > wfull, step < exact);
+    }
+    if (step + 1 == exact) {  // sum ds was to be dlse
+#pragma unroll
+      for (int b = 0; b < QW; ++b) {
+        delta[b] += half_sum(miss[b]) * power_of_two(-static_cast<int>(kPLog2<T>));
+        if (a.dlse != nullptr) delta[b] -= a.dlse[row_at(b)] * by[b];
       }
+      store_stats();
     }
     bits = next, next = after;
     tile_barrier();
   }
+  if (a.out == nullptr) return;
 #pragma unroll
   for (int b = 0; b < QW; ++b) {
     if (wrow + b * 32 + c32 >= rows) continue;
-    const int64_t at = (s.q0 + qi[b]) * a.hq + head * a.group + qg[b];
-    store_owned<T, DP>(static_cast<T*>(a.out) + at * a.dim, a.dim, h, acc[b], size[b], false);
+    store_owned<T, DP>(static_cast<T*>(a.out) + row_at(b) * a.dim, a.dim, h, acc[b], size[b], false);
   }
 }
+
+__device__ const float kPastRows[2] = {INFINITY, 0.0f};
 
 // dk and dv. A workgroup owns NW * QW * 32 keys of one key head (keys and values in
 // registers) and walks the packed query rows that read the head in tiles of 64 (queries and
@@ -251,20 +311,26 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
 // head sum in registers. Rows past the segment and rows that saw no key have lse = +infinity:
 // their probabilities are zero.
 template <typename T, int DP, int NW, int QW, bool Z, bool SPLIT>
-__global__ __launch_bounds__(64 * NW, 2) void attend_dkv_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(AttnArgs a) {
   constexpr int KEYS = NW * QW * 32, KS = DP / 16, DB = DP / 32, PAIR = 2 * kKT * DP * 2, CH = DP / 8;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   float* stats = reinterpret_cast<float*>(smem + 2 * PAIR);  // [2][lse, D][64]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c32 = lane & 31, h = lane >> 5;
-  const int64_t id = xcd_remap(blockIdx.x, gridDim.x);
   int head, split = 0, slot;
-  if (a.head_minor) {
-    head = static_cast<int>(id % a.hk), slot = static_cast<int>(id / a.hk);
-    if constexpr (SPLIT) split = slot % a.splits, slot /= a.splits;
+  if (a.causal) {  // slot by slot, so that the first keys, which see the most rows, come first
+    const int of = a.hk * a.splits;
+    head = blockIdx.x % of, slot = blockIdx.x / of;
+    if constexpr (SPLIT) split = head / a.hk, head -= split * a.hk;
   } else {
-    slot = static_cast<int>(id % a.slots), head = static_cast<int>(id / a.slots);
-    if constexpr (SPLIT) split = head % a.splits, head /= a.splits;
+    const int64_t id = xcd_remap(blockIdx.x, gridDim.x);
+    if (a.head_minor) {
+      head = static_cast<int>(id % a.hk), slot = static_cast<int>(id / a.hk);
+      if constexpr (SPLIT) split = slot % a.splits, slot /= a.splits;
+    } else {
+      slot = static_cast<int>(id % a.slots), head = static_cast<int>(id / a.slots);
+      if constexpr (SPLIT) split = head % a.splits, head /= a.splits;
+    }
   }
   Segment s;
   find_segment(a.cu_k, a.len_k, a.batch, a.total_k, 1, KEYS, slot, s);
@@ -307,21 +373,22 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dkv_kernel(AttnArgs a) {
                                                  static_cast<int64_t>(head) * a.group * a.q_h);
   const int64_t row_at = s.q0 * a.hq + head * a.group;  // of lse, D and dout
   const char* dp_ = reinterpret_cast<const char*>(static_cast<const T*>(a.dout) + row_at * a.dim);
+  const uint32_t q_row = static_cast<uint32_t>(a.q_n) * 2, q_head = static_cast<uint32_t>(a.q_h) * 2, d_head = a.dim * 2;
   auto load = [&](int t, int buf) {
+    int i0, g0;
+    split_row(a, t * kKT, i0, g0);  // the tile's first query: offsets from it fit 32 bits
+    const int lane = fresh_lane();
+    const char *x = qp + i0 * a.q_n * 2, *y = dp_ + static_cast<int64_t>(i0) * a.hq * a.dim * 2;
 #pragma unroll
     for (int i = 0; i < CH / NW; ++i) {
-      const int u = (wave + i * NW) * 64 + lane;
-      const int row = u / CH, c = (u % CH) ^ row_xor<DP>(row);
-      int qi, qg;
+      int row, c, qi, qg;
+      tile_chunk<DP, NW>(i, wave, lane, row, c);
+      if (Z && c * 8 >= a.dim) continue;
       split_row(a, min(t * kKT + row, rows - 1), qi, qg);
-      const char* x = qp + (qi * a.q_n + qg * a.q_h) * 2 + c * 16;
-      const char* y = dp_ + (static_cast<int64_t>(qi) * a.hq + qg) * a.dim * 2 + c * 16;
-      if constexpr (Z) {
-        if (c * 8 >= a.dim) x = y = reinterpret_cast<const char*>(&kZeroChunk);
-      }
+      const uint32_t from = qi - i0;
       char* to = smem + buf * PAIR + (wave + i * NW) * 1024;
-      lds_dma16(x, to);
-      lds_dma16(y, to + kKT * DP * 2);
+      lds_dma16(x + (from * q_row + qg * q_head + c * 16), to);
+      lds_dma16(y + ((from * a.hq + qg) * d_head + c * 16), to + kKT * DP * 2);
     }
   };
   // the scale of ds of this segment and head, from the bounds that the dq kernel's waves left
@@ -338,86 +405,85 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dkv_kernel(AttnArgs a) {
     by = power_of_two(e - static_cast<int>(kPLog2<T>)), dk_by *= power_of_two(-e);
     dv_by = power_of_two(-static_cast<int>(kPLog2<T>));
   }
-  float lse = 0.0f, delta = 0.0f;
-  auto load_stats = [&](int t) {  // by the first wave: row t * 64 + lane
-    const int r = t * kKT + lane;
-    int qi, qg;
-    split_row(a, min(r, rows - 1), qi, qg);
-    const int64_t at = row_at + static_cast<int64_t>(qi) * a.hq + qg;
-    lse = r < rows ? a.lse[at] : -INFINITY, delta = a.delta[at];
+  // lse and D of a tile's rows, by the first wave; rows past the segment: +infinity and 0
+  const int64_t stats_at = (head * a.total_q + s.q0) * a.group;
+  auto load_stats = [&](int t, int buf) {
+    const int r = t * kKT + fresh_lane();
+    float* to = stats + buf * 128;
+    lds_dma4(r < rows ? a.lse2 + stats_at + r : &kPastRows[0], reinterpret_cast<char*>(to));
+    lds_dma4(r < rows ? a.delta + stats_at + r : &kPastRows[1], reinterpret_cast<char*>(to + 64));
   };
-  auto store_stats = [&](int buf) {  // used only here, so that the loads are not waited for before the tile's work
-    const bool none = lse == -INFINITY;
-    stats[buf * 128 + lane] = none ? INFINITY : lse * kLog2e - kPLog2<T>;
-    stats[buf * 128 + 64 + lane] = none ? 0.0f : delta * by;
-  };
-
   f32x16 dk[QW][DB] = {}, dv[QW][DB] = {};
+  // one tile; hide: some rows do not see some keys
+  auto walk = [&](const char* qt, const float* st, int t, bool hide) {
+    const char* dt = qt + kKT * DP * 2;
+#pragma unroll 1
+    for (int n = 0; n < 2; ++n) {
+      f32x16 sc[QW] = {}, dp[QW] = {};
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const u32x4 x = read_rows<DP>(qt, 32 * n + c32, k, h), y = read_rows<DP>(dt, 32 * n + c32, k, h);
+#pragma unroll
+        for (int b = 0; b < QW; ++b) Mfma<T>::run(x, kf[b][k], sc[b]), Mfma<T>::run(y, vf[b][k], dp[b]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (hide) {
+        asm volatile("");  // a branch, not 16 selects for every tile
+#pragma unroll
+        for (int b = 0; b < QW; ++b) {
+          const int l = fresh_lane();  // first packed row that sees the lane's key, from the lane's first on
+          const int seen = max(0, wkey + b * 32 + (l & 31) - off) * a.group - t * kKT - 32 * n - 4 * (l >> 5);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) sc[b][e] = seen <= 8 * (e >> 2) + (e & 3) ? sc[b][e] : -INFINITY;
+        }
+      }
+      u32x4 p[2][QW], ds[2][QW];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        f32x8 ps[QW], dss[QW];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const f32x4 l4 = *reinterpret_cast<const f32x4*>(st + 32 * n + 16 * k + 8 * g + 4 * h);
+          const f32x4 d4 = *reinterpret_cast<const f32x4*>(st + 64 + 32 * n + 16 * k + 8 * g + 4 * h);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int b = 0; b < QW; ++b) {
+              const int at = 8 * k + 4 * g + e;
+              const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][at], a.scale2, -l4[e]));
+              ps[b][4 * g + e] = x, dss[b][4 * g + e] = (x * by) * (dp[b][at] - d4[e]);
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < QW; ++b) p[k][b] = pack8<T>(ps[b]), ds[k][b] = pack8<T>(dss[b]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+          const u32x4 x = read_columns<DP>(dt, 32 * n + 16 * k, d, lane), y = read_columns<DP>(qt, 32 * n + 16 * k, d, lane);
+#pragma unroll
+          for (int b = 0; b < QW; ++b) Mfma<T>::run(x, p[k][b], dv[b][d]), Mfma<T>::run(y, ds[k][b], dk[b][d]);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  if (Z && a.dim < DP) clear_tiles(smem, 2 * PAIR);
   if (t0 < t1) {
     load(t0, 0);
-    if (wave == 0) load_stats(t0), store_stats(0);
+    if (wave == 0) load_stats(t0, 0);
   }
   tile_barrier();
   for (int t = t0, buf = 0; t < t1; ++t, buf ^= 1) {
     if (t + 1 < t1) {
       load(t + 1, buf ^ 1);
-      if (wave == 0) load_stats(t + 1);
+      if (wave == 0) load_stats(t + 1, buf ^ 1);
     }
     if ((t + 1) * kKT > wfirst) {
-      const char* qt = smem + buf * PAIR;
-      const char* dt = qt + kKT * DP * 2;
-      const float* st = stats + buf * 128;
-      const bool hide = t * kKT < wfull;
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        f32x16 sc[QW] = {}, dp[QW] = {};
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          const u32x4 x = read_rows<DP>(qt, 32 * n + c32, k, h), y = read_rows<DP>(dt, 32 * n + c32, k, h);
-#pragma unroll
-          for (int b = 0; b < QW; ++b) Mfma<T>::run(x, kf[b][k], sc[b]), Mfma<T>::run(y, vf[b][k], dp[b]);
-        }
-        if (hide) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            int qi, qg;
-            split_row(a, min(t * kKT + 32 * n + 8 * (e >> 2) + 4 * h + (e & 3), rows - 1), qi, qg);
-#pragma unroll
-            for (int b = 0; b < QW; ++b)
-              sc[b][e] = wkey + b * 32 + c32 <= qi + off ? sc[b][e] : -INFINITY;
-          }
-        }
-        u32x4 p[QW][2], ds[QW][2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          f32x8 ps[QW], dss[QW];
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const f32x4 l4 = *reinterpret_cast<const f32x4*>(st + 32 * n + 16 * k + 8 * g + 4 * h);
-            const f32x4 d4 = *reinterpret_cast<const f32x4*>(st + 64 + 32 * n + 16 * k + 8 * g + 4 * h);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-              for (int b = 0; b < QW; ++b) {
-                const int at = 8 * k + 4 * g + e;
-                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][at], a.scale2, -l4[e]));
-                ps[b][4 * g + e] = x, dss[b][4 * g + e] = x * __builtin_fmaf(dp[b][at], by, -d4[e]);
-              }
-          }
-#pragma unroll
-          for (int b = 0; b < QW; ++b) p[b][k] = pack8<T>(ps[b]), ds[b][k] = pack8<T>(dss[b]);
-        }
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int d = 0; d < DB; ++d) {
-            const u32x4 x = read_columns<DP>(dt, 32 * n + 16 * k, d, lane), y = read_columns<DP>(qt, 32 * n + 16 * k, d, lane);
-#pragma unroll
-            for (int b = 0; b < QW; ++b) Mfma<T>::run(x, p[b][k], dv[b][d]), Mfma<T>::run(y, ds[b][k], dk[b][d]);
-          }
-      }
+      walk(smem + buf * PAIR, stats + buf * 128, t, t * kKT < wfull);
     }
-    if (wave == 0 && t + 1 < t1) store_stats(buf ^ 1);
     tile_barrier();
   }
 #pragma unroll
@@ -524,7 +590,7 @@ int dkv_splits(const AttnArgs& a, int cus) {
   const int64_t average = ceil_div(a.total_k, a.batch), tile = average <= 32 ? 32 : 128;
   const int64_t blocks = a.batch * ceil_div(average, tile) * a.hk;
   const int64_t tiles = ceil_div(ceil_div(a.total_q * a.group, a.batch), kKT);
-  int64_t splits = 2 * static_cast<int64_t>(cus) * (tile == 32 ? 4 : 1) / (blocks > 0 ? blocks : 1);
+  int64_t splits = (a.causal ? 4 : 2) * static_cast<int64_t>(cus) * (tile == 32 ? 4 : 1) / (blocks > 0 ? blocks : 1);
   if (splits > tiles / 4) splits = tiles / 4;
   if (splits > 64) splits = 64;
   return splits < 1 ? 1 : static_cast<int>(splits);
@@ -539,8 +605,8 @@ void dq_tiles(AttnArgs& a) {
                                                   : ceil_div(static_cast<int64_t>(a.len_q) * a.group, a.dq_rows) * a.batch);
 }
 
-// Workspace: D, the bounds of dout's rows, the parts of dk and dv.
-int64_t delta_bytes(const AttnArgs& a) { return align_up(a.total_q * a.hq * 4, 256); }
+// Workspace: lse and D of the packed rows, the bounds of dout's rows, the parts of dk and dv.
+int64_t stats_bytes(const AttnArgs& a) { return align_up(a.total_q * a.hq * 4, 256); }
 int64_t bound_bytes(const AttnArgs& a) { return align_up(static_cast<int64_t>(a.hk) * a.dq_slots * a.dq_waves * 4, 256); }
 
 }  // namespace
@@ -561,7 +627,7 @@ int hi3d_attention_backward_workspace(const hi3d_attention_desc* d, int64_t* byt
   if (cus <= 0) cus = 256;  // without a device: the MI355X's
   const int splits = a.total_k > 0 ? dkv_splits(a, cus) : 1;
   dq_tiles(a);
-  *bytes = delta_bytes(a) + bound_bytes(a) + (splits > 1 ? splits * 2 * a.total_k * a.hk * a.dim * 4 : 0);
+  *bytes = 2 * stats_bytes(a) + bound_bytes(a) + (splits > 1 ? splits * 2 * a.total_k * a.hk * a.dim * 4 : 0);
   return HI3D_OK;
 }
 
@@ -574,6 +640,8 @@ int hi3d_attention_backward(const hi3d_attention_desc* d, const void* out, const
   if (rc == HI3D_OK) rc = hi3d_attention_backward_workspace(d, &need);
   if (rc != HI3D_OK) return rc;
   HI3D_REQUIRE((dk == nullptr) == (dv == nullptr), "dk and dv are formed together");
+  HI3D_REQUIRE(a.hq <= 65536 && (a.group - 1) * a.q_h < (1ll << 29) && a.q_h >= 0,
+               "the query heads of one key head must lie within 2^29 elements");
   if ((a.total_q == 0 && a.total_k == 0) || (dq == nullptr && dk == nullptr)) return HI3D_OK;
   HI3D_REQUIRE(a.batch > 0, "rows without a segment");
   if (a.total_q > 0) HI3D_REQUIRE(out != nullptr && lse != nullptr && dout != nullptr, "null pointer argument");
@@ -587,10 +655,11 @@ int hi3d_attention_backward(const hi3d_attention_desc* d, const void* out, const
   HI3D_REQUIRE(cus > 0, "cannot query the compute unit count");
   a.o = out, a.lse = const_cast<float*>(lse), a.dout = dout, a.dlse = dlse;
   a.out = dq, a.dk = dk, a.dv = dv;
-  a.delta = static_cast<float*>(workspace);
+  a.lse2 = static_cast<float*>(workspace);
+  a.delta = reinterpret_cast<float*>(static_cast<char*>(workspace) + stats_bytes(a));
   dq_tiles(a);
-  a.bound = reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes(a));
-  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes(a) + bound_bytes(a));
+  a.bound = reinterpret_cast<float*>(static_cast<char*>(workspace) + 2 * stats_bytes(a));
+  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + 2 * stats_bytes(a) + bound_bytes(a));
   a.splits = a.total_k > 0 ? dkv_splits(a, cus) : 1;
   hipStream_t stream = as_stream(stream_);
   return d->dtype == HI3D_F16 ? launch_grad_type<_Float16>(a, stream) : launch_grad_type<__bf16>(a, stream);
