@@ -8,6 +8,7 @@ device, so launches are ordered with PyTorch's own work on that stream.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from pathlib import Path
@@ -157,35 +158,51 @@ def check(rc: int) -> None:
 
 
 def call(name: str, *args) -> None:
-    check(getattr(lib(), name)(*args))
+    rc = getattr(_LIB or lib(), name)(*args)
+    if rc != OK:
+        check(rc)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream(device: torch.device) -> int:
     """Handle of the current HIP stream of ``device``."""
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)  # without a Stream object: 0.2 us for 2
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def on(device: torch.device):
+    """A context with ``device`` current; an empty one where it is already (1.5 us less)."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+_HERE = contextlib.nullcontext()
 
 
 def require_gpu(*tensors: torch.Tensor | None) -> torch.device:
     """Every tensor must live on one ROCm GPU; there is no host path."""
-    device = None
+    device, index = None, -1
     for t in tensors:
         if t is None:
             continue
-        if t.device.type != "cuda":
+        if not t.is_cuda:
             raise ValueError(
                 f"hi3d_amd runs on a ROCm GPU only; got a tensor on {t.device} (move it with .cuda())"
             )
         if device is None:
-            device = t.device
-        elif t.device != device:
+            device, index = t.device, t.get_device()
+        elif t.get_device() != index:
             raise ValueError(f"tensors on different devices: {device} and {t.device}")
     if device is None:
         raise ValueError("no tensor given")
-    lib()
+    if _LIB is None:
+        lib()
     return device
 
 
@@ -197,5 +214,5 @@ def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
 def query(name: str, *args) -> int:
     """Run a ``*_workspace`` size query and return the byte count."""
     out = ctypes.c_int64(0)
-    check(getattr(lib(), name)(*args, ctypes.byref(out)))
-    return int(out.value)
+    call(name, *args, ctypes.byref(out))
+    return out.value

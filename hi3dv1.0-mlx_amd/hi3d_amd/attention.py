@@ -39,42 +39,44 @@ def offsets(lengths, device: torch.device | str = "cuda") -> torch.Tensor:
     return torch.tensor(at, dtype=torch.int32).to(device)
 
 
-def _heads(x: torch.Tensor) -> torch.Tensor:
+def _heads(x: torch.Tensor) -> tuple[torch.Tensor, tuple[int, ...]]:
     """``x`` itself where the kernels can read it (adjacent values, 16-byte aligned heads and
-    rows, non-negative strides below 2^23), else a copy."""
-    inner = x.dim() - 2
-    ok = (x.shape[-1] == 1 or x.stride(-1) == 1) and x.data_ptr() % 16 == 0
-    ok = ok and all(s % 8 == 0 for s in x.stride()[:-1]) and x.stride(inner - 1) < 1 << 23
-    if ok:
-        return x
+    rows, non-negative strides below 2^23), else a copy; and its strides."""
+    strides = x.stride()
+    if (strides[-1] == 1 or x.shape[-1] == 1) and strides[-3] < 1 << 23 and not x.data_ptr() % 16:
+        bits = strides[-2] | strides[-3]
+        if not (bits | strides[0]) % 8:
+            return x, strides
     x = x.contiguous()
-    return x.clone() if x.data_ptr() % 16 else x
+    if x.data_ptr() % 16:
+        x = x.clone()
+    return x, x.stride()
 
 
-def _offsets_of(cu: torch.Tensor | None, what: str) -> torch.Tensor | None:
-    if cu is None:
-        return None
+def _offsets_of(cu: torch.Tensor, what: str) -> torch.Tensor:
     if cu.dim() != 1 or cu.dtype not in (torch.int32, torch.int64) or cu.numel() < 1:
         raise ValueError(f"{what} must be int32 offsets [segments + 1]")
-    return cu.to(torch.int32).contiguous()
+    return cu if cu.dtype == torch.int32 and cu.is_contiguous() else cu.to(torch.int32).contiguous()
 
 
 class _Problem:
     """One checked attention problem: the descriptor and the tensors it points into."""
 
     def __init__(self, q, k, v, cu_q, cu_k, lens_k, scale, causal, key_mask):
+        shape, key_shape, dtype = q.shape, k.shape, q.dtype
+        rank = len(shape)
         for name, x in (("q", q), ("k", k), ("v", v)):
-            if x.dim() != q.dim() or x.dim() not in (3, 4):
+            if x.dim() != rank or rank not in (3, 4):
                 raise ValueError(f"{name} must be [tokens, heads, dim], or [batch, length, heads, dim] like the others")
-            if x.dtype != q.dtype:
-                raise ValueError(f"q, k and v of different types: {q.dtype} and {x.dtype}")
-        if q.dtype not in (torch.float16, torch.bfloat16):
-            raise ValueError(f"attention takes fp16 or bf16 (got {q.dtype})")
-        if k.shape != v.shape:
-            raise ValueError(f"keys {list(k.shape)} and values {list(v.shape)} differ")
-        dim, hq, hk = int(q.shape[-1]), int(q.shape[-2]), int(k.shape[-2])
-        if k.shape[-1] != dim:
-            raise ValueError(f"heads of {dim} and {k.shape[-1]} values")
+            if x.dtype != dtype:
+                raise ValueError(f"q, k and v of different types: {dtype} and {x.dtype}")
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"attention takes fp16 or bf16 (got {dtype})")
+        if key_shape != v.shape:
+            raise ValueError(f"keys {list(key_shape)} and values {list(v.shape)} differ")
+        dim, hq, hk = shape[-1], shape[-2], key_shape[-2]
+        if key_shape[-1] != dim:
+            raise ValueError(f"heads of {dim} and {key_shape[-1]} values")
         if dim % 8 or not 8 <= dim <= 128:
             raise ValueError(f"head size must be a multiple of 8 up to 128 (got {dim})")
         if hk < 1 or hq < 1 or hq % hk:
@@ -82,68 +84,78 @@ class _Problem:
         scale = dim ** -0.5 if scale is None else float(scale)
         if not (scale > 0 and math.isfinite(scale)):
             raise ValueError("scale must be positive and finite")
-        cu_q, cu_k = _offsets_of(cu_q, "cu_q"), _offsets_of(cu_k, "cu_k")
-        if q.dim() == 4:
+        if cu_q is not None:
+            cu_q = _offsets_of(cu_q, "cu_q")
+        if cu_k is not None:
+            cu_k = _offsets_of(cu_k, "cu_k")
+        if rank == 4:
             if cu_q is not None or cu_k is not None:
                 raise ValueError("offsets belong to packed tokens [tokens, heads, dim]")
-            if q.shape[0] != k.shape[0]:
-                raise ValueError(f"{q.shape[0]} and {k.shape[0]} batch elements")
-            batch, len_q, len_k = int(q.shape[0]), int(q.shape[1]), int(k.shape[1])
+            batch, len_q, len_k = shape[0], shape[1], key_shape[1]
+            if key_shape[0] != batch:
+                raise ValueError(f"{batch} and {key_shape[0]} batch elements")
+            total_q, total_k = batch * len_q, batch * len_k
         else:
+            total_q, total_k = shape[0], key_shape[0]
             if cu_k is None and cu_q is not None:
-                if q.shape[0] != k.shape[0]:
+                if total_q != total_k:
                     raise ValueError("keys of other segments than the queries' need offsets of their own")
                 cu_k = cu_q
             if (cu_q is None) != (cu_k is None) or (cu_q is not None and cu_q.numel() != cu_k.numel()):
                 raise ValueError("queries and keys need offsets of the same segments")
-            batch, len_q, len_k = 1, int(q.shape[0]), int(k.shape[0])
+            batch, len_q, len_k = 1, total_q, total_k
             if cu_q is not None:
                 batch, len_q, len_k = cu_q.numel() - 1, 0, 0
-                if batch == 0 and (q.shape[0] or k.shape[0]):
+                if batch == 0 and (total_q or total_k):
                     raise ValueError("tokens without a segment")
         if lens_k is not None:
-            if q.dim() != 4 or lens_k.shape != (batch,) or lens_k.dtype not in (torch.int32, torch.int64):
+            if rank != 4 or lens_k.shape != (batch,) or lens_k.dtype not in (torch.int32, torch.int64):
                 raise ValueError("lens_k must be int32 [batch], for tokens [batch, length, heads, dim]")
             lens_k = lens_k.to(torch.int32).contiguous()
         if key_mask is not None:
-            if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.shape != k.shape[:-2]:
-                raise ValueError(f"key_mask must be bool {list(k.shape[:-2])}")
+            if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.shape != key_shape[:-2]:
+                raise ValueError(f"key_mask must be bool {list(key_shape[:-2])}")
             key_mask = key_mask.contiguous()
         self.device = _lib.require_gpu(q, k, v, cu_q, cu_k, lens_k, key_mask)
-        q, k, v = _heads(q), _heads(k), _heads(v)
-        self.keep = (q, k, v, cu_q, cu_k, lens_k, key_mask)
-        d = self.desc = _Desc()
-        d.q, d.k, d.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-        d.cu_q, d.cu_k, d.lens_k, d.key_mask = (_lib.ptr(t) for t in (cu_q, cu_k, lens_k, key_mask))
-        strides = []
-        for x in (q, k, v):
-            strides += [0, *x.stride()[:-1]] if x.dim() == 3 else x.stride()[:-1]
-        d.strides[:] = strides
-        d.total_q, d.total_k = q.numel() // (hq * dim), k.numel() // (hk * dim)
-        d.batch, d.len_q, d.len_k, d.heads_q, d.heads_k, d.dim = batch, len_q, len_k, hq, hk, dim
-        d.dtype, d.causal, d.scale = _lib.DTYPES[q.dtype], int(bool(causal)), scale
+        self.set((q, k, v, cu_q, cu_k, lens_k, key_mask),
+                 (total_q, total_k, batch, len_q, len_k, hq, hk, dim, _lib.DTYPES[dtype], 1 if causal else 0, scale))
+
+    @classmethod
+    def again(cls, tensors, sizes) -> _Problem:
+        """A problem that was checked before, of its ``tensors`` (or copies of them) and ``sizes``."""
+        p = cls.__new__(cls)
+        p.device = tensors[0].device
+        p.set(tensors, sizes)
+        return p
+
+    def set(self, tensors, sizes) -> None:
+        (q, q_s), (k, k_s), (v, v_s) = _heads(tensors[0]), _heads(tensors[1]), _heads(tensors[2])
+        self.tensors, self.sizes = (q, k, v, *tensors[3:]), sizes
+        strides = (0, *q_s[:2], 0, *k_s[:2], 0, *v_s[:2]) if len(q_s) == 3 else (*q_s[:3], *k_s[:3], *v_s[:3])
+        self.desc = _Desc(*[x if x is None else x.data_ptr() for x in self.tensors], strides, *sizes)
+        self.ref = ctypes.byref(self.desc)
 
     def forward(self, want_lse: bool) -> tuple[torch.Tensor, torch.Tensor | None]:
-        q = self.keep[0]
+        q, ref = self.tensors[0], self.ref
         out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
         lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=self.device) if want_lse else None
-        need = _lib.query("hi3d_attention_workspace", ctypes.byref(self.desc))
+        need = _lib.query("hi3d_attention_workspace", ref)
         work = _lib.workspace(need, self.device) if need else None
-        _lib.call("hi3d_attention_forward", ctypes.byref(self.desc), _lib.ptr(out), _lib.ptr(lse), _lib.ptr(work), need,
+        _lib.call("hi3d_attention_forward", ref, out.data_ptr(), _lib.ptr(lse), _lib.ptr(work), need,
                   _lib.stream(self.device))
         return out, lse
 
-
     def backward(self, out, lse, dout, dlse, want_q: bool, want_kv: bool):
-        q, k = self.keep[:2]
-        self.dense = [x if x is None else _dense(x) for x in (out, lse, dout, dlse)]
-        out, lse, dout, dlse = self.dense
+        q, k = self.tensors[:2]
+        ref = self.ref
+        out, lse, dout = _dense(out), _dense(lse), _dense(dout)
+        dlse = dlse if dlse is None else _dense(dlse)
         dq = torch.empty(q.shape, dtype=q.dtype, device=self.device) if want_q else None
         dk = torch.empty(k.shape, dtype=k.dtype, device=self.device) if want_kv else None
         dv = torch.empty(k.shape, dtype=k.dtype, device=self.device) if want_kv else None
-        need = _lib.query("hi3d_attention_backward_workspace", ctypes.byref(self.desc))
+        need = _lib.query("hi3d_attention_backward_workspace", ref)
         work = _lib.workspace(need, self.device) if need else None
-        _lib.call("hi3d_attention_backward", ctypes.byref(self.desc), out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
+        _lib.call("hi3d_attention_backward", ref, out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
                   _lib.ptr(dlse), _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), _lib.ptr(work), need, _lib.stream(self.device))
         return dq, dk, dv
 
@@ -157,22 +169,24 @@ class _Attend(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, lens_k, scale, causal, key_mask):
         p = _Problem(q, k, v, cu_q, cu_k, lens_k, scale, causal, key_mask)
-        out, lse = p.forward(True)
-        ctx.save_for_backward(q, k, v, cu_q, cu_k, lens_k, key_mask, out, lse)
-        ctx.how = (scale, causal)
+        with _lib.on(p.device):
+            out, lse = p.forward(True)
+        ctx.save_for_backward(*p.tensors, out, lse)
+        ctx.sizes = p.sizes
         ctx.set_materialize_grads(False)
         return out, lse
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout, dlse):
-        q, k, v, cu_q, cu_k, lens_k, key_mask, out, lse = ctx.saved_tensors
+        if torch.is_grad_enabled():
+            raise RuntimeError("attention is differentiable once")
         want_q, want_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         if (dout is None and dlse is None) or not (want_q or want_kv):
             return (None,) * 9
+        *tensors, out, lse = ctx.saved_tensors
         dout = torch.zeros_like(out) if dout is None else dout
-        p = _Problem(q, k, v, cu_q, cu_k, lens_k, *ctx.how, key_mask)
-        with torch.cuda.device(p.device):
+        p = _Problem.again(tensors, ctx.sizes)
+        with _lib.on(p.device):
             dq, dk, dv = p.backward(out, lse, dout, dlse, want_q, want_kv)
         return dq, dk, dv, None, None, None, None, None, None
 
@@ -208,7 +222,7 @@ def attend(
         out, lse = _Attend.apply(q, k, v, cu_q, cu_k, lens_k, scale, causal, key_mask)
         return (out, lse) if return_lse else out
     p = _Problem(q, k, v, cu_q, cu_k, lens_k, scale, causal, key_mask)
-    with torch.cuda.device(p.device):
+    with _lib.on(p.device):
         out, lse = p.forward(return_lse)
     return (out, lse) if return_lse else out
 
@@ -242,5 +256,5 @@ def attend_grad(
         if x is not None and (x.shape != shape or x.dtype != dtype):
             raise ValueError(f"{name} must be {list(shape)} of {dtype} (got {list(x.shape)} of {x.dtype})")
     _lib.require_gpu(q, out, lse, dout, dlse)
-    with torch.cuda.device(p.device), torch.no_grad():
+    with _lib.on(p.device), torch.no_grad():
         return p.backward(out, lse, dout, dlse, True, True)

@@ -74,22 +74,25 @@ def _tokens(x: torch.Tensor, what: str) -> torch.Tensor:
     return x.reshape(-1, *x.shape[-2:]) if x.dim() > 3 else x
 
 
-def _launch(xs: list[torch.Tensor], positions: torch.Tensor, freqs: torch.Tensor, interleaved: bool, scale: float,
+_Two, _TwoHeads, _FourStrides = ctypes.c_void_p * 2, ctypes.c_int32 * 2, ctypes.c_int64 * 4
+
+
+def _launch(xs, positions: torch.Tensor, freqs: torch.Tensor, interleaved: bool, scale: float,
             inverse: bool) -> list[torch.Tensor]:
     flat = [_tokens(x, "x") for x in xs]
-    n, dim = int(flat[0].shape[0]), int(flat[0].shape[2])
-    pos = positions.reshape(n, freqs.shape[0])
-    device = xs[0].device
-    outs = [torch.empty(x.shape, dtype=x.dtype, device=device) for x in xs]
-    pad = [None] * (2 - len(xs))
-    heads = [int(x.shape[1]) for x in flat] + [0] * len(pad)
-    strides = [s for x in flat for s in (x.stride(0), x.stride(1))] + [0, 0] * len(pad)
+    a, b = flat[0], flat[-1]
+    n, heads, dim = a.shape
+    a_s, b_s, axes = a.stride(), b.stride(), freqs.shape[0]
+    pos = positions if positions.shape == (n, axes) else positions.reshape(n, axes)
+    device, dtype = a.device, a.dtype
+    outs = [torch.empty(x.shape, dtype=dtype, device=device) for x in xs]
+    one = len(xs) == 1
     _lib.call(
-        "hi3d_rotary", (ctypes.c_void_p * 2)(*[x.data_ptr() for x in flat], *pad),
-        (ctypes.c_void_p * 2)(*[y.data_ptr() for y in outs], *pad), (ctypes.c_int32 * 2)(*heads),
-        (ctypes.c_int64 * 4)(*strides), _lib.DTYPES[xs[0].dtype], n, dim, 2 * int(freqs.shape[1]), pos.data_ptr(),
-        _POSITIONS[pos.dtype], pos.stride(0), pos.stride(1), int(freqs.shape[0]), freqs.data_ptr(), int(interleaved),
-        int(inverse), float(scale), _lib.stream(device),
+        "hi3d_rotary", _Two(a.data_ptr(), None if one else b.data_ptr()),
+        _Two(outs[0].data_ptr(), None if one else outs[1].data_ptr()), _TwoHeads(heads, 0 if one else b.shape[1]),
+        _FourStrides(a_s[0], a_s[1], b_s[0], b_s[1]), _lib.DTYPES[dtype], n, dim, 2 * freqs.shape[1], pos.data_ptr(),
+        _POSITIONS[pos.dtype], pos.stride(0), pos.stride(1), axes, freqs.data_ptr(), interleaved, inverse, scale,
+        _lib.stream(device),
     )
     return outs
 
@@ -102,7 +105,8 @@ class _Rotate(torch.autograd.Function):
         ctx.save_for_backward(positions, freqs)
         ctx.how = (interleaved, scale, inverse)
         ctx.set_materialize_grads(False)
-        return tuple(_launch(list(xs), positions, freqs, interleaved, scale, inverse))
+        with _lib.on(xs[0].device):
+            return tuple(_launch(xs, positions, freqs, interleaved, scale, inverse))
 
     @staticmethod
     def backward(ctx, *grads):
@@ -111,7 +115,12 @@ class _Rotate(torch.autograd.Function):
         out: list[torch.Tensor | None] = [None] * len(grads)
         given = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[5 + i]]
         if given:
-            back = _Rotate.apply(positions, freqs, interleaved, scale, not inverse, *[grads[i] for i in given])
+            way = (positions, freqs, interleaved, scale, not inverse)
+            if torch.is_grad_enabled():
+                back = _Rotate.apply(*way, *[grads[i] for i in given])
+            else:
+                with _lib.on(positions.device):
+                    back = _launch([grads[i] for i in given], *way)
             for i, g in zip(given, back):
                 out[i] = g
         return (None, None, None, None, None, *out)
@@ -140,9 +149,9 @@ def _rotate(xs: list[torch.Tensor], positions: torch.Tensor, freqs: torch.Tensor
         raise ValueError("scale must be finite")
     _lib.require_gpu(*xs, positions, freqs)
     freqs = freqs.contiguous()
-    with torch.cuda.device(xs[0].device):
-        if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
-            return _Rotate.apply(positions, freqs, layout == "interleaved", float(scale), False, *xs)
+    if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
+        return _Rotate.apply(positions, freqs, layout == "interleaved", float(scale), False, *xs)
+    with _lib.on(xs[0].device):
         return _launch(xs, positions, freqs, layout == "interleaved", float(scale), False)
 
 
