@@ -53,7 +53,7 @@ struct AttnArgs {
   int32_t hq, hk, group, dim;
   uint32_t group_magic;         // ceil(2^32 / group) for group > 1
   float scale, scale2;          // scale, scale * log2(e)
-  int32_t causal, splits, slots, head_minor, reverse;
+  int32_t causal, splits, slots, head_minor, reverse, few;
 };
 
 template <typename T>
@@ -233,6 +233,39 @@ __device__ __forceinline__ void load_pair(const char* x, int64_t x_n, const char
     lds_dma16(x + (from * xs + c * 16), to);
     lds_dma16(y + (from * ys + c * 16), to + kKT * DP * 2);
   }
+}
+
+// Lanes that see key j (lane half 0) or j + 4 (half 1) of a tile whose visible keys are `bits`:
+// a mask in scalar registers, so that a hidden key costs one vector select an element.
+__device__ __forceinline__ bool sees_key(uint64_t bits, int j) {
+  const uint64_t lo = (bits >> j) & 1 ? 0xffffffffull : 0, hi = (bits >> (j + 4)) & 1 ? 0xffffffffull << 32 : 0;
+  return __builtin_amdgcn_inverse_ballot_w64(lo | hi);
+}
+
+// Writes 32 accumulated rows (lane l: row l % 32, columns 32 d + 8 e + 4 (l / 32) ..) times
+// `by` as T. The lane halves exchange every second group of 4 columns, so that each stores 8
+// adjacent ones.
+template <typename T, int DP>
+__device__ __forceinline__ void store_row(T* to, int dim, int h, const f32x16* acc, int step, float by) {
+  typedef T t4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int e = 0; e < 4; e += 2) {
+      t4 x, y;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[j] = static_cast<T>(acc[d * step][4 * e + j] * by);
+        y[j] = static_cast<T>(acc[d * step][4 * e + 4 + j] * by);
+      }
+      const u32x2 a = __builtin_bit_cast(u32x2, x), b = __builtin_bit_cast(u32x2, y);
+      const uint32_t a0 = a[0], a1 = a[1], b0 = b[0], b1 = b[1];
+      const auto p = __builtin_amdgcn_permlane32_swap(a0, b0, false, false);
+      const auto q = __builtin_amdgcn_permlane32_swap(a1, b1, false, false);
+      const uint32_t p0 = p[0], p1 = p[1], q0 = q[0], q1 = q[1];
+      const int c = 32 * d + 8 * (e + h);
+      if (c < dim) *reinterpret_cast<u32x4*>(to + c) = u32x4{p0, q0, p1, q1};
+    }
 }
 
 // Zeroes LDS tiles, for heads that do not fill their rows. Ends with a barrier.

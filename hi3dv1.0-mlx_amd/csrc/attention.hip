@@ -5,6 +5,20 @@
 namespace hi3d {
 namespace {
 
+// Scores of the keys that `bits` leaves out become -infinity.
+template <int QW>
+__device__ __forceinline__ void hide_keys(f32x16 (&sc)[2][QW], uint64_t bits) {
+  if (bits == ~0ull) return;
+#pragma unroll
+  for (int n = 0; n < 2; ++n)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const bool on = sees_key(bits, 32 * n + 8 * (e >> 2) + (e & 3));
+#pragma unroll
+      for (int b = 0; b < QW; ++b) sc[n][b][e] = on ? sc[n][b][e] : -INFINITY;
+    }
+}
+
 // A workgroup owns NW * QW * 32 packed rows of one key head (QW blocks of 32 per wave,
 // their queries in registers) and walks the keys in tiles of 64 held twice in LDS: the
 // next tile's loads go straight to LDS while the present one is computed, one barrier per
@@ -128,20 +142,16 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_kernel(AttnArgs a) {
         }
       // keys that are hidden from a row
       if (bits != ~0ull || (t + 1) * kKT > wfull) {
+        hide_keys<QW>(sc, bits);
+        if (a.causal) {
 #pragma unroll
-        for (int b = 0; b < QW; ++b) {
-          uint64_t on = bits;
-          if (a.causal) {
-            const int n = qi[b] + off + 1 - t * kKT;  // keys of this tile that the row sees
-            on &= n >= 64 ? ~0ull : (n <= 0 ? 0ull : (1ull << n) - 1);
-          }
-          on >>= 4 * h;
+          for (int b = 0; b < QW; ++b) {
+            const int seen = qi[b] + off + 1 - t * kKT - 4 * h;  // keys of this tile that the row sees, from its half's first
 #pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            const uint32_t w = static_cast<uint32_t>(on >> (32 * n));
+            for (int n = 0; n < 2; ++n)
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-              sc[n][b][e] = (w >> (8 * (e >> 2) + (e & 3))) & 1 ? sc[n][b][e] : -INFINITY;
+              for (int e = 0; e < 16; ++e)
+                sc[n][b][e] = 32 * n + 8 * (e >> 2) + (e & 3) < seen ? sc[n][b][e] : -INFINITY;
           }
         }
       }
@@ -221,50 +231,272 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_kernel(AttnArgs a) {
       }
     } else {
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // no key seen: zeros
-      T* to = static_cast<T*>(a.out) + at * a.dim;
-#pragma unroll
-      for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int c = 32 * d + 8 * e + 4 * h;
-          typedef T t4 __attribute__((ext_vector_type(4)));
-          t4 x;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) x[j] = static_cast<T>(acc[d][b][4 * e + j] * inv);
-          if (c < a.dim) *reinterpret_cast<t4*>(to + c) = x;
-        }
+      store_row<T, DP>(static_cast<T*>(a.out) + at * a.dim, a.dim, h, &acc[0][b], QW, inv);
       if (a.lse != nullptr && h == 0) a.lse[at] = sum == 0.0f ? -INFINITY : (m[b] + __builtin_amdgcn_logf(sum)) * kLn2;
     }
   }
 }
 
-// Joins the splits of a row: a wave per row, each part weighed by exp2(m - max m) in fp32.
-// Reads splits * (dim + 2) * 4 bytes a row.
+// Short segments and small problems: waves that work on their own. A wave takes QW * 32
+// packed rows of one key head. Keys go from memory straight to matrix operands, values
+// through a tile of 64 rows in LDS for the transposed read; there is little to prefetch for,
+// so one tile is held and more waves are resident. Groups of 16 keys that are all hidden or
+// past the segment are skipped.
+//
+// KW = 1, segments of tens of rows and keys (windows of a serialized level): four tasks to a
+// workgroup, the heads of a segment side by side since they share its cache lines, no
+// barriers. KW > 1, too few rows to fill the chip: KW waves share the rows and take every
+// KW-th tile of the keys; their parts meet in LDS, weighed by exp2(m - max m) in fp32.
+template <typename T, int DP, int QW, int KW, bool Z>
+__global__ __launch_bounds__(KW == 1 ? 256 : 64 * KW, KW > 1 ? KW / 4 : (DP <= 32 ? 3 : (DP <= 64 ? 2 : 1))) void
+attend_short_kernel(AttnArgs a) {
+  constexpr int ROWS = QW * 32, KS = DP / 16, DB = DP / 32, TILE = kKT * DP * 2 + (KW > 1 ? DP * 4 : 0);
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c32 = lane & 31, h = lane >> 5;
+  char* vt = smem + wave * TILE;
+  const int64_t id = KW > 1 ? blockIdx.x : xcd_remap(blockIdx.x, gridDim.x) * 4 + wave;
+  const int head = static_cast<int>(id % a.hk), slot = static_cast<int>(id / a.hk);
+  if (slot >= a.slots) return;
+  Segment s;
+  find_segment(a.cu_q, a.len_q, a.batch, a.total_q, a.group, ROWS, slot, s);
+  segment_rows(a, s);
+  const int rows = s.lq * a.group, row0 = s.tile * ROWS;
+  if (s.tile < 0 || row0 >= rows) return;
+
+  const int off = s.lk - s.lq;
+  int qi[QW], qg[QW];
+  u32x4 qf[QW][KS];
+#pragma unroll
+  for (int b = 0; b < QW; ++b) {
+    split_row(a, min(row0 + b * 32 + c32, rows - 1), qi[b], qg[b]);
+    const T* src = static_cast<const T*>(a.q) + s.b * a.q_b + (a.cu_q != nullptr ? s.q0 + qi[b] : qi[b]) * a.q_n +
+                   static_cast<int64_t>(head * a.group + qg[b]) * a.q_h;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      const int c = 16 * k + 8 * h;
+      u32x4 x = {0, 0, 0, 0};
+      if (!Z || c < a.dim) x = *reinterpret_cast<const u32x4*>(src + c);
+      qf[b][k] = x;
+    }
+  }
+  int kend = s.lk, full = s.lk;  // keys that some row sees, that every row sees
+  if (a.causal) {
+    int i, g;
+    split_row(a, min(rows, row0 + ROWS) - 1, i, g);
+    kend = min(kend, i + off + 1);
+    split_row(a, row0, i, g);
+    full = min(full, i + off + 1);
+  }
+  const T* kp = static_cast<const T*>(a.k) + s.b * a.k_b + head * a.k_h + (a.cu_k != nullptr ? s.k0 * a.k_n : 0);
+  const char* vp = reinterpret_cast<const char*>(static_cast<const T*>(a.v) + s.b * a.v_b + head * a.v_h +
+                                                 (a.cu_k != nullptr ? s.k0 * a.v_n : 0));
+  if (Z && a.dim < DP)
+    for (int i = lane * 16; i < kKT * DP * 2; i += 1024) *reinterpret_cast<u32x4*>(vt + i) = u32x4{0, 0, 0, 0};
+  if (Z) wait_lgkm0();
+
+  f32x16 acc[DB][QW] = {};
+  float m[QW], l[QW];
+#pragma unroll
+  for (int b = 0; b < QW; ++b) m[b] = -INFINITY, l[b] = 0.0f;
+  const int start = KW > 1 ? wave * kKT : 0;
+  for (int k0 = start; k0 < kend; k0 += KW * kKT) {
+    bool shown = k0 + lane < s.lk;
+    if (Z && a.mask != nullptr) shown = shown && a.mask[s.k0 + (shown ? k0 + lane : 0)] != 0;
+    const uint64_t bits = __ballot(shown);
+    if (bits == 0) continue;
+    const int one = __builtin_ctzll(bits);  // stands in for the keys that are hidden or not there
+    asm volatile("" ::: "memory");  // the reads of the tile before are done: their products have waited for them
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i) {
+      int row, c;
+      tile_chunk<DP, 1>(i, 0, lane, row, c);
+      if (Z && c * 8 >= a.dim) continue;
+      const uint32_t from = (bits >> row) & 1 ? row : one;
+      lds_dma16(vp + k0 * a.v_n * 2 + (from * (static_cast<uint32_t>(a.v_n) * 2) + c * 16), vt + i * 1024);
+    }
+    f32x16 sc[2][QW] = {};
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      if ((bits >> (32 * n) & 0xffffffffull) == 0) continue;
+      const int row = 32 * n + c32;
+      const T* src = kp + k0 * a.k_n + ((bits >> row) & 1 ? row : one) * a.k_n;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const int c = 16 * k + 8 * h;
+        u32x4 x = {0, 0, 0, 0};
+        if (!Z || c < a.dim) x = *reinterpret_cast<const u32x4*>(src + c);
+#pragma unroll
+        for (int b = 0; b < QW; ++b) Mfma<T>::run(x, qf[b][k], sc[n][b]);
+      }
+    }
+    float top[QW];
+#pragma unroll
+    for (int b = 0; b < QW; ++b) top[b] = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint64_t some = bits >> (16 * k) & 0xffff;
+      if (some == 0) continue;
+      if (some != 0xffff) {
+#pragma unroll
+        for (int e = 8 * (k & 1); e < 8 * (k & 1) + 8; ++e) {
+          const bool on = sees_key(bits, 32 * (k >> 1) + 8 * (e >> 2) + (e & 3));
+#pragma unroll
+          for (int b = 0; b < QW; ++b) sc[k >> 1][b][e] = on ? sc[k >> 1][b][e] : -INFINITY;
+        }
+      }
+      if (k0 + 16 * k + 16 > full && a.causal) {
+#pragma unroll
+        for (int b = 0; b < QW; ++b) {
+          const int seen = qi[b] + off + 1 - k0 - 4 * h;
+#pragma unroll
+          for (int e = 8 * (k & 1); e < 8 * (k & 1) + 8; ++e)
+            sc[k >> 1][b][e] = 32 * (k >> 1) + 8 * (e >> 2) + (e & 3) < seen ? sc[k >> 1][b][e] : -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < QW; ++b)
+#pragma unroll
+        for (int e = 8 * (k & 1); e < 8 * (k & 1) + 8; ++e) top[b] = fmaxf(top[b], sc[k >> 1][b][e]);
+    }
+#pragma unroll
+    for (int b = 0; b < QW; ++b) {
+      const float to = fmaxf(m[b], half_max(top[b]) * a.scale2);
+      if (k0 > start) {
+        const float by = m[b] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[b] - to);
+        l[b] *= by;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) acc[d][b] *= by;
+      }
+      m[b] = to;
+    }
+    wait_vmcnt<0>();  // the value tile
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if ((bits >> (16 * k) & 0xffff) == 0) continue;
+      u32x4 p[QW];
+#pragma unroll
+      for (int b = 0; b < QW; ++b) {
+        const float ref = m[b] == -INFINITY ? 0.0f : m[b];
+        f32x8 x;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[k >> 1][b][8 * (k & 1) + e], a.scale2, -ref));
+          l[b] += x[e];
+        }
+        p[b] = pack8<T>(x);
+      }
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const u32x4 x = read_columns<DP>(vt, 16 * k, d, lane);
+#pragma unroll
+        for (int b = 0; b < QW; ++b) Mfma<T>::run(x, p[b], acc[d][b]);
+      }
+    }
+  }
+  if constexpr (KW > 1) {
+    // parts in LDS as [column / 4][33 rows][4], so that neither side's accesses share banks
+    float* ml = reinterpret_cast<float*>(smem + KW * TILE);
+    if (h == 0) ml[wave * 32 + c32] = m[0];
+    l[0] = half_sum(l[0]);
+    if (h == 0) ml[(KW + wave) * 32 + c32] = l[0];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        *reinterpret_cast<f32x4*>(vt + ((8 * d + 2 * e + h) * 33 + c32) * 16) =
+            f32x4{acc[d][0][4 * e], acc[d][0][4 * e + 1], acc[d][0][4 * e + 2], acc[d][0][4 * e + 3]};
+    __syncthreads();
+    const int quads = a.dim / 4;
+    for (int i = threadIdx.x; i < 32 * quads; i += 64 * KW) {
+      const int row = i / quads, q = i - row * quads;
+      if (row0 + row >= rows) break;
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < KW; ++w) top = fmaxf(top, ml[w * 32 + row]);
+      const float ref = top == -INFINITY ? 0.0f : top;
+      f32x4 x = {0, 0, 0, 0};
+      float sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < KW; ++w) {
+        const float by = __builtin_amdgcn_exp2f(ml[w * 32 + row] - ref);
+        sum += ml[(KW + w) * 32 + row] * by;
+        x += *reinterpret_cast<const f32x4*>(smem + w * TILE + (q * 33 + row) * 16) * by;
+      }
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // no key seen: zeros
+      int r, g;
+      split_row(a, row0 + row, r, g);
+      const int64_t at = (s.q0 + r) * a.hq + head * a.group + g;
+      typedef T t4 __attribute__((ext_vector_type(4)));
+      *reinterpret_cast<t4*>(static_cast<T*>(a.out) + at * a.dim + 4 * q) =
+          t4{static_cast<T>(x[0] * inv), static_cast<T>(x[1] * inv), static_cast<T>(x[2] * inv), static_cast<T>(x[3] * inv)};
+      if (a.lse != nullptr && q == 0) a.lse[at] = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+    }
+    return;
+  }
+#pragma unroll
+  for (int b = 0; b < QW; ++b) {
+    if (row0 + b * 32 + c32 >= rows) continue;
+    const float sum = half_sum(l[b]), inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int64_t at = (s.q0 + qi[b]) * a.hq + head * a.group + qg[b];
+    store_row<T, DP>(static_cast<T*>(a.out) + at * a.dim, a.dim, h, &acc[0][b], QW, inv);
+    if (a.lse != nullptr && h == 0) a.lse[at] = sum == 0.0f ? -INFINITY : (m[b] + __builtin_amdgcn_logf(sum)) * kLn2;
+  }
+}
+
+// Joins the splits of a row: a workgroup per row. Every wave weighs the parts by exp2(m -
+// max m) (lane s: split s) and sums a quarter of them, two columns a lane, all loads in
+// flight together; the quarters meet in LDS in a fixed order. Reads splits * (dim + 2) * 4
+// bytes a row: 32 splits of 256 rows of 128 in 4.6 us.
 template <typename T>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a, int64_t rows) {
-  const int lane = threadIdx.x & 63;
-  const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (r >= rows) return;
-  float top = -INFINITY;
-  for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, a.part_ml[(s * rows + r) * 2]);
+  __shared__ float parts[4][128];
+  __shared__ float weights[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t r = blockIdx.x;
+  float m[4], l[4], top = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int s = j * 64 + lane;
+    const bool on = s < a.splits;
+    const float* ml = a.part_ml + ((on ? s : 0) * rows + r) * 2;
+    m[j] = on ? ml[0] : -INFINITY, l[j] = on ? ml[1] : 0.0f;
+    top = fmaxf(top, m[j]);
+  }
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
   const float ref = top == -INFINITY ? 0.0f : top;
   float sum = 0.0f;
-  for (int s = lane; s < a.splits; s += 64) {
-    const float* ml = a.part_ml + (s * rows + r) * 2;
-    sum += ml[1] * __builtin_amdgcn_exp2f(ml[0] - ref);
-  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) m[j] = __builtin_amdgcn_exp2f(m[j] - ref), sum += m[j] * l[j];
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  for (int c = lane; c < a.dim; c += 64) {
-    float x = 0.0f;
-    for (int s = 0; s < a.splits; ++s)
-      x += a.part[(s * rows + r) * a.dim + c] * __builtin_amdgcn_exp2f(a.part_ml[(s * rows + r) * 2] - ref);
-    static_cast<T*>(a.out)[r * a.dim + c] = static_cast<T>(x * inv);
+  // this wave's splits: wave, wave + 4, ...; at most 64
+  if ((lane & 3) == wave)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) weights[wave][j * 16 + (lane >> 2)] = m[j];
+  __syncthreads();
+  const int c = 2 * lane;
+  float x = 0.0f, y = 0.0f;
+  if (c < a.dim) {
+#pragma unroll 8
+    for (int s = wave; s < a.splits; s += 4) {
+      const float2 v = *reinterpret_cast<const float2*>(a.part + (s * rows + r) * a.dim + c);
+      const float w = weights[wave][s >> 2];
+      x = __builtin_fmaf(v.x, w, x), y = __builtin_fmaf(v.y, w, y);
+    }
   }
-  if (a.lse != nullptr && lane == 0) a.lse[r] = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+  parts[wave][c] = x, parts[wave][c + 1] = y;
+  __syncthreads();
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  if (threadIdx.x < a.dim) {
+    const int d = threadIdx.x;
+    static_cast<T*>(a.out)[r * a.dim + d] =
+        static_cast<T>(((parts[0][d] + parts[1][d]) + (parts[2][d] + parts[3][d])) * inv);
+  }
+  if (a.lse != nullptr && threadIdx.x == 0)
+    a.lse[r] = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
 template <typename T, int DP, int NW, int QW>
@@ -283,13 +515,43 @@ int launch_attend(AttnArgs a, hipStream_t stream) {
     else hipLaunchKernelGGL((attend_kernel<T, DP, NW, QW, false, true>), grid, block, lds, stream, a);
     HI3D_LAUNCH_CHECK();
     const int64_t n = a.total_q * a.hq;
-    hipLaunchKernelGGL(attend_join_kernel<T>, dim3(static_cast<unsigned>(ceil_div(n, 4))), dim3(256), 0, stream, a, n);
+    hipLaunchKernelGGL(attend_join_kernel<T>, dim3(static_cast<unsigned>(n)), dim3(256), 0, stream, a, n);
   } else {
     if (z) hipLaunchKernelGGL((attend_kernel<T, DP, NW, QW, true, false>), grid, block, lds, stream, a);
     else hipLaunchKernelGGL((attend_kernel<T, DP, NW, QW, false, false>), grid, block, lds, stream, a);
   }
   HI3D_LAUNCH_CHECK();
   return HI3D_OK;
+}
+
+template <typename T, int DP, int QW, int KW>
+int launch_short(AttnArgs a, hipStream_t stream) {
+  constexpr int rows = QW * 32;
+  constexpr size_t lds = KW == 1 ? 4 * kKT * DP * 2 : KW * (kKT * DP * 2 + DP * 4 + 256);
+  const int64_t per = a.cu_q != nullptr ? a.total_q * a.group / rows + a.batch
+                                        : ceil_div(static_cast<int64_t>(a.len_q) * a.group, rows) * a.batch;
+  HI3D_REQUIRE(per * a.hk < (1ll << 31), "too many rows for one launch");
+  a.slots = static_cast<int>(per);
+  const dim3 grid(static_cast<unsigned>(KW == 1 ? ceil_div(per * a.hk, 4) : per * a.hk)), block(KW == 1 ? 256 : 64 * KW);
+  const bool z = a.mask != nullptr || a.dim < DP;
+  if (lds > 65536)
+    HI3D_HIP_CHECK(hipFuncSetAttribute(z ? reinterpret_cast<const void*>(&attend_short_kernel<T, DP, QW, KW, true>)
+                                         : reinterpret_cast<const void*>(&attend_short_kernel<T, DP, QW, KW, false>),
+                                       hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
+  if (z) hipLaunchKernelGGL((attend_short_kernel<T, DP, QW, KW, true>), grid, block, lds, stream, a);
+  else hipLaunchKernelGGL((attend_short_kernel<T, DP, QW, KW, false>), grid, block, lds, stream, a);
+  HI3D_LAUNCH_CHECK();
+  return HI3D_OK;
+}
+
+// Few rows: 32-row blocks that leave compute units without a workgroup, over keys that 8
+// waves get through sooner than parts of them and a join: 517 x 517 x 8 heads x 64 takes
+// 8.1 us for 18.8, 1000 x 1000 10.9 for 22.9, 517 x 4000 26.5 for 29.1. Single tokens fill
+// little of a block and need more workgroups on their keys: 1030 keys x 33 heads x 64 in 9.7
+// us for 10.8, but 2048 keys x 8 heads x 128 in 23.7 for 12.4.
+bool few_rows(int64_t total_q, int64_t total_k, int batch, int hq, int hk, int dim, int cus) {
+  const int64_t average = ceil_div(total_q * (hq / hk), batch), keys = ceil_div(total_k, batch);
+  return batch * ceil_div(average, 32) * hk <= cus && keys * dim <= (average <= 32 ? 98304 : 262144);
 }
 
 // Rows of a workgroup: one wave where segments are short (a larger tile would be empty),
@@ -299,6 +561,9 @@ int64_t segment_average(const AttnArgs& a) { return ceil_div(a.total_q * a.group
 template <typename T, int DP>
 int launch_attend_dim(const AttnArgs& a, hipStream_t stream) {
   const int64_t average = segment_average(a);
+  if (average <= 64 && ceil_div(a.total_k, a.batch) <= 128)
+    return average <= 32 || DP > 64 ? launch_short<T, DP, 1, 1>(a, stream) : launch_short<T, DP, DP <= 64 ? 2 : 1, 1>(a, stream);
+  if (a.few) return launch_short<T, DP, 1, 8>(a, stream);
   if (average <= 32) return launch_attend<T, DP, 1, 1>(a, stream);
   if (average <= 64) return launch_attend<T, DP, 1, 2>(a, stream);
   if constexpr (DP <= 64) return launch_attend<T, DP, 4, 2>(a, stream);
@@ -316,7 +581,8 @@ int launch_attend_type(const AttnArgs& a, hipStream_t stream) {
 }
 
 // Splits of the key axis: as many as fill the chip twice over, each of at least 4 tiles.
-int attend_splits(int64_t total_q, int64_t total_k, int batch, int hq, int hk, int cus) {
+int attend_splits(int64_t total_q, int64_t total_k, int batch, int hq, int hk, int dim, int cus) {
+  if (few_rows(total_q, total_k, batch, hq, hk, dim, cus)) return 1;
   const int64_t rows = total_q * (hq / hk), average = ceil_div(rows, batch);
   const int tile = average <= 32 ? 32 : (average <= 64 ? 64 : 256);
   const int64_t blocks = (batch * ceil_div(average, tile)) * hk;
@@ -390,7 +656,7 @@ int hi3d_attention_workspace(const hi3d_attention_desc* d, int64_t* bytes) {
   // without a device (a size query on a build host) the MI355X's 256 compute units
   int cus = compute_units();
   if (cus <= 0) cus = 256;
-  const int splits = attend_splits(a.total_q, a.total_k, a.batch, a.hq, a.hk, cus);
+  const int splits = attend_splits(a.total_q, a.total_k, a.batch, a.hq, a.hk, a.dim, cus);
   if (splits > 1) *bytes = static_cast<int64_t>(splits) * a.total_q * a.hq * (a.dim + 2) * 4 + 256;
   return HI3D_OK;
 }
@@ -406,7 +672,8 @@ int hi3d_attention_forward(const hi3d_attention_desc* d, void* out, float* lse, 
   const int cus = compute_units();
   HI3D_REQUIRE(cus > 0, "cannot query the compute unit count");
   a.out = out, a.lse = lse;
-  int splits = attend_splits(a.total_q, a.total_k, a.batch, a.hq, a.hk, cus);
+  int splits = attend_splits(a.total_q, a.total_k, a.batch, a.hq, a.hk, a.dim, cus);
+  a.few = few_rows(a.total_q, a.total_k, a.batch, a.hq, a.hk, a.dim, cus);
   if (splits > 1) {
     const int64_t row_bytes = a.total_q * a.hq * 4;
     HI3D_REQUIRE(workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 &&
