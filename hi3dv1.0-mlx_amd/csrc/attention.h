@@ -103,6 +103,10 @@ __device__ __forceinline__ u32x4 read_columns(const char* tile, int row0, int db
   return u32x4{x[0], x[1], y[0], y[1]};
 }
 
+// v_maximum3_f32 by pairs. (fmaxf first quiets both operands, a vector operation each.) NaN
+// if one is: such a row's output is NaN whatever its reference.
+__device__ __forceinline__ float larger(float x, float y) { return __builtin_elementwise_maximum(x, y); }
+
 // The values of the two lanes (l, l ^ 32) that hold one owned row.
 __device__ __forceinline__ void both_halves(float x, float& lo, float& hi) {
   const uint32_t a = __builtin_bit_cast(uint32_t, x);

@@ -9,6 +9,7 @@ namespace {
 template <int QW>
 __device__ __forceinline__ void hide_keys(f32x16 (&sc)[2][QW], uint64_t bits) {
   if (bits == ~0ull) return;
+  asm volatile("");  // a branch, not a select a score in every tile
 #pragma unroll
   for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -144,6 +145,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_kernel(AttnArgs a) {
       if (bits != ~0ull || (t + 1) * kKT > wfull) {
         hide_keys<QW>(sc, bits);
         if (a.causal) {
+          asm volatile("");
 #pragma unroll
           for (int b = 0; b < QW; ++b) {
             const int seen = qi[b] + off + 1 - t * kKT - 4 * h;  // keys of this tile that the row sees, from its half's first
@@ -159,9 +161,9 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_kernel(AttnArgs a) {
       bool grow = false;
 #pragma unroll
       for (int b = 0; b < QW; ++b) {
-        float x = fmaxf(sc[0][b][0], sc[1][b][0]);
+        float x = larger(sc[0][b][0], sc[1][b][0]);
 #pragma unroll
-        for (int e = 1; e < 16; ++e) x = fmaxf(x, fmaxf(sc[0][b][e], sc[1][b][e]));
+        for (int e = 1; e < 16; ++e) x = larger(larger(x, sc[0][b][e]), sc[1][b][e]);
         top[b] = half_max(x) * a.scale2;
         grow = grow || top[b] > m[b] + 8.0f;
       }
@@ -357,7 +359,7 @@ attend_short_kernel(AttnArgs a) {
 #pragma unroll
       for (int b = 0; b < QW; ++b)
 #pragma unroll
-        for (int e = 8 * (k & 1); e < 8 * (k & 1) + 8; ++e) top[b] = fmaxf(top[b], sc[k >> 1][b][e]);
+        for (int e = 8 * (k & 1); e < 8 * (k & 1) + 8; ++e) top[b] = larger(top[b], sc[k >> 1][b][e]);
     }
 #pragma unroll
     for (int b = 0; b < QW; ++b) {
