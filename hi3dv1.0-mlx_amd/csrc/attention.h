@@ -15,9 +15,7 @@
 // for lane half h: the probabilities never leave the registers, and the first operand
 // comes from the same LDS tile through the transposing read ds_read_b64_tr_b16.
 //
-// LDS tiles are rows of DP values (DP = head size rounded up to 32), 16-byte chunk c of
-// row r at c ^ f(r): f spreads 8 consecutive rows over the banks for the row reads, and 4
-// consecutive rows over 32-byte pairs of chunks for the transposing reads.
+// LDS tiles are rows of DP values (DP = head size rounded up to 32).
 #pragma once
 
 #include "common.h"
@@ -74,33 +72,64 @@ __device__ __forceinline__ u32x4 pack8(f32x8 v) {
   return __builtin_bit_cast(u32x4, __builtin_convertvector(v, typename Vec8<T>::type));
 }
 
+// An LDS tile is DP / 8 blocks of 1024 bytes, each filled by one load of a wave, rows one after
+// another; with 128 values a row, 16 bytes lie between blocks. Chunk c of a row is kept at c ^
+// f(row). LDS serves 16 lanes' 16 bytes (row reads) or 32 lanes' 8 (transposing reads) a cycle
+// from 64 banks. Row reads take one chunk of 16 consecutive rows: f (and the gaps) spread those
+// that start at the same bank over all chunk places. Transposing reads take an aligned group
+// of 4 chunks of 4 consecutive rows: f moves rows of the same bank into different groups.
+// Counted: no bank conflicts (a third to a half of the LDS cycles with f of 8 rows alone).
+template <int DP>
+constexpr int kBlock = 1024 + (DP == 128 ? 16 : 0);
+template <int DP>
+constexpr int kTile = DP / 8 * kBlock<DP>;
+
 template <int DP>
 __device__ __forceinline__ int row_xor(int row) {
-  if constexpr (DP % 64 == 0) return ((row & 3) << 1) | ((row >> 2) & 1);
-  else return (row & 2) | ((row >> 2) & 1);
+  if constexpr (DP == 128) return (row & 3) << 2;
+  else if constexpr (DP == 64) return ((row & 2) << 1) | ((row >> 2) & 3);
+  else return (row >> 2) & 3;
+}
+template <int DP>
+__device__ __forceinline__ constexpr int row_place(int row) {
+  return row * 2 * DP + (DP == 128 ? (row >> 2) * 16 : 0);
 }
 
-// First operand of a score product: chunk 2 s + h of row `row` (a multiple of 32 plus l % 32).
+// Where a lane reads in a tile: base + (x ^ number of the chunk), bytes.
+struct TileLane {
+  int row, row_x;  // row reads: row l % 32, chunk l / 32
+  int col, col_x;  // transposing reads: row 4 h + i / 4, columns 16 (l / 16 % 2) + 4 (i % 4), i = l % 16
+};
+
 template <int DP>
-__device__ __forceinline__ u32x4 read_rows(const char* tile, int row, int s, int h) {
-  const int c = (2 * s + h) ^ row_xor<DP>(row);
-  return *reinterpret_cast<const u32x4*>(tile + row * (2 * DP) + c * 16);
+__device__ __forceinline__ TileLane tile_lane(int lane) {
+  const int r = lane & 31, h = lane >> 5, i = lane & 15, q = 4 * h + (i >> 2);
+  const int c = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+  if constexpr (DP == 128)  // f leaves the low bits of a chunk's number alone
+    return {row_place<DP>(r) + h * 16, row_xor<DP>(r) * 16, row_place<DP>(q) + c * 16 + (i & 1) * 8, row_xor<DP>(q) * 16};
+  return {row_place<DP>(r), (h ^ row_xor<DP>(r)) * 16, row_place<DP>(q) + (i & 1) * 8, (c ^ row_xor<DP>(q)) * 16};
+}
+
+// First operand of a score product: chunk 2 s + h of rows row0 + l % 32 (row0 a multiple of 32).
+template <int DP>
+__device__ __forceinline__ u32x4 read_rows(const char* tile, int row0, int s, const TileLane& at) {
+  const char* p = tile + row_place<DP>(row0) + at.row;
+  if constexpr (DP == 128) return *reinterpret_cast<const u32x4*>(p + (s & 1) * 32 + (at.row_x ^ (s >> 1) << 6));
+  else return *reinterpret_cast<const u32x4*>(p + (at.row_x ^ s << 5));
 }
 
 // First operand of a product over streamed rows: columns 32 db + l % 32 of rows
-// row0 + {4 h + 0..3, 8 + 4 h + 0..3}. A 16-lane group reads 4 rows x 16 columns and gets
-// them transposed (lane i: column i).
+// row0 + {4 h + 0..3, 8 + 4 h + 0..3} (row0 a multiple of 16). A 16-lane group reads 4 rows x
+// 16 columns and gets them transposed (lane i: column i).
 template <int DP>
-__device__ __forceinline__ u32x4 read_columns(const char* tile, int row0, int db, int lane) {
-  const int i = lane & 15, grp = (lane >> 4) & 1, h = lane >> 5;
-  const int row = 4 * h + (i >> 2);  // row0 is a multiple of 16: row_xor does not see it
-  const int c = (4 * db + 2 * grp + ((i & 3) >> 1)) ^ row_xor<DP>(row);
-  const char* p = tile + (row0 + row) * (2 * DP) + c * 16 + (i & 1) * 8;
+__device__ __forceinline__ u32x4 read_columns(const char* tile, int row0, int db, const TileLane& at) {
+  const char* p = tile + row_place<DP>(row0) + at.col;
+  const int x = at.col_x ^ db << 6, y = DP == 128 ? x : x ^ 32;  // f(row + 8) = f(row), or f(row) ^ 2
   typedef __attribute__((address_space(3))) s16x4* lds4;
-  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p));
-  const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 8 * 2 * DP));
-  const u32x2 x = __builtin_bit_cast(u32x2, a), y = __builtin_bit_cast(u32x2, b);
-  return u32x4{x[0], x[1], y[0], y[1]};
+  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + x));
+  const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + row_place<DP>(8) + y));
+  const u32x2 u = __builtin_bit_cast(u32x2, a), v = __builtin_bit_cast(u32x2, b);
+  return u32x4{u[0], u[1], v[0], v[1]};
 }
 
 // v_maximum3_f32 by pairs. (fmaxf first quiets both operands, a vector operation each.) NaN
@@ -210,7 +239,7 @@ __device__ __forceinline__ int fresh_lane() {
 template <int DP, int NW>
 __device__ __forceinline__ void tile_chunk(int i, int wave, int lane, int& row, int& c) {
   constexpr int CH = DP / 8, STEP = 64 * NW / CH;
-  if constexpr (64 * NW % CH == 0 && STEP % 8 == 0) {  // the same chunk of rows STEP apart
+  if constexpr (64 * NW % CH == 0 && STEP % 16 == 0) {  // the same chunk of rows STEP apart
     const int u = wave * 64 + lane;
     row = u / CH, c = (u % CH) ^ row_xor<DP>(row);
     row += i * STEP;
@@ -233,9 +262,9 @@ __device__ __forceinline__ void load_pair(const char* x, int64_t x_n, const char
     tile_chunk<DP, NW>(i, wave, lane, row, c);
     if (Z && c * 8 >= dim) continue;
     const uint32_t from = of(row);
-    char* to = tile + (wave + i * NW) * 1024;
+    char* to = tile + (wave + i * NW) * kBlock<DP>;
     lds_dma16(x + (from * xs + c * 16), to);
-    lds_dma16(y + (from * ys + c * 16), to + kKT * DP * 2);
+    lds_dma16(y + (from * ys + c * 16), to + kTile<DP>);
   }
 }
 
@@ -270,6 +299,24 @@ __device__ __forceinline__ void store_row(T* to, int dim, int h, const f32x16* a
       const int c = 32 * d + 8 * (e + h);
       if (c < dim) *reinterpret_cast<u32x4*>(to + c) = u32x4{p0, q0, p1, q1};
     }
+}
+
+// Launches kKernel, which may take more than 64 KB of LDS (asked for once a device).
+template <auto kKernel>
+int launch_tiles(const AttnArgs& a, int64_t blocks, int threads, size_t lds, hipStream_t stream) {
+  static uint64_t asked = 0;
+  if (lds > 65536) {
+    int dev = 0;
+    HI3D_HIP_CHECK(hipGetDevice(&dev));
+    if (dev >= 64 || !(__atomic_load_n(&asked, __ATOMIC_RELAXED) >> dev & 1)) {
+      HI3D_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kKernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(lds)));
+      if (dev < 64) __atomic_fetch_or(&asked, 1ull << dev, __ATOMIC_RELAXED);
+    }
+  }
+  hipLaunchKernelGGL(kKernel, dim3(static_cast<unsigned>(blocks)), dim3(threads), lds, stream, a);
+  HI3D_LAUNCH_CHECK();
+  return HI3D_OK;
 }
 
 // Zeroes LDS tiles, for heads that do not fill their rows. Ends with a barrier.

@@ -31,10 +31,11 @@ __device__ __forceinline__ void hide_keys(f32x16 (&sc)[2][QW], uint64_t bits) {
 // stay below 2^8, well inside fp16's and fp32's range, so the output is rescaled rarely.
 template <typename T, int DP, int NW, int QW, bool Z, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, 2) void attend_kernel(AttnArgs a) {
-  constexpr int ROWS = NW * QW * 32, KS = DP / 16, DB = DP / 32, PAIR = 2 * kKT * DP * 2;
+  constexpr int ROWS = NW * QW * 32, KS = DP / 16, DB = DP / 32, PAIR = 2 * kTile<DP>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c32 = lane & 31, h = lane >> 5;
+  const TileLane at = tile_lane<DP>(lane);
 
   // task: (head, split, slot), neighbours on one XCD so that they share its L2
   const int64_t id = xcd_remap(blockIdx.x, gridDim.x);
@@ -106,9 +107,9 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_kernel(AttnArgs a) {
   // probabilities are zero, and what a hidden key holds cannot reach a product
   auto load = [&](int t, uint64_t bits, int buf) {
     if (Z && bits == 0) return;
-    const int64_t at = static_cast<int64_t>(t) * kKT;
+    const int64_t from = static_cast<int64_t>(t) * kKT;
     const int last = s.lk - t * kKT - 1, shown = Z ? __builtin_ctzll(bits) : 0;
-    load_pair<DP, NW, Z>(kp + at * a.k_n * 2, a.k_n, vp + at * a.v_n * 2, a.v_n, a.dim, smem + buf * PAIR, wave, lane,
+    load_pair<DP, NW, Z>(kp + from * a.k_n * 2, a.k_n, vp + from * a.v_n * 2, a.v_n, a.dim, smem + buf * PAIR, wave, lane,
                          [&](int row) { return Z ? ((bits >> row) & 1 ? row : shown) : (row < last ? row : last); });
   };
 
@@ -131,13 +132,13 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_kernel(AttnArgs a) {
     if (t + 2 < t1) after = key_bits(t + 2);
     if (t * kKT < wkend && (!Z || bits != 0)) {
       const char* kt = smem + buf * PAIR;
-      const char* vt = kt + kKT * DP * 2;
+      const char* vt = kt + kTile<DP>;
       f32x16 sc[2][QW] = {};
 #pragma unroll
       for (int k = 0; k < KS; ++k)
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-          const u32x4 x = read_rows<DP>(kt, 32 * n + c32, k, h);
+          const u32x4 x = read_rows<DP>(kt, 32 * n, k, at);
 #pragma unroll
           for (int b = 0; b < QW; ++b) Mfma<T>::run(x, qf[b][k], sc[n][b]);
         }
@@ -201,7 +202,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_kernel(AttnArgs a) {
         }
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
-          const u32x4 x = read_columns<DP>(vt, 16 * k, d, lane);
+          const u32x4 x = read_columns<DP>(vt, 16 * k, d, at);
 #pragma unroll
           for (int b = 0; b < QW; ++b) Mfma<T>::run(x, p[b], acc[d][b]);
         }
@@ -215,9 +216,9 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_kernel(AttnArgs a) {
   for (int b = 0; b < QW; ++b) {
     if (wrow + b * 32 + c32 >= rows) continue;
     const float sum = half_sum(l[b]);
-    const int64_t at = (s.q0 + qi[b]) * a.hq + head * a.group + qg[b];
+    const int64_t place = (s.q0 + qi[b]) * a.hq + head * a.group + qg[b];
     if constexpr (SPLIT) {
-      float* to = a.part + (static_cast<int64_t>(split) * a.total_q * a.hq + at) * a.dim;
+      float* to = a.part + (static_cast<int64_t>(split) * a.total_q * a.hq + place) * a.dim;
 #pragma unroll
       for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -228,13 +229,13 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_kernel(AttnArgs a) {
                                                        acc[d][b][4 * e + 3]};
         }
       if (h == 0) {
-        float* ml = a.part_ml + (static_cast<int64_t>(split) * a.total_q * a.hq + at) * 2;
+        float* ml = a.part_ml + (static_cast<int64_t>(split) * a.total_q * a.hq + place) * 2;
         ml[0] = m[b], ml[1] = sum;
       }
     } else {
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // no key seen: zeros
-      store_row<T, DP>(static_cast<T*>(a.out) + at * a.dim, a.dim, h, &acc[0][b], QW, inv);
-      if (a.lse != nullptr && h == 0) a.lse[at] = sum == 0.0f ? -INFINITY : (m[b] + __builtin_amdgcn_logf(sum)) * kLn2;
+      store_row<T, DP>(static_cast<T*>(a.out) + place * a.dim, a.dim, h, &acc[0][b], QW, inv);
+      if (a.lse != nullptr && h == 0) a.lse[place] = sum == 0.0f ? -INFINITY : (m[b] + __builtin_amdgcn_logf(sum)) * kLn2;
     }
   }
 }
@@ -252,10 +253,11 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_kernel(AttnArgs a) {
 template <typename T, int DP, int QW, int KW, bool Z>
 __global__ __launch_bounds__(KW == 1 ? 256 : 64 * KW, KW > 1 ? KW / 4 : (DP <= 32 ? 3 : (DP <= 64 ? 2 : 1))) void
 attend_short_kernel(AttnArgs a) {
-  constexpr int ROWS = QW * 32, KS = DP / 16, DB = DP / 32, TILE = kKT * DP * 2 + (KW > 1 ? DP * 4 : 0);
+  constexpr int ROWS = QW * 32, KS = DP / 16, DB = DP / 32, TILE = KW > 1 && DP * 132 > kTile<DP> ? DP * 132 : kTile<DP>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c32 = lane & 31, h = lane >> 5;
+  const TileLane at = tile_lane<DP>(lane);
   char* vt = smem + wave * TILE;
   const int64_t id = KW > 1 ? blockIdx.x : xcd_remap(blockIdx.x, gridDim.x) * 4 + wave;
   const int head = static_cast<int>(id % a.hk), slot = static_cast<int>(id / a.hk);
@@ -294,7 +296,7 @@ attend_short_kernel(AttnArgs a) {
   const char* vp = reinterpret_cast<const char*>(static_cast<const T*>(a.v) + s.b * a.v_b + head * a.v_h +
                                                  (a.cu_k != nullptr ? s.k0 * a.v_n : 0));
   if (Z && a.dim < DP)
-    for (int i = lane * 16; i < kKT * DP * 2; i += 1024) *reinterpret_cast<u32x4*>(vt + i) = u32x4{0, 0, 0, 0};
+    for (int i = lane * 16; i < kTile<DP>; i += 1024) *reinterpret_cast<u32x4*>(vt + i) = u32x4{0, 0, 0, 0};
   if (Z) wait_lgkm0();
 
   f32x16 acc[DB][QW] = {};
@@ -315,7 +317,7 @@ attend_short_kernel(AttnArgs a) {
       tile_chunk<DP, 1>(i, 0, lane, row, c);
       if (Z && c * 8 >= a.dim) continue;
       const uint32_t from = (bits >> row) & 1 ? row : one;
-      lds_dma16(vp + k0 * a.v_n * 2 + (from * (static_cast<uint32_t>(a.v_n) * 2) + c * 16), vt + i * 1024);
+      lds_dma16(vp + k0 * a.v_n * 2 + (from * (static_cast<uint32_t>(a.v_n) * 2) + c * 16), vt + i * kBlock<DP>);
     }
     f32x16 sc[2][QW] = {};
 #pragma unroll
@@ -391,7 +393,7 @@ attend_short_kernel(AttnArgs a) {
       }
 #pragma unroll
       for (int d = 0; d < DB; ++d) {
-        const u32x4 x = read_columns<DP>(vt, 16 * k, d, lane);
+        const u32x4 x = read_columns<DP>(vt, 16 * k, d, at);
 #pragma unroll
         for (int b = 0; b < QW; ++b) Mfma<T>::run(x, p[b], acc[d][b]);
       }
@@ -441,9 +443,9 @@ attend_short_kernel(AttnArgs a) {
   for (int b = 0; b < QW; ++b) {
     if (row0 + b * 32 + c32 >= rows) continue;
     const float sum = half_sum(l[b]), inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const int64_t at = (s.q0 + qi[b]) * a.hq + head * a.group + qg[b];
-    store_row<T, DP>(static_cast<T*>(a.out) + at * a.dim, a.dim, h, &acc[0][b], QW, inv);
-    if (a.lse != nullptr && h == 0) a.lse[at] = sum == 0.0f ? -INFINITY : (m[b] + __builtin_amdgcn_logf(sum)) * kLn2;
+    const int64_t place = (s.q0 + qi[b]) * a.hq + head * a.group + qg[b];
+    store_row<T, DP>(static_cast<T*>(a.out) + place * a.dim, a.dim, h, &acc[0][b], QW, inv);
+    if (a.lse != nullptr && h == 0) a.lse[place] = sum == 0.0f ? -INFINITY : (m[b] + __builtin_amdgcn_logf(sum)) * kLn2;
   }
 }
 
@@ -510,18 +512,15 @@ int launch_attend(AttnArgs a, hipStream_t stream) {
   const int64_t blocks = per * a.hk * a.splits;
   HI3D_REQUIRE(blocks < (1ll << 31), "too many rows for one launch");
   a.slots = static_cast<int>(per);
-  const size_t lds = 4 * kKT * DP * 2;
-  const dim3 grid(static_cast<unsigned>(blocks)), block(64 * NW);
-  if (a.splits > 1) {
-    if (z) hipLaunchKernelGGL((attend_kernel<T, DP, NW, QW, true, true>), grid, block, lds, stream, a);
-    else hipLaunchKernelGGL((attend_kernel<T, DP, NW, QW, false, true>), grid, block, lds, stream, a);
-    HI3D_LAUNCH_CHECK();
-    const int64_t n = a.total_q * a.hq;
-    hipLaunchKernelGGL(attend_join_kernel<T>, dim3(static_cast<unsigned>(n)), dim3(256), 0, stream, a, n);
-  } else {
-    if (z) hipLaunchKernelGGL((attend_kernel<T, DP, NW, QW, true, false>), grid, block, lds, stream, a);
-    else hipLaunchKernelGGL((attend_kernel<T, DP, NW, QW, false, false>), grid, block, lds, stream, a);
-  }
+  constexpr size_t lds = 4 * kTile<DP>;
+  if (a.splits == 1)
+    return z ? launch_tiles<&attend_kernel<T, DP, NW, QW, true, false>>(a, blocks, 64 * NW, lds, stream)
+             : launch_tiles<&attend_kernel<T, DP, NW, QW, false, false>>(a, blocks, 64 * NW, lds, stream);
+  const int rc = z ? launch_tiles<&attend_kernel<T, DP, NW, QW, true, true>>(a, blocks, 64 * NW, lds, stream)
+                   : launch_tiles<&attend_kernel<T, DP, NW, QW, false, true>>(a, blocks, 64 * NW, lds, stream);
+  if (rc != HI3D_OK) return rc;
+  const int64_t n = a.total_q * a.hq;
+  hipLaunchKernelGGL(attend_join_kernel<T>, dim3(static_cast<unsigned>(n)), dim3(256), 0, stream, a, n);
   HI3D_LAUNCH_CHECK();
   return HI3D_OK;
 }
@@ -529,21 +528,17 @@ int launch_attend(AttnArgs a, hipStream_t stream) {
 template <typename T, int DP, int QW, int KW>
 int launch_short(AttnArgs a, hipStream_t stream) {
   constexpr int rows = QW * 32;
-  constexpr size_t lds = KW == 1 ? 4 * kKT * DP * 2 : KW * (kKT * DP * 2 + DP * 4 + 256);
+  constexpr int part = DP * 132 > kTile<DP> ? DP * 132 : kTile<DP>;  // a wave's tile, or its 32 rows of the output
+  constexpr size_t lds = KW == 1 ? 4 * kTile<DP> : KW * (part + 256);
   const int64_t per = a.cu_q != nullptr ? a.total_q * a.group / rows + a.batch
                                         : ceil_div(static_cast<int64_t>(a.len_q) * a.group, rows) * a.batch;
   HI3D_REQUIRE(per * a.hk < (1ll << 31), "too many rows for one launch");
   a.slots = static_cast<int>(per);
-  const dim3 grid(static_cast<unsigned>(KW == 1 ? ceil_div(per * a.hk, 4) : per * a.hk)), block(KW == 1 ? 256 : 64 * KW);
-  const bool z = a.mask != nullptr || a.dim < DP;
-  if (lds > 65536)
-    HI3D_HIP_CHECK(hipFuncSetAttribute(z ? reinterpret_cast<const void*>(&attend_short_kernel<T, DP, QW, KW, true>)
-                                         : reinterpret_cast<const void*>(&attend_short_kernel<T, DP, QW, KW, false>),
-                                       hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
-  if (z) hipLaunchKernelGGL((attend_short_kernel<T, DP, QW, KW, true>), grid, block, lds, stream, a);
-  else hipLaunchKernelGGL((attend_short_kernel<T, DP, QW, KW, false>), grid, block, lds, stream, a);
-  HI3D_LAUNCH_CHECK();
-  return HI3D_OK;
+  const int64_t blocks = KW == 1 ? ceil_div(per * a.hk, 4) : per * a.hk;
+  constexpr int threads = KW == 1 ? 256 : 64 * KW;
+  return a.mask != nullptr || a.dim < DP
+             ? launch_tiles<&attend_short_kernel<T, DP, QW, KW, true>>(a, blocks, threads, lds, stream)
+             : launch_tiles<&attend_short_kernel<T, DP, QW, KW, false>>(a, blocks, threads, lds, stream);
 }
 
 // Few rows: 32-row blocks that leave compute units without a workgroup, over keys that 8

@@ -81,10 +81,11 @@ constexpr int kExactTiles = 4;
 // the same K tile read transposed.
 template <typename T, int DP, int NW, int QW, bool Z>
 __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
-  constexpr int ROWS = NW * QW * 32, KS = DP / 16, DB = DP / 32, PAIR = 2 * kKT * DP * 2;
+  constexpr int ROWS = NW * QW * 32, KS = DP / 16, DB = DP / 32, PAIR = 2 * kTile<DP>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c32 = lane & 31, h = lane >> 5;
+  const TileLane place_of = tile_lane<DP>(lane);
   const int64_t id = xcd_remap(blockIdx.x, gridDim.x);
   int head, slot;
   if (a.head_minor) head = static_cast<int>(id % a.hk), slot = static_cast<int>(id / a.hk);
@@ -204,13 +205,13 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
   f32x16 acc[QW][DB] = {};
   // one tile; hide: some keys are hidden from some rows; exact_step: only sums ds
   auto walk = [&](const char* kt, int t, uint64_t bits, bool hide, bool exact_step) {
-    const char* vt = kt + kKT * DP * 2;
+    const char* vt = kt + kTile<DP>;
 #pragma unroll 2
     for (int n = 0; n < 2; ++n) {
       f32x16 sc[QW] = {}, dp[QW] = {};
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
-        const u32x4 x = read_rows<DP>(kt, 32 * n + c32, k, h), y = read_rows<DP>(vt, 32 * n + c32, k, h);
+        const u32x4 x = read_rows<DP>(kt, 32 * n, k, place_of), y = read_rows<DP>(vt, 32 * n, k, place_of);
 #pragma unroll
         for (int b = 0; b < QW; ++b) Mfma<T>::run(x, qf[b][k], sc[b]), Mfma<T>::run(y, df[b][k], dp[b]);
       }
@@ -258,7 +259,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
         for (int k = 0; k < 2; ++k) {
 #pragma unroll
           for (int d = 0; d < DB; ++d) {
-            const u32x4 x = read_columns<DP>(kt, 32 * n + 16 * k, d, lane);
+            const u32x4 x = read_columns<DP>(kt, 32 * n + 16 * k, d, place_of);
 #pragma unroll
             for (int b = 0; b < QW; ++b) Mfma<T>::run(x, pk[k][b], acc[b][d]);
           }
@@ -312,11 +313,12 @@ __device__ const float kPastRows[2] = {INFINITY, 0.0f};
 // their probabilities are zero.
 template <typename T, int DP, int NW, int QW, bool Z, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(AttnArgs a) {
-  constexpr int KEYS = NW * QW * 32, KS = DP / 16, DB = DP / 32, PAIR = 2 * kKT * DP * 2, CH = DP / 8;
+  constexpr int KEYS = NW * QW * 32, KS = DP / 16, DB = DP / 32, PAIR = 2 * kTile<DP>, CH = DP / 8;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   float* stats = reinterpret_cast<float*>(smem + 2 * PAIR);  // [2][lse, D][64]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c32 = lane & 31, h = lane >> 5;
+  const TileLane place_of = tile_lane<DP>(lane);
   int head, split = 0, slot;
   if (a.causal) {  // slot by slot, so that the first keys, which see the most rows, come first
     const int of = a.hk * a.splits;
@@ -386,9 +388,9 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
       if (Z && c * 8 >= a.dim) continue;
       split_row(a, min(t * kKT + row, rows - 1), qi, qg);
       const uint32_t from = qi - i0;
-      char* to = smem + buf * PAIR + (wave + i * NW) * 1024;
+      char* to = smem + buf * PAIR + (wave + i * NW) * kBlock<DP>;
       lds_dma16(x + (from * q_row + qg * q_head + c * 16), to);
-      lds_dma16(y + ((from * a.hq + qg) * d_head + c * 16), to + kKT * DP * 2);
+      lds_dma16(y + ((from * a.hq + qg) * d_head + c * 16), to + kTile<DP>);
     }
   };
   // the scale of ds of this segment and head, from the bounds that the dq kernel's waves left
@@ -416,13 +418,13 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
   f32x16 dk[QW][DB] = {}, dv[QW][DB] = {};
   // one tile; hide: some rows do not see some keys
   auto walk = [&](const char* qt, const float* st, int t, bool hide) {
-    const char* dt = qt + kKT * DP * 2;
+    const char* dt = qt + kTile<DP>;
 #pragma unroll 1
     for (int n = 0; n < 2; ++n) {
       f32x16 sc[QW] = {}, dp[QW] = {};
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
-        const u32x4 x = read_rows<DP>(qt, 32 * n + c32, k, h), y = read_rows<DP>(dt, 32 * n + c32, k, h);
+        const u32x4 x = read_rows<DP>(qt, 32 * n, k, place_of), y = read_rows<DP>(dt, 32 * n, k, place_of);
 #pragma unroll
         for (int b = 0; b < QW; ++b) Mfma<T>::run(x, kf[b][k], sc[b]), Mfma<T>::run(y, vf[b][k], dp[b]);
       }
@@ -462,7 +464,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
       for (int k = 0; k < 2; ++k) {
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
-          const u32x4 x = read_columns<DP>(dt, 32 * n + 16 * k, d, lane), y = read_columns<DP>(qt, 32 * n + 16 * k, d, lane);
+          const u32x4 x = read_columns<DP>(dt, 32 * n + 16 * k, d, place_of), y = read_columns<DP>(qt, 32 * n + 16 * k, d, place_of);
 #pragma unroll
           for (int b = 0; b < QW; ++b) Mfma<T>::run(x, p[k][b], dv[b][d]), Mfma<T>::run(y, ds[k][b], dk[b][d]);
         }
@@ -520,39 +522,26 @@ int launch_dq(AttnArgs a, hipStream_t stream) {
   HI3D_REQUIRE(static_cast<int64_t>(a.dq_slots) * a.hk < (1ll << 31), "too many rows for one launch");
   if (rows != a.dq_rows || NW != a.dq_waves) return fail(HI3D_ERR_INVALID, "the tile differs from the workspace's");
   a.slots = a.dq_slots;
-  const dim3 grid(static_cast<unsigned>(a.slots * a.hk)), block(64 * NW);
-  const size_t lds = 4 * kKT * DP * 2;
-  if (a.mask != nullptr || a.dim < DP) hipLaunchKernelGGL((attend_dq_kernel<T, DP, NW, QW, true>), grid, block, lds, stream, a);
-  else hipLaunchKernelGGL((attend_dq_kernel<T, DP, NW, QW, false>), grid, block, lds, stream, a);
-  HI3D_LAUNCH_CHECK();
-  return HI3D_OK;
-}
-
-template <typename T, int DP, int NW, int QW, bool Z, bool SPLIT>
-int launch_dkv_variant(const AttnArgs& a, dim3 grid, size_t lds, hipStream_t stream) {
-  if (lds > 65536)
-    HI3D_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&attend_dkv_kernel<T, DP, NW, QW, Z, SPLIT>),
-                                       hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
-  hipLaunchKernelGGL((attend_dkv_kernel<T, DP, NW, QW, Z, SPLIT>), grid, dim3(64 * NW), lds, stream, a);
-  HI3D_LAUNCH_CHECK();
-  return HI3D_OK;
+  const int64_t blocks = static_cast<int64_t>(a.slots) * a.hk;
+  constexpr size_t lds = 4 * kTile<DP>;
+  return a.mask != nullptr || a.dim < DP ? launch_tiles<&attend_dq_kernel<T, DP, NW, QW, true>>(a, blocks, 64 * NW, lds, stream)
+                                         : launch_tiles<&attend_dq_kernel<T, DP, NW, QW, false>>(a, blocks, 64 * NW, lds, stream);
 }
 
 template <typename T, int DP, int NW, int QW>
 int launch_dkv(AttnArgs a, hipStream_t stream) {
-  constexpr int keys = NW * QW * 32;
+  constexpr int keys = NW * QW * 32, threads = 64 * NW;
+  constexpr size_t lds = 4 * kTile<DP> + 1024;
   const int64_t per = a.cu_k != nullptr ? a.total_k / keys + a.batch : ceil_div(a.len_k, keys) * a.batch;
   const int64_t blocks = per * a.hk * a.splits;
   HI3D_REQUIRE(blocks < (1ll << 31), "too many rows for one launch");
   a.slots = static_cast<int>(per);
-  const dim3 grid(static_cast<unsigned>(blocks));
-  const size_t lds = 4 * kKT * DP * 2 + 1024;
   const bool z = a.mask != nullptr || a.dim < DP;
   if (a.splits == 1)
-    return z ? launch_dkv_variant<T, DP, NW, QW, true, false>(a, grid, lds, stream)
-             : launch_dkv_variant<T, DP, NW, QW, false, false>(a, grid, lds, stream);
-  const int rc = z ? launch_dkv_variant<T, DP, NW, QW, true, true>(a, grid, lds, stream)
-                   : launch_dkv_variant<T, DP, NW, QW, false, true>(a, grid, lds, stream);
+    return z ? launch_tiles<&attend_dkv_kernel<T, DP, NW, QW, true, false>>(a, blocks, threads, lds, stream)
+             : launch_tiles<&attend_dkv_kernel<T, DP, NW, QW, false, false>>(a, blocks, threads, lds, stream);
+  const int rc = z ? launch_tiles<&attend_dkv_kernel<T, DP, NW, QW, true, true>>(a, blocks, threads, lds, stream)
+                   : launch_tiles<&attend_dkv_kernel<T, DP, NW, QW, false, true>>(a, blocks, threads, lds, stream);
   if (rc != HI3D_OK) return rc;
   const int64_t all = a.total_k * a.hk * a.dim;
   hipLaunchKernelGGL(attend_dkv_join_kernel<T>, dim3(static_cast<unsigned>(ceil_div(2 * all, 1024))), dim3(256), 0, stream, a,
