@@ -51,7 +51,7 @@ struct AttnArgs {
   int32_t hq, hk, group, dim;
   uint32_t group_magic;         // ceil(2^32 / group) for group > 1
   float scale, scale2;          // scale, scale * log2(e)
-  int32_t causal, splits, slots, head_minor, reverse, few;
+  int32_t causal, splits, slots, head_minor, reverse, few, rows;
 };
 
 template <typename T>
@@ -189,6 +189,9 @@ __device__ __forceinline__ void segment_rows(const AttnArgs& a, Segment& s) {
 // floor(cu[b] * rows / T) + b to that of b + 1: at least ceil(length * rows / T) of them and
 // at most one more, so the launch needs only the total, and nothing is built beforehand.
 // The segment is found by 64-way search, first around the place an even split gives.
+// FIRST: every segment's first tile has a slot of its own, slot b, which needs no search; the
+// others follow from `batch` on, segment b's from floor(cu[b] * rows / T).
+template <bool FIRST = false>
 __device__ __forceinline__ void find_segment(const int32_t* cu, int len, int batch, int64_t total, int rows, int tile,
                                              int slot, Segment& s) {
   if (cu == nullptr) {
@@ -196,13 +199,20 @@ __device__ __forceinline__ void find_segment(const int32_t* cu, int len, int bat
     s.b = slot / per, s.tile = slot - s.b * per;
     return;
   }
+  if constexpr (FIRST) {
+    if (slot < batch) {
+      s.b = slot, s.tile = 0;
+      return;
+    }
+    slot -= batch;
+  }
   const int lane = threadIdx.x & 63;
   auto first = [&](int b) {
-    return static_cast<int>(static_cast<int64_t>(clamp_offset(cu[b], total)) * rows / tile) + b;
+    return static_cast<int>(static_cast<int64_t>(clamp_offset(cu[b], total)) * rows / tile) + (FIRST ? 0 : b);
   };
   int lo = 0, hi = batch;  // first(lo) <= slot < first(hi), hi exclusive of the answer
   if (batch > 64) {
-    const int64_t all = total * rows / tile + batch;
+    const int64_t all = total * rows / tile + (FIRST ? 0 : batch);
     int at = static_cast<int>(static_cast<int64_t>(slot) * batch / (all > 0 ? all : 1)) - 32;
     at = at < 0 ? 0 : (at > batch - 64 ? batch - 64 : at);
     const uint64_t le = __ballot(first(at + lane) <= slot);
@@ -218,7 +228,7 @@ __device__ __forceinline__ void find_segment(const int32_t* cu, int len, int bat
     hi = lo + step < hi ? lo + step : hi;
   }
   s.b = __builtin_amdgcn_readfirstlane(lo);
-  s.tile = slot - first(s.b);
+  s.tile = slot - first(s.b) + (FIRST ? 1 : 0);
 }
 
 __device__ __forceinline__ void split_row(const AttnArgs& a, int r, int& i, int& g) {

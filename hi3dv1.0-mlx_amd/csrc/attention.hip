@@ -30,7 +30,7 @@ __device__ __forceinline__ void hide_keys(f32x16 (&sc)[2][QW], uint64_t bits) {
 // included): any reference gives the same quotient, and between moves the probabilities
 // stay below 2^8, well inside fp16's and fp32's range, so the output is rescaled rarely.
 template <typename T, int DP, int NW, int QW, bool Z, bool SPLIT>
-__global__ __launch_bounds__(64 * NW, 2) void attend_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * NW, DP <= 64 && NW * QW == 4 ? 3 : 2) void attend_kernel(AttnArgs a) {
   constexpr int ROWS = NW * QW * 32, KS = DP / 16, DB = DP / 32, PAIR = 2 * kTile<DP>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -190,6 +190,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_kernel(AttnArgs a) {
             l[b] += sc[n][b][e];
           }
       }
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         u32x4 p[QW];
@@ -208,6 +209,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_kernel(AttnArgs a) {
         }
       }
     }
+    __builtin_amdgcn_s_setprio(0);
     bits = next, next = after;
     tile_barrier();
   }
@@ -240,20 +242,28 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_kernel(AttnArgs a) {
   }
 }
 
-// Short segments and small problems: waves that work on their own. A wave takes QW * 32
-// packed rows of one key head. Keys go from memory straight to matrix operands, values
-// through a tile of 64 rows in LDS for the transposed read; there is little to prefetch for,
-// so one tile is held and more waves are resident. Groups of 16 keys that are all hidden or
-// past the segment are skipped.
+// Short segments and small problems: waves that work on their own, on blocks of 32 packed
+// rows of one key head. Keys go from memory straight to matrix operands, values through a tile
+// of 64 rows in LDS for the transposed read; there is little to prefetch for, so one tile is
+// held and more waves are resident. Groups of 16 keys that are all hidden or past the segment
+// are skipped.
 //
 // KW = 1, segments of tens of rows and keys (windows of a serialized level): four tasks to a
 // workgroup, the heads of a segment side by side since they share its cache lines, no
-// barriers. KW > 1, too few rows to fill the chip: KW waves share the rows and take every
-// KW-th tile of the keys; their parts meet in LDS, weighed by exp2(m - max m) in fp32.
-template <typename T, int DP, int QW, int KW, bool Z>
-__global__ __launch_bounds__(KW == 1 ? 256 : 64 * KW, KW > 1 ? KW / 4 : (DP <= 32 ? 3 : (DP <= 64 ? 2 : 1))) void
+// barriers. A task is up to 256 rows of a segment, block after block, the next block's
+// queries on their way; keys and values that fit one tile are loaded once. KW > 1, too few
+// rows to fill the chip: KW waves share a block and take every KW-th tile of the keys; their
+// parts meet in LDS, weighed by exp2(m - max m) in fp32.
+//
+// Bound by memory latency and the waves that fit: 327,581 rows in windows of 48, 8 heads of 32
+// (671 MB) in 172 us, 3.9 TB/s; 204 as 64-row workgroups of attend_kernel.
+constexpr int kShortSpan = 256;
+
+template <typename T, int DP, int KW, bool Z>
+__global__ __launch_bounds__(KW == 1 ? 256 : 64 * KW, KW > 1 ? KW / 4 : (DP <= 32 ? 4 : (DP <= 64 ? 2 : 1))) void
 attend_short_kernel(AttnArgs a) {
-  constexpr int ROWS = QW * 32, KS = DP / 16, DB = DP / 32, TILE = KW > 1 && DP * 132 > kTile<DP> ? DP * 132 : kTile<DP>;
+  constexpr int SPAN = KW == 1 ? kShortSpan : 32, KS = DP / 16, DB = DP / 32;
+  constexpr int TILE = KW > 1 && DP * 132 > kTile<DP> ? DP * 132 : kTile<DP>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c32 = lane & 31, h = lane >> 5;
@@ -263,54 +273,43 @@ attend_short_kernel(AttnArgs a) {
   const int head = static_cast<int>(id % a.hk), slot = static_cast<int>(id / a.hk);
   if (slot >= a.slots) return;
   Segment s;
-  find_segment(a.cu_q, a.len_q, a.batch, a.total_q, a.group, ROWS, slot, s);
+  find_segment<KW == 1>(a.cu_q, a.len_q, a.batch, a.total_q, a.group, SPAN, slot, s);
   segment_rows(a, s);
-  const int rows = s.lq * a.group, row0 = s.tile * ROWS;
-  if (s.tile < 0 || row0 >= rows) return;
+  const int rows = s.lq * a.group, off = s.lk - s.lq, first = s.tile * SPAN, last = min(rows, first + SPAN);
+  if (s.tile < 0 || first >= last) return;
 
-  const int off = s.lk - s.lq;
-  int qi[QW], qg[QW];
-  u32x4 qf[QW][KS];
-#pragma unroll
-  for (int b = 0; b < QW; ++b) {
-    split_row(a, min(row0 + b * 32 + c32, rows - 1), qi[b], qg[b]);
-    const T* src = static_cast<const T*>(a.q) + s.b * a.q_b + (a.cu_q != nullptr ? s.q0 + qi[b] : qi[b]) * a.q_n +
-                   static_cast<int64_t>(head * a.group + qg[b]) * a.q_h;
-#pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      const int c = 16 * k + 8 * h;
-      u32x4 x = {0, 0, 0, 0};
-      if (!Z || c < a.dim) x = *reinterpret_cast<const u32x4*>(src + c);
-      qf[b][k] = x;
-    }
-  }
-  int kend = s.lk, full = s.lk;  // keys that some row sees, that every row sees
-  if (a.causal) {
-    int i, g;
-    split_row(a, min(rows, row0 + ROWS) - 1, i, g);
-    kend = min(kend, i + off + 1);
-    split_row(a, row0, i, g);
-    full = min(full, i + off + 1);
-  }
+  const T* qp = static_cast<const T*>(a.q) + s.b * a.q_b + (a.cu_q != nullptr ? s.q0 * a.q_n : 0) +
+                static_cast<int64_t>(head) * a.group * a.q_h;
   const T* kp = static_cast<const T*>(a.k) + s.b * a.k_b + head * a.k_h + (a.cu_k != nullptr ? s.k0 * a.k_n : 0);
   const char* vp = reinterpret_cast<const char*>(static_cast<const T*>(a.v) + s.b * a.v_b + head * a.v_h +
                                                  (a.cu_k != nullptr ? s.k0 * a.v_n : 0));
-  if (Z && a.dim < DP)
-    for (int i = lane * 16; i < kTile<DP>; i += 1024) *reinterpret_cast<u32x4*>(vt + i) = u32x4{0, 0, 0, 0};
-  if (Z) wait_lgkm0();
-
-  f32x16 acc[DB][QW] = {};
-  float m[QW], l[QW];
+  auto load_rows = [&](const T* src, u32x4 (&x)[KS]) {
 #pragma unroll
-  for (int b = 0; b < QW; ++b) m[b] = -INFINITY, l[b] = 0.0f;
-  const int start = KW > 1 ? wave * kKT : 0;
-  for (int k0 = start; k0 < kend; k0 += KW * kKT) {
+    for (int k = 0; k < KS; ++k) {
+      const int c = 16 * k + 8 * h;
+      u32x4 v = {0, 0, 0, 0};
+      if (!Z || c < a.dim) v = *reinterpret_cast<const u32x4*>(src + c);
+      x[k] = v;
+    }
+  };
+  auto load_queries = [&](int row0, u32x4 (&x)[KS]) {
+    int i, g;
+    split_row(a, min(row0 + c32, rows - 1), i, g);
+    load_rows(qp + i * a.q_n + g * a.q_h, x);
+  };
+  // a tile of keys, in registers, and of values, on their way to LDS; the keys that are there
+  u32x4 kf[2][KS];
+  auto load_keys = [&](int k0) -> uint64_t {
     bool shown = k0 + lane < s.lk;
     if (Z && a.mask != nullptr) shown = shown && a.mask[s.k0 + (shown ? k0 + lane : 0)] != 0;
     const uint64_t bits = __ballot(shown);
-    if (bits == 0) continue;
+    if (bits == 0) return bits;
     const int one = __builtin_ctzll(bits);  // stands in for the keys that are hidden or not there
     asm volatile("" ::: "memory");  // the reads of the tile before are done: their products have waited for them
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+      if ((bits >> (32 * n) & 0xffffffffull) != 0)
+        load_rows(kp + k0 * a.k_n + ((bits >> (32 * n + c32)) & 1 ? 32 * n + c32 : one) * a.k_n, kf[n]);
 #pragma unroll
     for (int i = 0; i < DP / 8; ++i) {
       int row, c;
@@ -319,133 +318,134 @@ attend_short_kernel(AttnArgs a) {
       const uint32_t from = (bits >> row) & 1 ? row : one;
       lds_dma16(vp + k0 * a.v_n * 2 + (from * (static_cast<uint32_t>(a.v_n) * 2) + c * 16), vt + i * kBlock<DP>);
     }
-    f32x16 sc[2][QW] = {};
+    return bits;
+  };
+
+  if (Z && a.dim < DP) {
+    for (int i = lane * 16; i < kTile<DP>; i += 1024) *reinterpret_cast<u32x4*>(vt + i) = u32x4{0, 0, 0, 0};
+    wait_lgkm0();
+  }
+  u32x4 qf[KS], qn[KS];
+  load_queries(first, qn);
+  const bool once = KW == 1 && s.lk <= kKT;
+  uint64_t bits = 0;
+  if (once) bits = load_keys(0);
+  for (int row0 = first; row0 < last; row0 += 32) {
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      if ((bits >> (32 * n) & 0xffffffffull) == 0) continue;
-      const int row = 32 * n + c32;
-      const T* src = kp + k0 * a.k_n + ((bits >> row) & 1 ? row : one) * a.k_n;
-#pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const int c = 16 * k + 8 * h;
-        u32x4 x = {0, 0, 0, 0};
-        if (!Z || c < a.dim) x = *reinterpret_cast<const u32x4*>(src + c);
-#pragma unroll
-        for (int b = 0; b < QW; ++b) Mfma<T>::run(x, qf[b][k], sc[n][b]);
-      }
+    for (int k = 0; k < KS; ++k) qf[k] = qn[k];
+    if (row0 + 32 < last) load_queries(row0 + 32, qn);
+    int qi, qg;
+    split_row(a, min(row0 + c32, rows - 1), qi, qg);
+    int kend = s.lk, full = s.lk;  // keys that some row sees, that every row sees
+    if (a.causal) {
+      int i, g;
+      split_row(a, min(rows, row0 + 32) - 1, i, g);
+      kend = min(kend, i + off + 1);
+      split_row(a, row0, i, g);
+      full = min(full, i + off + 1);
     }
-    float top[QW];
+    f32x16 acc[DB] = {};
+    float m = -INFINITY, l = 0.0f;
+    const int start = KW > 1 ? wave * kKT : 0;
+    for (int k0 = start; k0 < kend; k0 += KW * kKT) {
+      if (!once) bits = load_keys(k0);
+      if (bits == 0) continue;
+      f32x16 sc[2] = {};
 #pragma unroll
-    for (int b = 0; b < QW; ++b) top[b] = -INFINITY;
+      for (int n = 0; n < 2; ++n)
+        if ((bits >> (32 * n) & 0xffffffffull) != 0)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint64_t some = bits >> (16 * k) & 0xffff;
-      if (some == 0) continue;
-      if (some != 0xffff) {
+          for (int k = 0; k < KS; ++k) Mfma<T>::run(kf[n][k], qf[k], sc[n]);
+      float top = -INFINITY;
 #pragma unroll
-        for (int e = 8 * (k & 1); e < 8 * (k & 1) + 8; ++e) {
-          const bool on = sees_key(bits, 32 * (k >> 1) + 8 * (e >> 2) + (e & 3));
-#pragma unroll
-          for (int b = 0; b < QW; ++b) sc[k >> 1][b][e] = on ? sc[k >> 1][b][e] : -INFINITY;
-        }
-      }
-      if (k0 + 16 * k + 16 > full && a.causal) {
-#pragma unroll
-        for (int b = 0; b < QW; ++b) {
-          const int seen = qi[b] + off + 1 - k0 - 4 * h;
+      for (int k = 0; k < 4; ++k) {
+        const uint64_t some = bits >> (16 * k) & 0xffff;
+        if (some == 0) continue;
+        if (some != 0xffff) {
 #pragma unroll
           for (int e = 8 * (k & 1); e < 8 * (k & 1) + 8; ++e)
-            sc[k >> 1][b][e] = 32 * (k >> 1) + 8 * (e >> 2) + (e & 3) < seen ? sc[k >> 1][b][e] : -INFINITY;
+            sc[k >> 1][e] = sees_key(bits, 32 * (k >> 1) + 8 * (e >> 2) + (e & 3)) ? sc[k >> 1][e] : -INFINITY;
         }
+        if (k0 + 16 * k + 16 > full && a.causal) {
+          const int seen = qi + off + 1 - k0 - 4 * h;
+#pragma unroll
+          for (int e = 8 * (k & 1); e < 8 * (k & 1) + 8; ++e)
+            sc[k >> 1][e] = 32 * (k >> 1) + 8 * (e >> 2) + (e & 3) < seen ? sc[k >> 1][e] : -INFINITY;
+        }
+#pragma unroll
+        for (int e = 8 * (k & 1); e < 8 * (k & 1) + 8; ++e) top = larger(top, sc[k >> 1][e]);
       }
-#pragma unroll
-      for (int b = 0; b < QW; ++b)
-#pragma unroll
-        for (int e = 8 * (k & 1); e < 8 * (k & 1) + 8; ++e) top[b] = larger(top[b], sc[k >> 1][b][e]);
-    }
-#pragma unroll
-    for (int b = 0; b < QW; ++b) {
-      const float to = fmaxf(m[b], half_max(top[b]) * a.scale2);
+      const float to = fmaxf(m, half_max(top) * a.scale2);
       if (k0 > start) {
-        const float by = m[b] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[b] - to);
-        l[b] *= by;
+        const float by = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - to);
+        l *= by;
 #pragma unroll
-        for (int d = 0; d < DB; ++d) acc[d][b] *= by;
+        for (int d = 0; d < DB; ++d) acc[d] *= by;
       }
-      m[b] = to;
-    }
-    wait_vmcnt<0>();  // the value tile
-    asm volatile("" ::: "memory");
+      m = to;
+      const float ref = m == -INFINITY ? 0.0f : m;
+      if (!once || row0 == first) wait_vmcnt<0>();  // the value tile
+      asm volatile("" ::: "memory");
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if ((bits >> (16 * k) & 0xffff) == 0) continue;
-      u32x4 p[QW];
-#pragma unroll
-      for (int b = 0; b < QW; ++b) {
-        const float ref = m[b] == -INFINITY ? 0.0f : m[b];
+      for (int k = 0; k < 4; ++k) {
+        if ((bits >> (16 * k) & 0xffff) == 0) continue;
         f32x8 x;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[k >> 1][b][8 * (k & 1) + e], a.scale2, -ref));
-          l[b] += x[e];
+          x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[k >> 1][8 * (k & 1) + e], a.scale2, -ref));
+          l += x[e];
         }
-        p[b] = pack8<T>(x);
-      }
+        const u32x4 p = pack8<T>(x);
 #pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        const u32x4 x = read_columns<DP>(vt, 16 * k, d, at);
-#pragma unroll
-        for (int b = 0; b < QW; ++b) Mfma<T>::run(x, p[b], acc[d][b]);
+        for (int d = 0; d < DB; ++d) Mfma<T>::run(read_columns<DP>(vt, 16 * k, d, at), p, acc[d]);
       }
     }
-  }
-  if constexpr (KW > 1) {
-    // parts in LDS as [column / 4][33 rows][4], so that neither side's accesses share banks
-    float* ml = reinterpret_cast<float*>(smem + KW * TILE);
-    if (h == 0) ml[wave * 32 + c32] = m[0];
-    l[0] = half_sum(l[0]);
-    if (h == 0) ml[(KW + wave) * 32 + c32] = l[0];
+    if constexpr (KW > 1) {
+      // parts in LDS as [column / 4][33 rows][4], so that neither side's accesses share banks
+      float* ml = reinterpret_cast<float*>(smem + KW * TILE);
+      l = half_sum(l);
+      if (h == 0) ml[wave * 32 + c32] = m, ml[(KW + wave) * 32 + c32] = l;
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
+      for (int d = 0; d < DB; ++d)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        *reinterpret_cast<f32x4*>(vt + ((8 * d + 2 * e + h) * 33 + c32) * 16) =
-            f32x4{acc[d][0][4 * e], acc[d][0][4 * e + 1], acc[d][0][4 * e + 2], acc[d][0][4 * e + 3]};
-    __syncthreads();
-    const int quads = a.dim / 4;
-    for (int i = threadIdx.x; i < 32 * quads; i += 64 * KW) {
-      const int row = i / quads, q = i - row * quads;
-      if (row0 + row >= rows) break;
-      float top = -INFINITY;
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<f32x4*>(vt + ((8 * d + 2 * e + h) * 33 + c32) * 16) =
+              f32x4{acc[d][4 * e], acc[d][4 * e + 1], acc[d][4 * e + 2], acc[d][4 * e + 3]};
+      __syncthreads();
+      const int quads = a.dim / 4;
+      for (int i = threadIdx.x; i < 32 * quads; i += 64 * KW) {
+        const int row = i / quads, q = i - row * quads;
+        if (row0 + row >= rows) break;
+        float high = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < KW; ++w) top = fmaxf(top, ml[w * 32 + row]);
-      const float ref = top == -INFINITY ? 0.0f : top;
-      f32x4 x = {0, 0, 0, 0};
-      float sum = 0.0f;
+        for (int w = 0; w < KW; ++w) high = fmaxf(high, ml[w * 32 + row]);
+        const float from = high == -INFINITY ? 0.0f : high;
+        f32x4 x = {0, 0, 0, 0};
+        float sum = 0.0f;
 #pragma unroll
-      for (int w = 0; w < KW; ++w) {
-        const float by = __builtin_amdgcn_exp2f(ml[w * 32 + row] - ref);
-        sum += ml[(KW + w) * 32 + row] * by;
-        x += *reinterpret_cast<const f32x4*>(smem + w * TILE + (q * 33 + row) * 16) * by;
+        for (int w = 0; w < KW; ++w) {
+          const float by = __builtin_amdgcn_exp2f(ml[w * 32 + row] - from);
+          sum += ml[(KW + w) * 32 + row] * by;
+          x += *reinterpret_cast<const f32x4*>(smem + w * TILE + (q * 33 + row) * 16) * by;
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // no key seen: zeros
+        int r, g;
+        split_row(a, row0 + row, r, g);
+        const int64_t place = (s.q0 + r) * a.hq + head * a.group + g;
+        typedef T t4 __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<t4*>(static_cast<T*>(a.out) + place * a.dim + 4 * q) =
+            t4{static_cast<T>(x[0] * inv), static_cast<T>(x[1] * inv), static_cast<T>(x[2] * inv), static_cast<T>(x[3] * inv)};
+        if (a.lse != nullptr && q == 0)
+          a.lse[place] = sum == 0.0f ? -INFINITY : (high + __builtin_amdgcn_logf(sum)) * kLn2;
       }
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // no key seen: zeros
-      int r, g;
-      split_row(a, row0 + row, r, g);
-      const int64_t at = (s.q0 + r) * a.hq + head * a.group + g;
-      typedef T t4 __attribute__((ext_vector_type(4)));
-      *reinterpret_cast<t4*>(static_cast<T*>(a.out) + at * a.dim + 4 * q) =
-          t4{static_cast<T>(x[0] * inv), static_cast<T>(x[1] * inv), static_cast<T>(x[2] * inv), static_cast<T>(x[3] * inv)};
-      if (a.lse != nullptr && q == 0) a.lse[at] = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+    } else {
+      const float sum = half_sum(l), inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      if (row0 + c32 < rows) {
+        const int64_t place = (s.q0 + qi) * a.hq + head * a.group + qg;
+        store_row<T, DP>(static_cast<T*>(a.out) + place * a.dim, a.dim, h, acc, 1, inv);
+        if (a.lse != nullptr && h == 0) a.lse[place] = sum == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(sum)) * kLn2;
+      }
     }
-    return;
-  }
-#pragma unroll
-  for (int b = 0; b < QW; ++b) {
-    if (row0 + b * 32 + c32 >= rows) continue;
-    const float sum = half_sum(l[b]), inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const int64_t place = (s.q0 + qi[b]) * a.hq + head * a.group + qg[b];
-    store_row<T, DP>(static_cast<T*>(a.out) + place * a.dim, a.dim, h, &acc[0][b], QW, inv);
-    if (a.lse != nullptr && h == 0) a.lse[place] = sum == 0.0f ? -INFINITY : (m[b] + __builtin_amdgcn_logf(sum)) * kLn2;
   }
 }
 
@@ -525,9 +525,9 @@ int launch_attend(AttnArgs a, hipStream_t stream) {
   return HI3D_OK;
 }
 
-template <typename T, int DP, int QW, int KW>
+template <typename T, int DP, int KW>
 int launch_short(AttnArgs a, hipStream_t stream) {
-  constexpr int rows = QW * 32;
+  constexpr int rows = KW == 1 ? kShortSpan : 32;
   constexpr int part = DP * 132 > kTile<DP> ? DP * 132 : kTile<DP>;  // a wave's tile, or its 32 rows of the output
   constexpr size_t lds = KW == 1 ? 4 * kTile<DP> : KW * (part + 256);
   const int64_t per = a.cu_q != nullptr ? a.total_q * a.group / rows + a.batch
@@ -537,8 +537,8 @@ int launch_short(AttnArgs a, hipStream_t stream) {
   const int64_t blocks = KW == 1 ? ceil_div(per * a.hk, 4) : per * a.hk;
   constexpr int threads = KW == 1 ? 256 : 64 * KW;
   return a.mask != nullptr || a.dim < DP
-             ? launch_tiles<&attend_short_kernel<T, DP, QW, KW, true>>(a, blocks, threads, lds, stream)
-             : launch_tiles<&attend_short_kernel<T, DP, QW, KW, false>>(a, blocks, threads, lds, stream);
+             ? launch_tiles<&attend_short_kernel<T, DP, KW, true>>(a, blocks, threads, lds, stream)
+             : launch_tiles<&attend_short_kernel<T, DP, KW, false>>(a, blocks, threads, lds, stream);
 }
 
 // Few rows: 32-row blocks that leave compute units without a workgroup, over keys that 8
@@ -551,20 +551,29 @@ bool few_rows(int64_t total_q, int64_t total_k, int batch, int hq, int hk, int d
   return batch * ceil_div(average, 32) * hk <= cus && keys * dim <= (average <= 32 ? 98304 : 262144);
 }
 
-// Rows of a workgroup: one wave where segments are short (a larger tile would be empty),
-// else four.
 int64_t segment_average(const AttnArgs& a) { return ceil_div(a.total_q * a.group, a.batch); }
+
+// Rows of a workgroup: one wave where segments are short (a larger tile would be empty), else
+// four waves of one block of 32 rows, or of two where heads are small and that still leaves
+// four workgroups to each place on the chip: two blocks share their reads of LDS (20,011 x 33
+// heads x 64: 1865 us for 1926), one fills the chip more evenly (8,191 x 33 x 64 in four
+// segments: 193 us for 210).
+int attend_rows(int64_t total_q, int batch, int hq, int hk, int dim, int cus) {
+  const int64_t rows = total_q * (hq / hk), average = ceil_div(rows, batch);
+  if (average <= 64) return average <= 32 ? 32 : 64;
+  return dim <= 64 && ceil_div(rows, 256) * hk >= 8 * cus ? 256 : 128;
+}
 
 template <typename T, int DP>
 int launch_attend_dim(const AttnArgs& a, hipStream_t stream) {
   const int64_t average = segment_average(a);
-  if (average <= 64 && ceil_div(a.total_k, a.batch) <= 128)
-    return average <= 32 || DP > 64 ? launch_short<T, DP, 1, 1>(a, stream) : launch_short<T, DP, DP <= 64 ? 2 : 1, 1>(a, stream);
-  if (a.few) return launch_short<T, DP, 1, 8>(a, stream);
-  if (average <= 32) return launch_attend<T, DP, 1, 1>(a, stream);
-  if (average <= 64) return launch_attend<T, DP, 1, 2>(a, stream);
-  if constexpr (DP <= 64) return launch_attend<T, DP, 4, 2>(a, stream);
-  else return launch_attend<T, DP, 4, 1>(a, stream);
+  if (average <= 64 && ceil_div(a.total_k, a.batch) <= 128) return launch_short<T, DP, 1>(a, stream);
+  if (a.few) return launch_short<T, DP, 8>(a, stream);
+  if (a.rows == 32) return launch_attend<T, DP, 1, 1>(a, stream);
+  if (a.rows == 64) return launch_attend<T, DP, 1, 2>(a, stream);
+  if constexpr (DP <= 64)
+    if (a.rows == 256) return launch_attend<T, DP, 4, 2>(a, stream);
+  return launch_attend<T, DP, 4, 1>(a, stream);
 }
 
 template <typename T>
@@ -580,8 +589,8 @@ int launch_attend_type(const AttnArgs& a, hipStream_t stream) {
 // Splits of the key axis: as many as fill the chip twice over, each of at least 4 tiles.
 int attend_splits(int64_t total_q, int64_t total_k, int batch, int hq, int hk, int dim, int cus) {
   if (few_rows(total_q, total_k, batch, hq, hk, dim, cus)) return 1;
-  const int64_t rows = total_q * (hq / hk), average = ceil_div(rows, batch);
-  const int tile = average <= 32 ? 32 : (average <= 64 ? 64 : 256);
+  const int64_t average = ceil_div(total_q * (hq / hk), batch);
+  const int tile = attend_rows(total_q, batch, hq, hk, dim, cus);
   const int64_t blocks = (batch * ceil_div(average, tile)) * hk;
   const int64_t tiles = ceil_div(ceil_div(total_k, batch), kKT);
   const int64_t fill = static_cast<int64_t>(cus) * (tile <= 64 ? 8 : 2);
@@ -670,6 +679,7 @@ int hi3d_attention_forward(const hi3d_attention_desc* d, void* out, float* lse, 
   HI3D_REQUIRE(cus > 0, "cannot query the compute unit count");
   a.out = out, a.lse = lse;
   int splits = attend_splits(a.total_q, a.total_k, a.batch, a.hq, a.hk, a.dim, cus);
+  a.rows = attend_rows(a.total_q, a.batch, a.hq, a.hk, a.dim, cus);
   a.few = few_rows(a.total_q, a.total_k, a.batch, a.hq, a.hk, a.dim, cus);
   if (splits > 1) {
     const int64_t row_bytes = a.total_q * a.hq * 4;

@@ -255,7 +255,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
             for (int e = 0; e < 8; ++e) x[e] = dp[b][8 * k + e];
             pk[k][b] = pack8<T>(x);
           }
-  #pragma unroll
+          __builtin_amdgcn_s_setprio(1);
+#pragma unroll
         for (int k = 0; k < 2; ++k) {
 #pragma unroll
           for (int d = 0; d < DB; ++d) {
@@ -264,6 +265,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
             for (int b = 0; b < QW; ++b) Mfma<T>::run(x, pk[k][b], acc[b][d]);
           }
         }
+        __builtin_amdgcn_s_setprio(0);
         }
     }
   };
@@ -460,6 +462,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
         for (int b = 0; b < QW; ++b) p[k][b] = pack8<T>(ps[b]), ds[k][b] = pack8<T>(dss[b]);
       }
       __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
 #pragma unroll
@@ -469,6 +472,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
           for (int b = 0; b < QW; ++b) Mfma<T>::run(x, p[k][b], dv[b][d]), Mfma<T>::run(y, ds[k][b], dk[b][d]);
         }
       }
+      __builtin_amdgcn_s_setprio(0);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
