@@ -250,3 +250,23 @@ def test_attention_grad_c_refusals():
     assert query(total_q=4096, len_q=4096) > 4096 * 4 * 4 + 2 * 4 * 2 * 64 * 4
     with pytest.raises(ValueError, match="null"):
         _lib.query("hi3d_attention_backward_workspace", None)
+
+
+def test_token_attention_refusals():
+    from hi3d_amd import torso
+
+    for bad in ((100, 3), (96, 4, 3), (96, 0), (96, 24), (512, 2)):
+        with pytest.raises(ValueError):
+            torso.TokenAttention(*bad)
+    block = torso.TokenAttention(64, 1)
+    assert block.half().frequencies(torch.device("cpu")).dtype == torch.float64
+    cache = torso.KeyValueCache(2, 4, 1, 64, device="cpu")
+    cache.extend(0, torch.ones(3, 1, 64), torch.ones(3, 1, 64))
+    with pytest.raises(ValueError, match="no room for 2"):
+        cache.extend(0, torch.ones(2, 1, 64), torch.ones(2, 1, 64))
+    cache.append(torch.full((2, 1, 64), 2.0), torch.zeros(2, 1, 64))
+    assert cache.lens.tolist() == [4, 1] == cache.used and cache.k[0, 3, 0, 0] == 2 and cache.k[1, 0, 0, 0] == 2
+    with pytest.raises(ValueError, match="sequence 0 holds 4 of 4"):
+        cache.append(torch.ones(2, 1, 64), torch.ones(2, 1, 64))
+    with pytest.raises(ValueError, match="one sequence"):
+        block.float()(torch.zeros(2, 64), torch.zeros(2, 3, dtype=torch.int32), cache=cache)
