@@ -79,6 +79,12 @@ constexpr int kExactTiles = 4;
 // dout in registers) and walks the keys in tiles of 64 held twice in LDS, as the forward
 // does. Per 32 keys a wave forms S^T = K Q^T and dP^T = V dO^T, then dq += K^T dS^T with
 // the same K tile read transposed.
+//
+// One block of 32 rows a wave: two (half the LDS reads) need 1 wave a SIMD or spill, and ran
+// at half the speed (64 values a head: 560 us for 282). Bound by each wave's chain of
+// products and vector operations, which 2 or 3 waves a SIMD overlap in part: 8,191 rows x 33
+// heads x 64 fp16 in four segments 284 us (750 TFLOP/s of its 3 products), 8,192 causal x
+// 32/8 heads x 128 bf16 451 us (910).
 template <typename T, int DP, int NW, int QW, bool Z>
 __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
   constexpr int ROWS = NW * QW * 32, KS = DP / 16, DB = DP / 32, PAIR = 2 * kTile<DP>;
@@ -313,6 +319,15 @@ __device__ const float kPastRows[2] = {INFINITY, 0.0f};
 // dout, with lse and D of each row) held twice in LDS, so the query heads of a shared key
 // head sum in registers. Rows past the segment and rows that saw no key have lse = +infinity:
 // their probabilities are zero.
+//
+// Registers decide: keys, values and both sums take 192 of 256 at 128 values a head, and a
+// register spilled into the loop waits, when it is read again, for the tile loads in flight
+// (48 of them: 1628 us for 1000). So lse and D go straight to LDS, places are formed anew
+// from the lane, and masked and plain tiles share one path (two paths copied the sums). The
+// same figures as above: 365 us (775 TFLOP/s of its 4 products) and 552 us (1000).
+//
+// Causal: early keys see the most rows, so their blocks start first, and each block is split
+// at least in two, which levels the ends (1008 us to 623, with 25 for the join).
 template <typename T, int DP, int NW, int QW, bool Z, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(AttnArgs a) {
   constexpr int KEYS = NW * QW * 32, KS = DP / 16, DB = DP / 32, PAIR = 2 * kTile<DP>, CH = DP / 8;
@@ -508,7 +523,8 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
   }
 }
 
-// Sums the splits of dk and dv in order; 4 values a thread.
+// Sums the splits of dk and dv in order; 4 values a thread. 2 splits of 8,192 x 8 x 128: 25 us,
+// 5.3 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void attend_dkv_join_kernel(AttnArgs a, int64_t all) {
   const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
@@ -577,8 +593,8 @@ int launch_grad_type(const AttnArgs& a, hipStream_t stream) {
   }
 }
 
-// Splits of the query rows for dk and dv: as many as give every compute unit two workgroups,
-// each of at least 4 tiles of the average segment.
+// Splits of the query rows for dk and dv: as many as give every compute unit two workgroups
+// (four where causal blocks differ in length), each of at least 4 tiles of the average segment.
 int dkv_splits(const AttnArgs& a, int cus) {
   const int64_t average = ceil_div(a.total_k, a.batch), tile = average <= 32 ? 32 : 128;
   const int64_t blocks = a.batch * ceil_div(average, tile) * a.hk;

@@ -147,6 +147,8 @@ class _Problem:
 
     def backward(self, out, lse, dout, dlse, want_q: bool, want_kv: bool):
         q, k = self.tensors[:2]
+        if (q.shape[-2] // k.shape[-2] - 1) * q.stride(-2) >= 1 << 29:  # a tile's queries are addressed with 32 bits
+            self.set((q.contiguous(), *self.tensors[1:]), self.sizes)
         ref = self.ref
         out, lse, dout = _dense(out), _dense(lse), _dense(dout)
         dlse = dlse if dlse is None else _dense(dlse)

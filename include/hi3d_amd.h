@@ -636,7 +636,7 @@ int hi3d_rotary(const void* const x_dev[2], void* const y_dev[2], const int32_t 
  * causal: query i sees keys j <= i + lk - lq. key_mask (uint8, one per key row; optional):
  * keys with 0 are not seen, whatever they hold. A row that sees no key gives zeros and
  * lse = -infinity. F16 or BF16, dim a multiple of 8 up to 128, 16-byte aligned pointers,
- * strides multiples of 8, row strides below 2^23. */
+ * strides multiples of 8, row strides below 2^23; total_q * (heads_q / heads_k)^2 < 2^31. */
 typedef struct hi3d_attention_desc {
   const void* q;
   const void* k;
@@ -677,7 +677,7 @@ int hi3d_attention_backward_workspace(const hi3d_attention_desc* desc_host, int6
  * that of lse, dlse_dev fp32 [total_q, heads_q]. Probabilities are formed again from lse;
  * they and the scores' gradients are rounded once to the inputs' type for their products,
  * everything is summed in fp32 in a fixed order. Hidden keys and keys past those in use get
- * zeros. */
+ * zeros. The query heads of one key head must lie within 2^29 elements. */
 int hi3d_attention_backward(const hi3d_attention_desc* desc_host, const void* out_dev, const float* lse_dev,
                             const void* dout_dev, const float* dlse_dev, void* dq_dev, void* dk_dev, void* dv_dev,
                             void* workspace_dev, int64_t workspace_bytes, void* stream);
