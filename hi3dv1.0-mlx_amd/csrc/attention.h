@@ -329,6 +329,24 @@ int launch_tiles(const AttnArgs& a, int64_t blocks, int threads, size_t lds, hip
   return HI3D_OK;
 }
 
+// Masked keys: each tile has 64 numbers beside it in LDS, 0 for a key that is seen and
+// -infinity for one that is not, from which the score products start. Costs 8 reads of LDS a
+// tile, where selects cost 3 vector operations a score (or 8 scalar ones).
+__device__ __forceinline__ void store_bias(float* bias, uint64_t bits, int lane) {
+  bias[lane] = (bits >> lane) & 1 ? 0.0f : -INFINITY;
+}
+__device__ __forceinline__ f32x16 read_bias(const float* bias, int n, int h) {
+  f32x16 x;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(bias + 32 * n + 8 * g + 4 * h);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[4 * g + e] = v[e];
+  }
+  return x;
+}
+constexpr int kBiasBytes = 2 * kKT * 4;
+
 // Zeroes LDS tiles, for heads that do not fill their rows. Ends with a barrier.
 __device__ __forceinline__ void clear_tiles(char* smem, int bytes) {
   for (int i = threadIdx.x * 16; i < bytes; i += blockDim.x * 16) *reinterpret_cast<u32x4*>(smem + i) = u32x4{0, 0, 0, 0};

@@ -47,6 +47,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 && NW * QW == 4 ? 3 : 2) void att
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c32 = lane & 31, h = lane >> 5;
   const TileLane at = tile_lane<DP>(lane);
+  float* bias = reinterpret_cast<float*>(smem + 2 * PAIR);
 
   // task: (head, split, slot), neighbours on one XCD so that they share its L2
   const int64_t id = xcd_remap(blockIdx.x, gridDim.x);
@@ -118,6 +119,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 && NW * QW == 4 ? 3 : 2) void att
   // probabilities are zero, and what a hidden key holds cannot reach a product
   auto load = [&](int t, uint64_t bits, int buf) {
     if (Z && bits == 0) return;
+    if (Z && wave == 0) store_bias(bias + buf * kKT, bits, lane);
     const int64_t from = static_cast<int64_t>(t) * kKT;
     const int last = s.lk - t * kKT - 1, shown = Z ? __builtin_ctzll(bits) : 0;
     load_pair<DP, NW, Z>(kp + from * a.k_n * 2, a.k_n, vp + from * a.v_n * 2, a.v_n, a.dim, smem + buf * PAIR, wave, lane,
@@ -145,6 +147,14 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 && NW * QW == 4 ? 3 : 2) void att
       const char* kt = smem + buf * PAIR;
       const char* vt = kt + kTile<DP>;
       f32x16 sc[2][QW] = {};
+      if constexpr (Z) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const f32x16 x = read_bias(bias + buf * kKT, n, h);
+#pragma unroll
+          for (int b = 0; b < QW; ++b) sc[n][b] = x;
+        }
+      }
 #pragma unroll
       for (int k = 0; k < KS; ++k)
 #pragma unroll
@@ -154,8 +164,8 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 && NW * QW == 4 ? 3 : 2) void att
           for (int b = 0; b < QW; ++b) Mfma<T>::run(x, qf[b][k], sc[n][b]);
         }
       // keys that are hidden from a row
-      if (bits != ~0ull || (t + 1) * kKT > wfull) {
-        hide_keys<QW>(sc, bits);
+      if ((!Z && bits != ~0ull) || (t + 1) * kKT > wfull) {
+        if constexpr (!Z) hide_keys<QW>(sc, bits);
         if (a.causal) {
           asm volatile("");
 #pragma unroll
@@ -523,7 +533,7 @@ int launch_attend(AttnArgs a, hipStream_t stream) {
   const int64_t blocks = per * a.hk * a.splits;
   HI3D_REQUIRE(blocks < (1ll << 31), "too many rows for one launch");
   a.slots = static_cast<int>(per);
-  constexpr size_t lds = 4 * kTile<DP>;
+  const size_t lds = 4 * kTile<DP> + (z ? kBiasBytes : 0);
   if (a.splits == 1)
     return z ? launch_tiles<&attend_kernel<T, DP, NW, QW, true, false>>(a, blocks, 64 * NW, lds, stream)
              : launch_tiles<&attend_kernel<T, DP, NW, QW, false, false>>(a, blocks, 64 * NW, lds, stream);

@@ -92,6 +92,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c32 = lane & 31, h = lane >> 5;
   const TileLane place_of = tile_lane<DP>(lane);
+  float* bias = reinterpret_cast<float*>(smem + 2 * PAIR);
   const int64_t id = xcd_remap(blockIdx.x, gridDim.x);
   int head, slot;
   if (a.head_minor) head = static_cast<int>(id % a.hk), slot = static_cast<int>(id / a.hk);
@@ -202,6 +203,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
   // probabilities are zero, and what a hidden key holds cannot reach a product
   auto load = [&](int t, uint64_t bits, int buf) {
     if (Z && bits == 0) return;
+    if (Z && wave == 0) store_bias(bias + buf * kKT, bits, fresh_lane());
     const int64_t at = static_cast<int64_t>(t) * kKT;
     const int lane = fresh_lane(), last = s.lk - t * kKT - 1, shown = Z ? __builtin_ctzll(bits) : 0;
     load_pair<DP, NW, Z>(kp + at * a.k_n * 2, a.k_n, vp + at * a.v_n * 2, a.v_n, a.dim, smem + buf * PAIR, wave, lane,
@@ -210,11 +212,15 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
 
   f32x16 acc[QW][DB] = {};
   // one tile; hide: some keys are hidden from some rows; exact_step: only sums ds
-  auto walk = [&](const char* kt, int t, uint64_t bits, bool hide, bool exact_step) {
+  auto walk = [&](const char* kt, const float* tile_bias, int t, uint64_t bits, bool hide, bool exact_step) {
     const char* vt = kt + kTile<DP>;
 #pragma unroll 2
     for (int n = 0; n < 2; ++n) {
       f32x16 sc[QW] = {}, dp[QW] = {};
+      if constexpr (Z) {
+#pragma unroll
+        for (int b = 0; b < QW; ++b) sc[b] = read_bias(tile_bias, n, h);
+      }
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         const u32x4 x = read_rows<DP>(kt, 32 * n, k, place_of), y = read_rows<DP>(vt, 32 * n, k, place_of);
@@ -291,7 +297,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
     if (step + 2 < steps) after = key_bits(tile_of(step + 2));
     if (t * kKT < wkend && (!Z || bits != 0)) {
       const char* tile = smem + buf * PAIR;
-      walk(tile, t, bits, bits != ~0ull || (t + 1) * kKT > wfull, step < exact);
+      walk(tile, bias + buf * kKT, t, bits, (!Z && bits != ~0ull) || (t + 1) * kKT > wfull, step < exact);
     }
     if (step + 1 == exact) {  // sum ds was to be dlse
 #pragma unroll
@@ -544,7 +550,7 @@ int launch_dq(AttnArgs a, hipStream_t stream) {
   a.slots = a.dq_slots;
   const int64_t blocks = static_cast<int64_t>(a.slots) * a.hk;
   constexpr size_t lds = 4 * kTile<DP>;
-  return a.mask != nullptr || a.dim < DP ? launch_tiles<&attend_dq_kernel<T, DP, NW, QW, true>>(a, blocks, 64 * NW, lds, stream)
+  return a.mask != nullptr || a.dim < DP ? launch_tiles<&attend_dq_kernel<T, DP, NW, QW, true>>(a, blocks, 64 * NW, lds + kBiasBytes, stream)
                                          : launch_tiles<&attend_dq_kernel<T, DP, NW, QW, false>>(a, blocks, 64 * NW, lds, stream);
 }
 

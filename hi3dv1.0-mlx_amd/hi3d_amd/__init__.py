@@ -2,8 +2,8 @@
 
 Voxel-hash kernel maps, gather-MFMA sparse convolution (submanifold 3^3, 2x2x2/s2 and
 its transpose), the W8A8 int8 linear, the LayerNorm + adaLN row kernel and the torso's
-rotary positions and attention, as hand-written HIP kernels behind a C ABI (``include/hi3d_amd.h``), with the reference's
-Python call surfaces on top:
+rotary positions and attention, as hand-written HIP kernels behind a C ABI
+(``include/hi3d_amd.h``), with the reference's Python call surfaces on top:
 
 * :mod:`hi3d_amd.spconv` — the spconv 2.3.6 subset (``SubMConv3d``,
   ``SparseConvTensor``, ``ops.get_indice_pairs``, ``core.IndiceData``, ...);
