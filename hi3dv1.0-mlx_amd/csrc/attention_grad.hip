@@ -182,12 +182,6 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
     }
   }
   const int tiles = kend > 0 ? (kend + kKT - 1) / kKT : 0;
-  // walks over the tiles: the first one corrects D where the rows see few keys; none where
-  // only D and the bounds are wanted
-  const int exact = tiles <= kExactTiles ? tiles : 0;
-  const int steps = exact + (a.out != nullptr ? tiles : 0);
-  if (exact == 0) store_stats();
-  float miss[QW] = {};
 
   const char* kp = reinterpret_cast<const char*>(static_cast<const T*>(a.k) + s.b * a.k_b + head * a.k_h +
                                                  (a.cu_k != nullptr ? s.k0 * a.k_n : 0));
@@ -210,9 +204,10 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
                          [&](int row) { return Z ? ((bits >> row) & 1 ? row : shown) : (row < last ? row : last); });
   };
 
-  f32x16 acc[QW][DB] = {};
-  // one tile; hide: some keys are hidden from some rows; exact_step: only sums ds
-  auto walk = [&](const char* kt, const float* tile_bias, int t, uint64_t bits, bool hide, bool exact_step) {
+  f32x16 acc[QW][DB];
+  float miss[QW];
+  // one tile; hide: some keys are hidden from some rows; EXACT: only sums ds
+  auto walk = [&](const char* kt, const float* tile_bias, int t, uint64_t bits, bool hide, auto EXACT) {
     const char* vt = kt + kTile<DP>;
 #pragma unroll 2
     for (int n = 0; n < 2; ++n) {
@@ -250,8 +245,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
           const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][e], a.scale2, -ref[b]));
           dp[b][e] = p * __builtin_fmaf(dp[b][e], by[b], -delta[b]);
         }
-      if (exact_step) {
-        asm volatile("");
+      if constexpr (EXACT) {
 #pragma unroll
         for (int b = 0; b < QW; ++b)
 #pragma unroll
@@ -267,7 +261,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
             for (int e = 0; e < 8; ++e) x[e] = dp[b][8 * k + e];
             pk[k][b] = pack8<T>(x);
           }
-          __builtin_amdgcn_s_setprio(1);
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
 #pragma unroll
@@ -278,39 +272,43 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
           }
         }
         __builtin_amdgcn_s_setprio(0);
-        }
+      }
+    }
+  };
+  // one pass over the tiles
+  auto pass = [&](auto EXACT) {
+    uint64_t bits = key_bits(0), next = 0;
+    load(0, bits, 0);
+    if (tiles > 1) next = key_bits(1);
+    tile_barrier();
+    for (int t = 0, buf = 0; t < tiles; ++t, buf ^= 1) {
+      if (t + 1 < tiles) load(t + 1, next, buf ^ 1);
+      uint64_t after = 0;
+      if (t + 2 < tiles) after = key_bits(t + 2);
+      if (t * kKT < wkend && (!Z || bits != 0))
+        walk(smem + buf * PAIR, bias + buf * kKT, t, bits, (!Z && bits != ~0ull) || (t + 1) * kKT > wfull, EXACT);
+      bits = next, next = after;
+      tile_barrier();
     }
   };
   if (Z && a.dim < DP) clear_tiles(smem, 2 * PAIR);
-  uint64_t bits = 0, next = 0;
-  auto tile_of = [&](int step) { return step < exact ? step : step - exact; };
-  if (steps > 0) {
-    bits = key_bits(0);
-    load(0, bits, 0);
-    if (steps > 1) next = key_bits(tile_of(1));
-  }
-  tile_barrier();
-  for (int step = 0, buf = 0; step < steps; ++step, buf ^= 1) {
-    const int t = tile_of(step);
-    if (step + 1 < steps) load(tile_of(step + 1), next, buf ^ 1);
-    uint64_t after = 0;
-    if (step + 2 < steps) after = key_bits(tile_of(step + 2));
-    if (t * kKT < wkend && (!Z || bits != 0)) {
-      const char* tile = smem + buf * PAIR;
-      walk(tile, bias + buf * kKT, t, bits, (!Z && bits != ~0ull) || (t + 1) * kKT > wfull, step < exact);
-    }
-    if (step + 1 == exact) {  // sum ds was to be dlse
+  if (tiles > 0 && tiles <= kExactTiles) {
 #pragma unroll
-      for (int b = 0; b < QW; ++b) {
-        delta[b] += half_sum(miss[b]) * power_of_two(-static_cast<int>(kPLog2<T>));
-        if (a.dlse != nullptr) delta[b] -= a.dlse[row_at(b)] * by[b];
-      }
-      store_stats();
+    for (int b = 0; b < QW; ++b) miss[b] = 0.0f;
+    pass(std::true_type{});
+#pragma unroll
+    for (int b = 0; b < QW; ++b) {  // sum ds was to be dlse
+      delta[b] += half_sum(miss[b]) * power_of_two(-static_cast<int>(kPLog2<T>));
+      if (a.dlse != nullptr) delta[b] -= a.dlse[row_at(b)] * by[b];
     }
-    bits = next, next = after;
-    tile_barrier();
   }
-  if (a.out == nullptr) return;
+  store_stats();
+  if (a.out == nullptr) return;  // only D and the bounds are wanted
+#pragma unroll
+  for (int b = 0; b < QW; ++b)
+#pragma unroll
+    for (int d = 0; d < DB; ++d) acc[b][d] = f32x16{};
+  if (tiles > 0) pass(std::false_type{});
 #pragma unroll
   for (int b = 0; b < QW; ++b) {
     if (wrow + b * 32 + c32 >= rows) continue;
