@@ -440,7 +440,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
   // one tile; hide: some rows do not see some keys
   auto walk = [&](const char* qt, const float* st, int t, bool hide) {
     const char* dt = qt + kTile<DP>;
-#pragma unroll 1
+#pragma unroll 2
     for (int n = 0; n < 2; ++n) {
       f32x16 sc[QW] = {}, dp[QW] = {};
 #pragma unroll
