@@ -28,14 +28,23 @@ struct alignas(sizeof(T) * V) Chunk {
   T v[V];
 };
 
+// A chunk that is read once: past the caches, which keep what is written for its reader.
+template <typename C, typename T>
+__device__ __forceinline__ C load_once(const T* p) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  if constexpr (sizeof(C) == 16) return __builtin_bit_cast(C, __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)));
+  else return *reinterpret_cast<const C*>(p);
+}
+
 // A workgroup takes `tokens` tokens. It first forms cos and sin of their rot / 2 angles,
 // once for all heads: the angle in fp64, reduced to half a turn before it is rounded (an
 // angle of 10^5 radians would keep 2 digits in fp32), then sine and cosine in fp32 in LDS.
 // The heads then move as units of one 16-byte chunk (interleaved; or a copied chunk past
 // rot) or two (a half-layout unit is chunk c of the first half and of the second), so each
 // value is read and written once. V is 1 where sizes, strides or pointers do not allow
-// 16-byte chunks. Bound by HBM: 20,011 tokens x 66 heads x 64 fp16 by three axes in 80 us (4.2
-// TB/s), 65,536 x 40 x 128 bf16 in 268 us (5.0 TB/s); one token in 3 us.
+// 16-byte chunks. Bound by HBM: 20,011 tokens x 66 heads x 64 fp16 by three axes in 76 us (4.5
+// TB/s; 82 with loads through the caches), 65,536 x 40 x 128 bf16 in 278 us (4.8); one token
+// in 3 us.
 template <typename T, typename P, int V, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
   extern __shared__ float2 turns[];  // [tokens][rot / 2]
@@ -70,10 +79,10 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
       T* y = static_cast<T*>(a.y[which]) + ((first + t) * a.heads[which] + h) * a.dim;
       if (c >= turned) {
         const int d = a.rot + (c - turned) * V;
-        *reinterpret_cast<C*>(y + d) = *reinterpret_cast<const C*>(x + d);
+        *reinterpret_cast<C*>(y + d) = load_once<C>(x + d);
       } else if constexpr (!INTERLEAVED || V == 1) {
         const int d0 = INTERLEAVED ? 2 * c : c * V, d1 = INTERLEAVED ? d0 + 1 : d0 + half;
-        C p = *reinterpret_cast<const C*>(x + d0), q = *reinterpret_cast<const C*>(x + d1);
+        C p = load_once<C>(x + d0), q = load_once<C>(x + d1);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           const float2 r = w[c * V + e];
@@ -84,7 +93,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
         *reinterpret_cast<C*>(y + d0) = p;
         *reinterpret_cast<C*>(y + d1) = q;
       } else {
-        C p = *reinterpret_cast<const C*>(x + c * V);
+        C p = load_once<C>(x + c * V);
 #pragma unroll
         for (int e = 0; e < V / 2; ++e) {
           const float2 r = w[c * (V / 2) + e];
