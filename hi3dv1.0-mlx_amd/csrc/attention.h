@@ -52,6 +52,7 @@ struct AttnArgs {
   uint32_t group_magic;         // ceil(2^32 / group) for group > 1
   float scale, scale2;          // scale, scale * log2(e)
   int32_t causal, splits, slots, head_minor, reverse, few, rows;
+  int32_t once;                 // keys and values that no cache holds until they are read again
 };
 
 template <typename T>
@@ -259,9 +260,15 @@ __device__ __forceinline__ void tile_chunk(int i, int wave, int lane, int& row, 
   }
 }
 
+// 16 bytes a lane straight to LDS; ONCE: past the caches.
+template <bool ONCE>
+__device__ __forceinline__ void load_chunk(const void* src, char* to) {
+  __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void*)(to), 16, 0, ONCE ? 2 : 0);
+}
+
 // Copies a tile of 64 keys and their values from x and y on straight to LDS; row r comes from
 // row of(r). Chunks past the head size are left out (Z): they were zeroed once.
-template <int DP, int NW, bool Z, typename F>
+template <int DP, int NW, bool Z, bool ONCE, typename F>
 __device__ __forceinline__ void load_pair(const char* x, int64_t x_n, const char* y, int64_t y_n, int dim, char* tile,
                                           int wave, int lane, F of) {
   static_assert(DP / 8 % NW == 0, "the waves share a tile's loads evenly");
@@ -273,8 +280,8 @@ __device__ __forceinline__ void load_pair(const char* x, int64_t x_n, const char
     if (Z && c * 8 >= dim) continue;
     const uint32_t from = of(row);
     char* to = tile + (wave + i * NW) * kBlock<DP>;
-    lds_dma16(x + (from * xs + c * 16), to);
-    lds_dma16(y + (from * ys + c * 16), to + kTile<DP>);
+    load_chunk<ONCE>(x + (from * xs + c * 16), to);
+    load_chunk<ONCE>(y + (from * ys + c * 16), to + kTile<DP>);
   }
 }
 

@@ -38,8 +38,11 @@ __device__ __forceinline__ void hide_keys(f32x16 (&sc)[2][QW], uint64_t bits) {
 // TFLOP/s; 16,384 causal x 32/8 heads x 128 bf16: 1978 us, 1110 TFLOP/s.
 //
 // SPLIT, few rows over many keys: parts of the keys go to workgroups of their own, and their
-// outputs and (m, sum) to attend_join_kernel in fp32. Single tokens of 8 sequences over
-// caches of up to 65,536 x 8 x 128 bf16: 350 us, 5.3 TB/s, the keys and values read once.
+// outputs and (m, sum) to attend_join_kernel in fp32. One-wave workgroups then read keys and
+// values that no other one does; more of them than the chip's 256 MiB of cache go past it, as
+// the next token's call would not find them there. Single tokens of 8 sequences over caches of
+// up to 65,536 x 8 x 128 bf16 (1.9 GB): 326 us, 5.8 TB/s, 358 through the caches; below that
+// size the cache helps (8 x 4,096 keys, 134 MB: 30.8 us for 32.3).
 template <typename T, int DP, int NW, int QW, bool Z, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, DP <= 64 && NW * QW == 4 ? 3 : 2) void attend_kernel(AttnArgs a) {
   constexpr int ROWS = NW * QW * 32, KS = DP / 16, DB = DP / 32, PAIR = 2 * kTile<DP>;
@@ -122,8 +125,11 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 && NW * QW == 4 ? 3 : 2) void att
     if (Z && wave == 0) store_bias(bias + buf * kKT, bits, lane);
     const int64_t from = static_cast<int64_t>(t) * kKT;
     const int last = s.lk - t * kKT - 1, shown = Z ? __builtin_ctzll(bits) : 0;
-    load_pair<DP, NW, Z>(kp + from * a.k_n * 2, a.k_n, vp + from * a.v_n * 2, a.v_n, a.dim, smem + buf * PAIR, wave, lane,
-                         [&](int row) { return Z ? ((bits >> row) & 1 ? row : shown) : (row < last ? row : last); });
+    auto of = [&](int row) { return Z ? ((bits >> row) & 1 ? row : shown) : (row < last ? row : last); };
+    const char *x = kp + from * a.k_n * 2, *y = vp + from * a.v_n * 2;
+    char* to = smem + buf * PAIR;
+    if (SPLIT && NW == 1 && a.once) load_pair<DP, NW, Z, true>(x, a.k_n, y, a.v_n, a.dim, to, wave, lane, of);
+    else load_pair<DP, NW, Z, false>(x, a.k_n, y, a.v_n, a.dim, to, wave, lane, of);
   };
 
   f32x16 acc[DB][QW] = {};
@@ -664,6 +670,7 @@ int attention_args(const hi3d_attention_desc* d, AttnArgs& a) {
   // short segments: the heads of a row share its cache lines, so they run side by side
   a.head_minor = d->batch > 0 && d->total_k / d->batch <= 512;
   a.reverse = a.causal;
+  a.once = d->total_k * d->heads_k * d->dim * 4 > (256ll << 20);
   return HI3D_OK;
 }
 

@@ -200,7 +200,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
     if (Z && wave == 0) store_bias(bias + buf * kKT, bits, fresh_lane());
     const int64_t at = static_cast<int64_t>(t) * kKT;
     const int lane = fresh_lane(), last = s.lk - t * kKT - 1, shown = Z ? __builtin_ctzll(bits) : 0;
-    load_pair<DP, NW, Z>(kp + at * a.k_n * 2, a.k_n, vp + at * a.v_n * 2, a.v_n, a.dim, smem + buf * PAIR, wave, lane,
+    load_pair<DP, NW, Z, false>(kp + at * a.k_n * 2, a.k_n, vp + at * a.v_n * 2, a.v_n, a.dim, smem + buf * PAIR, wave, lane,
                          [&](int row) { return Z ? ((bits >> row) & 1 ? row : shown) : (row < last ? row : last); });
   };
 
