@@ -80,11 +80,11 @@ constexpr int kExactTiles = 4;
 // does. Per 32 keys a wave forms S^T = K Q^T and dP^T = V dO^T, then dq += K^T dS^T with
 // the same K tile read transposed.
 //
-// One block of 32 rows a wave: two (half the LDS reads) need 1 wave a SIMD or spill, and ran
-// at half the speed (64 values a head: 560 us for 282). Bound by each wave's chain of
-// products and vector operations, which 2 or 3 waves a SIMD overlap in part: 8,191 rows x 33
-// heads x 64 fp16 in four segments 284 us (750 TFLOP/s of its 3 products), 8,192 causal x
-// 32/8 heads x 128 bf16 451 us (910).
+// One block of 32 rows a wave: two (half the LDS reads) leave fewer waves a SIMD and ran at
+// lower speed (64 values a head: 294 us for 271). Bound by each wave's chain of products
+// and vector operations, which 2 or 3 waves a SIMD overlap in part: 8,191 rows x 33 heads x 64
+// fp16 in four segments 262 us (810 TFLOP/s of its 3 products), 8,192 causal x 32/8 heads x 128
+// bf16 412 us (1000).
 template <typename T, int DP, int NW, int QW, bool Z>
 __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
   constexpr int ROWS = NW * QW * 32, KS = DP / 16, DB = DP / 32, PAIR = 2 * kTile<DP>;
@@ -328,7 +328,7 @@ __device__ const float kPastRows[2] = {INFINITY, 0.0f};
 // register spilled into the loop waits, when it is read again, for the tile loads in flight
 // (48 of them: 1628 us for 1000). So lse and D go straight to LDS, places are formed anew
 // from the lane, and masked and plain tiles share one path (two paths copied the sums). The
-// same figures as above: 365 us (775 TFLOP/s of its 4 products) and 552 us (1000).
+// same figures as above: 350 us (810 TFLOP/s of its 4 products) and 545 us (1010).
 //
 // Causal: early keys see the most rows, so their blocks start first, and each block is split
 // at least in two, which levels the ends (1008 us to 623, with 25 for the join).
