@@ -84,14 +84,20 @@ class TokenAttention(nn.Module):
                 key_mask: torch.Tensor | None = None, cache: KeyValueCache | None = None) -> torch.Tensor:
         """``x [N, C]`` with ``positions [N, axes]``, objects one after another at ``offsets``
         (:func:`attention.offsets`; one object without). ``cache``: takes the keys and values of
-        the one sequence of a prompt."""
+        the one sequence of a prompt, or of its next part, which also sees the keys that the
+        cache holds already (as constants, where gradients are wanted)."""
         if cache is not None and (offsets is not None or len(cache.used) != 1):
             raise ValueError("a prompt fills the cache of one sequence")
         q, k, v = self.project(x, positions)
         if cache is not None:
+            held, recorded = cache.used[0], torch.is_grad_enabled() and k.requires_grad
             cache.extend(0, k, v)
+            if held and recorded:  # copies: autograd keeps them, and the cache changes with every token
+                k, v = torch.cat([cache.k[0, :held], k]), torch.cat([cache.v[0, :held], v])
+            elif held:
+                k, v = cache.k[0, :cache.used[0]], cache.v[0, :cache.used[0]]
         y = attention.attend(q, k, v, offsets, causal=self.causal, key_mask=key_mask)
-        return self.out(y.reshape(x.shape[0], -1))
+        return self.out(y.reshape(x.shape[0], self.heads * self.dim))
 
     @torch.no_grad()
     def step(self, x: torch.Tensor, positions: torch.Tensor, cache: KeyValueCache) -> torch.Tensor:
@@ -100,4 +106,4 @@ class TokenAttention(nn.Module):
         q, k, v = self.project(x, positions)
         cache.append(k, v)
         y = attention.attend(q[:, None], cache.k, cache.v, lens_k=cache.lens)
-        return self.out(y.reshape(x.shape[0], -1))
+        return self.out(y.reshape(x.shape[0], self.heads * self.dim))

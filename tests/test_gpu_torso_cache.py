@@ -1,0 +1,66 @@
+"""The torso's block over a cache on the GPU, against the block in float64. Tolerances as in
+``test_gpu_torso``: root mean square errors below 8 half steps of the type for outputs, 16 for
+gradients."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from test_gpu_torso import U, _plain, _rms
+
+pytestmark = pytest.mark.gpu
+
+
+def _block(dtype, heads=4, key_heads=2, dim=64, causal=True):
+    from hi3d_amd import torso
+
+    torch.manual_seed(1)
+    return torso.TokenAttention(dim * heads, heads, key_heads, axes=1, causal=causal, dtype=dtype, device="cuda")
+
+
+def _tokens(n, channels, dtype):
+    g = torch.Generator().manual_seed(4)
+    return torch.randn(n, channels, generator=g).to(dtype).cuda(), torch.arange(n, dtype=torch.int32).cuda()[:, None]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("chunks", [(200, 90), (1, 1, 64, 33, 200), (130, 0, 5)])
+def test_a_prompt_in_chunks(cuda, chunks, dtype):
+    from hi3d_amd import torso
+
+    block = _block(dtype)
+    x, positions = _tokens(310, 256, dtype)
+    want = _plain(block, x.double(), positions, [310], True)[0].detach()
+    cache, at, rows = torso.KeyValueCache(1, 310, 2, 64, dtype), 0, []
+    with torch.no_grad():
+        for n in chunks:
+            rows.append(block(x[at:at + n], positions[at:at + n], cache=cache))
+            at += n
+        for i in range(at, at + 3):
+            rows.append(block.step(x[i:i + 1], positions[i:i + 1], cache))
+    rows = torch.cat(rows).double()
+    assert _rms(rows - want[:at + 3]) <= 8 * U[dtype] * _rms(want[:at + 3])
+    assert _rms(rows[-3:] - want[at:at + 3]) <= 8 * U[dtype] * _rms(want[at:at + 3])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_gradients_of_a_chunk(cuda, dtype):
+    from hi3d_amd import torso
+
+    block = _block(dtype)
+    x, positions = _tokens(150, 256, dtype)
+    dout = _tokens(60, 256, dtype)[0]
+    cache = torso.KeyValueCache(1, 200, 2, 64, dtype)
+    with torch.no_grad():
+        block(x[:90], positions[:90], cache=cache)
+    leaf = x[90:].clone().requires_grad_(True)
+    out = block(leaf, positions[90:], cache=cache)
+    with torch.no_grad():
+        block.step(x[:1], positions[:1], cache)
+    out.backward(dout)
+    other = x[90:].double().requires_grad_(True)
+    want = _plain(block, torch.cat([x[:90].double(), other]), positions, [150], True)[0][90:]
+    want.backward(dout.double())
+    assert _rms(out.double() - want) <= 8 * U[dtype] * _rms(want)
+    assert _rms(leaf.grad.double() - other.grad) <= 16 * U[dtype] * _rms(other.grad)

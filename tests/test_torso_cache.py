@@ -1,0 +1,115 @@
+"""What the torso's block does with its cache, without a GPU: plain stand-ins in the inputs' own
+type (float64 here) for the two operators, so that the block's data flow is all that is tested.
+Tolerance: sums of a few hundred float64 products, 1e-12 of values near one."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+TOL = dict(rtol=1e-12, atol=1e-12)
+
+
+def _attend(q, k, v, cu_q=None, cu_k=None, *, lens_k=None, scale=None, causal=False, key_mask=None):
+    """``attention.attend`` from its definition: one packed segment, or equal room."""
+    assert cu_q is None and cu_k is None and k.shape == v.shape and k.shape[:-3] == q.shape[:-3]
+    if q.dim() == 4:
+        lens = [k.shape[1]] * k.shape[0] if lens_k is None else lens_k.tolist()
+        assert key_mask is None or key_mask.shape == k.shape[:2]
+        return torch.stack([_attend(q[b], k[b, :n], v[b, :n], causal=causal,
+                                    key_mask=None if key_mask is None else key_mask[b, :n]) for b, n in enumerate(lens)])
+    lq, lk, group = q.shape[0], k.shape[0], q.shape[1] // k.shape[1]
+    assert key_mask is None or key_mask.shape == (lk,)
+    k, v = k.repeat_interleave(group, 1), v.repeat_interleave(group, 1)
+    score = torch.einsum("ihd,jhd->hij", q, k) * (q.shape[-1] ** -0.5 if scale is None else scale)
+    if causal:
+        score = score.masked_fill(torch.arange(lk) > torch.arange(lq)[:, None] + (lk - lq), -math.inf)
+    if key_mask is not None:
+        score = score.masked_fill(~key_mask, -math.inf)
+    return torch.einsum("hij,jhd->ihd", score.softmax(-1).nan_to_num(0.0), v)
+
+
+def _turn(q, k, positions, freqs, *, layout):
+    angle = (positions.double() @ freqs)[:, None]
+    pad = q.shape[-1] // 2 - angle.shape[-1]
+    wave = torch.nn.functional.pad(torch.polar(torch.ones_like(angle), angle), (0, pad), value=1.0)
+    turned = lambda x: torch.view_as_real(torch.view_as_complex(x.unflatten(-1, (-1, 2))) * wave).flatten(-2)  # noqa: E731
+    assert layout == "interleaved"
+    return turned(q), turned(k)
+
+
+@pytest.fixture
+def plain(monkeypatch):
+    from hi3d_amd import attention, rotary
+
+    monkeypatch.setattr(attention, "attend", _attend)
+    monkeypatch.setattr(rotary, "rotate_qk", _turn)
+
+
+def _block(causal=True, heads=4, key_heads=2):
+    from hi3d_amd import torso
+
+    torch.manual_seed(0)
+    return torso.TokenAttention(8 * heads, heads, key_heads, axes=1, causal=causal, dtype=torch.float64)
+
+
+def _cache(block, batch=1, length=40):
+    from hi3d_amd import torso
+
+    return torso.KeyValueCache(batch, length, block.key_heads, block.dim, torch.float64, device="cpu")
+
+
+def _tokens(n, channels, seed=1):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(n, channels, generator=g, dtype=torch.float64), torch.arange(n, dtype=torch.int32)[:, None]
+
+
+@pytest.mark.parametrize("chunks", [(20,), (13, 7), (1, 1, 18), (5, 0, 15)])
+def test_a_prompt_in_chunks(plain, chunks):
+    """Every chunk sees what the cache holds already: the rows of one pass over all tokens."""
+    block = _block()
+    x, positions = _tokens(24, 32)
+    want, cache, at, rows = block(x, positions), _cache(block), 0, []
+    with torch.no_grad():
+        for n in chunks:
+            rows.append(block(x[at:at + n], positions[at:at + n], cache=cache))
+            at += n
+            assert cache.used == [at] == cache.lens.tolist()
+        for i in range(at, 24):
+            rows.append(block.step(x[i:i + 1], positions[i:i + 1], cache))
+    torch.testing.assert_close(torch.cat(rows), want.detach(), **TOL)
+    assert cache.used == [24]
+
+
+def test_a_chunk_after_steps_and_without_a_causal_limit(plain):
+    block = _block(causal=False)
+    x, positions = _tokens(12, 32)
+    cache = _cache(block)
+    with torch.no_grad():
+        block(x[:5], positions[:5], cache=cache)
+        block.step(x[5:6], positions[5:6], cache)
+        got = block(x[6:], positions[6:], cache=cache)
+    torch.testing.assert_close(got, block(x, positions).detach()[6:], **TOL)
+
+
+def test_gradients_of_a_chunk(plain):
+    """The chunk's own keys take gradients; those that the cache held are constants, and keys
+    that the cache takes later do not disturb the backward pass."""
+    block = _block()
+    x, positions = _tokens(20, 32)
+    cache = _cache(block)
+    with torch.no_grad():
+        block(x[:9], positions[:9], cache=cache)
+    leaf = x[9:].clone().requires_grad_(True)
+    out = block(leaf, positions[9:], cache=cache)
+    assert cache.used == [20] and not cache.k.requires_grad
+    with torch.no_grad():
+        block.step(x[:1], positions[:1], cache)
+    got, = torch.autograd.grad(out.square().sum(), leaf)
+    other = x[9:].clone().requires_grad_(True)
+    whole = block(torch.cat([x[:9], other]), positions)[9:]
+    want, = torch.autograd.grad(whole.square().sum(), other)
+    torch.testing.assert_close(out, whole, **TOL)
+    torch.testing.assert_close(got, want, **TOL)
