@@ -13,7 +13,8 @@ from . import attention, rotary
 
 class KeyValueCache:
     """Room for ``length`` keys and values of each of ``batch`` sequences, ``[batch, length,
-    heads, dim]``, and how many are in use: ``lens`` on the GPU, ``used`` on the host."""
+    heads, dim]``, and how many are in use: ``lens`` on the GPU, ``used`` on the host. ``mask``:
+    None, or bool ``[batch, length]`` with False at the keys that a prompt's mask hid."""
 
     def __init__(self, batch: int, length: int, heads: int, dim: int, dtype: torch.dtype = torch.float16,
                  device: torch.device | str = "cuda"):
@@ -21,16 +22,24 @@ class KeyValueCache:
         self.v = torch.zeros_like(self.k)
         self.lens = torch.zeros(batch, dtype=torch.int32, device=device)
         self.used = [0] * batch
+        self.mask: torch.Tensor | None = None
         self._rows = torch.arange(batch, device=device)
 
     def _room(self, which: int, count: int) -> None:
         if self.used[which] + count > self.k.shape[1]:
             raise ValueError(f"sequence {which} holds {self.used[which]} of {self.k.shape[1]} keys: no room for {count}")
 
-    def extend(self, which: int, k: torch.Tensor, v: torch.Tensor) -> None:
-        """Adds the keys and values ``[n, heads, dim]`` of a prompt to one sequence."""
+    def extend(self, which: int, k: torch.Tensor, v: torch.Tensor, key_mask: torch.Tensor | None = None) -> None:
+        """Adds the keys and values ``[n, heads, dim]`` of a prompt to one sequence; those where
+        ``key_mask [n]`` is False are there, but not seen."""
         n, at = int(k.shape[0]), self.used[which]
         self._room(which, n)
+        if key_mask is not None:
+            if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.shape != (n,):
+                raise ValueError(f"key_mask must be bool [{n}]")
+            if self.mask is None:
+                self.mask = torch.ones(self.k.shape[:2], dtype=torch.bool, device=self.k.device)
+            self.mask[which, at:at + n] = key_mask
         self.k[which, at:at + n] = k.detach()
         self.v[which, at:at + n] = v.detach()
         self.used[which] += n
@@ -85,13 +94,17 @@ class TokenAttention(nn.Module):
         """``x [N, C]`` with ``positions [N, axes]``, objects one after another at ``offsets``
         (:func:`attention.offsets`; one object without). ``cache``: takes the keys and values of
         the one sequence of a prompt, or of its next part, which also sees the keys that the
-        cache holds already (as constants, where gradients are wanted)."""
+        cache holds already (as constants, where gradients are wanted). ``key_mask``: of ``x``'s own
+        tokens; a cache keeps it for what comes after."""
         if cache is not None and (offsets is not None or len(cache.used) != 1):
             raise ValueError("a prompt fills the cache of one sequence")
         q, k, v = self.project(x, positions)
         if cache is not None:
             held, recorded = cache.used[0], torch.is_grad_enabled() and k.requires_grad
-            cache.extend(0, k, v)
+            cache.extend(0, k, v, key_mask)
+            if held and cache.mask is not None:
+                key_mask = cache.mask[0, :cache.used[0]]
+                key_mask = key_mask.clone() if recorded else key_mask
             if held and recorded:  # copies: autograd keeps them, and the cache changes with every token
                 k, v = torch.cat([cache.k[0, :held], k]), torch.cat([cache.v[0, :held], v])
             elif held:
@@ -102,8 +115,8 @@ class TokenAttention(nn.Module):
     @torch.no_grad()
     def step(self, x: torch.Tensor, positions: torch.Tensor, cache: KeyValueCache) -> torch.Tensor:
         """One new token ``x [batch, C]`` of every sequence of ``cache``, which takes its key and
-        value; each sees all keys of its sequence."""
+        value; each sees all keys of its sequence that no mask hid."""
         q, k, v = self.project(x, positions)
         cache.append(k, v)
-        y = attention.attend(q[:, None], cache.k, cache.v, lens_k=cache.lens)
+        y = attention.attend(q[:, None], cache.k, cache.v, lens_k=cache.lens, key_mask=cache.mask)
         return self.out(y.reshape(x.shape[0], self.heads * self.dim))

@@ -64,3 +64,37 @@ def test_gradients_of_a_chunk(cuda, dtype):
     want.backward(dout.double())
     assert _rms(out.double() - want) <= 8 * U[dtype] * _rms(want)
     assert _rms(leaf.grad.double() - other.grad) <= 16 * U[dtype] * _rms(other.grad)
+
+
+def _visible(block, x, positions, shown):
+    """The rows of the block in float64 where only the keys ``shown`` exist: row ``i`` is the last
+    of a causal pass over the visible tokens before it and itself."""
+    rows = []
+    for i in range(len(x)):
+        keep = shown[:i + 1].nonzero()[:, 0]
+        keep = keep if len(keep) and int(keep[-1]) == i else torch.cat([keep, torch.tensor([i], device=keep.device)])
+        rows.append(_plain(block, x[keep], positions[keep], [len(keep)], True)[0].detach()[-1])
+    return torch.stack(rows)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("chunks", [(90,), (70, 20)])
+def test_masked_prompts(cuda, chunks, dtype):
+    """Rows of visible tokens (a hidden token's own row does not see itself and is not compared)."""
+    from hi3d_amd import torso
+
+    block = _block(dtype)
+    x, positions = _tokens(97, 256, dtype)
+    shown = (torch.rand(97, generator=torch.Generator().manual_seed(2)) < 0.6).cuda()
+    shown[90:] = True
+    cache, at, rows = torso.KeyValueCache(1, 97, 2, 64, dtype), 0, []
+    with torch.no_grad():
+        for n in chunks:
+            rows.append(block(x[at:at + n], positions[at:at + n], cache=cache, key_mask=shown[at:at + n]))
+            at += n
+        for i in range(at, 97):
+            rows.append(block.step(x[i:i + 1], positions[i:i + 1], cache))
+    off, want = torch.cat(rows).double(), _visible(block, x.double(), positions, shown)
+    off = off - want
+    assert _rms(off[shown]) <= 8 * U[dtype] * _rms(want[shown])
+    assert _rms(off[90:]) <= 8 * U[dtype] * _rms(want[90:])

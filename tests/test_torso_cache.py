@@ -113,3 +113,54 @@ def test_gradients_of_a_chunk(plain):
     want, = torch.autograd.grad(whole.square().sum(), other)
     torch.testing.assert_close(out, whole, **TOL)
     torch.testing.assert_close(got, want, **TOL)
+
+
+@pytest.mark.parametrize("chunks", [(17,), (9, 8), (9, 0, 8)])
+@pytest.mark.parametrize("late", [False, True])
+def test_masked_prompts(plain, chunks, late):
+    """Keys that a prompt's mask hides stay hidden from later parts and steps; ``late``: only the
+    last part has a mask."""
+    block = _block()
+    x, positions = _tokens(22, 32)
+    mask = torch.rand(17, generator=torch.Generator().manual_seed(2)) < 0.6
+    if late:
+        mask[:17 - chunks[-1]] = True
+    shown = torch.cat([mask, torch.ones(5, dtype=torch.bool)])
+    want, cache, at, rows = block(x, positions, key_mask=shown).detach(), _cache(block), 0, []
+    with torch.no_grad():
+        for i, n in enumerate(chunks):
+            kw = {} if late and i + 1 < len(chunks) else dict(key_mask=mask[at:at + n])
+            rows.append(block(x[at:at + n], positions[at:at + n], cache=cache, **kw))
+            at += n
+        for i in range(17, 20):
+            rows.append(block.step(x[i:i + 1], positions[i:i + 1], cache))
+        rows.append(block(x[20:], positions[20:], cache=cache))
+    torch.testing.assert_close(torch.cat(rows), want, **TOL)
+
+
+def test_gradients_over_masked_keys(plain):
+    block = _block()
+    x, positions = _tokens(20, 32)
+    mask = torch.rand(20, generator=torch.Generator().manual_seed(3)) < 0.5
+    cache = _cache(block)
+    with torch.no_grad():
+        block(x[:9], positions[:9], cache=cache, key_mask=mask[:9])
+    leaf, other = (x[9:].clone().requires_grad_(True) for _ in range(2))
+    got, = torch.autograd.grad(block(leaf, positions[9:], cache=cache, key_mask=mask[9:]).square().sum(), leaf)
+    want, = torch.autograd.grad(block(torch.cat([x[:9], other]), positions, key_mask=mask)[9:].square().sum(), other)
+    torch.testing.assert_close(got, want, **TOL)
+
+
+def test_masks_of_several_sequences(plain):
+    """A mask belongs to its sequence; the others see all their keys."""
+    block = _block()
+    x, positions = _tokens(11, 32)
+    cache, mask = _cache(block, batch=2), torch.arange(10) % 3 != 1
+    with torch.no_grad():
+        _, k, v = block.project(x[:10], positions[:10])
+        cache.extend(0, k[:6], v[:6])
+        cache.extend(1, k, v, mask)
+        got = block.step(x[[6, 10]], positions[[6, 10]], cache)
+    torch.testing.assert_close(got[0], block(x[:7], positions[:7]).detach()[-1], **TOL)
+    shown = torch.cat([mask, mask.new_ones(1)])
+    torch.testing.assert_close(got[1], block(x, positions, key_mask=shown).detach()[-1], **TOL)
