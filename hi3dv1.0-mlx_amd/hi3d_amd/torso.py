@@ -25,18 +25,29 @@ class KeyValueCache:
         self.mask: torch.Tensor | None = None
         self._rows = torch.arange(batch, device=device)
 
+    def _check(self, count: int, k: torch.Tensor, v: torch.Tensor) -> None:
+        """What is refused is refused before anything is written."""
+        shape = (count, *self.k.shape[2:])
+        for name, x in (("k", k), ("v", v)):
+            if x.shape != shape or x.device != self.k.device:
+                raise ValueError(f"{name} must be {list(shape)} on {self.k.device} (got {list(x.shape)} on {x.device})")
+
     def _room(self, which: int, count: int) -> None:
+        if not 0 <= which < len(self.used):
+            raise ValueError(f"no sequence {which} of {len(self.used)}")
         if self.used[which] + count > self.k.shape[1]:
             raise ValueError(f"sequence {which} holds {self.used[which]} of {self.k.shape[1]} keys: no room for {count}")
 
     def extend(self, which: int, k: torch.Tensor, v: torch.Tensor, key_mask: torch.Tensor | None = None) -> None:
         """Adds the keys and values ``[n, heads, dim]`` of a prompt to one sequence; those where
         ``key_mask [n]`` is False are there, but not seen."""
-        n, at = int(k.shape[0]), self.used[which]
+        n = int(k.shape[0])
         self._room(which, n)
+        self._check(n, k, v)
+        at = self.used[which]
         if key_mask is not None:
-            if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.shape != (n,):
-                raise ValueError(f"key_mask must be bool [{n}]")
+            if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.shape != (n,) or key_mask.device != k.device:
+                raise ValueError(f"key_mask must be bool [{n}] on {k.device}")
             if self.mask is None:
                 self.mask = torch.ones(self.k.shape[:2], dtype=torch.bool, device=self.k.device)
             self.mask[which, at:at + n] = key_mask
@@ -47,6 +58,7 @@ class KeyValueCache:
 
     def append(self, k: torch.Tensor, v: torch.Tensor) -> None:
         """Adds one key and value ``[batch, heads, dim]`` to every sequence."""
+        self._check(len(self.used), k, v)
         for b in range(len(self.used)):
             self._room(b, 1)
         at = self.lens.long()
@@ -89,6 +101,11 @@ class TokenAttention(nn.Module):
         q, k = rotary.rotate_qk(q, k, positions, self.frequencies(x.device), layout=self.layout)
         return q, k, v
 
+    @staticmethod
+    def _check_type(cache: KeyValueCache, k: torch.Tensor) -> None:
+        if cache.k.dtype != k.dtype:
+            raise ValueError(f"the cache must be of the block's {k.dtype} (got {cache.k.dtype})")
+
     def forward(self, x: torch.Tensor, positions: torch.Tensor, offsets: torch.Tensor | None = None, *,
                 key_mask: torch.Tensor | None = None, cache: KeyValueCache | None = None) -> torch.Tensor:
         """``x [N, C]`` with ``positions [N, axes]``, objects one after another at ``offsets``
@@ -100,6 +117,7 @@ class TokenAttention(nn.Module):
             raise ValueError("a prompt fills the cache of one sequence")
         q, k, v = self.project(x, positions)
         if cache is not None:
+            self._check_type(cache, k)
             held, recorded = cache.used[0], torch.is_grad_enabled() and k.requires_grad
             cache.extend(0, k, v, key_mask)
             if held and cache.mask is not None:
@@ -117,6 +135,7 @@ class TokenAttention(nn.Module):
         """One new token ``x [batch, C]`` of every sequence of ``cache``, which takes its key and
         value; each sees all keys of its sequence that no mask hid."""
         q, k, v = self.project(x, positions)
+        self._check_type(cache, k)
         cache.append(k, v)
         y = attention.attend(q[:, None], cache.k, cache.v, lens_k=cache.lens, key_mask=cache.mask)
         return self.out(y.reshape(x.shape[0], self.heads * self.dim))

@@ -164,3 +164,61 @@ def test_masks_of_several_sequences(plain):
     torch.testing.assert_close(got[0], block(x[:7], positions[:7]).detach()[-1], **TOL)
     shown = torch.cat([mask, mask.new_ones(1)])
     torch.testing.assert_close(got[1], block(x, positions, key_mask=shown).detach()[-1], **TOL)
+
+
+def _state(cache):
+    return [x.clone() for x in (cache.k, cache.v, cache.lens)] + [list(cache.used), None if cache.mask is None else cache.mask.clone()]
+
+
+def _same(a, b):
+    return all(torch.equal(x, y) if torch.is_tensor(x) else x == y for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("masked", [False, True])
+def test_refused_keys_leave_the_cache_alone(masked):
+    from hi3d_amd import torso
+
+    cache = torso.KeyValueCache(3, 6, 2, 8, torch.float32, device="cpu")
+    if masked:
+        cache.extend(1, torch.ones(2, 2, 8), torch.ones(2, 2, 8), torch.tensor([True, False]))
+    before, ones = _state(cache), torch.ones
+    for k, v in [(ones(1, 2, 8), ones(1, 2, 8)), (ones(3, 1, 8), ones(3, 1, 8)), (ones(3, 2, 1), ones(3, 2, 1)),
+                 (ones(3, 2, 8), ones(1, 2, 8)), (ones(2, 8), ones(2, 8)),
+                 (ones(3, 2, 8, device="meta"), ones(3, 2, 8, device="meta")),
+                 (ones(3, 2, 8), ones(3, 2, 16)), (ones(4, 2, 8), ones(4, 2, 8))]:
+        with pytest.raises(ValueError, match="must be"):
+            cache.append(k, v)
+        assert _same(before, _state(cache))
+    for k, v, mask in [(ones(4, 1, 8), ones(4, 1, 8), None), (ones(4, 2, 8), ones(1, 2, 8), None),
+                       (ones(4, 2, 8), ones(4, 2, 1), None),
+                       (ones(2, 8), ones(2, 8), None), (ones(1, 4, 2, 8), ones(1, 4, 2, 8), None),
+                       (ones(4, 2, 8), ones(4, 2, 8), ones(4)), (ones(4, 2, 8), ones(4, 2, 8), ones(1, dtype=torch.bool)),
+                       (ones(4, 2, 8), ones(4, 2, 8), ones(4, dtype=torch.bool, device="meta"))]:
+        with pytest.raises(ValueError, match="must be"):
+            cache.extend(2, k, v, mask)
+        assert _same(before, _state(cache))
+    for which in (-1, 3):
+        with pytest.raises(ValueError, match="no sequence"):
+            cache.extend(which, ones(1, 2, 8), ones(1, 2, 8))
+        assert _same(before, _state(cache))
+
+
+def test_refused_tokens_leave_the_cache_alone(plain):
+    """Through the block: a token too few, a cache of another type or of other heads."""
+    from hi3d_amd import torso
+
+    block = _block()
+    x, positions = _tokens(6, 32)
+    for cache, batch in [(_cache(block, batch=3), 1), (_cache(block, batch=3), 2),
+                         (torso.KeyValueCache(2, 9, 2, 8, torch.float32, device="cpu"), 2),
+                         (torso.KeyValueCache(2, 9, 1, 8, torch.float64, device="cpu"), 2)]:
+        before = _state(cache)
+        with pytest.raises(ValueError, match="must be"):
+            block.step(x[:batch], positions[:batch], cache)
+        assert _same(before, _state(cache))
+    for cache in (torso.KeyValueCache(1, 9, 2, 8, torch.float32, device="cpu"),
+                  torso.KeyValueCache(1, 9, 1, 8, torch.float64, device="cpu")):
+        before = _state(cache)
+        with torch.no_grad(), pytest.raises(ValueError, match="must be"):
+            block(x, positions, cache=cache)
+        assert _same(before, _state(cache))
