@@ -219,7 +219,8 @@ def attend(
 
     Returns ``[..., hq, dim]`` (and with ``return_lse`` the float32 ``log(sum(exp(scores)))``
     per row and head, -inf for a row that sees no key). Differentiable once in ``q``, ``k`` and
-    ``v``, through both outputs; :func:`attend_grad` is the same without autograd."""
+    ``v`` (reverse mode), through both outputs; :func:`attend_grad` is the same without autograd."""
+    _lib.no_tangents("attention", q, k, v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = _Attend.apply(q, k, v, cu_q, cu_k, lens_k, scale, causal, key_mask)
         return (out, lse) if return_lse else out
@@ -252,6 +253,7 @@ def attend_grad(
     gradients are rounded once to the inputs' type for their products (in fp16 after a scaling
     by powers of two, so that small gradients of long rows keep their digits). Launches only:
     this is the form to capture into a graph, with no autograd node of another stream in it."""
+    _lib.no_tangents("attention", q, k, v, out, lse, dout, dlse)
     p = _Problem(q, k, v, cu_q, cu_k, lens_k, scale, causal, key_mask)
     for name, x, shape, dtype in (("out", out, q.shape, q.dtype), ("dout", dout, q.shape, q.dtype),
                                   ("lse", lse, q.shape[:-1], torch.float32), ("dlse", dlse, q.shape[:-1], torch.float32)):

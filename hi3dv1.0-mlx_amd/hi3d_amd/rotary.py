@@ -147,6 +147,7 @@ def _rotate(xs: list[torch.Tensor], positions: torch.Tensor, freqs: torch.Tensor
         raise ValueError(f"positions must be {[*lead, int(freqs.shape[0])]} (got {list(positions.shape)})")
     if not math.isfinite(scale):
         raise ValueError("scale must be finite")
+    _lib.no_tangents("rotary", *xs, freqs)
     _lib.require_gpu(*xs, positions, freqs)
     freqs = freqs.contiguous()
     if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
@@ -161,7 +162,7 @@ def rotate(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, *, lay
     of every head turned by ``positions [..., axes]`` (int32 or int64; ``[...]`` for one axis)
     and multiplied by ``scale``; the rest is copied. Pairs are ``(p, p + rot / 2)``
     (``layout="half"``) or ``(2 p, 2 p + 1)`` (``"interleaved"``). fp32 arithmetic, one
-    rounding; differentiable."""
+    rounding; differentiable (reverse mode)."""
     return _rotate([x], positions, freqs, layout, scale)[0]
 
 
