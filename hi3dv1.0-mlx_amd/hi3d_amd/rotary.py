@@ -147,6 +147,8 @@ def _rotate(xs: list[torch.Tensor], positions: torch.Tensor, freqs: torch.Tensor
         raise ValueError(f"positions must be {[*lead, int(freqs.shape[0])]} (got {list(positions.shape)})")
     if not math.isfinite(scale):
         raise ValueError("scale must be finite")
+    if freqs.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError("frequencies are constants: no gradient is formed of them (pass freqs.detach())")
     _lib.no_tangents("rotary", *xs, freqs)
     _lib.require_gpu(*xs, positions, freqs)
     freqs = freqs.contiguous()

@@ -48,3 +48,15 @@ def test_rotary_refuses_tangents():
                      lambda: rotary.rotate(x, p, forward_ad.make_dual(f, torch.ones_like(f)))):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 call()
+
+
+def test_rotary_refuses_gradients_of_frequencies():
+    """Frequencies are constants: a leaf that waits for their gradient would get none."""
+    from hi3d_amd import rotary
+
+    x, p, f = torch.randn(4, 2, 64), torch.zeros(4, 1, dtype=torch.int32), rotary.frequencies(64).requires_grad_(True)
+    for call in (lambda: rotary.rotate(x, p, f), lambda: rotary.rotate(x.requires_grad_(True), p, f)):
+        with pytest.raises(NotImplementedError, match="frequencies"):
+            call()
+    with torch.no_grad(), pytest.raises(ValueError, match="ROCm GPU only"):
+        rotary.rotate(x, p, f)
