@@ -47,10 +47,13 @@ def _heads(x: torch.Tensor) -> tuple[torch.Tensor, tuple[int, ...]]:
         bits = strides[-2] | strides[-3]
         if not (bits | strides[0]) % 8:
             return x, strides
+    if 1 in x.shape[:-1]:  # the stride of a dimension of one says nothing, and contiguous() leaves it
+        if any(s and n == 1 for s, n in zip(strides, x.shape)):
+            return _heads(x.as_strided(x.shape, [0 if n == 1 else s for s, n in zip(strides, x.shape)]))
     x = x.contiguous()
     if x.data_ptr() % 16:
         x = x.clone()
-    return x, x.stride()
+    return x, [0 if n == 1 else s for s, n in zip(x.stride(), x.shape)]
 
 
 def _offsets_of(cu: torch.Tensor, what: str) -> torch.Tensor:
