@@ -355,6 +355,7 @@ attend_short_kernel(AttnArgs a) {
   u32x4 qf[KS], qn[KS];
   load_queries(first, qn);
   const bool once = KW == 1 && s.lk <= kKT;
+  bool landed = false;  // once: the value tile has been waited for (a block that sees no key does not)
   uint64_t bits = 0;
   if (once) bits = load_keys(0);
   for (int row0 = first; row0 < last; row0 += 32) {
@@ -411,7 +412,8 @@ attend_short_kernel(AttnArgs a) {
       }
       m = to;
       const float ref = m == -INFINITY ? 0.0f : m;
-      if (!once || row0 == first) wait_vmcnt<0>();  // the value tile
+      if (!once || !landed) wait_vmcnt<0>();  // the value tile
+      landed = true;
       asm volatile("" ::: "memory");
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -474,6 +476,7 @@ attend_short_kernel(AttnArgs a) {
       }
     }
   }
+  if (once && !landed) wait_vmcnt<0>();  // no block saw a key: the wave must not leave loads to LDS behind
 }
 
 // Joins the splits of a row: a workgroup per row. Every wave weighs the parts by exp2(m -
