@@ -1,9 +1,19 @@
 // Attention over packed segments: out = softmax(scale q k^T) v, with grouped heads, a
 // causal limit aligned to the last query and key, and a mask of keys.
+#include <type_traits>
+
 #include "attention.h"
 
 namespace hi3d {
 namespace {
+
+// How far below a row's maximum its reference is kept, in powers of two. fp16 holds 2^-24 to
+// 2^16: with probabilities of up to 2^7 beside a reference at the maximum, 10^5 keys whose
+// scores lie 25 powers of two below it still count (they hold 0.3 % of the row; from a
+// reference at the maximum all of it was lost). The quotient and lse take it out again. bf16
+// has fp32's range.
+template <typename T>
+constexpr float kBelow = std::is_same_v<T, _Float16> ? 7.0f : 0.0f;
 
 // Scores of the keys that `bits` leaves out become -infinity.
 template <int QW>
@@ -26,9 +36,11 @@ __device__ __forceinline__ void hide_keys(f32x16 (&sc)[2][QW], uint64_t bits) {
 // tile. Per 64 keys a wave forms S^T = K Q^T, keeps the running reference m and sum of
 // exp2(s - m) of its rows in fp32, and adds V^T P^T to the output it holds.
 //
-// m only moves when some row's maximum has grown by more than 2^8 over it (the first tile
-// included): any reference gives the same quotient, and between moves the probabilities
-// stay below 2^8, well inside fp16's and fp32's range, so the output is rescaled rarely.
+// m is kBelow under the row's maximum and only moves when that has grown by more than 2^8 (the
+// first tile included): any reference gives the same quotient, and between moves the
+// probabilities stay below 2^15, inside fp16's and fp32's range, so the output is rescaled
+// rarely. In fp16 a tile's probabilities are summed before they join the row's sum, which
+// would round away keys 24 powers of two below the first one by one.
 //
 // Bound by the two waves of a SIMD sharing its matrix and vector units: per 64 keys and 32
 // rows 32 * DP / 128 matrix instructions of 32 cycles, and about 140 vector operations for
@@ -192,7 +204,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 && NW * QW == 4 ? 3 : 2) void att
         float x = larger(sc[0][b][0], sc[1][b][0]);
 #pragma unroll
         for (int e = 1; e < 16; ++e) x = larger(larger(x, sc[0][b][e]), sc[1][b][e]);
-        top[b] = half_max(x) * a.scale2;
+        top[b] = half_max(x) * a.scale2 - kBelow<T>;
         grow = grow || top[b] > m[b] + 8.0f;
       }
       if (__any(grow)) {
@@ -209,13 +221,16 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 && NW * QW == 4 ? 3 : 2) void att
 #pragma unroll
       for (int b = 0; b < QW; ++b) {
         const float ref = m[b] == -INFINITY ? 0.0f : m[b];
+        constexpr bool APART = kBelow<T> > 0;  // bf16's own rounding is far coarser than the sum's
+        float sum = APART ? 0.0f : l[b];
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             sc[n][b][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][b][e], a.scale2, -ref));
-            l[b] += sc[n][b][e];
+            sum += sc[n][b][e];
           }
+        l[b] = APART ? l[b] + sum : sum;
       }
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
@@ -403,7 +418,7 @@ attend_short_kernel(AttnArgs a) {
 #pragma unroll
         for (int e = 8 * (k & 1); e < 8 * (k & 1) + 8; ++e) top = larger(top, sc[k >> 1][e]);
       }
-      const float to = fmaxf(m, half_max(top) * a.scale2);
+      const float to = fmaxf(m, half_max(top) * a.scale2 - kBelow<T>);
       if (k0 > start) {
         const float by = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - to);
         l *= by;

@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -34,3 +36,30 @@ def _segments(lq, lk, hq, hk, d, dtype, seed=0, causal=False, mask=None, grads=T
     ([100, 33] * 20, [64, 1] * 20)])
 def test_short_segments_whose_first_rows_see_no_key(cuda, lq, lk, d, dtype):
     _segments(lq, lk, 3, 3, d, dtype, causal=True, grads=False)
+
+
+@pytest.mark.parametrize("bits", [24.6, 25.25, 26.0])
+@pytest.mark.parametrize("nq,nk,heads,d", [
+    (8192, 100_000, 8, 64),  # 256 rows to a workgroup
+    (8192, 100_000, 8, 128),  # 128 rows
+    (1, 100_000, 2, 64),  # split over the keys
+    (20, 2000, 2, 64),  # eight waves on a block
+    (20, 100, 2, 64)])  # a wave on its own
+def test_many_keys_far_below_the_first(cuda, nq, nk, heads, d, bits):
+    """A key of score s, value 0, before many keys of score 0, value 1: out = n / (e^s + n). In
+    fp16 a probability is off by 2^-11 of itself or, below the normal range, by 2^-25 where the
+    row's largest is 2^7 or more: 2^-32 of the row's sum a key."""
+    from hi3d_amd import attention
+
+    dtype, scale, n = torch.float16, 0.125, nk - 1
+    first = float(torch.tensor(bits * 0.6931471805599453).half())  # the score, exact in fp16
+    q = torch.zeros(nq, heads, d, dtype=dtype, device="cuda")
+    k, v = (torch.zeros(nk, heads, d, dtype=dtype, device="cuda") for _ in range(2))
+    q[..., 3], k[0, :, 3], v[1:] = 8.0, first, 1.0
+    out, lse = attention.attend(q, k, v, scale=scale, return_lse=True)
+    total = math.exp(first) + n
+    want = n / total
+    pe = 2 * (d + 4) * 2.0 ** -24 * first + (16 + nk) * 2.0 ** -24
+    room = (2.0 ** -11 + pe) * want + 2.0 ** -32 * n + 2.0 ** -11 * want + 2.0 ** -24
+    assert float((out.double() - want).abs().max()) <= room
+    assert float((lse.double() - math.log(total)).abs().max()) <= pe + 4 * 2.0 ** -24 * first + 8 * 2.0 ** -24
