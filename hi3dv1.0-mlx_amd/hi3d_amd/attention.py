@@ -222,7 +222,8 @@ def attend(
 
     Returns ``[..., hq, dim]`` (and with ``return_lse`` the float32 ``log(sum(exp(scores)))``
     per row and head, -inf for a row that sees no key). Differentiable once in ``q``, ``k`` and
-    ``v`` (reverse mode), through both outputs; :func:`attend_grad` is the same without autograd."""
+    ``v`` (reverse mode), through both outputs; :func:`attend_grad` is the same without autograd
+    (and says for which values fp16 gradients are formed)."""
     _lib.no_tangents("attention", q, k, v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = _Attend.apply(q, k, v, cu_q, cu_k, lens_k, scale, causal, key_mask)
@@ -254,7 +255,9 @@ def attend_grad(
 
     Sums run in a fixed order: the same bits every time. fp32 sums; probabilities and score
     gradients are rounded once to the inputs' type for their products (in fp16 after a scaling
-    by powers of two, so that small gradients of long rows keep their digits). Launches only:
+    by powers of two, so that small gradients of long rows keep their digits; with values of 8190
+    and more that scaling can leave fp16's range, and the gradients of such a row are not finite
+    then: take bf16 there). Launches only:
     this is the form to capture into a graph, with no autograd node of another stream in it."""
     _lib.no_tangents("attention", q, k, v, out, lse, dout, dlse)
     p = _Problem(q, k, v, cu_q, cu_k, lens_k, scale, causal, key_mask)

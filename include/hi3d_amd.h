@@ -676,8 +676,9 @@ int hi3d_attention_backward_workspace(const hi3d_attention_desc* desc_host, int6
  * out_dev and lse_dev, the gradient dout_dev [total_q, heads_q, dim] of out and optionally
  * that of lse, dlse_dev fp32 [total_q, heads_q]. Probabilities are formed again from lse;
  * they and the scores' gradients are rounded once to the inputs' type for their products,
- * everything is summed in fp32 in a fixed order. Hidden keys and keys past those in use get
- * zeros. The query heads of one key head must lie within 2^29 elements. */
+ * everything is summed in fp32 in a fixed order. F16 takes |v| < 8190: from there on a score's
+ * gradient can pass the type's range and become infinite. Hidden keys and keys past those in
+ * use get zeros. The query heads of one key head must lie within 2^29 elements. */
 int hi3d_attention_backward(const hi3d_attention_desc* desc_host, const void* out_dev, const float* lse_dev,
                             const void* dout_dev, const float* dlse_dev, void* dq_dev, void* dk_dev, void* dv_dev,
                             void* workspace_dev, int64_t workspace_bytes, void* stream);

@@ -63,3 +63,21 @@ def test_many_keys_far_below_the_first(cuda, nq, nk, heads, d, bits):
     room = (2.0 ** -11 + pe) * want + 2.0 ** -32 * n + 2.0 ** -11 * want + 2.0 ** -24
     assert float((out.double() - want).abs().max()) <= room
     assert float((lse.double() - math.log(total)).abs().max()) <= pe + 4 * 2.0 ** -24 * first + 8 * 2.0 ** -24
+
+
+def test_fp16_gradients_of_the_largest_values(cuda):
+    """The range that fp16 gradients are formed in: values of up to 8189, output gradients all of
+    one sign, two keys of probability 1/2 and opposite values, where |ds| is largest: by the
+    formulas p (1 - p) 2 sum |dout| max |v|."""
+    from hi3d_amd import attention
+
+    for gain in (2.0 ** -10, 1.0, 1.999):  # sum |dout| at both ends of a power of two
+        q = torch.randn(40, 1, 64, generator=torch.Generator().manual_seed(0)).half().cuda()
+        k, v = torch.zeros(2, 1, 64, dtype=torch.float16, device="cuda"), torch.empty(2, 1, 64, dtype=torch.float16, device="cuda")
+        k[0, 0, 0], k[1, 0, 0] = 2.0 ** -10, -2.0 ** -10
+        v[0], v[1] = 8188.0, -8188.0
+        dout = torch.full((40, 1, 64), gain / 64 * 2.0 ** -8, dtype=torch.float16, device="cuda")
+        grads = _grads(q, k, v, dout)
+        assert all(bool(x.isfinite().all()) for x in grads)
+        _check(grads, q, k, v, dout, [0, 40], [0, 2])
+        assert attention.attend(q, k, v).isfinite().all()
