@@ -157,7 +157,7 @@ __device__ __forceinline__ float half_sum(float x) {
 
 struct Segment {
   int b, tile;          // segment and the workgroup's tile of it
-  int lq, lk;
+  int lq, lk, room;     // queries, keys in use, keys there are
   int64_t q0, k0;       // first row of the segment among all queries / keys
 };
 
@@ -166,32 +166,41 @@ __device__ __forceinline__ int clamp_offset(int v, int64_t total) {
 }
 
 // Lengths and first rows of segment b. Offsets are clamped to the rows there are, so no
-// offset can lead outside the tensors.
+// offset can lead outside the tensors. Rows outside the offsets are segments too, -1 in front
+// and `batch` behind, whose keys are not in use: their outputs and gradients are zeros.
 __device__ __forceinline__ void segment_rows(const AttnArgs& a, Segment& s) {
+  const bool front = s.b < 0, back = s.b >= a.batch;
+  const int from = front ? 0 : s.b, to = back ? a.batch : s.b + 1;
   if (a.cu_q != nullptr) {
-    const int q0 = clamp_offset(a.cu_q[s.b], a.total_q), q1 = clamp_offset(a.cu_q[s.b + 1], a.total_q);
+    const int q0 = front ? 0 : clamp_offset(a.cu_q[from], a.total_q);
+    const int q1 = back ? static_cast<int>(a.total_q) : clamp_offset(a.cu_q[to], a.total_q);
     s.q0 = q0, s.lq = q1 > q0 ? q1 - q0 : 0;
   } else {
     s.q0 = static_cast<int64_t>(s.b) * a.len_q, s.lq = a.len_q;
   }
   if (a.cu_k != nullptr) {
-    const int k0 = clamp_offset(a.cu_k[s.b], a.total_k), k1 = clamp_offset(a.cu_k[s.b + 1], a.total_k);
-    s.k0 = k0, s.lk = k1 > k0 ? k1 - k0 : 0;
+    const int k0 = front ? 0 : clamp_offset(a.cu_k[from], a.total_k);
+    const int k1 = back ? static_cast<int>(a.total_k) : clamp_offset(a.cu_k[to], a.total_k);
+    s.k0 = k0, s.room = k1 > k0 ? k1 - k0 : 0, s.lk = front || back ? 0 : s.room;
   } else {
-    s.k0 = static_cast<int64_t>(s.b) * a.len_k, s.lk = a.len_k;
-    if (a.lens_k != nullptr) {
+    s.k0 = static_cast<int64_t>(s.b) * a.len_k, s.room = a.len_k, s.lk = front || back ? 0 : a.len_k;
+    if (a.lens_k != nullptr && s.lk > 0) {
       const int n = a.lens_k[s.b];
       s.lk = n < 0 ? 0 : (n < s.lk ? n : s.lk);
     }
   }
 }
 
-// Which segment and tile slot `slot` is. Segment b owns the slots from
-// floor(cu[b] * rows / T) + b to that of b + 1: at least ceil(length * rows / T) of them and
-// at most one more, so the launch needs only the total, and nothing is built beforehand.
-// The segment is found by 64-way search, first around the place an even split gives.
-// FIRST: every segment's first tile has a slot of its own, slot b, which needs no search; the
-// others follow from `batch` on, segment b's from floor(cu[b] * rows / T).
+// Slots of a launch over packed rows: see find_segment.
+inline int64_t packed_slots(int64_t total, int64_t rows, int tile, int batch) { return total * rows / tile + batch + 2; }
+
+// Which segment and tile slot `slot` is. Segment b, from -1 (the rows in front of the offsets)
+// to batch (those behind), owns the slots from floor(cu[b] * rows / T) + b + 1 to those of b + 1
+// (cu[-1] = 0): at least ceil(length * rows / T) of them and at most one more, so the launch
+// needs only the total, and nothing is built beforehand. The segment is found by 64-way search,
+// first around the place an even split gives.
+// FIRST: every segment's first tile has a slot of its own, slot b + 1, which needs no search; the
+// others follow from batch + 2 on, segment b's from floor(cu[b] * rows / T).
 template <bool FIRST = false>
 __device__ __forceinline__ void find_segment(const int32_t* cu, int len, int batch, int64_t total, int rows, int tile,
                                              int slot, Segment& s) {
@@ -201,19 +210,19 @@ __device__ __forceinline__ void find_segment(const int32_t* cu, int len, int bat
     return;
   }
   if constexpr (FIRST) {
-    if (slot < batch) {
-      s.b = slot, s.tile = 0;
+    if (slot < batch + 2) {
+      s.b = slot - 1, s.tile = 0;
       return;
     }
-    slot -= batch;
+    slot -= batch + 2;
   }
   const int lane = threadIdx.x & 63;
   auto first = [&](int b) {
-    return static_cast<int>(static_cast<int64_t>(clamp_offset(cu[b], total)) * rows / tile) + (FIRST ? 0 : b);
+    return static_cast<int>(static_cast<int64_t>(clamp_offset(cu[b], total)) * rows / tile) + (FIRST ? 0 : b + 1);
   };
-  int lo = 0, hi = batch;  // first(lo) <= slot < first(hi), hi exclusive of the answer
+  int lo = 0, hi = batch + 1;  // lo is 0 or first(lo) <= slot; the answer is below hi
   if (batch > 64) {
-    const int64_t all = total * rows / tile + (FIRST ? 0 : batch);
+    const int64_t all = total * rows / tile + (FIRST ? 0 : batch + 2);
     int at = static_cast<int>(static_cast<int64_t>(slot) * batch / (all > 0 ? all : 1)) - 32;
     at = at < 0 ? 0 : (at > batch - 64 ? batch - 64 : at);
     const uint64_t le = __ballot(first(at + lane) <= slot);
@@ -224,12 +233,13 @@ __device__ __forceinline__ void find_segment(const int32_t* cu, int len, int bat
   while (hi - lo > 1) {
     const int step = (hi - lo + 63) / 64;
     const int at = lo + lane * step;
-    const uint64_t le = __ballot(at < hi && first(at < hi ? at : lo) <= slot);  // bit 0 is always set
+    const uint64_t le = __ballot(at < hi && first(at < hi ? at : lo) <= slot);  // bit 0 is set unless lo is 0
     lo += (63 - __builtin_clzll(le | 1)) * step;
     hi = lo + step < hi ? lo + step : hi;
   }
   s.b = __builtin_amdgcn_readfirstlane(lo);
   s.tile = slot - first(s.b) + (FIRST ? 1 : 0);
+  if (s.tile < (FIRST ? 1 : 0)) s.b = -1, s.tile = slot + (FIRST ? 1 : 0);  // in front of all offsets
 }
 
 __device__ __forceinline__ void split_row(const AttnArgs& a, int r, int& i, int& g) {

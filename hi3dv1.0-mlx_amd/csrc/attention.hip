@@ -552,7 +552,7 @@ template <typename T, int DP, int NW, int QW>
 int launch_attend(AttnArgs a, hipStream_t stream) {
   constexpr int rows = NW * QW * 32;
   const bool z = a.mask != nullptr || a.dim < DP;
-  const int64_t per = a.cu_q != nullptr ? a.total_q * a.group / rows + a.batch
+  const int64_t per = a.cu_q != nullptr ? packed_slots(a.total_q, a.group, rows, a.batch)
                                         : ceil_div(static_cast<int64_t>(a.len_q) * a.group, rows) * a.batch;
   const int64_t blocks = per * a.hk * a.splits;
   HI3D_REQUIRE(blocks < (1ll << 31), "too many rows for one launch");
@@ -575,7 +575,7 @@ int launch_short(AttnArgs a, hipStream_t stream) {
   constexpr int rows = KW == 1 ? kShortSpan : 32;
   constexpr int part = DP * 132 > kTile<DP> ? DP * 132 : kTile<DP>;  // a wave's tile, or its 32 rows of the output
   constexpr size_t lds = KW == 1 ? 4 * kTile<DP> : KW * (part + 256);
-  const int64_t per = a.cu_q != nullptr ? a.total_q * a.group / rows + a.batch
+  const int64_t per = a.cu_q != nullptr ? packed_slots(a.total_q, a.group, rows, a.batch)
                                         : ceil_div(static_cast<int64_t>(a.len_q) * a.group, rows) * a.batch;
   HI3D_REQUIRE(per * a.hk < (1ll << 31), "too many rows for one launch");
   a.slots = static_cast<int>(per);

@@ -358,12 +358,11 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
   Segment s;
   find_segment(a.cu_k, a.len_k, a.batch, a.total_k, 1, KEYS, slot, s);
   segment_rows(a, s);
-  const int room = a.cu_k != nullptr ? s.lk : a.len_k;  // keys past those in use get zeros
   const int key0 = s.tile * KEYS;
-  if (s.tile < 0 || key0 >= room) return;
+  if (s.tile < 0 || key0 >= s.room) return;  // keys past those in use get zeros
 
   const int wkey = key0 + wave * (QW * 32);
-  const int off = s.lk - s.lq, rows = s.lq * a.group;
+  const int off = s.lk - s.lq, rows = s.lk > 0 ? s.lq * a.group : 0;
   u32x4 kf[QW][KS], vf[QW][KS];
   bool on[QW];
 #pragma unroll
@@ -418,7 +417,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
   float by = 1.0f, dk_by = a.scale, dv_by = 1.0f;
   if constexpr (std::is_same_v<T, _Float16>) {
     const int64_t slot0 = a.cu_q != nullptr
-                              ? static_cast<int64_t>(clamp_offset(a.cu_q[s.b], a.total_q)) * a.group / a.dq_rows + s.b
+                              ? s.q0 * a.group / a.dq_rows + s.b + 1
                               : s.b * ((static_cast<int64_t>(a.len_q) * a.group + a.dq_rows - 1) / a.dq_rows);
     const float* bounds = a.bound + (static_cast<int64_t>(head) * a.dq_slots + slot0) * a.dq_waves;
     const int count = (rows + a.dq_rows - 1) / a.dq_rows * a.dq_waves;
@@ -514,7 +513,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
 #pragma unroll
   for (int b = 0; b < QW; ++b) {
     const int j = wkey + b * 32 + c32;
-    if (j >= room) continue;
+    if (j >= s.room) continue;
     const int64_t at = ((s.k0 + j) * a.hk + head) * a.dim;
     if constexpr (SPLIT) {
       const int64_t all = a.total_k * a.hk * a.dim;
@@ -556,7 +555,7 @@ template <typename T, int DP, int NW, int QW>
 int launch_dkv(AttnArgs a, hipStream_t stream) {
   constexpr int keys = NW * QW * 32, threads = 64 * NW;
   constexpr size_t lds = 4 * kTile<DP> + 1024;
-  const int64_t per = a.cu_k != nullptr ? a.total_k / keys + a.batch : ceil_div(a.len_k, keys) * a.batch;
+  const int64_t per = a.cu_k != nullptr ? packed_slots(a.total_k, 1, keys, a.batch) : ceil_div(a.len_k, keys) * a.batch;
   const int64_t blocks = per * a.hk * a.splits;
   HI3D_REQUIRE(blocks < (1ll << 31), "too many rows for one launch");
   a.slots = static_cast<int>(per);
@@ -614,7 +613,7 @@ int dkv_splits(const AttnArgs& a, int cus) {
 void dq_tiles(AttnArgs& a) {
   a.dq_waves = ceil_div(a.total_q * a.group, a.batch) <= 32 ? 1 : 4;
   a.dq_rows = 32 * a.dq_waves;
-  a.dq_slots = static_cast<int>(a.cu_q != nullptr ? a.total_q * a.group / a.dq_rows + a.batch
+  a.dq_slots = static_cast<int>(a.cu_q != nullptr ? packed_slots(a.total_q, a.group, a.dq_rows, a.batch)
                                                   : ceil_div(static_cast<int64_t>(a.len_q) * a.group, a.dq_rows) * a.batch);
 }
 

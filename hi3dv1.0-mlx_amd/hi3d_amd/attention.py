@@ -212,9 +212,10 @@ def attend(
     """``softmax(scale * q k^T) v`` within each segment, ``scale`` = ``dim ** -0.5`` by default.
 
     ``q [Nq, hq, dim]``, ``k`` and ``v [Nk, hk, dim]`` with offsets ``cu_q`` / ``cu_k`` (int32,
-    ascending from 0 to ``Nq`` / ``Nk``; ``cu_k`` = ``cu_q`` by default; one segment without
-    offsets), or ``[B, L, heads, dim]``, where ``lens_k [B]`` says how many keys of each are in
-    use (a cache). Query head ``h`` reads key head ``h // (hq // hk)``. ``causal``: query ``i``
+    ascending, within ``Nq`` / ``Nk``; ``cu_k`` = ``cu_q`` by default; one segment without
+    offsets; rows before the first offset and from the last one on give zeros and take no
+    part), or ``[B, L, heads, dim]``, where ``lens_k [B]`` says how many keys of each are in use
+    (a cache). Query head ``h`` reads key head ``h // (hq // hk)``. ``causal``: query ``i``
     of ``lq`` sees the keys ``j <= i + lk - lq`` (a later key whose value is not finite can still
     reach it: such keys belong in ``key_mask``). ``key_mask`` (bool, one per key): False keys
     are not seen, whatever they hold. A row that sees no key gives zeros. Views with other

@@ -629,8 +629,9 @@ int hi3d_rotary(const void* const x_dev[2], void* const y_dev[2], const int32_t 
 /* One attention problem: `batch` segments, each with its own queries and keys.
  * Element (segment b, row i, head h, d) of q lies at b * strides[0] + i * strides[1] +
  * h * strides[2] + d, of k at strides[3..5], of v at strides[6..8]. With offsets cu_q / cu_k
- * (int32 [batch + 1], ascending from 0 to the row count) the rows of all segments follow one
- * another, row cu[b] + i, and the segment stride is not used; without, every segment has
+ * (int32 [batch + 1], ascending) the rows of all segments follow one another, row cu[b] + i,
+ * and the segment stride is not used; rows before the first offset and from the last one on
+ * belong to no segment: their outputs and gradients are zeros. Without, every segment has
  * len_q / len_k rows, of which lens_k (int32 [batch], optional) keys are in use.
  * heads_q is a multiple of heads_k; query head h reads key head h / (heads_q / heads_k).
  * causal: query i sees keys j <= i + lk - lq. key_mask (uint8, one per key row; optional):
