@@ -81,3 +81,97 @@ def test_fp16_gradients_of_the_largest_values(cuda):
         assert all(bool(x.isfinite().all()) for x in grads)
         _check(grads, q, k, v, dout, [0, 40], [0, 2])
         assert attention.attend(q, k, v).isfinite().all()
+
+
+ROWS_33_TO_64 = [
+    ([40, 64, 33, 0, 50] * 30, [200, 129, 300, 150, 140] * 30),  # 64 rows to a wave, keys whole
+    ([50, 64, 35], [9001, 12000, 8500]),  # and split
+]
+ROWS_TO_32 = [
+    ([20, 32, 1, 0, 9] * 60, [200, 129, 300, 150, 140] * 60),
+    ([1, 32, 5], [9001, 12000, 8500]),
+]
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("d", [32, 64, 88, 96, 128])
+@pytest.mark.parametrize("case", range(4))
+def test_one_wave_over_many_keys(cuda, case, d, masked, causal):
+    lq, lk = (ROWS_33_TO_64 + ROWS_TO_32)[case]
+    mask = (torch.rand(sum(lk), generator=torch.Generator().manual_seed(case)) < 0.7).cuda() if masked else None
+    _segments(lq, lk, 2, 2, d, DTYPES[d % 3 == 0], seed=case, causal=causal, mask=mask, grads=False)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_many_heads_on_one_key_head_over_a_cache(cuda, d):
+    """64 query heads of one token, and 16 tokens of 4 heads: 64 packed rows over long caches."""
+    _segments([1, 1], [9000, 300], 64, 1, d, torch.bfloat16, grads=False)
+    _segments([16, 9], [9000, 8000], 8, 2, d, torch.float16, causal=True, grads=False)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("lq,lk", [
+    ([2] * 200 + [3000], None), ([3000] + [0] * 90 + [1] * 150, None), ([5] * 100 + [400], [100] * 100 + [2500]),
+    ([30] * 50 + [1], [3] * 50 + [4000])])
+def test_segments_far_from_their_average(cuda, lq, lk, causal):
+    """The rules go by the average; a segment many times longer is right all the same."""
+    _segments(lq, lq if lk is None else lk, 2, 1, 64, torch.float16, causal=causal)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal,masked", [(True, False), (False, True), (True, True)])
+@pytest.mark.parametrize("nq,cache,hq,hk,d,lens", [
+    (9, 150, 4, 2, 64, [150, 0, 1, 77]), (70, 300, 3, 3, 88, [300, 69, 71, 0]), (1, 5000, 8, 2, 128, [5000, 17, 0, 4999]),
+    (130, 2000, 2, 1, 32, [2000, 1, 130, 1999]), (50, 9000, 2, 2, 96, [9000, 40, 8999, 64])])
+def test_several_rows_over_caches(cuda, nq, cache, hq, hk, d, lens, causal, masked, dtype):
+    """Rows end at the last key in use; what lies past those, or is hidden, may hold anything."""
+    from hi3d_amd import attention
+
+    batch = len(lens)
+    q, k, v = _tensors(batch * nq, batch * cache, hq, hk, d, dtype)
+    dout = _tensors(batch * nq, 1, hq, 1, d, dtype, seed=1)[0]
+    used = torch.cat([torch.arange(cache) < n for n in lens]).cuda()
+    shown = (torch.rand(batch * cache, generator=torch.Generator().manual_seed(2)) < 0.6).cuda() if masked else None
+    kk, vv, mask = k[used], v[used], None if shown is None else shown[used]
+    hidden = ~used if shown is None else ~used | ~shown
+    k[hidden], v[hidden] = float("nan"), float("inf")
+    room = lambda x, n: x.reshape(batch, n, *x.shape[1:])  # noqa: E731
+    kw = dict(lens_k=torch.tensor(lens, dtype=torch.int32).cuda(), causal=causal,
+              key_mask=None if shown is None else room(shown, cache))
+    out, lse = attention.attend(room(q, nq), room(k, cache), room(v, cache), return_lse=True, **kw)
+    cu_q, cu_k = _cu([nq] * batch), _cu(lens)
+    _check_forward(out.flatten(0, 1), lse.flatten(0, 1), q, kk, vv, cu_q, cu_k, causal=causal, mask=mask)
+    dq, dk, dv = attention.attend_grad(room(q, nq), room(k, cache), room(v, cache), out, lse, room(dout, nq), **kw)
+    dk, dv = dk.flatten(0, 1), dv.flatten(0, 1)
+    assert not dk[hidden].any() and not dv[hidden].any()
+    _check((dq.flatten(0, 1), dk[used], dv[used]), q, kk, vv, dout, cu_q, cu_k, causal=causal, mask=mask)
+
+
+@pytest.mark.parametrize("d,masked", [(88, False), (88, True), (128, True), (40, False)])
+def test_streamed_caches_with_masks_and_narrow_heads(cuda, d, masked):
+    """Caches past 256 MB whose heads do not fill their rows, or whose mask hides single keys and
+    whole tiles."""
+    from hi3d_amd import attention
+
+    batch, hq, hk = 5, 8, 4
+    room = -(-(280 << 20) // (4 * batch * hk * d))
+    g = torch.Generator(device="cuda").manual_seed(0)
+    k, v = (torch.randn((batch, room, hk, d), generator=g, device="cuda").half() for _ in range(2))
+    q = torch.randn((batch, 1, hq, d), generator=g, device="cuda").half()
+    lens = torch.tensor([room, 17, 0, room - 12, room // 3], dtype=torch.int32, device="cuda")
+    mask = torch.rand((batch, room), generator=g, device="cuda") < 0.7
+    mask[0, 64 * 20:64 * 90], mask[3, :room // 2], mask[1, :17] = False, False, False
+    mask = mask if masked else torch.ones_like(mask)
+    k[~mask], v[~mask] = float("nan"), float("nan")
+    out = attention.attend(q, k, v, lens_k=lens, key_mask=mask if masked else None)
+    assert k.numel() * 4 > 256 << 20
+    for b, n in enumerate(lens.tolist()):
+        on = mask[b, :n]
+        kk, vv = (x[b, :n][on].double().repeat_interleave(hq // hk, 1).transpose(0, 1) for x in (k, v))
+        s = (kk * q[b, 0].double()[:, None]).sum(-1) * d ** -0.5
+        p = torch.softmax(s, -1) if int(on.sum()) else s
+        want, size = (p[..., None] * vv).sum(1), (p[..., None] * vv.abs()).sum(1)
+        # p and the output rounded to half a step each; fp32 sums of up to 400,000 terms in parts: 2^-14
+        room_ = 2.0 ** -11 * (size + want.abs()) + 2.0 ** -14 * size + 2.0 ** -24
+        assert bool(((out[b, 0].double() - want).abs() <= room_).all())
