@@ -561,13 +561,17 @@ int launch_attend(AttnArgs a, hipStream_t stream) {
   if (a.splits == 1)
     return z ? launch_tiles<&attend_kernel<T, DP, NW, QW, true, false>>(a, blocks, 64 * NW, lds, stream)
              : launch_tiles<&attend_kernel<T, DP, NW, QW, false, false>>(a, blocks, 64 * NW, lds, stream);
-  const int rc = z ? launch_tiles<&attend_kernel<T, DP, NW, QW, true, true>>(a, blocks, 64 * NW, lds, stream)
-                   : launch_tiles<&attend_kernel<T, DP, NW, QW, false, true>>(a, blocks, 64 * NW, lds, stream);
-  if (rc != HI3D_OK) return rc;
-  const int64_t n = a.total_q * a.hq;
-  hipLaunchKernelGGL(attend_join_kernel<T>, dim3(static_cast<unsigned>(n)), dim3(256), 0, stream, a, n);
-  HI3D_LAUNCH_CHECK();
-  return HI3D_OK;
+  if constexpr (NW * QW == 8) {  // rows that fill the chip four times over are not split
+    return fail(HI3D_ERR_INVALID, "256 rows to a workgroup are not split");
+  } else {
+    const int rc = z ? launch_tiles<&attend_kernel<T, DP, NW, QW, true, true>>(a, blocks, 64 * NW, lds, stream)
+                     : launch_tiles<&attend_kernel<T, DP, NW, QW, false, true>>(a, blocks, 64 * NW, lds, stream);
+    if (rc != HI3D_OK) return rc;
+    const int64_t n = a.total_q * a.hq;
+    hipLaunchKernelGGL(attend_join_kernel<T>, dim3(static_cast<unsigned>(n)), dim3(256), 0, stream, a, n);
+    HI3D_LAUNCH_CHECK();
+    return HI3D_OK;
+  }
 }
 
 template <typename T, int DP, int KW>

@@ -75,7 +75,7 @@ __device__ __forceinline__ float wave_max(float x) {
 // down to 1.42 (sqrt 2); above that many keys the miss is below a tenth of ds's rounding.
 constexpr int kExactTiles = 4;
 
-// dq and D. A workgroup owns NW * QW * 32 packed query rows of one key head (queries and
+// dq and D. A workgroup owns NW * 32 packed query rows of one key head (queries and
 // dout in registers) and walks the keys in tiles of 64 held twice in LDS, as the forward
 // does. Per 32 keys a wave forms S^T = K Q^T and dP^T = V dO^T, then dq += K^T dS^T with
 // the same K tile read transposed.
@@ -85,9 +85,9 @@ constexpr int kExactTiles = 4;
 // and vector operations, which 2 or 3 waves a SIMD overlap in part: 8,191 rows x 33 heads x 64
 // fp16 in four segments 262 us (810 TFLOP/s of its 3 products), 8,192 causal x 32/8 heads x 128
 // bf16 412 us (1000).
-template <typename T, int DP, int NW, int QW, bool Z>
+template <typename T, int DP, int NW, bool Z>
 __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
-  constexpr int ROWS = NW * QW * 32, KS = DP / 16, DB = DP / 32, PAIR = 2 * kTile<DP>;
+  constexpr int ROWS = NW * 32, KS = DP / 16, DB = DP / 32, PAIR = 2 * kTile<DP>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c32 = lane & 31, h = lane >> 5;
@@ -102,72 +102,57 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
   find_segment(a.cu_q, a.len_q, a.batch, a.total_q, a.group, ROWS, slot, s);
   segment_rows(a, s);
   const int rows = s.lq * a.group, row0 = s.tile * ROWS;
-  const int wrow = row0 + wave * (QW * 32);
+  const int wrow = row0 + wave * 32;
   float* bound = a.bound + (static_cast<int64_t>(head) * a.slots + slot) * NW + wave;
   if (s.tile < 0 || row0 >= rows) return;
 
   const int off = s.lk - s.lq;
-  // place of this lane's row of block b among [total_q, hq]
-  auto row_at = [&](int b) -> int64_t {
+  // place of this lane's row among [total_q, hq]
+  auto row_at = [&]() -> int64_t {
     int i, g;
-    split_row(a, min(wrow + b * 32 + (fresh_lane() & 31), rows - 1), i, g);
+    split_row(a, min(wrow + (fresh_lane() & 31), rows - 1), i, g);
     return (s.q0 + i) * a.hq + head * a.group + g;
   };
-  u32x4 qf[QW][KS], df[QW][KS];
-  bool none[QW];
-  float ref[QW], delta[QW], size[QW];  // log2 of the scaled p's divisor, D, sum |dout|
+  u32x4 qf[KS], df[KS];
+  int qi, qg;
+  split_row(a, min(wrow + c32, rows - 1), qi, qg);
+  const int64_t at = (s.q0 + qi) * a.hq + head * a.group + qg;
+  const T* src = static_cast<const T*>(a.q) + s.b * a.q_b + (a.cu_q != nullptr ? s.q0 + qi : qi) * a.q_n +
+                 static_cast<int64_t>(head * a.group + qg) * a.q_h;
+  load_owned<DP>(reinterpret_cast<const char*>(src), a.dim, h, true, qf);
+  load_owned<DP>(reinterpret_cast<const char*>(static_cast<const T*>(a.dout) + at * a.dim), a.dim, h, true, df);
+  u32x4 of[KS];
+  load_owned<DP>(reinterpret_cast<const char*>(static_cast<const T*>(a.o) + at * a.dim), a.dim, h, true, of);
+  float x = 0.0f, y = 0.0f;
 #pragma unroll
-  for (int b = 0; b < QW; ++b) {
-    const int r = wrow + b * 32 + c32;
-    int i, g;
-    split_row(a, r < rows ? r : rows - 1, i, g);
-    const int64_t at = (s.q0 + i) * a.hq + head * a.group + g;
-    const T* src = static_cast<const T*>(a.q) + s.b * a.q_b + (a.cu_q != nullptr ? s.q0 + i : i) * a.q_n +
-                   static_cast<int64_t>(head * a.group + g) * a.q_h;
-    load_owned<DP>(reinterpret_cast<const char*>(src), a.dim, h, true, qf[b]);
-    load_owned<DP>(reinterpret_cast<const char*>(static_cast<const T*>(a.dout) + at * a.dim), a.dim, h, true, df[b]);
-    u32x4 of[KS];
-    load_owned<DP>(reinterpret_cast<const char*>(static_cast<const T*>(a.o) + at * a.dim), a.dim, h, true, of);
-    float x = 0.0f, y = 0.0f;
+  for (int k = 0; k < KS; ++k) {
+    const auto u = __builtin_bit_cast(typename Vec8<T>::type, df[k]), v = __builtin_bit_cast(typename Vec8<T>::type, of[k]);
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      const auto u = __builtin_bit_cast(typename Vec8<T>::type, df[b][k]), v = __builtin_bit_cast(typename Vec8<T>::type, of[k]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x = __builtin_fmaf(static_cast<float>(u[e]), static_cast<float>(v[e]), x);
-        y += __builtin_fabsf(static_cast<float>(u[e]));
-      }
+    for (int e = 0; e < 8; ++e) {
+      x = __builtin_fmaf(static_cast<float>(u[e]), static_cast<float>(v[e]), x);
+      y += __builtin_fabsf(static_cast<float>(u[e]));
     }
-    delta[b] = half_sum(x), size[b] = half_sum(y);
-    if (a.dlse != nullptr) {
-      const float z = a.dlse[at];
-      delta[b] -= z, size[b] = fmaxf(size[b], __builtin_fabsf(z));
-    }
-    const float lse = a.lse[at];
-    none[b] = lse == -INFINITY;  // a row that sees no key: all its scores are hidden
-    ref[b] = (none[b] ? 0.0f : lse * kLog2e) - kPLog2<T>;
   }
+  float delta = half_sum(x), size = half_sum(y);  // D, sum |dout|
+  if (a.dlse != nullptr) {
+    const float z = a.dlse[at];
+    delta -= z, size = fmaxf(size, __builtin_fabsf(z));
+  }
+  const float lse = a.lse[at];
+  const bool none = lse == -INFINITY;  // a row that sees no key: all its scores are hidden
+  const float ref = (none ? 0.0f : lse * kLog2e) - kPLog2<T>;  // log2 of the scaled p's divisor
   if constexpr (std::is_same_v<T, _Float16>) {  // (a row repeated past the end changes no maximum)
-    float x = size[0];
-#pragma unroll
-    for (int b = 1; b < QW; ++b) x = fmaxf(x, size[b]);
-    x = wave_max(x);
+    const float x = wave_max(size);
     if (lane == 0) *bound = wrow < rows ? x : 0.0f;
   }
-  float by[QW];  // of dp - D: the scale of ds without that of p
-#pragma unroll
-  for (int b = 0; b < QW; ++b) {
-    const int e = ds_exponent<T>(size[b]);
-    by[b] = power_of_two(e - static_cast<int>(kPLog2<T>)), delta[b] *= by[b];
-    size[b] = a.scale * power_of_two(-e);  // takes the scale out of dq
-  }
+  const int exponent = ds_exponent<T>(size);
+  const float by = power_of_two(exponent - static_cast<int>(kPLog2<T>));  // of dp - D: the scale of ds without that of p
+  delta *= by;
+  const float dq_by = a.scale * power_of_two(-exponent);  // takes the scale out of dq
   auto store_stats = [&]() {  // for the rows' part in dk and dv: lse in powers of two, and D
-#pragma unroll
-    for (int b = 0; b < QW; ++b) {
-      const int r = wrow + b * 32 + c32;
-      const int64_t at = (head * a.total_q + s.q0) * a.group + r;
-      if (h == 0 && r < rows) a.lse2[at] = none[b] ? INFINITY : ref[b], a.delta[at] = none[b] ? 0.0f : delta[b] / by[b];
-    }
+    const int r = wrow + c32;
+    const int64_t at = (head * a.total_q + s.q0) * a.group + r;
+    if (h == 0 && r < rows) a.lse2[at] = none ? INFINITY : ref, a.delta[at] = none ? 0.0f : delta / by;
   };
   int kend = s.lk, wkend = wrow < rows ? s.lk : 0, wfull = s.lk;  // keys of the workgroup; of the wave; of all its rows
   if (a.causal) {
@@ -175,7 +160,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
     split_row(a, min(rows, row0 + ROWS) - 1, i, g);
     kend = min(kend, i + off + 1);
     if (wrow < rows) {
-      split_row(a, min(rows, wrow + QW * 32) - 1, i, g);
+      split_row(a, min(rows, wrow + 32) - 1, i, g);
       wkend = min(wkend, i + off + 1);
       split_row(a, wrow, i, g);
       wfull = min(wfull, i + off + 1);
@@ -204,71 +189,57 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
                          [&](int row) { return Z ? ((bits >> row) & 1 ? row : shown) : (row < last ? row : last); });
   };
 
-  f32x16 acc[QW][DB];
-  float miss[QW];
+  f32x16 acc[DB];
+  float miss;
   // one tile; hide: some keys are hidden from some rows; EXACT: only sums ds
   auto walk = [&](const char* kt, const float* tile_bias, int t, uint64_t bits, bool hide, auto EXACT) {
     const char* vt = kt + kTile<DP>;
 #pragma unroll 2
     for (int n = 0; n < 2; ++n) {
-      f32x16 sc[QW] = {}, dp[QW] = {};
-      if constexpr (Z) {
-#pragma unroll
-        for (int b = 0; b < QW; ++b) sc[b] = read_bias(tile_bias, n, h);
-      }
+      f32x16 sc = {}, dp = {};
+      if constexpr (Z) sc = read_bias(tile_bias, n, h);
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         const u32x4 x = read_rows<DP>(kt, 32 * n, k, place_of), y = read_rows<DP>(vt, 32 * n, k, place_of);
-#pragma unroll
-        for (int b = 0; b < QW; ++b) Mfma<T>::run(x, qf[b][k], sc[b]), Mfma<T>::run(y, df[b][k], dp[b]);
+        Mfma<T>::run(x, qf[k], sc), Mfma<T>::run(y, df[k], dp);
       }
       if (hide) {
         asm volatile("");  // a branch, not 16 selects for every tile
-#pragma unroll
-        for (int b = 0; b < QW; ++b) {
-          uint64_t on = bits;
-          if (a.causal) {
-            int i, g;
-            split_row(a, min(wrow + b * 32 + (fresh_lane() & 31), rows - 1), i, g);
-            const int seen = i + off + 1 - t * kKT;  // keys of this tile that the row sees
-            on &= seen >= 64 ? ~0ull : (seen <= 0 ? 0ull : (1ull << seen) - 1);
-          }
-          const uint32_t w = static_cast<uint32_t>(on >> (32 * n)) >> (4 * h);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) sc[b][e] = (w >> (8 * (e >> 2) + (e & 3))) & 1 ? sc[b][e] : -INFINITY;
+        uint64_t on = bits;
+        if (a.causal) {
+          int i, g;
+          split_row(a, min(wrow + (fresh_lane() & 31), rows - 1), i, g);
+          const int seen = i + off + 1 - t * kKT;  // keys of this tile that the row sees
+          on &= seen >= 64 ? ~0ull : (seen <= 0 ? 0ull : (1ull << seen) - 1);
         }
+        const uint32_t w = static_cast<uint32_t>(on >> (32 * n)) >> (4 * h);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[e] = (w >> (8 * (e >> 2) + (e & 3))) & 1 ? sc[e] : -INFINITY;
       }
 #pragma unroll
-      for (int b = 0; b < QW; ++b)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][e], a.scale2, -ref[b]));
-          dp[b][e] = p * __builtin_fmaf(dp[b][e], by[b], -delta[b]);
-        }
+      for (int e = 0; e < 16; ++e) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], a.scale2, -ref));
+        dp[e] = p * __builtin_fmaf(dp[e], by, -delta);
+      }
       if constexpr (EXACT) {
 #pragma unroll
-        for (int b = 0; b < QW; ++b)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) miss[b] += dp[b][e];
+        for (int e = 0; e < 16; ++e) miss += dp[e];
       } else {
-        u32x4 pk[2][QW];
+        u32x4 pk[2];
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int k = 0; k < 2; ++k) {
+          f32x8 x;
 #pragma unroll
-          for (int b = 0; b < QW; ++b) {
-            f32x8 x;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = dp[b][8 * k + e];
-            pk[k][b] = pack8<T>(x);
-          }
+          for (int e = 0; e < 8; ++e) x[e] = dp[8 * k + e];
+          pk[k] = pack8<T>(x);
+        }
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
 #pragma unroll
           for (int d = 0; d < DB; ++d) {
             const u32x4 x = read_columns<DP>(kt, 32 * n + 16 * k, d, place_of);
-#pragma unroll
-            for (int b = 0; b < QW; ++b) Mfma<T>::run(x, pk[k][b], acc[b][d]);
+            Mfma<T>::run(x, pk[k], acc[d]);
           }
         }
         __builtin_amdgcn_s_setprio(0);
@@ -293,32 +264,24 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
   };
   if (Z && a.dim < DP) clear_tiles(smem, 2 * PAIR);
   if (tiles > 0 && tiles <= kExactTiles) {
-#pragma unroll
-    for (int b = 0; b < QW; ++b) miss[b] = 0.0f;
+    miss = 0.0f;
     pass(std::true_type{});
-#pragma unroll
-    for (int b = 0; b < QW; ++b) {  // sum ds was to be dlse
-      delta[b] += half_sum(miss[b]) * power_of_two(-static_cast<int>(kPLog2<T>));
-      if (a.dlse != nullptr) delta[b] -= a.dlse[row_at(b)] * by[b];
-    }
+    // sum ds was to be dlse
+    delta += half_sum(miss) * power_of_two(-static_cast<int>(kPLog2<T>));
+    if (a.dlse != nullptr) delta -= a.dlse[row_at()] * by;
   }
   store_stats();
   if (a.out == nullptr) return;  // only D and the bounds are wanted
 #pragma unroll
-  for (int b = 0; b < QW; ++b)
-#pragma unroll
-    for (int d = 0; d < DB; ++d) acc[b][d] = f32x16{};
+  for (int d = 0; d < DB; ++d) acc[d] = f32x16{};
   if (tiles > 0) pass(std::false_type{});
-#pragma unroll
-  for (int b = 0; b < QW; ++b) {
-    if (wrow + b * 32 + c32 >= rows) continue;
-    store_owned<T, DP>(static_cast<T*>(a.out) + row_at(b) * a.dim, a.dim, h, acc[b], size[b], false);
-  }
+  if (wrow + c32 >= rows) return;
+  store_owned<T, DP>(static_cast<T*>(a.out) + row_at() * a.dim, a.dim, h, acc, dq_by, false);
 }
 
 __device__ const float kPastRows[2] = {INFINITY, 0.0f};
 
-// dk and dv. A workgroup owns NW * QW * 32 keys of one key head (keys and values in
+// dk and dv. A workgroup owns NW * 32 keys of one key head (keys and values in
 // registers) and walks the packed query rows that read the head in tiles of 64 (queries and
 // dout, with lse and D of each row) held twice in LDS, so the query heads of a shared key
 // head sum in registers. Rows past the segment and rows that saw no key have lse = +infinity:
@@ -332,9 +295,9 @@ __device__ const float kPastRows[2] = {INFINITY, 0.0f};
 //
 // Causal: early keys see the most rows, so their blocks start first, and each block is split
 // at least in two, which levels the ends (1008 us to 623, with 25 for the join).
-template <typename T, int DP, int NW, int QW, bool Z, bool SPLIT>
+template <typename T, int DP, int NW, bool Z, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(AttnArgs a) {
-  constexpr int KEYS = NW * QW * 32, KS = DP / 16, DB = DP / 32, PAIR = 2 * kTile<DP>, CH = DP / 8;
+  constexpr int KEYS = NW * 32, KS = DP / 16, DB = DP / 32, PAIR = 2 * kTile<DP>, CH = DP / 8;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   float* stats = reinterpret_cast<float*>(smem + 2 * PAIR);  // [2][lse, D][64]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -361,27 +324,23 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
   const int key0 = s.tile * KEYS;
   if (s.tile < 0 || key0 >= s.room) return;  // keys past those in use get zeros
 
-  const int wkey = key0 + wave * (QW * 32);
+  const int wkey = key0 + wave * 32;
   const int off = s.lk - s.lq, rows = s.lk > 0 ? s.lq * a.group : 0;
-  u32x4 kf[QW][KS], vf[QW][KS];
-  bool on[QW];
-#pragma unroll
-  for (int b = 0; b < QW; ++b) {
-    const int j = wkey + b * 32 + c32;
-    on[b] = j < s.lk;
-    if (Z && a.mask != nullptr) on[b] = on[b] && a.mask[s.k0 + (j < s.lk ? j : 0)] != 0;
-    const int64_t row = (a.cu_k != nullptr ? s.k0 : 0) + (j < s.lk ? j : 0);
-    load_owned<DP>(reinterpret_cast<const char*>(static_cast<const T*>(a.k) + s.b * a.k_b + row * a.k_n + head * a.k_h),
-                   a.dim, h, on[b], kf[b]);
-    load_owned<DP>(reinterpret_cast<const char*>(static_cast<const T*>(a.v) + s.b * a.v_b + row * a.v_n + head * a.v_h),
-                   a.dim, h, on[b], vf[b]);
-  }
+  u32x4 kf[KS], vf[KS];
+  const int key = wkey + c32;
+  bool on = key < s.lk;
+  const int64_t row = (a.cu_k != nullptr ? s.k0 : 0) + (on ? key : 0);
+  if (Z && a.mask != nullptr) on = on && a.mask[s.k0 + (on ? key : 0)] != 0;
+  load_owned<DP>(reinterpret_cast<const char*>(static_cast<const T*>(a.k) + s.b * a.k_b + row * a.k_n + head * a.k_h),
+                 a.dim, h, on, kf);
+  load_owned<DP>(reinterpret_cast<const char*>(static_cast<const T*>(a.v) + s.b * a.v_b + row * a.v_n + head * a.v_h),
+                 a.dim, h, on, vf);
   // packed rows that see a key of the workgroup, of the wave, and all keys of the wave: i >= key - off
   int first = 0, wfirst = wkey < s.lk ? 0 : rows, wfull = 0;
   if (a.causal) {
     first = min(s.lq, max(0, key0 - off)) * a.group;
     if (wkey < s.lk) wfirst = min(s.lq, max(0, wkey - off)) * a.group;
-    wfull = min(s.lq, max(0, wkey + QW * 32 - 1 - off)) * a.group;
+    wfull = min(s.lq, max(0, wkey + 31 - off)) * a.group;
   }
   const int tiles = key0 < s.lk ? (rows + kKT - 1) / kKT : 0;
   int t0 = first / kKT, t1 = tiles;
@@ -435,49 +394,42 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
     lds_dma4(r < rows ? a.lse2 + stats_at + r : &kPastRows[0], reinterpret_cast<char*>(to));
     lds_dma4(r < rows ? a.delta + stats_at + r : &kPastRows[1], reinterpret_cast<char*>(to + 64));
   };
-  f32x16 dk[QW][DB] = {}, dv[QW][DB] = {};
+  f32x16 dk[DB] = {}, dv[DB] = {};
   // one tile; hide: some rows do not see some keys
   auto walk = [&](const char* qt, const float* st, int t, bool hide) {
     const char* dt = qt + kTile<DP>;
 #pragma unroll 2
     for (int n = 0; n < 2; ++n) {
-      f32x16 sc[QW] = {}, dp[QW] = {};
+      f32x16 sc = {}, dp = {};
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         const u32x4 x = read_rows<DP>(qt, 32 * n, k, place_of), y = read_rows<DP>(dt, 32 * n, k, place_of);
-#pragma unroll
-        for (int b = 0; b < QW; ++b) Mfma<T>::run(x, kf[b][k], sc[b]), Mfma<T>::run(y, vf[b][k], dp[b]);
+        Mfma<T>::run(x, kf[k], sc), Mfma<T>::run(y, vf[k], dp);
       }
       __builtin_amdgcn_sched_barrier(0);
       if (hide) {
         asm volatile("");  // a branch, not 16 selects for every tile
+        const int l = fresh_lane();  // first packed row that sees the lane's key, from the lane's first on
+        const int seen = max(0, wkey + (l & 31) - off) * a.group - t * kKT - 32 * n - 4 * (l >> 5);
 #pragma unroll
-        for (int b = 0; b < QW; ++b) {
-          const int l = fresh_lane();  // first packed row that sees the lane's key, from the lane's first on
-          const int seen = max(0, wkey + b * 32 + (l & 31) - off) * a.group - t * kKT - 32 * n - 4 * (l >> 5);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) sc[b][e] = seen <= 8 * (e >> 2) + (e & 3) ? sc[b][e] : -INFINITY;
-        }
+        for (int e = 0; e < 16; ++e) sc[e] = seen <= 8 * (e >> 2) + (e & 3) ? sc[e] : -INFINITY;
       }
-      u32x4 p[2][QW], ds[2][QW];
+      u32x4 p[2], ds[2];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        f32x8 ps[QW], dss[QW];
+        f32x8 ps, dss;
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
           const f32x4 l4 = *reinterpret_cast<const f32x4*>(st + 32 * n + 16 * k + 8 * g + 4 * h);
           const f32x4 d4 = *reinterpret_cast<const f32x4*>(st + 64 + 32 * n + 16 * k + 8 * g + 4 * h);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-#pragma unroll
-            for (int b = 0; b < QW; ++b) {
-              const int at = 8 * k + 4 * g + e;
-              const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][at], a.scale2, -l4[e]));
-              ps[b][4 * g + e] = x, dss[b][4 * g + e] = (x * by) * (dp[b][at] - d4[e]);
-            }
+          for (int e = 0; e < 4; ++e) {
+            const int at = 8 * k + 4 * g + e;
+            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[at], a.scale2, -l4[e]));
+            ps[4 * g + e] = x, dss[4 * g + e] = (x * by) * (dp[at] - d4[e]);
+          }
         }
-#pragma unroll
-        for (int b = 0; b < QW; ++b) p[k][b] = pack8<T>(ps[b]), ds[k][b] = pack8<T>(dss[b]);
+        p[k] = pack8<T>(ps), ds[k] = pack8<T>(dss);
       }
       __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_s_setprio(1);
@@ -486,8 +438,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
           const u32x4 x = read_columns<DP>(dt, 32 * n + 16 * k, d, place_of), y = read_columns<DP>(qt, 32 * n + 16 * k, d, place_of);
-#pragma unroll
-          for (int b = 0; b < QW; ++b) Mfma<T>::run(x, p[k][b], dv[b][d]), Mfma<T>::run(y, ds[k][b], dk[b][d]);
+          Mfma<T>::run(x, p[k], dv[d]), Mfma<T>::run(y, ds[k], dk[d]);
         }
       }
       __builtin_amdgcn_s_setprio(0);
@@ -505,24 +456,18 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
       load(t + 1, buf ^ 1);
       if (wave == 0) load_stats(t + 1, buf ^ 1);
     }
-    if ((t + 1) * kKT > wfirst) {
-      walk(smem + buf * PAIR, stats + buf * 128, t, t * kKT < wfull);
-    }
+    if ((t + 1) * kKT > wfirst) walk(smem + buf * PAIR, stats + buf * 128, t, t * kKT < wfull);
     tile_barrier();
   }
-#pragma unroll
-  for (int b = 0; b < QW; ++b) {
-    const int j = wkey + b * 32 + c32;
-    if (j >= s.room) continue;
-    const int64_t at = ((s.k0 + j) * a.hk + head) * a.dim;
-    if constexpr (SPLIT) {
-      const int64_t all = a.total_k * a.hk * a.dim;
-      store_owned<float, DP>(a.part + split * 2 * all + at, a.dim, h, dk[b], dk_by, !on[b]);
-      store_owned<float, DP>(a.part + (split * 2 + 1) * all + at, a.dim, h, dv[b], dv_by, !on[b]);
-    } else {
-      store_owned<T, DP>(static_cast<T*>(a.dk) + at, a.dim, h, dk[b], dk_by, !on[b]);
-      store_owned<T, DP>(static_cast<T*>(a.dv) + at, a.dim, h, dv[b], dv_by, !on[b]);
-    }
+  if (key >= s.room) return;
+  const int64_t to = ((s.k0 + key) * a.hk + head) * a.dim;
+  if constexpr (SPLIT) {
+    const int64_t all = a.total_k * a.hk * a.dim;
+    store_owned<float, DP>(a.part + split * 2 * all + to, a.dim, h, dk, dk_by, !on);
+    store_owned<float, DP>(a.part + (split * 2 + 1) * all + to, a.dim, h, dv, dv_by, !on);
+  } else {
+    store_owned<T, DP>(static_cast<T*>(a.dk) + to, a.dim, h, dk, dk_by, !on);
+    store_owned<T, DP>(static_cast<T*>(a.dv) + to, a.dim, h, dv, dv_by, !on);
   }
 }
 
@@ -539,21 +484,21 @@ __global__ __launch_bounds__(256) void attend_dkv_join_kernel(AttnArgs a, int64_
   *reinterpret_cast<t4*>(to) = t4{static_cast<T>(x[0]), static_cast<T>(x[1]), static_cast<T>(x[2]), static_cast<T>(x[3])};
 }
 
-template <typename T, int DP, int NW, int QW>
+template <typename T, int DP, int NW>
 int launch_dq(AttnArgs a, hipStream_t stream) {
-  constexpr int rows = NW * QW * 32;
+  constexpr int rows = NW * 32;
   HI3D_REQUIRE(static_cast<int64_t>(a.dq_slots) * a.hk < (1ll << 31), "too many rows for one launch");
   if (rows != a.dq_rows || NW != a.dq_waves) return fail(HI3D_ERR_INVALID, "the tile differs from the workspace's");
   a.slots = a.dq_slots;
   const int64_t blocks = static_cast<int64_t>(a.slots) * a.hk;
   constexpr size_t lds = 4 * kTile<DP>;
-  return a.mask != nullptr || a.dim < DP ? launch_tiles<&attend_dq_kernel<T, DP, NW, QW, true>>(a, blocks, 64 * NW, lds + kBiasBytes, stream)
-                                         : launch_tiles<&attend_dq_kernel<T, DP, NW, QW, false>>(a, blocks, 64 * NW, lds, stream);
+  return a.mask != nullptr || a.dim < DP ? launch_tiles<&attend_dq_kernel<T, DP, NW, true>>(a, blocks, 64 * NW, lds + kBiasBytes, stream)
+                                         : launch_tiles<&attend_dq_kernel<T, DP, NW, false>>(a, blocks, 64 * NW, lds, stream);
 }
 
-template <typename T, int DP, int NW, int QW>
+template <typename T, int DP, int NW>
 int launch_dkv(AttnArgs a, hipStream_t stream) {
-  constexpr int keys = NW * QW * 32, threads = 64 * NW;
+  constexpr int keys = NW * 32, threads = 64 * NW;
   constexpr size_t lds = 4 * kTile<DP> + 1024;
   const int64_t per = a.cu_k != nullptr ? packed_slots(a.total_k, 1, keys, a.batch) : ceil_div(a.len_k, keys) * a.batch;
   const int64_t blocks = per * a.hk * a.splits;
@@ -561,10 +506,10 @@ int launch_dkv(AttnArgs a, hipStream_t stream) {
   a.slots = static_cast<int>(per);
   const bool z = a.mask != nullptr || a.dim < DP;
   if (a.splits == 1)
-    return z ? launch_tiles<&attend_dkv_kernel<T, DP, NW, QW, true, false>>(a, blocks, threads, lds, stream)
-             : launch_tiles<&attend_dkv_kernel<T, DP, NW, QW, false, false>>(a, blocks, threads, lds, stream);
-  const int rc = z ? launch_tiles<&attend_dkv_kernel<T, DP, NW, QW, true, true>>(a, blocks, threads, lds, stream)
-                   : launch_tiles<&attend_dkv_kernel<T, DP, NW, QW, false, true>>(a, blocks, threads, lds, stream);
+    return z ? launch_tiles<&attend_dkv_kernel<T, DP, NW, true, false>>(a, blocks, threads, lds, stream)
+             : launch_tiles<&attend_dkv_kernel<T, DP, NW, false, false>>(a, blocks, threads, lds, stream);
+  const int rc = z ? launch_tiles<&attend_dkv_kernel<T, DP, NW, true, true>>(a, blocks, threads, lds, stream)
+                   : launch_tiles<&attend_dkv_kernel<T, DP, NW, false, true>>(a, blocks, threads, lds, stream);
   if (rc != HI3D_OK) return rc;
   const int64_t all = a.total_k * a.hk * a.dim;
   hipLaunchKernelGGL(attend_dkv_join_kernel<T>, dim3(static_cast<unsigned>(ceil_div(2 * all, 1024))), dim3(256), 0, stream, a,
@@ -577,13 +522,13 @@ template <typename T, int DP>
 int launch_grad_dim(const AttnArgs& a, hipStream_t stream) {
   if (a.total_q > 0) {
     int rc = HI3D_OK;
-    if (a.dq_waves == 1) rc = launch_dq<T, DP, 1, 1>(a, stream);
-    else rc = launch_dq<T, DP, 4, 1>(a, stream);
+    if (a.dq_waves == 1) rc = launch_dq<T, DP, 1>(a, stream);
+    else rc = launch_dq<T, DP, 4>(a, stream);
     if (rc != HI3D_OK) return rc;
   }
   if (a.total_k == 0 || a.dk == nullptr) return HI3D_OK;
-  if (ceil_div(a.total_k, a.batch) <= 32) return launch_dkv<T, DP, 1, 1>(a, stream);
-  return launch_dkv<T, DP, 4, 1>(a, stream);
+  if (ceil_div(a.total_k, a.batch) <= 32) return launch_dkv<T, DP, 1>(a, stream);
+  return launch_dkv<T, DP, 4>(a, stream);
 }
 
 template <typename T>
