@@ -289,8 +289,9 @@ __device__ const float kPastRows[2] = {INFINITY, 0.0f};
 //
 // Registers decide: keys, values and both sums take 192 of 256 at 128 values a head, and a
 // register spilled into the loop waits, when it is read again, for the tile loads in flight
-// (48 of them: 1628 us for 1000). So lse and D go straight to LDS, places are formed anew
-// from the lane, and masked and plain tiles share one path (two paths copied the sums). The
+// (48 of them: 1628 us for 1000; one: 540 for 520). So lse and D go straight to LDS, places are
+// formed anew from the lane, at 128 values those in LDS too, for every tile, and masked and
+// plain tiles share one path (two paths copied the sums): no register is spilled. The
 // same figures as above: 350 us (810 TFLOP/s of its 4 products) and 545 us (1010).
 //
 // Causal: early keys see the most rows, so their blocks start first, and each block is split
@@ -302,7 +303,6 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
   float* stats = reinterpret_cast<float*>(smem + 2 * PAIR);  // [2][lse, D][64]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c32 = lane & 31, h = lane >> 5;
-  const TileLane place_of = tile_lane<DP>(lane);
   int head, split = 0, slot;
   if (a.causal) {  // slot by slot, so that the first keys, which see the most rows, come first
     const int of = a.hk * a.splits;
@@ -397,6 +397,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
   f32x16 dk[DB] = {}, dv[DB] = {};
   // one tile; hide: some rows do not see some keys
   auto walk = [&](const char* qt, const float* st, int t, bool hide) {
+    const TileLane place_of = tile_lane<DP>(DP == 128 ? fresh_lane() : lane);
     const char* dt = qt + kTile<DP>;
 #pragma unroll 2
     for (int n = 0; n < 2; ++n) {
