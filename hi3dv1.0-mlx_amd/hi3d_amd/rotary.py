@@ -33,10 +33,12 @@ def frequencies(
     they are.
 
     ``stretch`` > 1 fits positions past the trained length. ``scaling`` says how:
-    ``"linear"`` divides every frequency by it; ``"base"`` raises the base to ``base *
-    stretch ** (m / (m - 1))``, which leaves the fastest pair and divides the slowest by
-    ``stretch``; ``"blend"`` leaves pairs that turn 32 times or more within ``trained``
-    positions, divides those that turn once or less, and goes between by the number of turns.
+    ``"linear"`` (position interpolation, Chen et al., 2023) divides every frequency by it;
+    ``"base"`` (the "NTK-aware" change of base) raises the base to ``base * stretch ** (m / (m -
+    1))``, which leaves the fastest pair and divides the slowest by ``stretch``; ``"blend"``
+    (by parts, as in YaRN, Peng et al., 2023, without its temperature) leaves pairs that turn 32
+    times or more within ``trained`` positions, divides those that turn once or less, and goes
+    between by the number of turns.
     """
     if rot < 0 or rot % 2:
         raise ValueError(f"the number of turned values must be even (got {rot})")

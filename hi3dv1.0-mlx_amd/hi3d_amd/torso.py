@@ -1,7 +1,9 @@
 """Self attention of a torso block on the token operators: projection, rotary positions,
 attention within each object and the output projection, trainable; and the same block
-stepping one token at a time over a cache (the refiner's block structure:
-src/sparc3d/nn/sparse/attention/modules.py, src/sparc3d/nn/rope.py)."""
+stepping one token at a time over a cache. The refiner's attention modules
+(src/sparc3d/nn/sparse/attention/modules.py, src/sparc3d/nn/rope.py) have this order of
+steps and a root mean square norm of queries and keys besides, which is not formed here:
+this is not a drop-in for them, and the refiner itself keeps no cache."""
 
 from __future__ import annotations
 
