@@ -46,15 +46,15 @@ __device__ __forceinline__ void hide_keys(f32x16 (&sc)[2][QW], uint64_t bits) {
 // rows 32 * DP / 128 matrix instructions of 32 cycles, and about 140 vector operations for
 // the softmax (32 exponentials of 8 cycles), which at 64 values a head take longer. Matrix
 // products run at a higher wave priority, so that the other wave's softmax fills in behind
-// them (1.5 % at 64). 20,011 tokens x 33 heads x 64 fp16 in two objects: 1865 us, 910
-// TFLOP/s; 16,384 causal x 32/8 heads x 128 bf16: 1978 us, 1110 TFLOP/s.
+// them (1.5 % at 64). 20,011 tokens x 33 heads x 64 fp16 in two objects: 1880 us, 900
+// TFLOP/s; 16,384 causal x 32/8 heads x 128 bf16: 2045 us, 1075 TFLOP/s.
 //
 // SPLIT, few rows over many keys: parts of the keys go to workgroups of their own, and their
 // outputs and (m, sum) to attend_join_kernel in fp32. One-wave workgroups then read keys and
 // values that no other one does; more of them than the chip's 256 MiB of cache go past it, as
 // the next token's call would not find them there. Single tokens of 8 sequences over caches of
-// up to 65,536 x 8 x 128 bf16 (1.9 GB): 326 us, 5.8 TB/s, 358 through the caches; below that
-// size the cache helps (8 x 4,096 keys, 134 MB: 30.8 us for 32.3).
+// up to 65,536 x 8 x 128 bf16 (1.9 GB): 308 us, 6.1 TB/s (326 for 358 through the caches, in
+// turn on a slower card); below that size the cache helps (8 x 4,096 keys, 134 MB: 30.8 us for 32.3).
 template <typename T, int DP, int NW, int QW, bool Z, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, DP <= 64 && NW * QW == 4 ? 3 : 2) void attend_kernel(AttnArgs a) {
   constexpr int ROWS = NW * QW * 32, KS = DP / 16, DB = DP / 32, PAIR = 2 * kTile<DP>;
@@ -298,7 +298,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 && NW * QW == 4 ? 3 : 2) void att
 // parts meet in LDS, weighed by exp2(m - max m) in fp32.
 //
 // Bound by memory latency and the waves that fit: 327,581 rows in windows of 48, 8 heads of 32
-// (671 MB) in 172 us, 3.9 TB/s; 204 as 64-row workgroups of attend_kernel.
+// (671 MB) in 166 us, 4.05 TB/s; a fifth more as 64-row workgroups of attend_kernel.
 constexpr int kShortSpan = 256;
 
 template <typename T, int DP, int KW, bool Z>

@@ -83,8 +83,8 @@ constexpr int kExactTiles = 4;
 // One block of 32 rows a wave: two (half the LDS reads) leave fewer waves a SIMD and ran at
 // lower speed (64 values a head: 294 us for 271). Bound by each wave's chain of products
 // and vector operations, which 2 or 3 waves a SIMD overlap in part: 8,191 rows x 33 heads x 64
-// fp16 in four segments 262 us (810 TFLOP/s of its 3 products), 8,192 causal x 32/8 heads x 128
-// bf16 412 us (1000).
+// fp16 in four segments 264 us (805 TFLOP/s of its 3 products), 8,192 causal x 32/8 heads x 128
+// bf16 414 us (995).
 template <typename T, int DP, int NW, bool Z>
 __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(AttnArgs a) {
   constexpr int ROWS = NW * 32, KS = DP / 16, DB = DP / 32, PAIR = 2 * kTile<DP>;
@@ -289,10 +289,10 @@ __device__ const float kPastRows[2] = {INFINITY, 0.0f};
 //
 // Registers decide: keys, values and both sums take 192 of 256 at 128 values a head, and a
 // register spilled into the loop waits, when it is read again, for the tile loads in flight
-// (48 of them: 1628 us for 1000; one: 540 for 520). So lse and D go straight to LDS, places are
+// (48 of them: 1628 us for 1000; one: 545 for 532). So lse and D go straight to LDS, places are
 // formed anew from the lane, at 128 values those in LDS too, for every tile, and masked and
 // plain tiles share one path (two paths copied the sums): no register is spilled. The
-// same figures as above: 350 us (810 TFLOP/s of its 4 products) and 545 us (1010).
+// same figures as above: 355 us (795 TFLOP/s of its 4 products) and 532 us (1035).
 //
 // Causal: early keys see the most rows, so their blocks start first, and each block is split
 // at least in two, which levels the ends (1008 us to 623, with 25 for the join).
