@@ -53,6 +53,8 @@ class KeyValueCache:
             if self.mask is None:
                 self.mask = torch.ones(self.k.shape[:2], dtype=torch.bool, device=self.k.device)
             self.mask[which, at:at + n] = key_mask
+        elif self.mask is not None:
+            self.mask[which, at:at + n] = True
         self.k[which, at:at + n] = k.detach()
         self.v[which, at:at + n] = v.detach()
         self.used[which] += n
@@ -66,6 +68,8 @@ class KeyValueCache:
         at = self.lens.long()
         self.k[self._rows, at] = k.detach().to(self.k.dtype)
         self.v[self._rows, at] = v.detach().to(self.v.dtype)
+        if self.mask is not None:
+            self.mask[self._rows, at] = True
         self.lens += 1
         self.used = [n + 1 for n in self.used]
 

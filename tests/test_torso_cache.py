@@ -222,3 +222,18 @@ def test_refused_tokens_leave_the_cache_alone(plain):
         with torch.no_grad(), pytest.raises(ValueError, match="must be"):
             block(x, positions, cache=cache)
         assert _same(before, _state(cache))
+
+
+def test_a_cache_that_starts_again(plain):
+    """A program that takes a cache again from its first key: the old mask hides nothing new."""
+    block = _block()
+    x, positions = _tokens(14, 32)
+    cache = _cache(block)
+    with torch.no_grad():
+        block(x[:12], positions[:12], cache=cache, key_mask=torch.arange(12) % 2 == 0)
+        cache.used[0] = 0
+        cache.lens.zero_()
+        rows = [block(x[:6], positions[:6], cache=cache)]
+        rows += [block.step(x[i:i + 1], positions[i:i + 1], cache) for i in range(6, 9)]
+        rows.append(block(x[9:], positions[9:], cache=cache))
+    torch.testing.assert_close(torch.cat(rows), block(x, positions).detach(), **TOL)
