@@ -329,8 +329,8 @@ __device__ __forceinline__ void store_row(T* to, int dim, int h, const f32x16* a
 }
 
 // Launches kKernel, which may take more than 64 KB of LDS (asked for once a device).
-template <auto kKernel>
-int launch_tiles(const AttnArgs& a, int64_t blocks, int threads, size_t lds, hipStream_t stream) {
+template <auto kKernel, typename Args>
+int launch_tiles(const Args& a, int64_t blocks, int threads, size_t lds, hipStream_t stream) {
   static uint64_t asked = 0;
   if (lds > 65536) {
     int dev = 0;
@@ -377,5 +377,7 @@ __device__ __forceinline__ void tile_barrier() {
   wait_vmcnt<0>();
   __syncthreads();
 }
+
+int attention_args(const hi3d_attention_desc* d, AttnArgs& a);
 
 }  // namespace hi3d

@@ -1,0 +1,211 @@
+// Terms of attention scores beside scale q k: a cap, a cost that grows with the distance, a
+// learned bias by relative position, and keys that every query of a causal segment sees.
+//
+// Row i of a segment with lq queries and lk keys stands at place i + lk - lq among the keys; r =
+// j - place is the relative position of key j. With x = scale q k:
+//   s = cap tanh(x / cap)      (or x)
+//     - slope[head] |r|
+//     + bias[map[clamp(r, -far, far) + far], head]
+// and a causal row sees the keys with r <= 0 or j < prefix.
+//
+// All in powers of two (times log2 e). cap tanh(x / cap) = cap (1 - 2 u), u = 1 / (1 + exp(2 x /
+// cap)): an exponential and a reciprocal, 1 ulp each, so a capped score is off by at most 10 e
+// cap (e = 2^-24; caps end at 1024, where that is 6e-4); its derivative is 4 u (1 - u). What is left is kept as a sum mul * score + add that goes into the
+// softmax's own multiply-add: a capped score stays -u with mul = 2 cap, a distance costs one
+// multiply-add where a tile lies on one side of the rows (its constant part is in add), and a bias
+// costs nothing where a tile lies past `far`: there it is one number. Tiles between look it up
+// in LDS, where every query head of the workgroup has its bias by relative position, extended on
+// both sides by what a tile can reach past `far`, so that a lane's places are one address with
+// constant offsets.
+#pragma once
+
+#include <type_traits>
+
+#include "attention.h"
+
+namespace hi3d {
+
+constexpr float kHideBelow = -1e30f;  // a bias below hides its key (-infinity; the lowest numbers of a type too)
+constexpr int kPad = kKT, kPadKeys = 128;  // what the rows' and the keys' kernels look up past `far`
+constexpr int kMostTermBytes = 72 * 1024, kMostLds = 160 * 1024;
+
+struct TermArgs : AttnArgs {
+  float cap2, cap_in;           // log2(e) cap, and 2 log2(e) scale / cap; 0 without a cap
+  float per_mul;                // 1 / mul of a score without a bias
+  const float* slopes;          // [hq], or null
+  const void* bias;             // [buckets, hq], or null
+  const int32_t* map;           // [2 far + 1]
+  int32_t bias_type, buckets, far;
+  int32_t stride, stride_keys;  // floats of a head's bias in LDS, in the kernels over rows and over keys
+  const int32_t* prefix;        // [batch], or null
+  // the keys are the common beginning of `per`-row sequences (rows of segment 0 one after another):
+  const int32_t* own_lens;      // keys in use of each sequence behind it, or null: own_len
+  int32_t per, own_len;
+  int32_t share;                // backward: query heads of a key head, where hk counts query heads
+  float* dbias;                 // backward: [hq, slots, 2 far + 2 kPad + 1] parts, or null
+};
+
+template <bool TERMS>
+using ArgsOf = std::conditional_t<TERMS, TermArgs, AttnArgs>;
+
+// Floats of a head's bias in LDS: its length, up to the next number after which the lanes' heads
+// (32 / group rows of each) start at banks of their own.
+inline int bias_stride(int far, int pad, int group) {
+  const int want = group >= 32 ? 1 : 32 / group, length = 2 * far + 2 * pad + 1;
+  return length + ((want - length) % 64 + 64) % 64;
+}
+template <bool TERMS>
+int term_bytes(const ArgsOf<TERMS>& a) {
+  if constexpr (TERMS) return a.bias != nullptr ? a.group * a.stride * 4 : 0;
+  else return 0;
+}
+
+__device__ __forceinline__ float load_bias(const TermArgs& a, int at) {
+  if (a.bias_type == HI3D_F32) return static_cast<const float*>(a.bias)[at];
+  if (a.bias_type == HI3D_F16) return static_cast<float>(static_cast<const _Float16*>(a.bias)[at]);
+  return static_cast<float>(static_cast<const __bf16*>(a.bias)[at]);
+}
+
+// Which bucket place x of a padded bias belongs to. (Numbers outside the table count as the nearest.)
+__device__ __forceinline__ int bucket_at(const TermArgs& a, int x, int pad) {
+  const int b = a.map[min(max(x - pad, 0), 2 * a.far)];
+  return min(max(b, 0), a.buckets - 1);
+}
+
+// Places x0 to x1 of the bias of `count` query heads from `head0` on into LDS, in powers of two.
+template <int PAD>
+__device__ __forceinline__ void stage_bias(const TermArgs& a, float* to, int stride, int head0, int count, int x0, int x1,
+                                           int thread, int threads) {
+  for (int x = x0 + thread; x < x1; x += threads) {
+    const int at = bucket_at(a, x, PAD) * a.hq + head0;
+    for (int g = 0; g < count; ++g) {
+      const float v = load_bias(a, at + g);
+      to[g * stride + x] = v < kHideBelow ? -INFINITY : v * kLog2e;
+    }
+  }
+}
+
+__device__ __forceinline__ float minus_u(const TermArgs& a, float score) {
+  return __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(score * a.cap_in));
+}
+
+// A lane's rows (QW blocks of 32 of a wave) in the kernels whose lanes own query rows.
+template <int QW>
+struct RowTerms {
+  float slope[QW];       // log2(e) slope
+  int place[QW];         // among the keys
+  const float* bias[QW]; // of the row's head, in LDS
+  int first, last;       // least and largest place of the wave's rows
+};
+
+// Keys of a segment that all of its rows see.
+template <bool TERMS>
+__device__ __forceinline__ int first_keys(const ArgsOf<TERMS>& a, const Segment& s) {
+  if constexpr (TERMS)
+    if (a.prefix != nullptr && s.b >= 0 && s.b < a.batch) return min(max(a.prefix[s.b], 0), s.lk);
+  return 0;
+}
+
+// What the terms of a lane's rows depend on: rows r = wrow + 32 b + lane % 32 of queries i and heads g.
+template <int QW>
+__device__ __forceinline__ void row_terms(const TermArgs& a, const Segment& s, RowTerms<QW>& w, const float* table, int head,
+                                          int wrow, int rows, const int (&i)[QW], const int (&g)[QW]) {
+  const int off = s.lk - s.lq;
+  int least = 0x7fffffff, most = -0x7fffffff - 1;
+#pragma unroll
+  for (int b = 0; b < QW; ++b) {
+    w.slope[b] = a.slopes != nullptr ? a.slopes[head * a.group + g[b]] * kLog2e : 0.0f;
+    w.bias[b] = table + g[b] * a.stride;
+    w.place[b] = i[b] + off;
+    if (a.per > 0) {
+      const int of = i[b] / a.per;
+      int own = a.own_len;
+      if (a.own_lens != nullptr) own = min(max(a.own_lens[of], 0), own);
+      w.place[b] = s.lk + own - a.per + i[b] - of * a.per;
+      least = min(least, w.place[b]), most = max(most, w.place[b]);
+    }
+  }
+  if (a.per > 0) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) least = min(least, __shfl_xor(least, d)), most = max(most, __shfl_xor(most, d));
+    w.first = __builtin_amdgcn_readfirstlane(least), w.last = __builtin_amdgcn_readfirstlane(most);
+    return;
+  }
+  int x, y;
+  split_row(a, min(wrow, rows - 1), x, y);
+  w.first = x + off;
+  split_row(a, min(wrow + QW * 32, rows) - 1, x, y);
+  w.last = x + off;
+}
+
+// Adds a tile's terms to its scores sc[n][b] (keys k0 + 32 (n0 + n) + 8 (e / 4) + 4 h + e % 4). Scores
+// in powers of two are then sc * (returned factor) + add[b]. KEEP: derivative of the cap.
+template <int N, int QW, bool KEEP>
+__device__ __forceinline__ float add_terms(const TermArgs& a, const RowTerms<QW>& w, f32x16 (&sc)[N][QW], int k0, int n0,
+                                           int h, float (&add)[QW], f32x16* bend) {
+  float mul = a.scale2;
+#pragma unroll
+  for (int b = 0; b < QW; ++b) add[b] = 0.0f;
+  if (a.cap2 > 0.0f) {
+    mul = 2.0f * a.cap2;
+#pragma unroll
+    for (int b = 0; b < QW; ++b) {
+      add[b] = a.cap2;
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float u = minus_u(a, sc[n][b][e]);
+          sc[n][b][e] = u;
+          if constexpr (KEEP) (*bend)[e] = __builtin_fmaf(-4.0f * u, u, -4.0f * u);
+        }
+    }
+  }
+  if (a.slopes != nullptr) {
+    const bool before = k0 + kKT - 1 <= w.first, after = k0 >= w.last;
+#pragma unroll
+    for (int b = 0; b < QW; ++b) {
+      const float from = static_cast<float>(k0 + 4 * h - w.place[b]);
+      if (before || after) {
+        const float s = after ? -w.slope[b] : w.slope[b], t = s * a.per_mul;
+        add[b] = __builtin_fmaf(s, from, add[b]);
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            sc[n][b][e] = __builtin_fmaf(t, static_cast<float>(32 * (n0 + n) + 8 * (e >> 2) + (e & 3)), sc[n][b][e]);
+      } else {
+        const float t = -w.slope[b] * a.per_mul;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            sc[n][b][e] = __builtin_fmaf(
+                t, __builtin_fabsf(from + static_cast<float>(32 * (n0 + n) + 8 * (e >> 2) + (e & 3))), sc[n][b][e]);
+      }
+    }
+  }
+  if (a.bias != nullptr) {
+    if (k0 + kKT - 1 - w.first <= -a.far) {
+#pragma unroll
+      for (int b = 0; b < QW; ++b) add[b] += w.bias[b][0];
+    } else if (k0 - w.last >= a.far) {
+#pragma unroll
+      for (int b = 0; b < QW; ++b) add[b] += w.bias[b][2 * (a.far + kPad)];
+    } else {
+#pragma unroll
+      for (int b = 0; b < QW; ++b) {
+        const float* at = w.bias[b] + min(max(k0 + 4 * h - w.place[b] + a.far + kPad, 0), 2 * a.far + kPad);
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            sc[n][b][e] = __builtin_fmaf(sc[n][b][e], mul, at[32 * (n0 + n) + 8 * (e >> 2) + (e & 3)]);
+      }
+      mul = 1.0f;
+    }
+  }
+  return mul;
+}
+
+}  // namespace hi3d

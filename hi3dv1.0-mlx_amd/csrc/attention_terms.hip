@@ -1,0 +1,186 @@
+// Attention with terms beside scale q k (attention_terms.h), and attention over keys that many
+// sequences share in front of their own.
+#include "attention_forward.h"
+
+namespace hi3d {
+
+int term_args(const hi3d_attention_desc* d, const hi3d_attention_terms* t, TermArgs& a) {
+  a = TermArgs{};
+  const int rc = attention_args(d, a);
+  if (rc != HI3D_OK) return rc;
+  HI3D_REQUIRE(t != nullptr, "null terms");
+  HI3D_REQUIRE(t->cap == 0.0f || (t->cap >= 1e-6f && t->cap <= 1024.0f), "a cap must be at most 1024 (got %g)", t->cap);
+  HI3D_REQUIRE(t->slopes == nullptr || d->scale >= 1e-30f, "scores with slopes need a scale of 1e-30 or more");
+  HI3D_REQUIRE(t->prefix == nullptr || d->causal, "keys that all queries see belong to causal segments");
+  if (t->bias != nullptr) {
+    HI3D_REQUIRE(t->bias_dtype == HI3D_F32 || t->bias_dtype == HI3D_F16 || t->bias_dtype == HI3D_BF16,
+                 "the bias must be fp32, fp16 or bf16 (got type %d)", t->bias_dtype);
+    HI3D_REQUIRE(t->bucket_map != nullptr, "null pointer argument");
+    HI3D_REQUIRE(t->buckets >= 1 && static_cast<int64_t>(t->buckets) * d->heads_q < (1 << 30), "bad number of buckets (%d)",
+                 t->buckets);
+    HI3D_REQUIRE(t->far >= 0 && t->far <= 1024, "a bias reaches at most 1024 keys (got %d)", t->far);
+    a.bias = t->bias, a.map = t->bucket_map, a.bias_type = t->bias_dtype, a.buckets = t->buckets, a.far = t->far;
+    a.stride = bias_stride(a.far, kPad, a.group), a.stride_keys = bias_stride(a.far, kPadKeys, a.group);
+    HI3D_REQUIRE(static_cast<int64_t>(a.group) * a.stride_keys * 4 <= kMostTermBytes,
+                 "a bias that reaches %d keys takes at most %d query heads to a key head (got %d)", a.far,
+                 kMostTermBytes / 4 / a.stride_keys, a.group);
+  }
+  if (t->cap > 0.0f) a.cap2 = t->cap * kLog2e, a.cap_in = 2.0f * kLog2e * d->scale / t->cap;
+  a.per_mul = 1.0f / (t->cap > 0.0f ? 2.0f * a.cap2 : a.scale2);
+  a.slopes = t->slopes, a.prefix = t->prefix, a.share = 1;
+  return HI3D_OK;
+}
+
+namespace {
+
+// Kernel, tile and splits of the key axis.
+void choose(TermArgs& a, int cus) {
+  a.few = few_rows(a.total_q, a.total_k, a.batch, a.hq, a.hk, a.dim, cus, term_bytes<true>(a));
+  a.splits = attend_splits(a.total_q, a.total_k, a.batch, a.hq, a.hk, a.dim, cus, a.few);
+  a.rows = attend_rows(a.total_q, a.batch, a.hq, a.hk, a.dim, cus);
+}
+
+int64_t part_bytes(const TermArgs& a, int splits) { return static_cast<int64_t>(splits) * a.total_q * a.hq * (a.dim + 2) * 4; }
+
+// The two halves of attention over shared keys: all rows over the keys that they share, as one
+// segment, and each sequence over its own. Each half leaves parts of the rows, in at most 128 splits.
+void choose_halves(const TermArgs& a, const hi3d_attention_shared* s, TermArgs& shared, TermArgs& own, int cus) {
+  own = shared = a;
+  shared.k = s->k, shared.v = s->v, shared.mask = s->key_mask;
+  shared.k_b = shared.v_b = 0, shared.k_n = s->strides[0], shared.k_h = s->strides[1];
+  shared.v_n = s->strides[2], shared.v_h = s->strides[3];
+  shared.batch = 1, shared.len_q = static_cast<int32_t>(a.total_q), shared.len_k = s->len, shared.total_k = s->len;
+  shared.lens_k = nullptr, shared.causal = shared.reverse = 0;
+  shared.own_lens = a.lens_k, shared.own_len = a.len_k, shared.per = a.len_q;
+  shared.head_minor = s->len <= 512;
+  shared.once = static_cast<int64_t>(s->len) * a.hk * a.dim * 4 > (256ll << 20);
+  for (TermArgs* x : {&shared, &own}) {
+    const int rows = attend_rows(x->total_q, x->batch, x->hq, x->hk, x->dim, cus);
+    x->rows = rows > 128 ? 128 : rows;
+    const int splits = attend_splits(x->total_q, x->total_k, x->batch, x->hq, x->hk, x->dim, cus, false);
+    x->splits = splits > 128 ? 128 : splits;
+  }
+}
+
+template <typename T, int DP>
+int launch_part(const TermArgs& a, hipStream_t stream) {
+  if (a.rows == 32) return launch_attend<T, DP, 1, 1, true>(a, stream, true);
+  if (a.rows == 64) return launch_attend<T, DP, 1, 2, true>(a, stream, true);
+  return launch_attend<T, DP, 4, 1, true>(a, stream, true);
+}
+
+template <typename T>
+int launch_shared(const TermArgs& shared, const TermArgs& own, hipStream_t stream) {
+  for (const TermArgs* a : {&shared, &own}) {
+    int rc = HI3D_OK;
+    switch ((a->dim + 31) / 32) {
+      case 1: rc = launch_part<T, 32>(*a, stream); break;
+      case 2: rc = launch_part<T, 64>(*a, stream); break;
+      case 3: rc = launch_part<T, 96>(*a, stream); break;
+      default: rc = launch_part<T, 128>(*a, stream);
+    }
+    if (rc != HI3D_OK) return rc;
+  }
+  TermArgs all = shared;
+  all.splits = shared.splits + own.splits;
+  return launch_join<T>(all, stream);
+}
+
+int shared_args(const hi3d_attention_desc* d, const hi3d_attention_terms* t, const hi3d_attention_shared* s, TermArgs& a) {
+  const int rc = term_args(d, t, a);
+  if (rc != HI3D_OK) return rc;
+  HI3D_REQUIRE(s != nullptr, "null shared keys");
+  HI3D_REQUIRE(d->cu_q == nullptr && d->cu_k == nullptr, "shared keys stand in front of sequences of equal room, not of offsets");
+  HI3D_REQUIRE(t->prefix == nullptr, "shared keys are seen by all queries as they are");
+  HI3D_REQUIRE(s->len >= 0, "bad sizes");
+  HI3D_REQUIRE(s->len == 0 || (s->k != nullptr && s->v != nullptr), "null pointer argument");
+  HI3D_REQUIRE((reinterpret_cast<uintptr_t>(s->k) | reinterpret_cast<uintptr_t>(s->v)) % 16 == 0,
+               "the shared keys and values must be 16-byte aligned");
+  for (int i = 0; i < 4; ++i) HI3D_REQUIRE(s->strides[i] % 8 == 0, "strides must be multiples of 8 elements");
+  for (int i : {0, 2})
+    HI3D_REQUIRE(s->strides[i] >= 0 && s->strides[i] < (1ll << 23), "row strides must be below 2^23 elements");
+  return HI3D_OK;
+}
+
+}  // namespace
+}  // namespace hi3d
+
+using namespace hi3d;
+
+extern "C" {
+
+int hi3d_attention_terms_workspace(const hi3d_attention_desc* d, const hi3d_attention_terms* t, int64_t* bytes) {
+  TermArgs a;
+  const int rc = term_args(d, t, a);
+  if (rc != HI3D_OK) return rc;
+  HI3D_REQUIRE(bytes != nullptr, "null pointer argument");
+  *bytes = 0;
+  if (a.total_q == 0 || a.batch == 0) return HI3D_OK;
+  const int cus = compute_units();
+  choose(a, cus > 0 ? cus : 256);  // without a device (a size query on a build host): the MI355X's
+  if (a.splits > 1) *bytes = part_bytes(a, a.splits) + 256;
+  return HI3D_OK;
+}
+
+int hi3d_attention_terms_forward(const hi3d_attention_desc* d, const hi3d_attention_terms* t, void* out, float* lse,
+                                 void* workspace, int64_t workspace_bytes, void* stream_) {
+  TermArgs a;
+  const int rc = term_args(d, t, a);
+  if (rc != HI3D_OK) return rc;
+  if (a.total_q == 0) return HI3D_OK;
+  HI3D_REQUIRE(a.batch > 0, "rows without a segment");
+  HI3D_REQUIRE(out != nullptr && reinterpret_cast<uintptr_t>(out) % 16 == 0, "out must be 16-byte aligned");
+  const int cus = compute_units();
+  HI3D_REQUIRE(cus > 0, "cannot query the compute unit count");
+  a.out = out, a.lse = lse;
+  choose(a, cus);
+  if (a.splits > 1) {
+    HI3D_REQUIRE(workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 &&
+                     workspace_bytes >= part_bytes(a, a.splits),
+                 "workspace too small (%lld bytes)", static_cast<long long>(workspace_bytes));
+    a.part = static_cast<float*>(workspace);
+    a.part_ml = a.part + static_cast<int64_t>(a.splits) * a.total_q * a.hq * a.dim;
+  }
+  hipStream_t stream = as_stream(stream_);
+  return d->dtype == HI3D_F16 ? launch_attend_type<_Float16, true>(a, stream) : launch_attend_type<__bf16, true>(a, stream);
+}
+
+int hi3d_attention_shared_workspace(const hi3d_attention_desc* d, const hi3d_attention_terms* t,
+                                    const hi3d_attention_shared* s, int64_t* bytes) {
+  TermArgs a, shared, own;
+  const int rc = shared_args(d, t, s, a);
+  if (rc != HI3D_OK) return rc;
+  HI3D_REQUIRE(bytes != nullptr, "null pointer argument");
+  *bytes = 0;
+  if (a.total_q == 0 || a.batch == 0) return HI3D_OK;
+  const int cus = compute_units();
+  choose_halves(a, s, shared, own, cus > 0 ? cus : 256);
+  *bytes = part_bytes(a, shared.splits + own.splits) + 256;
+  return HI3D_OK;
+}
+
+int hi3d_attention_shared_forward(const hi3d_attention_desc* d, const hi3d_attention_terms* t, const hi3d_attention_shared* s,
+                                  void* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream_) {
+  TermArgs a, shared, own;
+  const int rc = shared_args(d, t, s, a);
+  if (rc != HI3D_OK) return rc;
+  if (a.total_q == 0) return HI3D_OK;
+  HI3D_REQUIRE(out != nullptr && reinterpret_cast<uintptr_t>(out) % 16 == 0, "out must be 16-byte aligned");
+  const int cus = compute_units();
+  HI3D_REQUIRE(cus > 0, "cannot query the compute unit count");
+  a.out = out, a.lse = lse;
+  choose_halves(a, s, shared, own, cus);
+  const int splits = shared.splits + own.splits;
+  HI3D_REQUIRE(workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 &&
+                   workspace_bytes >= part_bytes(a, splits),
+               "workspace too small (%lld bytes)", static_cast<long long>(workspace_bytes));
+  const int64_t rows = a.total_q * a.hq;
+  shared.part = static_cast<float*>(workspace);
+  shared.part_ml = shared.part + splits * rows * a.dim;
+  own.part = shared.part + shared.splits * rows * a.dim;
+  own.part_ml = shared.part_ml + shared.splits * rows * 2;
+  hipStream_t stream = as_stream(stream_);
+  return d->dtype == HI3D_F16 ? launch_shared<_Float16>(shared, own, stream) : launch_shared<__bf16>(shared, own, stream);
+}
+
+}  // extern "C"

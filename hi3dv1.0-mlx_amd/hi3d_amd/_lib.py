@@ -105,6 +105,12 @@ _SIGNATURES = {
     "hi3d_attention_forward": [_p, _p, _p, _p, _i64, _p],
     "hi3d_attention_backward_workspace": [_p, _p],
     "hi3d_attention_backward": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _p],
+    "hi3d_attention_terms_workspace": [_p, _p, _p],
+    "hi3d_attention_terms_forward": [_p, _p, _p, _p, _p, _i64, _p],
+    "hi3d_attention_terms_backward_workspace": [_p, _p, _p],
+    "hi3d_attention_terms_backward": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _p],
+    "hi3d_attention_shared_workspace": [_p, _p, _p, _p],
+    "hi3d_attention_shared_forward": [_p, _p, _p, _p, _p, _p, _i64, _p],
 }
 _RESTYPES = {"hi3d_last_error": ctypes.c_char_p, "hi3d_version": ctypes.c_char_p, "hi3d_conv_tile_rows": _i32,
              "hi3d_gather_conv_group16": _i32, "hi3d_w8a8_gemm_kernel": _i32,

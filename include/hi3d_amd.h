@@ -684,6 +684,63 @@ int hi3d_attention_backward(const hi3d_attention_desc* desc_host, const void* ou
                             const void* dout_dev, const float* dlse_dev, void* dq_dev, void* dk_dev, void* dv_dev,
                             void* workspace_dev, int64_t workspace_bytes, void* stream);
 
+/* Terms of attention scores beside x = scale q k. With r = j - (i + lk - lq) the position of key j
+ * relative to query i of a segment, the score is
+ *   cap tanh(x / cap) (x where cap is 0) - slopes[head] |r|
+ *     + bias[bucket_map[clamp(r, -far, far) + far], head]
+ * slopes_dev: fp32 [heads_q]; bias: F32, F16 or BF16 [buckets, heads_q], with bucket_map int32 [2 far
+ * + 1] (numbers outside 0 .. buckets - 1 count as the nearest), far <= 1024; either may be null. A
+ * bias below -1e30 hides its keys, as -infinity does. prefix: int32 [batch] or null: in
+ * a causal segment keys j < prefix[b] are seen by all queries. cap is 0 or 1e-6 to 1024; with slopes the scale is
+ * at least 1e-30; a bias takes LDS for the query heads of a key head: (heads_q / heads_k) * (2 far
+ * + 257 and up to 63 more) * 4 bytes <= 72 KB. */
+typedef struct hi3d_attention_terms {
+  const float* slopes;
+  const void* bias;
+  const int32_t* bucket_map;
+  const int32_t* prefix;
+  int32_t bias_dtype;
+  int32_t buckets;
+  int32_t far;
+  float cap;
+} hi3d_attention_terms;
+
+/* hi3d_attention_workspace, hi3d_attention_forward and the gradients with those terms. dbias_dev
+ * [buckets, heads_q] in the bias's type (may be null): the sums of the scores' gradients by bucket,
+ * in a fixed order. No gradient is formed of slopes. */
+int hi3d_attention_terms_workspace(const hi3d_attention_desc* desc_host, const hi3d_attention_terms* terms_host,
+                                   int64_t* bytes_host);
+int hi3d_attention_terms_forward(const hi3d_attention_desc* desc_host, const hi3d_attention_terms* terms_host,
+                                 void* out_dev, float* lse_dev, void* workspace_dev, int64_t workspace_bytes,
+                                 void* stream);
+int hi3d_attention_terms_backward_workspace(const hi3d_attention_desc* desc_host,
+                                            const hi3d_attention_terms* terms_host, int64_t* bytes_host);
+int hi3d_attention_terms_backward(const hi3d_attention_desc* desc_host, const hi3d_attention_terms* terms_host,
+                                  const void* out_dev, const float* lse_dev, const void* dout_dev,
+                                  const float* dlse_dev, void* dq_dev, void* dk_dev, void* dv_dev, void* dbias_dev,
+                                  void* workspace_dev, int64_t workspace_bytes, void* stream);
+
+/* Keys and values [len, heads_k, dim] that all sequences of a batch share in front of their own:
+ * element (j, h, d) at j * strides[0] + h * strides[1] + d of k, strides[2], [3] of v; key_mask uint8
+ * [len] or null. */
+typedef struct hi3d_attention_shared {
+  const void* k;
+  const void* v;
+  const uint8_t* key_mask;
+  int64_t strides[4];
+  int32_t len;
+} hi3d_attention_shared;
+
+/* hi3d_attention_terms_forward of segments without offsets whose queries all see the shared keys
+ * first, read once for the batch; relative positions count from a sequence's own keys on, so shared key j
+ * stands at j - len. desc's lens_k, causal and key_mask belong to the sequences' own keys;
+ * terms_host->prefix is null. Forward only. */
+int hi3d_attention_shared_workspace(const hi3d_attention_desc* desc_host, const hi3d_attention_terms* terms_host,
+                                    const hi3d_attention_shared* shared_host, int64_t* bytes_host);
+int hi3d_attention_shared_forward(const hi3d_attention_desc* desc_host, const hi3d_attention_terms* terms_host,
+                                  const hi3d_attention_shared* shared_host, void* out_dev, float* lse_dev,
+                                  void* workspace_dev, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
