@@ -18,6 +18,8 @@
 // LDS tiles are rows of DP values (DP = head size rounded up to 32).
 #pragma once
 
+#include <type_traits>
+
 #include "common.h"
 #include "conv_tile.h"
 
@@ -302,11 +304,20 @@ __device__ __forceinline__ bool sees_key(uint64_t bits, int j) {
   return __builtin_amdgcn_inverse_ballot_w64(lo | hi);
 }
 
+// fp16 holds what its own rounding took from the output times 2^11.
+template <typename T>
+constexpr float kRest = std::is_same_v<T, _Float16> ? 2048.0f : 1.0f;
+
 // Writes 32 accumulated rows (lane l: row l % 32, columns 32 d + 8 e + 4 (l / 32) ..) times
 // `by` as T. The lane halves exchange every second group of 4 columns, so that each stores 8
-// adjacent ones.
-template <typename T, int DP>
+// adjacent ones. REST: what that rounding takes.
+template <typename T, int DP, bool REST = false>
 __device__ __forceinline__ void store_row(T* to, int dim, int h, const f32x16* acc, int step, float by) {
+  auto rounded = [&](float x) -> T {
+    x *= by;
+    if constexpr (!REST) return static_cast<T>(x);
+    else return static_cast<T>((x - static_cast<float>(static_cast<T>(x))) * kRest<T>);
+  };
   typedef T t4 __attribute__((ext_vector_type(4)));
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d)
@@ -315,8 +326,8 @@ __device__ __forceinline__ void store_row(T* to, int dim, int h, const f32x16* a
       t4 x, y;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        x[j] = static_cast<T>(acc[d * step][4 * e + j] * by);
-        y[j] = static_cast<T>(acc[d * step][4 * e + 4 + j] * by);
+        x[j] = rounded(acc[d * step][4 * e + j]);
+        y[j] = rounded(acc[d * step][4 * e + 4 + j]);
       }
       const u32x2 a = __builtin_bit_cast(u32x2, x), b = __builtin_bit_cast(u32x2, y);
       const uint32_t a0 = a[0], a1 = a[1], b0 = b[0], b1 = b[1];

@@ -95,7 +95,7 @@ int hi3d_attention_forward(const hi3d_attention_desc* d, void* out, float* lse, 
     a.part_ml = a.part + static_cast<int64_t>(splits) * a.total_q * a.hq * a.dim;
   }
   hipStream_t stream = as_stream(stream_);
-  return d->dtype == HI3D_F16 ? launch_attend_type<_Float16, false>(a, stream) : launch_attend_type<__bf16, false>(a, stream);
+  return d->dtype == HI3D_F16 ? launch_attend_type<_Float16, 0>(a, stream) : launch_attend_type<__bf16, 0>(a, stream);
 }
 
 }  // extern "C"

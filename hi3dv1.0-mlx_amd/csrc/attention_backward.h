@@ -73,39 +73,76 @@ __device__ __forceinline__ float wave_max(float x) {
 // just that. Rows that see at most 4 tiles of keys take one walk more to find and mend it:
 // gradients of 16 to 128 causal keys come from 1.7-1.55 times the error of a single rounding
 // down to 1.42 (sqrt 2); above that many keys the miss is below a tenth of ds's rounding.
+// Scores with terms are sharp in rows of many keys too (a cap lets them be, slopes leave few keys). There
+// the forward also keeps what its rounding took from the output (TermArgs::rest), which gives D its
+// digits, and where it did not the walk is taken for every row: dq and dk of capped scores of
+// standard deviation 4 come from 2.0 times the error of a single rounding down to 1.2.
 constexpr int kExactTiles = 4;
 
-// The bias's gradient: ds of a tile (without the cap's derivative; `unscale` takes its scale out and
-// is 0 for rows that are not there) joins the sums of its relative positions in `sums`, this lane
-// half's own; past `far` only the side counts.
-__device__ __forceinline__ void sum_bias(const TermArgs& a, const RowTerms<1>& w, const f32x16& ds, int k0, int n, int h,
-                                         float unscale, float* sums, float (&far_sums)[2]) {
+// The bias's gradient, one query head of a wave's 32 rows at consecutive places. ds of 8 keys at a time
+// (without the cap's derivative; `unscale` takes its scale out and is 0 for rows that are not there)
+// goes to LDS row by row, and each lane sums one relative position down its 8 keys (rows of zeros
+// stand in for those outside): rows of 9, so that neither side's accesses share banks. LDS float
+// atomics took 175 cycles each here (dq of 8,191 rows x 33 heads x 64: 838 us for TODO). Of the 63
+// positions that 32 keys give the lower half is complete, and each is written once in a wave's life; the
+// upper half waits in `carry` for the next 32 keys. Keys of tiles past `far` only count by their side.
+struct BiasSums {
+  float carry = 0.0f, far[2] = {0.0f, 0.0f};
+  int next = 0;      // place (of sums) of lane 0 in the next 32 keys
+  bool open = false;  // carry holds something
+};
+
+__device__ __forceinline__ void close_sums(BiasSums& b, float* sums, int lane) {
+  if (b.open && lane >= 32 && lane < 63) sums[b.next + lane - 32] = b.carry;
+  b.carry = 0.0f, b.open = false;
+}
+
+__device__ __forceinline__ void sum_bias(const TermArgs& a, const RowTerms<1>& w, const f32x16& ds, int k0, int n, float unscale,
+                                         float* skew, float* sums, BiasSums& b) {
   const bool before = k0 + kKT - 1 - w.first <= -a.far, after = k0 - w.last >= a.far;
   if (before || after) {
     float x = 0.0f;
 #pragma unroll
     for (int e = 0; e < 16; ++e) x += ds[e];
-    if (before) far_sums[0] += x;
-    else far_sums[1] += x;
-  } else {
-    float* at = sums + min(max(k0 + 4 * h - w.place[0] + a.far + kPad, 0), 2 * a.far + kPad) + 32 * n;
-#pragma unroll
-    for (int e = 0; e < 16; ++e)
-      __hip_atomic_fetch_add(at + 8 * (e >> 2) + (e & 3), ds[e] * unscale, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    if (before) b.far[0] += x;
+    else b.far[1] += x;
+    return;
   }
+  const int lane = fresh_lane(), c32 = lane & 31, h = lane >> 5;
+  const int at = k0 + 32 * n - w.first - 31 + a.far + kPadSums;  // of lane 0's position
+  if (b.open && b.next != at) close_sums(b, sums, lane);
+  float* to = skew + (7 + c32) * kSkewRow + 4 * h;
+  float x = 0.0f;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    asm volatile("" ::: "memory");  // a wave's LDS operations run in order
+#pragma unroll
+    for (int e = 0; e < 4; ++e) to[e] = ds[4 * g + e] * unscale;
+    asm volatile("" ::: "memory");
+    const int row = 38 + 8 * g - lane;  // of the lane's first key
+    const float* from = skew + min(max(row, 0), 38) * kSkewRow;
+    float y = 0.0f, z = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) y += from[j * (kSkewRow + 1)], z += from[(j + 1) * (kSkewRow + 1)];
+    x += row >= 0 && row <= 38 ? y + z : 0.0f;
+  }
+  asm volatile("" ::: "memory");
+  float lo, hi;
+  both_halves(b.carry, lo, hi);
+  if (lane < 32) sums[at + lane] = x + hi;
+  b.carry = x, b.next = at + 32, b.open = true;
 }
 
-// A workgroup's sums by relative position for attend_dbias_kernel: those of its waves' lane halves in
-// order, or zeros.
+// A workgroup's sums by relative position for attend_dbias_kernel: those of its waves in order, or zeros.
 template <int NW>
 __device__ __forceinline__ void write_part(const TermArgs& a, int head, int slot, const float* sums) {
-  const int length = 2 * (a.far + kPad) + 1;
+  const int length = sum_length(a.far);
   float* to = a.dbias + (static_cast<int64_t>(head) * a.slots + slot) * length;
   for (int x = threadIdx.x; x < length; x += 64 * NW) {
     float v = 0.0f;
     if (sums != nullptr) {
 #pragma unroll
-      for (int c = 0; c < 2 * NW; ++c) v += sums[c * a.stride + x];
+      for (int c = 0; c < NW; ++c) v += sums[c * sum_stride(a.far) + x];
     }
     to[x] = v;
   }
@@ -121,7 +158,7 @@ __device__ __forceinline__ void write_part(const TermArgs& a, int head, int slot
 // and vector operations, which 2 or 3 waves a SIMD overlap in part: 8,191 rows x 33 heads x 64
 // fp16 in four segments 264 us (805 TFLOP/s of its 3 products), 8,192 causal x 32/8 heads x 128
 // bf16 414 us (995).
-template <typename T, int DP, int NW, bool Z, bool TERMS>
+template <typename T, int DP, int NW, bool Z, int TERMS>
 __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(ArgsOf<TERMS> a) {
   constexpr int ROWS = NW * 32, KS = DP / 16, DB = DP / 32, PAIR = 2 * kTile<DP>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -142,9 +179,9 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(ArgsOf<TERMS> a) 
   float* bound = a.bound + (static_cast<int64_t>(head) * a.slots + slot) * NW + wave;
   int key_head = head;
   bool sums = false;  // the bias's gradient is formed too
-  if constexpr (TERMS) key_head = head / a.share, sums = a.dbias != nullptr;  // rows of one query head (group is 1)
+  if constexpr (TERMS != 0) key_head = head / a.share, sums = has_bias<TERMS>(a) && a.dbias != nullptr;  // rows of one query head (group is 1)
   if (s.tile < 0 || row0 >= rows) {
-    if constexpr (TERMS)
+    if constexpr (TERMS != 0)
       if (sums) write_part<NW>(a, head, slot, nullptr);
     return;
   }
@@ -164,9 +201,14 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(ArgsOf<TERMS> a) 
                  static_cast<int64_t>(head * a.group + qg) * a.q_h;
   load_owned<DP>(reinterpret_cast<const char*>(src), a.dim, h, true, qf);
   load_owned<DP>(reinterpret_cast<const char*>(static_cast<const T*>(a.dout) + at * a.dim), a.dim, h, true, df);
-  u32x4 of[KS];
+  u32x4 of[KS], rest[KS];
   load_owned<DP>(reinterpret_cast<const char*>(static_cast<const T*>(a.o) + at * a.dim), a.dim, h, true, of);
-  float x = 0.0f, y = 0.0f;
+  bool with_rest = false;
+  if constexpr (TERMS != 0) {
+    with_rest = a.rest != nullptr;
+    load_owned<DP>(reinterpret_cast<const char*>(static_cast<const T*>(a.rest) + at * a.dim), a.dim, h, with_rest, rest);
+  }
+  float x = 0.0f, y = 0.0f, z = 0.0f;
 #pragma unroll
   for (int k = 0; k < KS; ++k) {
     const auto u = __builtin_bit_cast(typename Vec8<T>::type, df[k]), v = __builtin_bit_cast(typename Vec8<T>::type, of[k]);
@@ -175,11 +217,17 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(ArgsOf<TERMS> a) 
       x = __builtin_fmaf(static_cast<float>(u[e]), static_cast<float>(v[e]), x);
       y += __builtin_fabsf(static_cast<float>(u[e]));
     }
+    if constexpr (TERMS != 0) {
+      const auto r = __builtin_bit_cast(typename Vec8<T>::type, rest[k]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) z = __builtin_fmaf(static_cast<float>(u[e]), static_cast<float>(r[e]), z);
+    }
   }
+  if constexpr (TERMS != 0) x = __builtin_fmaf(z, 1.0f / kRest<T>, x);
   float delta = half_sum(x), size = half_sum(y);  // D, sum |dout|
   if (a.dlse != nullptr) {
-    const float z = a.dlse[at];
-    delta -= z, size = fmaxf(size, __builtin_fabsf(z));
+    const float dlse = a.dlse[at];
+    delta -= dlse, size = fmaxf(size, __builtin_fabsf(dlse));
   }
   const float lse = a.lse[at];
   const bool none = lse == -INFINITY;  // a row that sees no key: all its scores are hidden
@@ -189,13 +237,14 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(ArgsOf<TERMS> a) 
     if (lane == 0) *bound = wrow < rows ? x : 0.0f;
   }
   const int exponent = ds_exponent<T>(size);
-  const float by = power_of_two(exponent - static_cast<int>(kPLog2<T>));  // of dp - D: the scale of ds without that of p
+  float by = power_of_two(exponent - static_cast<int>(kPLog2<T>));  // of dp - D: the scale of ds without that of p
+  if constexpr (TERMS != 0) by *= has_cap<TERMS>(a) ? -4.0f : 1.0f;  // add_terms keeps the cap's derivative times -1/4
   delta *= by;
   const float dq_by = a.scale * power_of_two(-exponent);  // takes the scale out of dq
   auto store_stats = [&]() {  // for the rows' part in dk and dv: lse in powers of two, and D
     const int r = wrow + c32;
     int64_t at = (head * a.total_q + s.q0) * a.group + r;
-    if constexpr (TERMS) at = (key_head * a.total_q + s.q0 + r) * a.share + (head - key_head * a.share);
+    if constexpr (TERMS != 0) at = (key_head * a.total_q + s.q0 + r) * a.share + (head - key_head * a.share);
     if (h == 0 && r < rows) a.lse2[at] = none ? INFINITY : ref, a.delta[at] = none ? 0.0f : delta / by;
   };
   const int seen_by_all = first_keys<TERMS>(a, s);
@@ -235,24 +284,29 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(ArgsOf<TERMS> a) 
                          [&](int row) { return Z ? ((bits >> row) & 1 ? row : shown) : (row < last ? row : last); });
   };
 
-  // TERMS: the head's bias in LDS, and behind it the sums of its gradient, a copy for each lane half
-  // of each wave: one lane adds to a place in one instruction, so the order is always the same
+  // TERMS: the head's bias in LDS, and behind it each wave's sums of its gradient and room for a tile's part
   RowTerms<1> terms;
   bool capped = false;
-  float* table = nullptr;
-  float far_sums[2] = {0.0f, 0.0f};  // of keys past `far`, before and behind the row
-  if constexpr (TERMS) {
-    capped = a.cap2 > 0.0f;
+  float *table = nullptr, *bias_sums = nullptr, *skew = nullptr;
+  BiasSums part;
+  if constexpr (TERMS != 0) {
+    capped = has_cap<TERMS>(a);
     table = reinterpret_cast<float*>(smem + 2 * PAIR + (Z ? kBiasBytes : 0));
     const int is[1] = {qi}, gs[1] = {0};
     row_terms<1>(a, s, terms, table, head, wrow, rows, is, gs);
-    if (a.bias != nullptr) {  // the barrier in front of the first tile is these loops' too
+    if (has_bias<TERMS>(a)) {  // the barrier in front of the first tile is these loops' too
       stage_bias<kPad>(a, table, a.stride, head, 1, 0, 2 * (a.far + kPad) + 1, threadIdx.x, 64 * NW);
-      if (sums)
-        for (int x = threadIdx.x; x < 2 * NW * a.stride; x += 64 * NW) table[a.stride + x] = 0.0f;
+      if (sums) {
+        bias_sums = table + a.stride + wave * sum_stride(a.far);
+        skew = table + a.stride + NW * sum_stride(a.far) + wave * kSkew;
+        for (int x = threadIdx.x; x < NW * (sum_stride(a.far) + kSkew); x += 64 * NW) table[a.stride + x] = 0.0f;
+      }
     }
   }
-  const float unscale = wrow + c32 < rows ? power_of_two(-exponent) : 0.0f;  // takes the scale out of ds
+  constexpr bool FOLD = TERMS == kSlopes;
+  std::conditional_t<FOLD, SideProduct<T>, char> side;
+  if constexpr (FOLD) side.set(terms.slope[0] * a.per_mul, h);
+  const float unscale = wrow + c32 < rows ? power_of_two(-exponent) * (capped ? -0.25f : 1.0f) : 0.0f;  // of ds
   f32x16 acc[DB];
   float miss;
   // one tile; hide: some keys are hidden from some rows; EXACT: only sums ds
@@ -263,13 +317,21 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(ArgsOf<TERMS> a) 
       f32x16 scs[1][1] = {}, dp = {}, bend;
       f32x16& sc = scs[0][0];
       if (Z && !capped) sc = read_bias(tile_bias, n, h);
+      bool folded = false;
+      if constexpr (FOLD) {
+        const bool after = t * kKT >= terms.last;
+        folded = side.on && (after || (t + 1) * kKT - 1 <= terms.first);
+        // a product with zeros where it does not hold: a branch would copy the scores
+        const u32x4 slope = (side.slope ^ (after ? 0x80008000u : 0u)) & (folded ? ~0u : 0u);
+        Mfma<T>::run(SideProduct<T>::keys(n, c32), slope, sc);
+      }
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         const u32x4 x = read_rows<DP>(kt, 32 * n, k, place_of), y = read_rows<DP>(vt, 32 * n, k, place_of);
         Mfma<T>::run(x, qf[k], sc), Mfma<T>::run(y, df[k], dp);
       }
       float mul = a.scale2, add[1];
-      if constexpr (TERMS) mul = add_terms<1, 1, true>(a, terms, scs, t * kKT, n, h, add, &bend);
+      if constexpr (TERMS != 0) mul = add_terms<TERMS, 1, 1, true>(a, terms, scs, t * kKT, n, h, folded, add, &bend);
       const float less = TERMS ? add[0] - ref : -ref;
       if (hide) {
         asm volatile("");  // a branch, not 16 selects for every tile
@@ -293,8 +355,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(ArgsOf<TERMS> a) 
 #pragma unroll
         for (int e = 0; e < 16; ++e) miss += dp[e];
       } else {
-        if constexpr (TERMS) {
-          if (sums) sum_bias(a, terms, dp, t * kKT, n, h, unscale, table + (1 + 2 * wave + h) * a.stride, far_sums);
+        if constexpr (TERMS != 0) {
+          if (sums) sum_bias(a, terms, dp, t * kKT, n, unscale, skew, bias_sums, part);
           if (capped) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) dp[e] *= bend[e];
@@ -338,7 +400,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(ArgsOf<TERMS> a) 
     }
   };
   if (Z && a.dim < DP) clear_tiles(smem, 2 * PAIR);
-  if (tiles > 0 && tiles <= kExactTiles) {
+  if (tiles > 0 && (tiles <= kExactTiles || (TERMS && !with_rest))) {
     miss = 0.0f;
     pass(std::true_type{});
     // sum ds was to be dlse
@@ -350,14 +412,16 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(ArgsOf<TERMS> a) 
 #pragma unroll
   for (int d = 0; d < DB; ++d) acc[d] = f32x16{};
   if (tiles > 0) pass(std::false_type{});
-  if constexpr (TERMS)
+  if constexpr (TERMS != 0)
     if (sums) {
+      close_sums(part, bias_sums, lane);
+      asm volatile("" ::: "memory");
 #pragma unroll
       for (int side = 0; side < 2; ++side) {
-        float x = half_sum(far_sums[side] * unscale);
+        float x = half_sum(part.far[side] * unscale);
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) x += __shfl_xor(x, d);
-        if (lane == 0) table[(1 + 2 * wave) * a.stride + side * 2 * (a.far + kPad)] += x;
+        if (lane == 0) bias_sums[side * (sum_length(a.far) - 1)] += x;
       }
       __syncthreads();
       write_part<NW>(a, head, slot, table + a.stride);
@@ -389,22 +453,22 @@ __device__ __forceinline__ TileSides tile_sides(const TermArgs& a, const Segment
   return {key0 + KEYS - 1 <= first, key0 >= last, !left && !right, left};
 }
 
-template <int KEYS>
+template <int TERMS, int KEYS>
 __device__ __forceinline__ void stage_key_terms(const TermArgs& a, const Segment& s, int key0, int head, int r, int t, int rows,
                                                 const float* table, float* to) {
-  if (a.slopes == nullptr && a.bias == nullptr) return;
+  if (!has_slopes<TERMS>(a) && !has_bias<TERMS>(a)) return;
   const TileSides side = tile_sides<KEYS>(a, s, key0, t, rows);
   int i, g;
   split_row(a, min(r, rows - 1), i, g);
   const int lane = r - t * kKT, place = i + s.lk - s.lq - key0;
   float constant = 0.0f;
-  if (a.slopes != nullptr) {
+  if (has_slopes<TERMS>(a)) {
     const float slope = a.slopes[head * a.group + g] * kLog2e, by = side.before ? slope : -slope;
     if (side.before || side.after) constant = -by * static_cast<float>(place);
     to[kKT + lane] = by;
     to[2 * kKT + lane] = static_cast<float>(place);
   }
-  if (a.bias != nullptr) {
+  if (has_bias<TERMS>(a)) {
     const float* of = table + g * a.stride_keys;
     if (!side.near) constant += of[side.left ? 0 : 2 * (a.far + kPadKeys)];
     reinterpret_cast<int*>(to)[3 * kKT + lane] = g * a.stride_keys + a.far + kPadKeys - min(max(place, -a.far), a.far + kPadKeys);
@@ -412,71 +476,77 @@ __device__ __forceinline__ void stage_key_terms(const TermArgs& a, const Segment
   to[lane] = constant;
 }
 
-// Takes D from dp and adds the terms to scores sc of rows 32 n + 8 (e / 4) + 4 h + e % 4 of the tile
-// and the lane's key `key` of the workgroup; with a cap dp takes its derivative. Scores in powers of
-// two are then sc times the returned factor.
-template <int KEYS>
-__device__ __forceinline__ float add_key_terms(const TermArgs& a, const Segment& s, f32x16& sc, f32x16& dp, const float* st,
-                                               int key0, int key, int t, int n, int rows, const float* table) {
+// Takes D from dp and adds the terms to scores sc of rows 32 n + 8 (e / 4) + 4 h + e % 4 of the tile and
+// the lane's key `key` of the workgroup. Scores in powers of two are then sc * mul + base; with a cap dp
+// takes its derivative, times -1/4. folded: distances are in the scores already.
+template <int TERMS, int KEYS>
+__device__ __forceinline__ void add_key_terms(const TermArgs& a, f32x16& sc, f32x16& dp, const float* st, int key, int n,
+                                              const float* table, const TileSides& side, bool folded, float& mul, float& base) {
+  typedef int i32x4 __attribute__((ext_vector_type(4)));
   const int from = 32 * n + 4 * (fresh_lane() >> 5);
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
     const f32x4 d4 = *reinterpret_cast<const f32x4*>(st + kKT + from + 8 * g);
 #pragma unroll
     for (int e = 0; e < 4; ++e) dp[4 * g + e] -= d4[e];
+    __builtin_amdgcn_sched_barrier(0);  // four numbers in flight: more would cost registers that are not there
   }
-  float mul = a.scale2;
-  if (a.cap2 > 0.0f) {
-    mul = 2.0f * a.cap2;
+  // each term behind a branch of its own, also where it is the only one: in one straight line they are
+  // scheduled into registers that keys and values then have to leave
+  mul = a.scale2, base = 0.0f;
+  if (has_cap<kAll>(a)) {
+    mul = 2.0f * a.cap2, base = a.cap2;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       const float u = minus_u(a, sc[e]);
       sc[e] = u;
-      dp[e] *= __builtin_fmaf(-4.0f * u, u, -4.0f * u);
+      dp[e] *= __builtin_fmaf(u, u, u);
     }
   }
-  if (a.cap2 > 0.0f || a.slopes != nullptr || a.bias != nullptr) {
-    const bool more = a.slopes != nullptr || a.bias != nullptr;
+  const bool slopes = has_slopes<kAll>(a) && !folded, bias = has_bias<kAll>(a);
+  if (bias && !slopes && !side.near && a.group == 1) {
+    base += table[side.left ? 0 : 2 * (a.far + kPadKeys)];
+    return;
+  }
+  if (!slopes && !bias) return;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      f32x4 c4 = {0, 0, 0, 0};
-      if (more) c4 = *reinterpret_cast<const f32x4*>(st + 2 * kKT + from + 8 * g);
+  for (int g = 0; g < 4; ++g) {
+    const f32x4 c4 = *reinterpret_cast<const f32x4*>(st + 2 * kKT + from + 8 * g);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sc[4 * g + e] = __builtin_fmaf(sc[4 * g + e], mul, c4[e] + a.cap2);
-    }
-    mul = 1.0f;
-    if (!more) return mul;
-    const TileSides side = tile_sides<KEYS>(a, s, key0, t, rows);
-    if (a.slopes != nullptr) {
-      const float x = static_cast<float>(key);
-      if (side.before || side.after) {
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const f32x4 s4 = *reinterpret_cast<const f32x4*>(st + 3 * kKT + from + 8 * g);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sc[4 * g + e] = __builtin_fmaf(s4[e], x, sc[4 * g + e]);
-        }
-      } else {
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const f32x4 s4 = *reinterpret_cast<const f32x4*>(st + 3 * kKT + from + 8 * g);
-          const f32x4 p4 = *reinterpret_cast<const f32x4*>(st + 4 * kKT + from + 8 * g);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sc[4 * g + e] = __builtin_fmaf(s4[e], __builtin_fabsf(x - p4[e]), sc[4 * g + e]);
-        }
-      }
-    }
-    if (a.bias != nullptr && side.near) {
-      typedef int i32x4 __attribute__((ext_vector_type(4)));
+    for (int e = 0; e < 4; ++e) sc[4 * g + e] = __builtin_fmaf(sc[4 * g + e], mul, c4[e]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  mul = 1.0f;
+  if (slopes) {
+    const float x = static_cast<float>(key);
+    if (side.before || side.after) {
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const i32x4 x4 = *reinterpret_cast<const i32x4*>(st + 5 * kKT + from + 8 * g);
+        const f32x4 s4 = *reinterpret_cast<const f32x4*>(st + 3 * kKT + from + 8 * g);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[4 * g + e] += table[x4[e] + key];
+        for (int e = 0; e < 4; ++e) sc[4 * g + e] = __builtin_fmaf(s4[e], x, sc[4 * g + e]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 s4 = *reinterpret_cast<const f32x4*>(st + 3 * kKT + from + 8 * g);
+        const f32x4 p4 = *reinterpret_cast<const f32x4*>(st + 4 * kKT + from + 8 * g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[4 * g + e] = __builtin_fmaf(s4[e], __builtin_fabsf(x - p4[e]), sc[4 * g + e]);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
-  return mul;
+  if (bias && side.near) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const i32x4 x4 = *reinterpret_cast<const i32x4*>(st + 5 * kKT + from + 8 * g);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sc[4 * g + e] += table[x4[e] + key];
+    }
+  }
+  __builtin_amdgcn_sched_barrier(0);
 }
 
 // dk and dv. A workgroup owns NW * 32 keys of one key head (keys and values in
@@ -494,7 +564,7 @@ __device__ __forceinline__ float add_key_terms(const TermArgs& a, const Segment&
 //
 // Causal: early keys see the most rows, so their blocks start first, and each block is split
 // at least in two, which levels the ends (1008 us to 623, with 25 for the join).
-template <typename T, int DP, int NW, bool Z, bool SPLIT, bool TERMS>
+template <typename T, int DP, int NW, bool Z, bool SPLIT, int TERMS>
 __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(ArgsOf<TERMS> a) {
   constexpr int KEYS = NW * 32, KS = DP / 16, DB = DP / 32, PAIR = 2 * kTile<DP>, CH = DP / 8;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -591,8 +661,8 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
     dv_by = power_of_two(-static_cast<int>(kPLog2<T>));
   }
   float* table = stats + 2 * STATS;
-  if constexpr (TERMS)
-    if (a.bias != nullptr) {
+  if constexpr (TERMS != 0)
+    if (has_bias<TERMS>(a)) {
       stage_bias<kPadKeys>(a, table, a.stride_keys, head * a.group, a.group, 0, 2 * (a.far + kPadKeys) + 1, threadIdx.x,
                            64 * NW);
       __syncthreads();
@@ -602,29 +672,59 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
   auto load_stats = [&](int t, int buf) {
     const int r = t * kKT + fresh_lane();
     float* to = stats + buf * STATS;
-    if constexpr (TERMS) stage_key_terms<KEYS>(a, s, key0, head, r, t, rows, table, to + 2 * kKT);
+    if constexpr (TERMS != 0) stage_key_terms<TERMS, KEYS>(a, s, key0, head, r, t, rows, table, to + 2 * kKT);
     lds_dma4(r < rows ? a.lse2 + stats_at + r : &kPastRows[0], reinterpret_cast<char*>(to));
     lds_dma4(r < rows ? a.delta + stats_at + r : &kPastRows[1], reinterpret_cast<char*>(to + 64));
   };
+  constexpr bool FOLD = TERMS == kSlopes;
+  bool folds = false;
+  u32x4* side_at = reinterpret_cast<u32x4*>(table);  // [2][64], no bias then
+  if constexpr (FOLD) {
+    if (64 % a.group == 0) {
+      float most = 0.0f;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {  // every wave the same
+        const int r = 32 * n + c32, i = r / a.group;
+        const float t = a.slopes[head * a.group + r - i * a.group] * kLog2e * a.per_mul;
+        side_at[n * 64 + lane] = SideProduct<T>::of_row(t, i, h);
+        most = fmaxf(most, __builtin_fabsf(t));
+      }
+      folds = !__any(most > 1000.0f);
+    }
+  }
+  if constexpr (TERMS != 0) by *= has_cap<TERMS>(a) ? -4.0f : 1.0f;  // add_key_terms has the derivative times -1/4
   f32x16 dk[DB] = {}, dv[DB] = {};
   // one tile; hide: some rows do not see some keys
   auto walk = [&](const char* qt, const float* st, int t, bool hide) {
-    const TileLane place_of = tile_lane<DP>(DP == 128 ? fresh_lane() : lane);
+    const TileLane place_of = tile_lane<DP>(DP == 128 || TERMS ? fresh_lane() : lane);
     const char* dt = qt + kTile<DP>;
+    TileSides side = {};
+    bool folded = false;
+    int distance = 0;  // of the segment's first key to the tile's first row
+    if constexpr (TERMS != 0) {
+      if (has_slopes<kAll>(a) || has_bias<kAll>(a)) side = tile_sides<KEYS>(a, s, key0, t, rows);
+      if constexpr (FOLD) {
+        distance = -(t * kKT / a.group + off);
+        folded = folds && (side.before || side.after) && max(abs(distance + key0), abs(distance + key0 + KEYS)) <= SideProduct<T>::kFarthest;
+      }
+    }
 #pragma unroll 2
     for (int n = 0; n < 2; ++n) {
       f32x16 sc = {}, dp = {};
+      if constexpr (FOLD) {  // a product with zeros where it does not hold: a branch would copy the scores
+        const int l = fresh_lane();
+        const u32x4 far = SideProduct<T>::of_key(distance + wkey + (l & 31), l >> 5) ^ (side.after ? 0x80008000u : 0u);
+        Mfma<T>::run(side_at[n * 64 + l], far & (folded ? ~0u : 0u), sc);
+      }
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         const u32x4 x = read_rows<DP>(qt, 32 * n, k, place_of), y = read_rows<DP>(dt, 32 * n, k, place_of);
         Mfma<T>::run(x, kf[k], sc), Mfma<T>::run(y, vf[k], dp);
       }
       __builtin_amdgcn_sched_barrier(0);
-      float mul = a.scale2;
-      if constexpr (TERMS) {
-        mul = add_key_terms<KEYS>(a, s, sc, dp, st, key0, wkey - key0 + (fresh_lane() & 31), t, n, rows, table);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+      float mul = a.scale2, base = 0.0f;  // scores in powers of two are sc * mul + base
+      if constexpr (TERMS != 0)
+        add_key_terms<TERMS, KEYS>(a, sc, dp, st, wkey - key0 + (fresh_lane() & 31), n, table, side, folded, mul, base);
       if (hide) {
         asm volatile("");  // a branch, not 16 selects for every tile
         const int l = fresh_lane();  // first packed row that sees the lane's key, from the lane's first on
@@ -645,7 +745,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int at = 8 * k + 4 * g + e;
-            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[at], mul, -l4[e]));
+            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[at], mul, TERMS ? base - l4[e] : -l4[e]));
             ps[4 * g + e] = x, dss[4 * g + e] = (x * by) * (TERMS ? dp[at] : dp[at] - d4[e]);
           }
         }
@@ -727,12 +827,12 @@ __global__ __launch_bounds__(256) void attend_dbias_sum_kernel(const float* from
 __global__ __launch_bounds__(256) void attend_dbias_kernel(TermArgs a, const float* parts, int64_t count, void* out) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   float* total = reinterpret_cast<float*>(smem);
-  const int length = 2 * (a.far + kPad) + 1, head = blockIdx.x;
+  const int length = sum_length(a.far), head = blockIdx.x;
   int* bucket = reinterpret_cast<int*>(total + length);
   for (int x = threadIdx.x; x < length; x += 256) {
     float v = 0.0f;
     for (int64_t i = 0; i < count; ++i) v += parts[(head * count + i) * length + x];
-    total[x] = v, bucket[x] = bucket_at(a, x, kPad);
+    total[x] = v, bucket[x] = bucket_at(a, x, kPadSums);
   }
   __syncthreads();
   const int lane = threadIdx.x & 63;
@@ -749,7 +849,7 @@ __global__ __launch_bounds__(256) void attend_dbias_kernel(TermArgs a, const flo
   }
 }
 
-template <typename T, int DP, int NW, bool TERMS>
+template <typename T, int DP, int NW, int TERMS>
 int launch_dq(ArgsOf<TERMS> a, hipStream_t stream) {
   constexpr int rows = NW * 32;
   HI3D_REQUIRE(static_cast<int64_t>(a.dq_slots) * a.hk < (1ll << 31), "too many rows for one launch");
@@ -757,17 +857,18 @@ int launch_dq(ArgsOf<TERMS> a, hipStream_t stream) {
   a.slots = a.dq_slots;
   const int64_t blocks = static_cast<int64_t>(a.slots) * a.hk;
   size_t lds = 4 * kTile<DP>;
-  if constexpr (TERMS) lds += term_bytes<true>(a) * (a.dbias != nullptr ? 1 + 2 * NW : 1);
+  if constexpr (TERMS != 0) lds += term_bytes<kAll>(a) + (a.dbias != nullptr ? NW * (sum_stride(a.far) + kSkew) * 4 : 0);
   return a.mask != nullptr || a.dim < DP
              ? launch_tiles<&attend_dq_kernel<T, DP, NW, true, TERMS>>(a, blocks, 64 * NW, lds + kBiasBytes, stream)
              : launch_tiles<&attend_dq_kernel<T, DP, NW, false, TERMS>>(a, blocks, 64 * NW, lds, stream);
 }
 
-template <typename T, int DP, int NW, bool TERMS>
+template <typename T, int DP, int NW, int TERMS>
 int launch_dkv(ArgsOf<TERMS> a, hipStream_t stream) {
   constexpr int keys = NW * 32, threads = 64 * NW;
   size_t lds = 4 * kTile<DP> + (TERMS ? 6 : 2) * kKT * 8;
-  if constexpr (TERMS) lds += a.bias != nullptr ? a.group * a.stride_keys * 4 : 0;
+  if constexpr (TERMS == kSlopes) lds += 2048;
+  else if constexpr (TERMS != 0) lds += a.bias != nullptr ? a.group * a.stride_keys * 4 : 0;
   const int64_t per = a.cu_k != nullptr ? packed_slots(a.total_k, 1, keys, a.batch) : ceil_div(a.len_k, keys) * a.batch;
   const int64_t blocks = per * a.hk * a.splits;
   HI3D_REQUIRE(blocks < (1ll << 31), "too many rows for one launch");
@@ -786,36 +887,40 @@ int launch_dkv(ArgsOf<TERMS> a, hipStream_t stream) {
   return HI3D_OK;
 }
 
-template <typename T, int DP, bool TERMS>
+// WIDE: workgroups of four waves only.
+template <typename T, int DP, int TERMS, bool WIDE>
 int launch_dq_dim(const ArgsOf<TERMS>& a, hipStream_t stream) {
-  return a.dq_waves == 1 ? launch_dq<T, DP, 1, TERMS>(a, stream) : launch_dq<T, DP, 4, TERMS>(a, stream);
+  if constexpr (!WIDE)
+    if (a.dq_waves == 1) return launch_dq<T, DP, 1, TERMS>(a, stream);
+  return launch_dq<T, DP, 4, TERMS>(a, stream);
 }
 
-template <typename T, int DP, bool TERMS>
+template <typename T, int DP, int TERMS, bool WIDE>
 int launch_grad_dim(const ArgsOf<TERMS>& a, hipStream_t stream) {
   if (a.total_q > 0) {
     int rc = HI3D_OK;
-    if constexpr (TERMS) {  // rows of one query head to a workgroup: one bias in LDS, with its sums
+    if constexpr (TERMS != 0) {  // rows of one query head to a workgroup: one bias in LDS, with its sums
       TermArgs b = a;
-      b.share = a.group, b.hk = a.hq, b.group = 1, b.stride = bias_stride(a.far, kPad, 1);
-      rc = launch_dq_dim<T, DP, true>(b, stream);
+      b.share = a.group, b.hk = a.hq, b.group = 1, b.stride = 2 * (a.far + kPad) + 4;
+      rc = launch_dq_dim<T, DP, TERMS, WIDE>(b, stream);
     } else {
-      rc = launch_dq_dim<T, DP, false>(a, stream);
+      rc = launch_dq_dim<T, DP, 0, WIDE>(a, stream);
     }
     if (rc != HI3D_OK) return rc;
   }
   if (a.total_k == 0 || a.dk == nullptr) return HI3D_OK;
-  if (ceil_div(a.total_k, a.batch) <= 32) return launch_dkv<T, DP, 1, TERMS>(a, stream);
+  if constexpr (!WIDE)
+    if (ceil_div(a.total_k, a.batch) <= 32) return launch_dkv<T, DP, 1, TERMS>(a, stream);
   return launch_dkv<T, DP, 4, TERMS>(a, stream);
 }
 
-template <typename T, bool TERMS>
+template <typename T, int TERMS, bool WIDE = false>
 int launch_grad_type(const ArgsOf<TERMS>& a, hipStream_t stream) {
   switch ((a.dim + 31) / 32) {
-    case 1: return launch_grad_dim<T, 32, TERMS>(a, stream);
-    case 2: return launch_grad_dim<T, 64, TERMS>(a, stream);
-    case 3: return launch_grad_dim<T, 96, TERMS>(a, stream);
-    default: return launch_grad_dim<T, 128, TERMS>(a, stream);
+    case 1: return launch_grad_dim<T, 32, TERMS, WIDE>(a, stream);
+    case 2: return launch_grad_dim<T, 64, TERMS, WIDE>(a, stream);
+    case 3: return launch_grad_dim<T, 96, TERMS, WIDE>(a, stream);
+    default: return launch_grad_dim<T, 128, TERMS, WIDE>(a, stream);
   }
 }
 

@@ -58,7 +58,7 @@ __device__ __forceinline__ void hide_keys(f32x16 (&sc)[2][QW], uint64_t bits) {
 // the next token's call would not find them there. Single tokens of 8 sequences over caches of
 // up to 65,536 x 8 x 128 bf16 (1.9 GB): 308 us, 6.1 TB/s (326 for 358 through the caches, in
 // turn on a slower card); below that size the cache helps (8 x 4,096 keys, 134 MB: 30.8 us for 32.3).
-template <typename T, int DP, int NW, int QW, bool Z, bool SPLIT, bool TERMS>
+template <typename T, int DP, int NW, int QW, bool Z, bool SPLIT, int TERMS>
 __global__ __launch_bounds__(64 * NW, DP <= 64 && NW * QW == 4 ? 3 : 2) void attend_kernel(ArgsOf<TERMS> a) {
   constexpr int ROWS = NW * QW * 32, KS = DP / 16, DB = DP / 32, PAIR = 2 * kTile<DP>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -95,7 +95,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 && NW * QW == 4 ? 3 : 2) void att
     split_row(a, r < rows ? r : rows - 1, qi[b], qg[b]);
     const T* src = static_cast<const T*>(a.q) + s.b * a.q_b + (a.cu_q != nullptr ? s.q0 + qi[b] : qi[b]) * a.q_n +
                    static_cast<int64_t>(head * a.group + qg[b]) * a.q_h;
-    if constexpr (TERMS)
+    if constexpr (TERMS != 0)
       if (a.per > 0) {  // rows of many sequences over what they share
         const int of = qi[b] / a.per;
         src += of * a.q_b - static_cast<int64_t>(of) * a.per * a.q_n;
@@ -156,17 +156,35 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 && NW * QW == 4 ? 3 : 2) void att
 
   RowTerms<QW> terms;
   bool capped = false;
-  if constexpr (TERMS) {
-    capped = a.cap2 > 0.0f;
+  if constexpr (TERMS != 0) {
+    capped = has_cap<TERMS>(a);
     float* table = reinterpret_cast<float*>(smem + 2 * PAIR + (Z ? kBiasBytes : 0));
     row_terms<QW>(a, s, terms, table, head, wrow, rows, qi, qg);
-    if (a.bias != nullptr)  // the barrier in front of the first tile is this one's too
+    if (has_bias<TERMS>(a))  // the barrier in front of the first tile is this one's too
       stage_bias<kPad>(a, table, a.stride, head * a.group, a.group, 0, 2 * (a.far + kPad) + 1, threadIdx.x, 64 * NW);
   }
   f32x16 acc[DB][QW] = {};
   float m[QW], l[QW];
 #pragma unroll
   for (int b = 0; b < QW; ++b) m[b] = -INFINITY, l[b] = 0.0f;
+  float lr[QW] = {};  // TERMS: sums of the rounded probabilities
+  // Capped scores of bf16 need no maximum: from a reference of zero, probabilities of 2^-80 to 2^80 and their
+  // sums are far inside fp32's range and bf16's.
+  bool bounded = false;
+  if constexpr (TERMS == kCap && kBelow<T> == 0) {
+    bounded = a.cap2 <= 80.0f;
+    if (bounded)
+#pragma unroll
+      for (int b = 0; b < QW; ++b) m[b] = 0.0f;
+  }
+  constexpr bool FOLD = TERMS == kSlopes;
+  std::conditional_t<FOLD, SideProduct<T>, char> side[QW];
+  bool folds = false;
+  if constexpr (FOLD) {
+    folds = true;
+#pragma unroll
+    for (int b = 0; b < QW; ++b) side[b].set(terms.slope[b] * a.per_mul, h), folds = folds && side[b].on;
+  }
 
   if (Z && a.dim < DP) clear_tiles(smem, 2 * PAIR);
   uint64_t bits = 0, next = 0;
@@ -192,6 +210,19 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 && NW * QW == 4 ? 3 : 2) void att
           for (int b = 0; b < QW; ++b) sc[n][b] = x;
         }
       }
+      bool folded = false;
+      if constexpr (FOLD) {
+        const bool after = t * kKT >= terms.last;
+        folded = folds && (after || (t + 1) * kKT - 1 <= terms.first);
+        // a product with zeros where it does not hold: a branch would copy the scores
+        const uint32_t turn = after ? 0x80008000u : 0u, keep = folded ? ~0u : 0u;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const u32x4 x = SideProduct<T>::keys(n, c32);
+#pragma unroll
+          for (int b = 0; b < QW; ++b) Mfma<T>::run(x, (side[b].slope ^ turn) & keep, sc[n][b]);
+        }
+      }
 #pragma unroll
       for (int k = 0; k < KS; ++k)
 #pragma unroll
@@ -201,7 +232,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 && NW * QW == 4 ? 3 : 2) void att
           for (int b = 0; b < QW; ++b) Mfma<T>::run(x, qf[b][k], sc[n][b]);
         }
       float mul = a.scale2, add[QW];  // scores in powers of two are sc * mul (+ add)
-      if constexpr (TERMS) mul = add_terms<2, QW, false>(a, terms, sc, t * kKT, 0, h, add, nullptr);
+      if constexpr (TERMS != 0) mul = add_terms<TERMS, 2, QW, false>(a, terms, sc, t * kKT, 0, h, folded, add, nullptr);
       // keys that are hidden from a row
       if (((!Z || capped) && bits != ~0ull) || (t + 1) * kKT > wfull) {
         if (!Z || capped) hide_keys<QW>(sc, bits);
@@ -220,12 +251,13 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 && NW * QW == 4 ? 3 : 2) void att
       }
       float top[QW];
       bool grow = false;
+      if (!bounded)
 #pragma unroll
       for (int b = 0; b < QW; ++b) {
         float x = larger(sc[0][b][0], sc[1][b][0]);
 #pragma unroll
         for (int e = 1; e < 16; ++e) x = larger(larger(x, sc[0][b][e]), sc[1][b][e]);
-        if constexpr (TERMS) top[b] = half_max(__builtin_fmaf(x, mul, add[b])) - kBelow<T>;
+        if constexpr (TERMS != 0) top[b] = half_max(__builtin_fmaf(x, mul, add[b])) - kBelow<T>;
         else top[b] = half_max(x) * a.scale2 - kBelow<T>;
         grow = grow || top[b] > m[b] + 8.0f;
       }
@@ -236,6 +268,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 && NW * QW == 4 ? 3 : 2) void att
           const float by = m[b] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[b] - to);
           m[b] = to;
           l[b] *= by;
+          if constexpr (TERMS != 0) lr[b] *= by;
 #pragma unroll
           for (int d = 0; d < DB; ++d) acc[d][b] *= by;
         }
@@ -265,6 +298,13 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 && NW * QW == 4 ? 3 : 2) void att
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] = sc[k >> 1][b][8 * (k & 1) + e];
           p[b] = pack8<T>(x);
+          if constexpr (TERMS && !SPLIT)
+            if (a.rest != nullptr) {
+              float pair = 0.0f;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) pair = add_pair<T>(p[b][e], pair);
+              lr[b] += pair;
+            }
         }
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
@@ -300,8 +340,15 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 && NW * QW == 4 ? 3 : 2) void att
         ml[0] = m[b], ml[1] = sum;
       }
     } else {
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // no key seen: zeros
+      float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // no key seen: zeros
+      if constexpr (TERMS != 0)
+        if (a.rest != nullptr) {
+          const float rounded = half_sum(lr[b]);
+          inv = rounded == 0.0f ? 0.0f : 1.0f / rounded;
+        }
       store_row<T, DP>(static_cast<T*>(a.out) + place * a.dim, a.dim, h, &acc[0][b], QW, inv);
+      if constexpr (TERMS != 0)
+        if (a.rest != nullptr) store_row<T, DP, true>(static_cast<T*>(a.rest) + place * a.dim, a.dim, h, &acc[0][b], QW, inv);
       if (a.lse != nullptr && h == 0) a.lse[place] = sum == 0.0f ? -INFINITY : (m[b] + __builtin_amdgcn_logf(sum)) * kLn2;
     }
   }
@@ -324,8 +371,9 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 && NW * QW == 4 ? 3 : 2) void att
 // (671 MB) in 166 us, 4.05 TB/s; a fifth more as 64-row workgroups of attend_kernel.
 constexpr int kShortSpan = 256;
 
-template <typename T, int DP, int KW, bool Z, bool TERMS>
-__global__ __launch_bounds__(KW == 1 ? 256 : 64 * KW, KW > 1 ? KW / 4 : (DP <= 32 ? 4 : (DP <= 64 ? 2 : 1))) void
+template <typename T, int DP, int KW, bool Z, int TERMS>
+__global__ __launch_bounds__(KW == 1 ? 256 : 64 * KW,
+                             KW > 1 ? KW / 4 : (DP <= 32 ? (TERMS ? 3 : 4) : (DP <= 64 ? 2 : 1))) void
 attend_short_kernel(ArgsOf<TERMS> a) {
   constexpr int SPAN = KW == 1 ? kShortSpan : 32, KS = DP / 16, DB = DP / 32;
   constexpr int TILE = KW > 1 && DP * 132 > kTile<DP> ? DP * 132 : kTile<DP>;
@@ -394,8 +442,8 @@ attend_short_kernel(ArgsOf<TERMS> a) {
   auto seen_by = [&](int i) { return TERMS ? max(i + off + 1, seen_by_all) : i + off + 1; };
   RowTerms<1> terms;
   float* table = nullptr;
-  if constexpr (TERMS) {
-    if (a.bias != nullptr) {
+  if constexpr (TERMS != 0) {
+    if (has_bias<TERMS>(a)) {
       // a wave's own copy (its rows and keys reach no further), or the workgroup's
       table = reinterpret_cast<float*>(smem + (KW == 1 ? 4 * kTile<DP> : KW * (TILE + 256)));
       int x0 = 0, x1 = 2 * (a.far + kPad) + 1;
@@ -440,7 +488,7 @@ attend_short_kernel(ArgsOf<TERMS> a) {
       split_row(a, row0, i, g);
       full = min(full, seen_by(i));
     }
-    if constexpr (TERMS) {
+    if constexpr (TERMS != 0) {
       const int is[1] = {qi}, gs[1] = {qg};
       row_terms<1>(a, s, terms, table, head, row0, rows, is, gs);
     }
@@ -457,7 +505,7 @@ attend_short_kernel(ArgsOf<TERMS> a) {
 #pragma unroll
           for (int k = 0; k < KS; ++k) Mfma<T>::run(kf[n][k], qf[k], sc[n][0]);
       float mul = a.scale2, add[1];
-      if constexpr (TERMS) mul = add_terms<2, 1, false>(a, terms, sc, k0, 0, h, add, nullptr);
+      if constexpr (TERMS != 0) mul = add_terms<TERMS, 2, 1, false>(a, terms, sc, k0, 0, h, false, add, nullptr);
       float top = -INFINITY;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -477,7 +525,7 @@ attend_short_kernel(ArgsOf<TERMS> a) {
 #pragma unroll
         for (int e = 8 * (k & 1); e < 8 * (k & 1) + 8; ++e) top = larger(top, sc[k >> 1][0][e]);
       }
-      if constexpr (TERMS) top = half_max(__builtin_fmaf(top, mul, add[0]));
+      if constexpr (TERMS != 0) top = half_max(__builtin_fmaf(top, mul, add[0]));
       else top = half_max(top) * a.scale2;
       const float to = fmaxf(m, top - kBelow<T>);
       if (k0 > start) {
@@ -618,7 +666,7 @@ int launch_join(const AttnArgs& a, hipStream_t stream) {
 }
 
 // split: parts of the rows alone, also where there is one, for a join that takes more of them
-template <typename T, int DP, int NW, int QW, bool TERMS>
+template <typename T, int DP, int NW, int QW, int TERMS>
 int launch_attend(ArgsOf<TERMS> a, hipStream_t stream, bool split = false) {
   constexpr int rows = NW * QW * 32;
   const bool z = a.mask != nullptr || a.dim < DP;
@@ -640,7 +688,7 @@ int launch_attend(ArgsOf<TERMS> a, hipStream_t stream, bool split = false) {
   }
 }
 
-template <typename T, int DP, int KW, bool TERMS>
+template <typename T, int DP, int KW, int TERMS>
 int launch_short(ArgsOf<TERMS> a, hipStream_t stream) {
   constexpr int rows = KW == 1 ? kShortSpan : 32;
   constexpr int part = DP * 132 > kTile<DP> ? DP * 132 : kTile<DP>;  // a wave's tile, or its 32 rows of the output
@@ -681,20 +729,43 @@ int attend_rows(int64_t total_q, int batch, int hq, int hk, int dim, int cus) {
   return dim <= 64 && ceil_div(rows, 256) * hk >= 8 * cus ? 256 : 128;
 }
 
-template <typename T, int DP, bool TERMS>
-int launch_attend_dim(const ArgsOf<TERMS>& a, hipStream_t stream) {
-  const int64_t average = segment_average(a);
-  if (average <= 64 && ceil_div(a.total_k, a.batch) <= 128 && 4 * (kTile<DP> + term_bytes<TERMS>(a)) <= 160 * 1024)
-    return launch_short<T, DP, 1, TERMS>(a, stream);
-  if (a.few) return launch_short<T, DP, 8, TERMS>(a, stream);
-  if (a.rows == 32) return launch_attend<T, DP, 1, 1, TERMS>(a, stream);
-  if (a.rows == 64) return launch_attend<T, DP, 1, 2, TERMS>(a, stream);
+// Segments of tens of rows and keys: a wave each.
+template <int TERMS>
+bool short_segments(const ArgsOf<TERMS>& a) {
+  const int tile = a.dim > 96 ? kTile<128> : static_cast<int>(ceil_div(a.dim, 32)) * kTile<32>;
+  return segment_average(a) <= 64 && ceil_div(a.total_k, a.batch) <= 128 && 4 * (tile + term_bytes<TERMS>(a)) <= 160 * 1024;
+}
+
+// Rows of four waves each, not split: the kernels that are built for one term.
+template <typename T, int DP, int TERMS>
+int launch_wide(const ArgsOf<TERMS>& a, hipStream_t stream) {
   if constexpr (DP <= 64)
     if (a.rows == 256) return launch_attend<T, DP, 4, 2, TERMS>(a, stream);
   return launch_attend<T, DP, 4, 1, TERMS>(a, stream);
 }
 
-template <typename T, bool TERMS>
+template <typename T, int TERMS>
+int launch_wide_type(const ArgsOf<TERMS>& a, hipStream_t stream) {
+  switch ((a.dim + 31) / 32) {
+    case 1: return launch_wide<T, 32, TERMS>(a, stream);
+    case 2: return launch_wide<T, 64, TERMS>(a, stream);
+    case 3: return launch_wide<T, 96, TERMS>(a, stream);
+    default: return launch_wide<T, 128, TERMS>(a, stream);
+  }
+}
+
+template <typename T, int DP, int TERMS>
+int launch_attend_dim(const ArgsOf<TERMS>& a, hipStream_t stream) {
+  if (short_segments<TERMS>(a))
+    return launch_short<T, DP, 1, TERMS>(a, stream);
+  if (a.few) return launch_short<T, DP, 8, TERMS>(a, stream);
+  if (a.rows == 32) return launch_attend<T, DP, 1, 1, TERMS>(a, stream);
+  if constexpr (TERMS == 0)
+    if (a.rows == 64) return launch_attend<T, DP, 1, 2, TERMS>(a, stream);
+  return launch_wide<T, DP, TERMS>(a, stream);
+}
+
+template <typename T, int TERMS>
 int launch_attend_type(const ArgsOf<TERMS>& a, hipStream_t stream) {
   switch ((a.dim + 31) / 32) {
     case 1: return launch_attend_dim<T, 32, TERMS>(a, stream);

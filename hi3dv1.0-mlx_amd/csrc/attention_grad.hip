@@ -51,7 +51,7 @@ int hi3d_attention_backward(const hi3d_attention_desc* d, const void* out, const
   a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + 2 * stats_bytes(a) + bound_bytes(a, a.hk));
   a.splits = a.total_k > 0 ? dkv_splits(a, cus) : 1;
   hipStream_t stream = as_stream(stream_);
-  return d->dtype == HI3D_F16 ? launch_grad_type<_Float16, false>(a, stream) : launch_grad_type<__bf16, false>(a, stream);
+  return d->dtype == HI3D_F16 ? launch_grad_type<_Float16, 0>(a, stream) : launch_grad_type<__bf16, 0>(a, stream);
 }
 
 }  // extern "C"

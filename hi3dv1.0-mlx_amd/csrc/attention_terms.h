@@ -27,6 +27,7 @@ namespace hi3d {
 
 constexpr float kHideBelow = -1e30f;  // a bias below hides its key (-infinity; the lowest numbers of a type too)
 constexpr int kPad = kKT, kPadKeys = 128;  // what the rows' and the keys' kernels look up past `far`
+constexpr int kPadSums = 93;               // what a wave's 32 rows and a tile's 64 keys reach past it together
 constexpr int kMostTermBytes = 72 * 1024, kMostLds = 160 * 1024;
 
 struct TermArgs : AttnArgs {
@@ -42,11 +43,20 @@ struct TermArgs : AttnArgs {
   const int32_t* own_lens;      // keys in use of each sequence behind it, or null: own_len
   int32_t per, own_len;
   int32_t share;                // backward: query heads of a key head, where hk counts query heads
-  float* dbias;                 // backward: [hq, slots, 2 far + 2 kPad + 1] parts, or null
+  float* dbias;                 // backward: [hq, slots, sum_length(far)] parts, or null
+  void* rest;                   // [total_q, hq, d] what rounding took from out, times kRest; or null
 };
 
-template <bool TERMS>
-using ArgsOf = std::conditional_t<TERMS, TermArgs, AttnArgs>;
+// Which terms a kernel is built for: none, one of them, or any (each asked for when it runs).
+constexpr int kCap = 1, kSlopes = 2, kBias = 4, kAll = 7;
+template <int TERMS>
+using ArgsOf = std::conditional_t<TERMS != 0, TermArgs, AttnArgs>;
+template <int TERMS>
+__device__ __forceinline__ bool has_cap(const TermArgs& a) { return TERMS == kAll ? a.cap2 > 0.0f : (TERMS & kCap) != 0; }
+template <int TERMS>
+__device__ __forceinline__ bool has_slopes(const TermArgs& a) { return TERMS == kAll ? a.slopes != nullptr : (TERMS & kSlopes) != 0; }
+template <int TERMS>
+__device__ __forceinline__ bool has_bias(const TermArgs& a) { return TERMS == kAll ? a.bias != nullptr : (TERMS & kBias) != 0; }
 
 // Floats of a head's bias in LDS: its length, up to the next number after which the lanes' heads
 // (32 / group rows of each) start at banks of their own.
@@ -54,9 +64,14 @@ inline int bias_stride(int far, int pad, int group) {
   const int want = group >= 32 ? 1 : 32 / group, length = 2 * far + 2 * pad + 1;
   return length + ((want - length) % 64 + 64) % 64;
 }
-template <bool TERMS>
+__host__ __device__ constexpr int sum_length(int far) { return 2 * (far + kPadSums) + 1; }
+__host__ __device__ constexpr int sum_stride(int far) { return (sum_length(far) + 3) / 4 * 4; }
+// A wave's score gradients of 32 rows and 8 keys in LDS, between 7 rows of zeros on either side.
+constexpr int kSkewRow = 9, kSkew = (7 + 32 + 7) * kSkewRow + 2;
+
+template <int TERMS>
 int term_bytes(const ArgsOf<TERMS>& a) {
-  if constexpr (TERMS) return a.bias != nullptr ? a.group * a.stride * 4 : 0;
+  if constexpr (TERMS != 0) return a.bias != nullptr ? a.group * a.stride * 4 : 0;
   else return 0;
 }
 
@@ -89,6 +104,15 @@ __device__ __forceinline__ float minus_u(const TermArgs& a, float score) {
   return __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(score * a.cap_in));
 }
 
+// x + the two values in a word of T.
+template <typename T>
+__device__ __forceinline__ float add_pair(uint32_t word, float x) {
+  typedef T t2 __attribute__((ext_vector_type(2)));
+  const t2 one = {static_cast<T>(1.0f), static_cast<T>(1.0f)};
+  if constexpr (std::is_same_v<T, _Float16>) return __builtin_amdgcn_fdot2(__builtin_bit_cast(t2, word), one, x, false);
+  else return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(t2, word), one, x, false);
+}
+
 // A lane's rows (QW blocks of 32 of a wave) in the kernels whose lanes own query rows.
 template <int QW>
 struct RowTerms {
@@ -99,9 +123,9 @@ struct RowTerms {
 };
 
 // Keys of a segment that all of its rows see.
-template <bool TERMS>
+template <int TERMS>
 __device__ __forceinline__ int first_keys(const ArgsOf<TERMS>& a, const Segment& s) {
-  if constexpr (TERMS)
+  if constexpr (TERMS != 0)
     if (a.prefix != nullptr && s.b >= 0 && s.b < a.batch) return min(max(a.prefix[s.b], 0), s.lk);
   return 0;
 }
@@ -138,42 +162,98 @@ __device__ __forceinline__ void row_terms(const TermArgs& a, const Segment& s, R
   w.last = x + off;
 }
 
+// Distances to the keys of one side, as one more step of the score product: slope * (number of the key in
+// its tile), with the slope in three numbers of the inputs' type (22 bits and more) and the key's
+// number, which has one. It takes a matrix instruction a 32 x 32 block where a multiply-add a score takes
+// 16 vector ones, in loops that vector operations bound (20,011 rows x 33 heads x 64: TODO).
+template <typename T>
+struct SideProduct {
+  u32x4 slope;  // second operand: the lane's row (with the signs turned: keys behind it)
+  bool on;      // within the type's range in all lanes
+
+  __device__ __forceinline__ static void split(float t, T (&x)[3]) {
+    x[0] = static_cast<T>(t);
+    const float r = t - static_cast<float>(x[0]);
+    x[1] = static_cast<T>(r), x[2] = static_cast<T>(r - static_cast<float>(x[1]));
+  }
+  __device__ __forceinline__ void set(float t, int h) {
+    T x[3];
+    split(t, x);
+    const T zero = static_cast<T>(0.0f);
+    const typename Vec8<T>::type v = {x[0], x[1], x[2], zero, zero, zero, zero, zero};
+    slope = h == 0 ? __builtin_bit_cast(u32x4, v) : u32x4{0, 0, 0, 0};
+    on = !__any(__builtin_fabsf(t) > 16384.0f);
+  }
+  // Lanes that own keys: t * (key - place of the row) where the heads of a tile's 64 rows are the same in
+  // every tile (the group divides 64). A row's slope in three numbers meets the key's distance to
+  // the tile's first row in numbers of 8 (11) bits, and its own distance from there, slope times row /
+  // group in three numbers, meets -1: 12 of the 16 products of a step, all exact.
+  __device__ __forceinline__ static u32x4 of_row(float t, int row, int h) {
+    T x[3], y[3];
+    split(t, x), split(-t * static_cast<float>(row), y);
+    const T zero = static_cast<T>(0.0f);
+    const typename Vec8<T>::type a = {x[0], x[1], x[2], x[0], x[1], x[2], x[0], x[1]}, b = {x[2], y[0], y[1], y[2], zero, zero, zero, zero};
+    return h == 0 ? __builtin_bit_cast(u32x4, a) : __builtin_bit_cast(u32x4, b);
+  }
+  static constexpr int kBits = std::is_same_v<T, _Float16> ? 11 : 8;
+  static constexpr int kFarthest = std::is_same_v<T, _Float16> ? 65504 : (1 << 24) - 1;
+  __device__ __forceinline__ static u32x4 of_key(int distance, int h) {
+    const int far = distance < 0 ? -distance : distance, low = (1 << kBits) - 1;
+    auto number = [&](int x) { return static_cast<T>(static_cast<float>(distance < 0 ? -x : x)); };
+    const T b0 = number(far & low), b1 = number(far & low << kBits), b2 = number(far & ~(low << kBits | low));
+    const T one = static_cast<T>(1.0f), zero = static_cast<T>(0.0f);
+    const typename Vec8<T>::type a = {b0, b0, b0, b1, b1, b1, b2, b2}, b = {b2, one, one, one, zero, zero, zero, zero};
+    return h == 0 ? __builtin_bit_cast(u32x4, a) : __builtin_bit_cast(u32x4, b);
+  }
+  // first operand: keys 32 n + l % 32
+  __device__ __forceinline__ static u32x4 keys(int n, int c32) {
+    const T j = static_cast<T>(static_cast<float>(32 * n + c32)), zero = static_cast<T>(0.0f);
+    const typename Vec8<T>::type v = {j, j, j, zero, zero, zero, zero, zero};
+    return __builtin_bit_cast(u32x4, v);
+  }
+};
+
 // Adds a tile's terms to its scores sc[n][b] (keys k0 + 32 (n0 + n) + 8 (e / 4) + 4 h + e % 4). Scores
-// in powers of two are then sc * (returned factor) + add[b]. KEEP: derivative of the cap.
-template <int N, int QW, bool KEEP>
+// in powers of two are then sc * (returned factor) + add[b]. KEEP: derivative of the cap, times -1/4. folded:
+// the distances within a tile on one side are in the scores already.
+template <int TERMS, int N, int QW, bool KEEP>
 __device__ __forceinline__ float add_terms(const TermArgs& a, const RowTerms<QW>& w, f32x16 (&sc)[N][QW], int k0, int n0,
-                                           int h, float (&add)[QW], f32x16* bend) {
+                                           int h, bool folded, float (&add)[QW], f32x16* bend) {
   float mul = a.scale2;
 #pragma unroll
   for (int b = 0; b < QW; ++b) add[b] = 0.0f;
-  if (a.cap2 > 0.0f) {
+  if (has_cap<TERMS>(a)) {
     mul = 2.0f * a.cap2;
 #pragma unroll
     for (int b = 0; b < QW; ++b) {
       add[b] = a.cap2;
 #pragma unroll
-      for (int n = 0; n < N; ++n)
+      for (int n = 0; n < N; ++n) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const float u = minus_u(a, sc[n][b][e]);
           sc[n][b][e] = u;
-          if constexpr (KEEP) (*bend)[e] = __builtin_fmaf(-4.0f * u, u, -4.0f * u);
+          if constexpr (KEEP) (*bend)[e] = __builtin_fmaf(u, u, u);
         }
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
   }
-  if (a.slopes != nullptr) {
+  if (has_slopes<TERMS>(a)) {
     const bool before = k0 + kKT - 1 <= w.first, after = k0 >= w.last;
 #pragma unroll
     for (int b = 0; b < QW; ++b) {
       const float from = static_cast<float>(k0 + 4 * h - w.place[b]);
       if (before || after) {
         const float s = after ? -w.slope[b] : w.slope[b], t = s * a.per_mul;
-        add[b] = __builtin_fmaf(s, from, add[b]);
+        add[b] = __builtin_fmaf(s, folded ? static_cast<float>(k0 - w.place[b]) : from, add[b]);
+        if (!folded) {
 #pragma unroll
-        for (int n = 0; n < N; ++n)
+          for (int n = 0; n < N; ++n)
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            sc[n][b][e] = __builtin_fmaf(t, static_cast<float>(32 * (n0 + n) + 8 * (e >> 2) + (e & 3)), sc[n][b][e]);
+            for (int e = 0; e < 16; ++e)
+              sc[n][b][e] = __builtin_fmaf(t, static_cast<float>(32 * (n0 + n) + 8 * (e >> 2) + (e & 3)), sc[n][b][e]);
+        }
       } else {
         const float t = -w.slope[b] * a.per_mul;
 #pragma unroll
@@ -185,7 +265,7 @@ __device__ __forceinline__ float add_terms(const TermArgs& a, const RowTerms<QW>
       }
     }
   }
-  if (a.bias != nullptr) {
+  if (has_bias<TERMS>(a)) {
     if (k0 + kKT - 1 - w.first <= -a.far) {
 #pragma unroll
       for (int b = 0; b < QW; ++b) add[b] += w.bias[b][0];
@@ -197,15 +277,29 @@ __device__ __forceinline__ float add_terms(const TermArgs& a, const RowTerms<QW>
       for (int b = 0; b < QW; ++b) {
         const float* at = w.bias[b] + min(max(k0 + 4 * h - w.place[b] + a.far + kPad, 0), 2 * a.far + kPad);
 #pragma unroll
-        for (int n = 0; n < N; ++n)
+        for (int n = 0; n < N; ++n) {
 #pragma unroll
           for (int e = 0; e < 16; ++e)
             sc[n][b][e] = __builtin_fmaf(sc[n][b][e], mul, at[32 * (n0 + n) + 8 * (e >> 2) + (e & 3)]);
+          __builtin_amdgcn_sched_barrier(0);  // 16 look-ups in flight: more spill registers
+        }
       }
       mul = 1.0f;
     }
   }
   return mul;
 }
+
+// The one term of a problem, or kAll.
+inline int one_term(const TermArgs& a) {
+  const int kind = (a.cap2 > 0.0f ? kCap : 0) | (a.slopes != nullptr ? kSlopes : 0) | (a.bias != nullptr ? kBias : 0);
+  return kind == kCap || kind == kSlopes || kind == kBias ? kind : kAll;
+}
+
+// Workgroups of four waves whose rows are not parts (attention_terms_one.hip), and the gradients over them
+// (attention_terms_grad_one.hip), built for one term each: with the others' registers gone they need
+// no spills.
+int launch_rows_of_one(const TermArgs& a, int dtype, int kind, hipStream_t stream);
+int launch_grad_of_one(const TermArgs& a, int dtype, int kind, hipStream_t stream);
 
 }  // namespace hi3d

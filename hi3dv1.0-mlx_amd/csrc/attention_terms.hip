@@ -33,12 +33,18 @@ int term_args(const hi3d_attention_desc* d, const hi3d_attention_terms* t, TermA
 
 namespace {
 
-// Kernel, tile and splits of the key axis.
+// Kernel, tile and splits of the key axis. 33 to 64 rows take workgroups of four waves too: two blocks of 32 rows
+// a wave spill 30 to 300 registers with terms.
 void choose(TermArgs& a, int cus) {
-  a.few = few_rows(a.total_q, a.total_k, a.batch, a.hq, a.hk, a.dim, cus, term_bytes<true>(a));
+  a.few = few_rows(a.total_q, a.total_k, a.batch, a.hq, a.hk, a.dim, cus, term_bytes<kAll>(a));
   a.splits = attend_splits(a.total_q, a.total_k, a.batch, a.hq, a.hk, a.dim, cus, a.few);
   a.rows = attend_rows(a.total_q, a.batch, a.hq, a.hk, a.dim, cus);
+  if (a.rows == 64) a.rows = 128;
 }
+
+// Rows whose gradients take what rounding leaves of the output: those of attend_kernel's own rows. Short and
+// few rows, and those of which parts are joined, have the backward's walk for it.
+bool keeps_rest(const TermArgs& a) { return a.splits == 1 && !a.few && !short_segments<kAll>(a); }
 
 int64_t part_bytes(const TermArgs& a, int splits) { return static_cast<int64_t>(splits) * a.total_q * a.hq * (a.dim + 2) * 4; }
 
@@ -56,7 +62,7 @@ void choose_halves(const TermArgs& a, const hi3d_attention_shared* s, TermArgs& 
   shared.once = static_cast<int64_t>(s->len) * a.hk * a.dim * 4 > (256ll << 20);
   for (TermArgs* x : {&shared, &own}) {
     const int rows = attend_rows(x->total_q, x->batch, x->hq, x->hk, x->dim, cus);
-    x->rows = rows > 128 ? 128 : rows;
+    x->rows = rows > 32 ? 128 : rows;
     const int splits = attend_splits(x->total_q, x->total_k, x->batch, x->hq, x->hk, x->dim, cus, false);
     x->splits = splits > 128 ? 128 : splits;
   }
@@ -64,9 +70,8 @@ void choose_halves(const TermArgs& a, const hi3d_attention_shared* s, TermArgs& 
 
 template <typename T, int DP>
 int launch_part(const TermArgs& a, hipStream_t stream) {
-  if (a.rows == 32) return launch_attend<T, DP, 1, 1, true>(a, stream, true);
-  if (a.rows == 64) return launch_attend<T, DP, 1, 2, true>(a, stream, true);
-  return launch_attend<T, DP, 4, 1, true>(a, stream, true);
+  if (a.rows == 32) return launch_attend<T, DP, 1, 1, kAll>(a, stream, true);
+  return launch_attend<T, DP, 4, 1, kAll>(a, stream, true);
 }
 
 template <typename T>
@@ -109,20 +114,22 @@ using namespace hi3d;
 
 extern "C" {
 
-int hi3d_attention_terms_workspace(const hi3d_attention_desc* d, const hi3d_attention_terms* t, int64_t* bytes) {
+int hi3d_attention_terms_workspace(const hi3d_attention_desc* d, const hi3d_attention_terms* t, int32_t* rest, int64_t* bytes) {
   TermArgs a;
   const int rc = term_args(d, t, a);
   if (rc != HI3D_OK) return rc;
   HI3D_REQUIRE(bytes != nullptr, "null pointer argument");
   *bytes = 0;
+  if (rest != nullptr) *rest = 0;
   if (a.total_q == 0 || a.batch == 0) return HI3D_OK;
   const int cus = compute_units();
   choose(a, cus > 0 ? cus : 256);  // without a device (a size query on a build host): the MI355X's
+  if (rest != nullptr) *rest = keeps_rest(a);
   if (a.splits > 1) *bytes = part_bytes(a, a.splits) + 256;
   return HI3D_OK;
 }
 
-int hi3d_attention_terms_forward(const hi3d_attention_desc* d, const hi3d_attention_terms* t, void* out, float* lse,
+int hi3d_attention_terms_forward(const hi3d_attention_desc* d, const hi3d_attention_terms* t, void* out, void* rest, float* lse,
                                  void* workspace, int64_t workspace_bytes, void* stream_) {
   TermArgs a;
   const int rc = term_args(d, t, a);
@@ -132,8 +139,10 @@ int hi3d_attention_terms_forward(const hi3d_attention_desc* d, const hi3d_attent
   HI3D_REQUIRE(out != nullptr && reinterpret_cast<uintptr_t>(out) % 16 == 0, "out must be 16-byte aligned");
   const int cus = compute_units();
   HI3D_REQUIRE(cus > 0, "cannot query the compute unit count");
-  a.out = out, a.lse = lse;
+  a.out = out, a.rest = rest, a.lse = lse;
   choose(a, cus);
+  HI3D_REQUIRE(rest == nullptr || (keeps_rest(a) && reinterpret_cast<uintptr_t>(rest) % 16 == 0),
+               "no rest of the output is kept of these rows, or it is not 16-byte aligned");
   if (a.splits > 1) {
     HI3D_REQUIRE(workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 &&
                      workspace_bytes >= part_bytes(a, a.splits),
@@ -142,7 +151,9 @@ int hi3d_attention_terms_forward(const hi3d_attention_desc* d, const hi3d_attent
     a.part_ml = a.part + static_cast<int64_t>(a.splits) * a.total_q * a.hq * a.dim;
   }
   hipStream_t stream = as_stream(stream_);
-  return d->dtype == HI3D_F16 ? launch_attend_type<_Float16, true>(a, stream) : launch_attend_type<__bf16, true>(a, stream);
+  if (!a.few && !short_segments<kAll>(a) && a.rows > 32 && a.splits == 1 && one_term(a) != kAll)
+    return launch_rows_of_one(a, d->dtype, one_term(a), stream);
+  return d->dtype == HI3D_F16 ? launch_attend_type<_Float16, kAll>(a, stream) : launch_attend_type<__bf16, kAll>(a, stream);
 }
 
 int hi3d_attention_shared_workspace(const hi3d_attention_desc* d, const hi3d_attention_terms* t,

@@ -10,7 +10,7 @@ namespace {
 
 // Parts of the bias's gradient: one a workgroup of the dq kernel, then one a run of them.
 constexpr int kRun = 64;
-int64_t bias_length(const TermArgs& a) { return 2 * (a.far + kPad) + 1; }
+int64_t bias_length(const TermArgs& a) { return sum_length(a.far); }
 int64_t bias_runs(const TermArgs& a) { return a.dq_slots <= kRun ? 0 : ceil_div(a.dq_slots, kRun); }
 int64_t dbias_bytes(const TermArgs& a) {
   return align_up((a.dq_slots + bias_runs(a)) * a.hq * bias_length(a) * 4, 256);
@@ -59,8 +59,8 @@ int hi3d_attention_terms_backward_workspace(const hi3d_attention_desc* d, const 
 }
 
 int hi3d_attention_terms_backward(const hi3d_attention_desc* d, const hi3d_attention_terms* t, const void* out,
-                                  const float* lse, const void* dout, const float* dlse, void* dq, void* dk, void* dv,
-                                  void* dbias, void* workspace, int64_t workspace_bytes, void* stream_) {
+                                  const void* rest, const float* lse, const void* dout, const float* dlse, void* dq,
+                                  void* dk, void* dv, void* dbias, void* workspace, int64_t workspace_bytes, void* stream_) {
   TermArgs a;
   int64_t need = 0;
   int rc = term_args(d, t, a);
@@ -77,7 +77,7 @@ int hi3d_attention_terms_backward(const hi3d_attention_desc* d, const hi3d_atten
   if (a.total_q > 0) HI3D_REQUIRE(out != nullptr && lse != nullptr && dout != nullptr, "null pointer argument");
   const uintptr_t at = reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(dout) | reinterpret_cast<uintptr_t>(dq) |
                        reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv) |
-                       reinterpret_cast<uintptr_t>(workspace);
+                       reinterpret_cast<uintptr_t>(workspace) | reinterpret_cast<uintptr_t>(rest);
   HI3D_REQUIRE(at % 16 == 0, "out, dout, the gradients and the workspace must be 16-byte aligned");
   HI3D_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), "workspace too small (%lld bytes, need %lld)",
                static_cast<long long>(workspace_bytes), static_cast<long long>(need));
@@ -85,7 +85,7 @@ int hi3d_attention_terms_backward(const hi3d_attention_desc* d, const hi3d_atten
   if (!rows) return launch_dbias(a, dbias, stream);
   const int cus = compute_units();
   HI3D_REQUIRE(cus > 0, "cannot query the compute unit count");
-  a.o = out, a.lse = const_cast<float*>(lse), a.dout = dout, a.dlse = dlse;
+  a.o = out, a.lse = const_cast<float*>(lse), a.dout = dout, a.dlse = dlse, a.rest = const_cast<void*>(rest);
   a.out = dq, a.dk = dk, a.dv = dv;
   dq_tiles(a, 1);
   char* at_ws = static_cast<char*>(workspace);
@@ -101,7 +101,9 @@ int hi3d_attention_terms_backward(const hi3d_attention_desc* d, const hi3d_atten
   }
   a.part = reinterpret_cast<float*>(at_ws);
   a.splits = a.total_k > 0 ? dkv_splits(a, cus) : 1;
-  rc = d->dtype == HI3D_F16 ? launch_grad_type<_Float16, true>(a, stream) : launch_grad_type<__bf16, true>(a, stream);
+  const int kind = one_term(a);
+  if (kind != kAll && a.dq_waves == 4 && ceil_div(a.total_k, a.batch) > 32) rc = launch_grad_of_one(a, d->dtype, kind, stream);
+  else rc = d->dtype == HI3D_F16 ? launch_grad_type<_Float16, kAll>(a, stream) : launch_grad_type<__bf16, kAll>(a, stream);
   if (rc != HI3D_OK || dbias == nullptr) return rc;
   return launch_dbias(a, dbias, stream);
 }

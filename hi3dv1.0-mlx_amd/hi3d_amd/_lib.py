@@ -105,10 +105,10 @@ _SIGNATURES = {
     "hi3d_attention_forward": [_p, _p, _p, _p, _i64, _p],
     "hi3d_attention_backward_workspace": [_p, _p],
     "hi3d_attention_backward": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _p],
-    "hi3d_attention_terms_workspace": [_p, _p, _p],
-    "hi3d_attention_terms_forward": [_p, _p, _p, _p, _p, _i64, _p],
+    "hi3d_attention_terms_workspace": [_p, _p, _p, _p],
+    "hi3d_attention_terms_forward": [_p, _p, _p, _p, _p, _p, _i64, _p],
     "hi3d_attention_terms_backward_workspace": [_p, _p, _p],
-    "hi3d_attention_terms_backward": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _p],
+    "hi3d_attention_terms_backward": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _p],
     "hi3d_attention_shared_workspace": [_p, _p, _p, _p],
     "hi3d_attention_shared_forward": [_p, _p, _p, _p, _p, _p, _i64, _p],
 }

@@ -252,7 +252,8 @@ class _Problem:
         self.desc = _Desc(*[x if x is None else x.data_ptr() for x in self.tensors], strides, *sizes)
         self.ref = ctypes.byref(self.desc)
 
-    def forward(self, want_lse: bool) -> tuple[torch.Tensor, torch.Tensor | None]:
+    def forward(self, want_lse: bool, want_rest: bool = False) -> tuple[torch.Tensor, ...]:
+        """``out`` and ``lse``; with ``want_rest`` and terms also what rounding took from ``out``, where it is kept."""
         q, ref = self.tensors[0], self.ref
         out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
         lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=self.device) if want_lse else None
@@ -262,13 +263,15 @@ class _Problem:
             _lib.call("hi3d_attention_forward", ref, out.data_ptr(), _lib.ptr(lse), _lib.ptr(work), need,
                       _lib.stream(self.device))
             return out, lse
-        need = _lib.query("hi3d_attention_terms_workspace", ref, self.terms_ref)
+        kept = ctypes.c_int32(0)
+        need = _lib.query("hi3d_attention_terms_workspace", ref, self.terms_ref, ctypes.byref(kept))
         work = _lib.workspace(need, self.device) if need else None
-        _lib.call("hi3d_attention_terms_forward", ref, self.terms_ref, out.data_ptr(), _lib.ptr(lse), _lib.ptr(work), need,
-                  _lib.stream(self.device))
-        return out, lse
+        rest = torch.empty_like(out) if want_rest and kept.value else None
+        _lib.call("hi3d_attention_terms_forward", ref, self.terms_ref, out.data_ptr(), _lib.ptr(rest), _lib.ptr(lse),
+                  _lib.ptr(work), need, _lib.stream(self.device))
+        return (out, lse, rest) if want_rest else (out, lse)
 
-    def backward(self, out, lse, dout, dlse, want_q: bool, want_kv: bool, want_bias: bool = False):
+    def backward(self, out, lse, dout, dlse, want_q: bool, want_kv: bool, want_bias: bool = False, rest=None):
         q, k = self.tensors[:2]
         if (q.shape[-2] // k.shape[-2] - 1) * q.stride(-2) >= 1 << 29:  # a tile's queries are addressed with 32 bits
             self.set((q.contiguous(), *self.tensors[1:]), self.sizes)
@@ -287,9 +290,9 @@ class _Problem:
         dbias = torch.empty_like(self.terms.bias) if want_bias else None
         need = _lib.query("hi3d_attention_terms_backward_workspace", ref, self.terms_ref)
         work = _lib.workspace(need, self.device) if need else None
-        _lib.call("hi3d_attention_terms_backward", ref, self.terms_ref, out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
-                  _lib.ptr(dlse), _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), _lib.ptr(dbias), _lib.ptr(work), need,
-                  _lib.stream(self.device))
+        _lib.call("hi3d_attention_terms_backward", ref, self.terms_ref, out.data_ptr(), _lib.ptr(rest), lse.data_ptr(),
+                  dout.data_ptr(), _lib.ptr(dlse), _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), _lib.ptr(dbias), _lib.ptr(work),
+                  need, _lib.stream(self.device))
         return dq, dk, dv, dbias
 
 
@@ -302,15 +305,15 @@ class _Attend(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, bias, cu_q, cu_k, lens_k, scale, causal, key_mask, terms):
         p = _Problem(q, k, v, cu_q, cu_k, lens_k, scale, causal, key_mask, terms)
-        with _lib.on(p.device):
-            out, lse = p.forward(True)
-        ctx.terms = None
-        if terms is not None:
-            ctx.terms = terms.cap
-            ctx.save_for_backward(*p.tensors, out, lse, terms.slopes, terms.bias, terms.buckets, terms.prefix)
-        else:
-            ctx.save_for_backward(*p.tensors, out, lse)
         ctx.sizes, ctx.with_terms = p.sizes, terms is not None
+        with _lib.on(p.device):
+            if terms is None:
+                out, lse = p.forward(True)
+                ctx.save_for_backward(*p.tensors, out, lse)
+            else:
+                ctx.cap = terms.cap
+                out, lse, rest = p.forward(True, True)
+                ctx.save_for_backward(*p.tensors, out, lse, rest, terms.slopes, terms.bias, terms.buckets, terms.prefix)
         ctx.set_materialize_grads(False)
         return out, lse
 
@@ -323,13 +326,13 @@ class _Attend(torch.autograd.Function):
         if (dout is None and dlse is None) or not (want_q or want_kv or want_bias):
             return (None,) * 11
         saved = ctx.saved_tensors
-        tensors, out, lse, terms = saved[:7], saved[7], saved[8], None
+        tensors, out, lse, rest, terms = saved[:7], saved[7], saved[8], None, None
         if ctx.with_terms:
-            terms = _Terms(ctx.terms, *saved[9:])
+            rest, terms = saved[9], _Terms(ctx.cap, *saved[10:])
         dout = torch.zeros_like(out) if dout is None else dout
         p = _Problem.again(tensors, ctx.sizes, terms)
         with _lib.on(p.device):
-            dq, dk, dv, dbias = p.backward(out, lse, dout, dlse, want_q, want_kv, want_bias)
+            dq, dk, dv, dbias = p.backward(out, lse, dout, dlse, want_q, want_kv, want_bias, rest)
         return dq, dk, dv, dbias, None, None, None, None, None, None, None
 
 
@@ -413,6 +416,8 @@ def attend_grad(
 ) -> tuple[torch.Tensor, ...]:
     """``dq``, ``dk`` and ``dv`` (and ``dbias``, where there is a bias) of :func:`attend` from its
     arguments, its ``out`` and ``lse``, the gradient ``dout`` of ``out`` and optionally ``dlse`` of ``lse``.
+    (With terms autograd keeps more digits of ``out`` than its type holds; from ``out`` alone this
+    walks over the keys once more for them.)
 
     Sums run in a fixed order: the same bits every time. fp32 sums; probabilities and score
     gradients are rounded once to the inputs' type for their products (in fp16 after a scaling

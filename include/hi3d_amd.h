@@ -705,20 +705,23 @@ typedef struct hi3d_attention_terms {
   float cap;
 } hi3d_attention_terms;
 
-/* hi3d_attention_workspace, hi3d_attention_forward and the gradients with those terms. dbias_dev
- * [buckets, heads_q] in the bias's type (may be null): the sums of the scores' gradients by bucket,
- * in a fixed order. No gradient is formed of slopes. */
+/* hi3d_attention_workspace, hi3d_attention_forward and the gradients with those terms. Terms make rows
+ * sharp, and a sharp row's gradients need more digits of its output than 16 bits hold: where rest_host
+ * says 1, rest_dev [total_q, heads_q, dim] (may be null) takes what rounding leaves (times 2^11 in F16), out_dev is
+ * the quotient with the sum of the rounded probabilities then, and the gradients take it; without it
+ * they walk over the keys once more. dbias_dev [buckets, heads_q] in the bias's type (may be null): the
+ * sums of the scores' gradients by bucket, in a fixed order. No gradient is formed of slopes. */
 int hi3d_attention_terms_workspace(const hi3d_attention_desc* desc_host, const hi3d_attention_terms* terms_host,
-                                   int64_t* bytes_host);
+                                   int32_t* rest_host, int64_t* bytes_host);
 int hi3d_attention_terms_forward(const hi3d_attention_desc* desc_host, const hi3d_attention_terms* terms_host,
-                                 void* out_dev, float* lse_dev, void* workspace_dev, int64_t workspace_bytes,
+                                 void* out_dev, void* rest_dev, float* lse_dev, void* workspace_dev, int64_t workspace_bytes,
                                  void* stream);
 int hi3d_attention_terms_backward_workspace(const hi3d_attention_desc* desc_host,
                                             const hi3d_attention_terms* terms_host, int64_t* bytes_host);
 int hi3d_attention_terms_backward(const hi3d_attention_desc* desc_host, const hi3d_attention_terms* terms_host,
-                                  const void* out_dev, const float* lse_dev, const void* dout_dev,
-                                  const float* dlse_dev, void* dq_dev, void* dk_dev, void* dv_dev, void* dbias_dev,
-                                  void* workspace_dev, int64_t workspace_bytes, void* stream);
+                                  const void* out_dev, const void* rest_dev, const float* lse_dev,
+                                  const void* dout_dev, const float* dlse_dev, void* dq_dev, void* dk_dev,
+                                  void* dv_dev, void* dbias_dev, void* workspace_dev, int64_t workspace_bytes, void* stream);
 
 /* Keys and values [len, heads_k, dim] that all sequences of a batch share in front of their own:
  * element (j, h, d) at j * strides[0] + h * strides[1] + d of k, strides[2], [3] of v; key_mask uint8

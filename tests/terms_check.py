@@ -64,10 +64,16 @@ def within(got, want, room, what):
     assert (off <= room).all(), f"{what}: {np.max(off / np.maximum(room, 1e-300))} of the room"
 
 
-def check_rows(out, lse, f, dtype, what="out"):
-    """One head's output ``[lq, d]`` and lse against ``oracle.attention_terms.head``'s ``f``."""
+def check_rows(out, lse, f, dtype, what="out", for_grad=False):
+    """One head's output ``[lq, d]`` and lse against ``oracle.attention_terms.head``'s ``f``.
+
+    ``for_grad``: for gradients rows may be divided by the sum of the rounded probabilities, w_j = p_j (1 +
+    t_j) with |t_j| <= u: sum_j w_j v_j / sum_j w_j is off from out by sum_j p_j t_j (v_j - out) / (1 +
+    sum_j p_j t_j), at most u (sum_j p_j |v_j| + |out|) to first order: u |out| more than for the
+    quotient with the sum of the p_j."""
     u, tiny = U[dtype], TINY[dtype]
-    within(out, f["out"], f["out_off"] * 1.01 + u * f["size"] + tiny * f["vsum"] + u * np.abs(f["out"]) + 2 * tiny, what)
+    rounded = u * np.abs(f["out"]) * (2 if for_grad else 1)
+    within(out, f["out"], f["out_off"] * 1.01 + u * f["size"] + tiny * f["vsum"] + rounded + 2 * tiny, what)
     if lse is not None:
         got, none = host(lse), np.isneginf(f["lse"])
         assert np.array_equal(np.isneginf(got), none)
@@ -119,7 +125,8 @@ def check_all(q, k, v, lengths_q, lengths_k, out, lse, grads, *, dout=None, dlse
             g = h // (hq // hk)
             pre = 0 if prefix is None else int(min(max(prefix[s], 0), e - c))
             f = oterms.head(qh[a:b, h], kh[c:e, g], vh[c:e, g], h, scale, causal, None if mh is None else mh[c:e] > 0, pre, **on)
-            check_rows(out[a:b, h], None if lse is None else lse[a:b, h], f, dtype, f"out of segment {s} head {h}")
+            check_rows(out[a:b, h], None if lse is None else lse[a:b, h], f, dtype, f"out of segment {s} head {h}",
+                       dout is not None)
             if dout is None or c == e:
                 continue
             r = oterms.head_grad(f, qh[a:b, h], dh[a:b, h], scale, u + 4 * E, tiny, floor, None if zh is None else zh[a:b, h])
