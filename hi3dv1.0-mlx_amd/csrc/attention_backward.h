@@ -433,6 +433,13 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(ArgsOf<TERMS> a) 
 
 __device__ const float kPastRows[2] = {INFINITY, 0.0f};
 
+// Numbers of a row in LDS beside its queries and dout: lse and D; a constant; its slope and place; where its
+// bias stands.
+template <int TERMS>
+constexpr int kStats = TERMS == 0 || TERMS == kCap ? 2 : (TERMS == kSlopes ? 5 : (TERMS == kBias ? 4 : 6));
+template <int TERMS>
+constexpr int kBiasAt = kStats<TERMS> - 1;
+
 // What the terms of a score take in the kernel whose lanes own keys, for row r of a tile's 64 (a lane
 // each, one wave): a constant; the slope that multiplies the key's number in the workgroup, with
 // the side's sign; and for tiles between, the row's place from the workgroup's first key on and where
@@ -471,7 +478,7 @@ __device__ __forceinline__ void stage_key_terms(const TermArgs& a, const Segment
   if (has_bias<TERMS>(a)) {
     const float* of = table + g * a.stride_keys;
     if (!side.near) constant += of[side.left ? 0 : 2 * (a.far + kPadKeys)];
-    reinterpret_cast<int*>(to)[3 * kKT + lane] = g * a.stride_keys + a.far + kPadKeys - min(max(place, -a.far), a.far + kPadKeys);
+    reinterpret_cast<int*>(to)[(kBiasAt<TERMS> - 2) * kKT + lane] = g * a.stride_keys + a.far + kPadKeys - min(max(place, -a.far), a.far + kPadKeys);
   }
   to[lane] = constant;
 }
@@ -541,7 +548,7 @@ __device__ __forceinline__ void add_key_terms(const TermArgs& a, f32x16& sc, f32
   if (bias && side.near) {
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const i32x4 x4 = *reinterpret_cast<const i32x4*>(st + 5 * kKT + from + 8 * g);
+      const i32x4 x4 = *reinterpret_cast<const i32x4*>(st + kBiasAt<TERMS> * kKT + from + 8 * g);
 #pragma unroll
       for (int e = 0; e < 4; ++e) sc[4 * g + e] += table[x4[e] + key];
     }
@@ -568,10 +575,14 @@ template <typename T, int DP, int NW, bool Z, bool SPLIT, int TERMS>
 __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(ArgsOf<TERMS> a) {
   constexpr int KEYS = NW * 32, KS = DP / 16, DB = DP / 32, PAIR = 2 * kTile<DP>, CH = DP / 8;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  constexpr int STATS = (TERMS ? 6 : 2) * kKT;
+  constexpr int STATS = kStats<TERMS> * kKT;
   float* stats = reinterpret_cast<float*>(smem + 2 * PAIR);  // [2][lse, D, and what the terms take][64]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c32 = lane & 31, h = lane >> 5;
+  // with terms the last of the values' operands is in LDS: 256 registers do not hold it at 128 values a head, and
+  // a spilled operand waits for the tile loads in flight when it is read again
+  constexpr bool LAST = TERMS != 0 && DP == 128;
+  u32x4* last_of = reinterpret_cast<u32x4*>(stats + 2 * STATS) + wave * 64;
   int head, split = 0, slot;
   if (a.causal) {  // slot by slot, so that the first keys, which see the most rows, come first
     const int of = a.hk * a.splits;
@@ -606,6 +617,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
                  a.dim, h, on, vf);
   // packed rows that see a key of the workgroup, of the wave, and all keys of the wave: i >= key - off
   int first = 0, wfirst = wkey < s.lk ? 0 : rows, wfull = 0;
+  if constexpr (LAST) last_of[lane] = vf[KS - 1];
   const int seen_by_all = first_keys<TERMS>(a, s);
   if (a.causal) {
     auto sees = [&](int key) { return TERMS && key < seen_by_all ? 0 : min(s.lq, max(0, key - off)) * a.group; };
@@ -660,7 +672,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
     by = power_of_two(e - static_cast<int>(kPLog2<T>)), dk_by *= power_of_two(-e);
     dv_by = power_of_two(-static_cast<int>(kPLog2<T>));
   }
-  float* table = stats + 2 * STATS;
+  float* table = stats + 2 * STATS + (LAST ? NW * 256 : 0);
   if constexpr (TERMS != 0)
     if (has_bias<TERMS>(a)) {
       stage_bias<kPadKeys>(a, table, a.stride_keys, head * a.group, a.group, 0, 2 * (a.far + kPadKeys) + 1, threadIdx.x,
@@ -719,7 +731,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         const u32x4 x = read_rows<DP>(qt, 32 * n, k, place_of), y = read_rows<DP>(dt, 32 * n, k, place_of);
-        Mfma<T>::run(x, kf[k], sc), Mfma<T>::run(y, vf[k], dp);
+        Mfma<T>::run(x, kf[k], sc), Mfma<T>::run(y, LAST && k == KS - 1 ? last_of[fresh_lane()] : vf[k], dp);
       }
       __builtin_amdgcn_sched_barrier(0);
       float mul = a.scale2, base = 0.0f;  // scores in powers of two are sc * mul + base
@@ -813,6 +825,7 @@ __global__ __launch_bounds__(256) void attend_dbias_sum_kernel(const float* from
   const int64_t end = first + run < count ? first + run : count;
   float v = 0.0f;
   if (x < length)
+#pragma unroll 8
     for (int64_t i = first + of; i < end; i += 4) v += from[(head * count + i) * length + x];
   quarter[of][threadIdx.x & 63] = v;
   __syncthreads();
@@ -822,8 +835,8 @@ __global__ __launch_bounds__(256) void attend_dbias_sum_kernel(const float* from
   }
 }
 
-// A workgroup a head sums what is left by relative position, then each wave every fourth bucket: a
-// lane takes every 64th place and those of the bucket are summed in a fixed order.
+// A workgroup a head sums what is left by relative position, then each wave eight buckets at a time: a
+// lane takes every 64th place, and the lanes' sums are joined in a fixed order.
 __global__ __launch_bounds__(256) void attend_dbias_kernel(TermArgs a, const float* parts, int64_t count, void* out) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   float* total = reinterpret_cast<float*>(smem);
@@ -831,21 +844,33 @@ __global__ __launch_bounds__(256) void attend_dbias_kernel(TermArgs a, const flo
   int* bucket = reinterpret_cast<int*>(total + length);
   for (int x = threadIdx.x; x < length; x += 256) {
     float v = 0.0f;
+#pragma unroll 16
     for (int64_t i = 0; i < count; ++i) v += parts[(head * count + i) * length + x];
     total[x] = v, bucket[x] = bucket_at(a, x, kPadSums);
   }
   __syncthreads();
   const int lane = threadIdx.x & 63;
-  for (int b = threadIdx.x >> 6; b < a.buckets; b += 4) {
-    float v = 0.0f;
-    for (int x = lane; x < length; x += 64) v += bucket[x] == b ? total[x] : 0.0f;
+  for (int first = (threadIdx.x >> 6) * 8; first < a.buckets; first += 32) {  // a wave's eight buckets
+    float v[8] = {};
+    for (int x = lane; x < length; x += 64) {
+      const int b = bucket[x] - first;
+      const float add = total[x];
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
-    if (lane != 0) continue;
-    const int64_t at = static_cast<int64_t>(b) * a.hq + head;
-    if (a.bias_type == HI3D_F32) static_cast<float*>(out)[at] = v;
-    else if (a.bias_type == HI3D_F16) static_cast<_Float16*>(out)[at] = static_cast<_Float16>(v);
-    else static_cast<__bf16*>(out)[at] = static_cast<__bf16>(v);
+      for (int j = 0; j < 8; ++j) v[j] += b == j ? add : 0.0f;
+    }
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float x = half_sum(v[j]);
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) x += __shfl_xor(x, d);
+      sum = lane == j ? x : sum;
+    }
+    if (lane >= 8 || first + lane >= a.buckets) continue;
+    const int64_t at = static_cast<int64_t>(first + lane) * a.hq + head;
+    if (a.bias_type == HI3D_F32) static_cast<float*>(out)[at] = sum;
+    else if (a.bias_type == HI3D_F16) static_cast<_Float16*>(out)[at] = static_cast<_Float16>(sum);
+    else static_cast<__bf16*>(out)[at] = static_cast<__bf16>(sum);
   }
 }
 
@@ -866,7 +891,7 @@ int launch_dq(ArgsOf<TERMS> a, hipStream_t stream) {
 template <typename T, int DP, int NW, int TERMS>
 int launch_dkv(ArgsOf<TERMS> a, hipStream_t stream) {
   constexpr int keys = NW * 32, threads = 64 * NW;
-  size_t lds = 4 * kTile<DP> + (TERMS ? 6 : 2) * kKT * 8;
+  size_t lds = 4 * kTile<DP> + kStats<TERMS> * kKT * 8 + (TERMS != 0 && DP == 128 ? threads * 16 : 0);
   if constexpr (TERMS == kSlopes) lds += 2048;
   else if constexpr (TERMS != 0) lds += a.bias != nullptr ? a.group * a.stride_keys * 4 : 0;
   const int64_t per = a.cu_k != nullptr ? packed_slots(a.total_k, 1, keys, a.batch) : ceil_div(a.len_k, keys) * a.batch;

@@ -59,7 +59,7 @@ __device__ __forceinline__ void hide_keys(f32x16 (&sc)[2][QW], uint64_t bits) {
 // up to 65,536 x 8 x 128 bf16 (1.9 GB): 308 us, 6.1 TB/s (326 for 358 through the caches, in
 // turn on a slower card); below that size the cache helps (8 x 4,096 keys, 134 MB: 30.8 us for 32.3).
 template <typename T, int DP, int NW, int QW, bool Z, bool SPLIT, int TERMS>
-__global__ __launch_bounds__(64 * NW, DP <= 64 && NW * QW == 4 ? 3 : 2) void attend_kernel(ArgsOf<TERMS> a) {
+__device__ __forceinline__ void attend_rows_of(const ArgsOf<TERMS>& a, int64_t block, int64_t blocks) {
   constexpr int ROWS = NW * QW * 32, KS = DP / 16, DB = DP / 32, PAIR = 2 * kTile<DP>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -68,7 +68,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 && NW * QW == 4 ? 3 : 2) void att
   float* bias = reinterpret_cast<float*>(smem + 2 * PAIR);
 
   // task: (head, split, slot), neighbours on one XCD so that they share its L2
-  const int64_t id = xcd_remap(blockIdx.x, gridDim.x);
+  const int64_t id = xcd_remap(block, blocks);
   int head, split = 0, slot;
   if (a.head_minor) {
     head = static_cast<int>(id % a.hk), slot = static_cast<int>(id / a.hk);
@@ -160,19 +160,32 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 && NW * QW == 4 ? 3 : 2) void att
     capped = has_cap<TERMS>(a);
     float* table = reinterpret_cast<float*>(smem + 2 * PAIR + (Z ? kBiasBytes : 0));
     row_terms<QW>(a, s, terms, table, head, wrow, rows, qi, qg);
-    if (has_bias<TERMS>(a))  // the barrier in front of the first tile is this one's too
-      stage_bias<kPad>(a, table, a.stride, head * a.group, a.group, 0, 2 * (a.far + kPad) + 1, threadIdx.x, 64 * NW);
+    if (has_bias<TERMS>(a)) {  // the barrier in front of the first tile is this one's too
+      int x0 = 0, x1 = 2 * (a.far + kPad) + 1;
+      if (a.per == 0) {  // what the workgroup's rows and keys reach (add_terms reads 64 places from a clamped one on)
+        int i, g;
+        split_row(a, min(rows, row0 + ROWS) - 1, i, g);
+        x0 = min(max(t0 * kKT - (i + off) + a.far + kPad, 0), 2 * a.far + kPad);
+        split_row(a, row0, i, g);
+        x1 = min(x1, max(t1 * kKT - (i + off) + a.far + kPad, kKT));
+      }
+      stage_bias<kPad>(a, table, a.stride, head * a.group, a.group, x0, max(x1, x0 + 1), threadIdx.x, 64 * NW);
+    }
   }
   f32x16 acc[DB][QW] = {};
   float m[QW], l[QW];
 #pragma unroll
   for (int b = 0; b < QW; ++b) m[b] = -INFINITY, l[b] = 0.0f;
   float lr[QW] = {};  // TERMS: sums of the rounded probabilities
+  // For gradients the reference is the maximum itself: what a sharp row hangs on rounds to a power of two then,
+  // without an error, and D keeps its digits.
+  float slack = 8.0f;
+  if constexpr (TERMS != 0) slack = a.rest != nullptr ? 0.0f : 8.0f;
   // Capped scores of bf16 need no maximum: from a reference of zero, probabilities of 2^-80 to 2^80 and their
   // sums are far inside fp32's range and bf16's.
   bool bounded = false;
   if constexpr (TERMS == kCap && kBelow<T> == 0) {
-    bounded = a.cap2 <= 80.0f;
+    bounded = a.cap2 <= 80.0f && a.rest == nullptr;
     if (bounded)
 #pragma unroll
       for (int b = 0; b < QW; ++b) m[b] = 0.0f;
@@ -259,7 +272,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 && NW * QW == 4 ? 3 : 2) void att
         for (int e = 1; e < 16; ++e) x = larger(larger(x, sc[0][b][e]), sc[1][b][e]);
         if constexpr (TERMS != 0) top[b] = half_max(__builtin_fmaf(x, mul, add[b])) - kBelow<T>;
         else top[b] = half_max(x) * a.scale2 - kBelow<T>;
-        grow = grow || top[b] > m[b] + 8.0f;
+        grow = grow || top[b] > m[b] + slack;
       }
       if (__any(grow)) {
 #pragma unroll
@@ -354,6 +367,11 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 && NW * QW == 4 ? 3 : 2) void att
   }
 }
 
+template <typename T, int DP, int NW, int QW, bool Z, bool SPLIT, int TERMS>
+__global__ __launch_bounds__(64 * NW, DP <= 64 && NW * QW == 4 ? 3 : 2) void attend_kernel(ArgsOf<TERMS> a) {
+  attend_rows_of<T, DP, NW, QW, Z, SPLIT, TERMS>(a, blockIdx.x, gridDim.x);
+}
+
 // Short segments and small problems: waves that work on their own, on blocks of 32 packed
 // rows of one key head. Keys go from memory straight to matrix operands, values through a tile
 // of 64 rows in LDS for the transposed read; there is little to prefetch for, so one tile is
@@ -440,26 +458,26 @@ attend_short_kernel(ArgsOf<TERMS> a) {
   }
   const int seen_by_all = first_keys<TERMS>(a, s);
   auto seen_by = [&](int i) { return TERMS ? max(i + off + 1, seen_by_all) : i + off + 1; };
+  u32x4 qf[KS], qn[KS];
+  load_queries(first, qn);
+  const bool once = KW == 1 && s.lk <= kKT;
+  bool landed = false;  // once: the value tile has been waited for (a block that sees no key does not)
+  uint64_t bits = 0;
+  if (once) bits = load_keys(0);
   RowTerms<1> terms;
   float* table = nullptr;
   if constexpr (TERMS != 0) {
     if (has_bias<TERMS>(a)) {
-      // a wave's own copy (its rows and keys reach no further), or the workgroup's
       table = reinterpret_cast<float*>(smem + (KW == 1 ? 4 * kTile<DP> : KW * (TILE + 256)));
       int x0 = 0, x1 = 2 * (a.far + kPad) + 1;
-      if constexpr (KW == 1) {
+      if constexpr (KW == 1) {  // a wave's own copy, of the places that its rows and keys reach
         table += wave * a.group * a.stride;
         int i, g;
-        split_row(a, first, i, g);
-        const int hi = s.lk - 1 - (i + off) + a.far + kPad;
         split_row(a, last - 1, i, g);
-        const int lo = a.far + kPad - (i + off);
-        x0 = min(max(lo, 0), 2 * a.far + kPad), x1 = min(x1, max(hi, 0) + kKT + 1);
+        x0 = min(max(a.far + kPad - (i + off), 0), 2 * a.far + kPad);
+        split_row(a, first, i, g);
+        x1 = min(x1, max(s.lk - (i + off) + a.far + kPad, x0 + 1));
         stage_bias<kPad>(a, table, a.stride, head * a.group, a.group, x0, x1, lane, 64);
-        if (lane < 2) {  // one number for tiles past `far`
-          const int x = lane * (2 * (a.far + kPad));
-          stage_bias<kPad>(a, table, a.stride, head * a.group, a.group, x, x + 1, 0, 1);
-        }
         wait_lgkm0();
         asm volatile("" ::: "memory");
       } else {
@@ -468,12 +486,6 @@ attend_short_kernel(ArgsOf<TERMS> a) {
       }
     }
   }
-  u32x4 qf[KS], qn[KS];
-  load_queries(first, qn);
-  const bool once = KW == 1 && s.lk <= kKT;
-  bool landed = false;  // once: the value tile has been waited for (a block that sees no key does not)
-  uint64_t bits = 0;
-  if (once) bits = load_keys(0);
   for (int row0 = first; row0 < last; row0 += 32) {
 #pragma unroll
     for (int k = 0; k < KS; ++k) qf[k] = qn[k];
@@ -665,9 +677,8 @@ int launch_join(const AttnArgs& a, hipStream_t stream) {
   return HI3D_OK;
 }
 
-// split: parts of the rows alone, also where there is one, for a join that takes more of them
 template <typename T, int DP, int NW, int QW, int TERMS>
-int launch_attend(ArgsOf<TERMS> a, hipStream_t stream, bool split = false) {
+int launch_attend(ArgsOf<TERMS> a, hipStream_t stream) {
   constexpr int rows = NW * QW * 32;
   const bool z = a.mask != nullptr || a.dim < DP;
   const int64_t per = a.cu_q != nullptr ? packed_slots(a.total_q, a.group, rows, a.batch)
@@ -676,7 +687,7 @@ int launch_attend(ArgsOf<TERMS> a, hipStream_t stream, bool split = false) {
   HI3D_REQUIRE(blocks < (1ll << 31), "too many rows for one launch");
   a.slots = static_cast<int>(per);
   const size_t lds = 4 * kTile<DP> + (z ? kBiasBytes : 0) + term_bytes<TERMS>(a);
-  if (a.splits == 1 && !split)
+  if (a.splits == 1)
     return z ? launch_tiles<&attend_kernel<T, DP, NW, QW, true, false, TERMS>>(a, blocks, 64 * NW, lds, stream)
              : launch_tiles<&attend_kernel<T, DP, NW, QW, false, false, TERMS>>(a, blocks, 64 * NW, lds, stream);
   if constexpr (NW * QW == 8) {  // rows that fill the chip four times over are not split
@@ -684,7 +695,7 @@ int launch_attend(ArgsOf<TERMS> a, hipStream_t stream, bool split = false) {
   } else {
     const int rc = z ? launch_tiles<&attend_kernel<T, DP, NW, QW, true, true, TERMS>>(a, blocks, 64 * NW, lds, stream)
                      : launch_tiles<&attend_kernel<T, DP, NW, QW, false, true, TERMS>>(a, blocks, 64 * NW, lds, stream);
-    return rc != HI3D_OK || split ? rc : launch_join<T>(a, stream);
+    return rc != HI3D_OK ? rc : launch_join<T>(a, stream);
   }
 }
 

@@ -91,7 +91,10 @@ __device__ __forceinline__ int bucket_at(const TermArgs& a, int x, int pad) {
 template <int PAD>
 __device__ __forceinline__ void stage_bias(const TermArgs& a, float* to, int stride, int head0, int count, int x0, int x1,
                                            int thread, int threads) {
-  for (int x = x0 + thread; x < x1; x += threads) {
+  // and the two ends, which stand for all places past `far`
+  const int end = 2 * (a.far + PAD), places = x1 - x0 + (x0 > 0) + (x1 <= end);
+  for (int i = thread; i < places; i += threads) {
+    const int x = i < x1 - x0 ? x0 + i : (i == x1 - x0 && x0 > 0 ? 0 : end);
     const int at = bucket_at(a, x, PAD) * a.hq + head0;
     for (int g = 0; g < count; ++g) {
       const float v = load_bias(a, at + g);

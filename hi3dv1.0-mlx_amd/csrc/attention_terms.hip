@@ -1,5 +1,7 @@
 // Attention with terms beside scale q k (attention_terms.h), and attention over keys that many
 // sequences share in front of their own.
+#include <algorithm>
+
 #include "attention_forward.h"
 
 namespace hi3d {
@@ -48,9 +50,24 @@ bool keeps_rest(const TermArgs& a) { return a.splits == 1 && !a.few && !short_se
 
 int64_t part_bytes(const TermArgs& a, int splits) { return static_cast<int64_t>(splits) * a.total_q * a.hq * (a.dim + 2) * 4; }
 
-// The two halves of attention over shared keys: all rows over the keys that they share, as one
-// segment, and each sequence over its own. Each half leaves parts of the rows, in at most 128 splits.
-void choose_halves(const TermArgs& a, const hi3d_attention_shared* s, TermArgs& shared, TermArgs& own, int cus) {
+// Attention over shared keys in one launch: all rows over the keys that they share, as one segment, and each
+// sequence's rows over its own. Both leave parts of the rows, which are joined. Workgroups of four
+// waves in both: where a sequence has few rows three of them only help to load.
+struct Halves {
+  TermArgs of[2];
+  int64_t blocks[2];
+};
+
+template <typename T, int DP, bool Z>
+__global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void attend_shared_kernel(Halves p) {
+  const int which = blockIdx.x >= p.blocks[0];
+  attend_rows_of<T, DP, 4, 1, Z, true, kAll>(p.of[which], blockIdx.x - (which ? p.blocks[0] : 0), p.blocks[which]);
+}
+
+// Splits of the keys so that all workgroups, two to a compute unit, walk over about as many keys, and at least
+// four tiles.
+void choose_halves(const TermArgs& a, const hi3d_attention_shared* s, Halves& p, int cus) {
+  TermArgs &shared = p.of[0], &own = p.of[1];
   own = shared = a;
   shared.k = s->k, shared.v = s->v, shared.mask = s->key_mask;
   shared.k_b = shared.v_b = 0, shared.k_n = s->strides[0], shared.k_h = s->strides[1];
@@ -59,36 +76,40 @@ void choose_halves(const TermArgs& a, const hi3d_attention_shared* s, TermArgs& 
   shared.lens_k = nullptr, shared.causal = shared.reverse = 0;
   shared.own_lens = a.lens_k, shared.own_len = a.len_k, shared.per = a.len_q;
   shared.head_minor = s->len <= 512;
-  shared.once = static_cast<int64_t>(s->len) * a.hk * a.dim * 4 > (256ll << 20);
+  int64_t keys = 0;
   for (TermArgs* x : {&shared, &own}) {
-    const int rows = attend_rows(x->total_q, x->batch, x->hq, x->hk, x->dim, cus);
-    x->rows = rows > 32 ? 128 : rows;
-    const int splits = attend_splits(x->total_q, x->total_k, x->batch, x->hq, x->hk, x->dim, cus, false);
-    x->splits = splits > 128 ? 128 : splits;
+    x->slots = static_cast<int>(ceil_div(static_cast<int64_t>(x->len_q) * x->group, 128) * x->batch);
+    keys += static_cast<int64_t>(x->slots) * x->hk * x->len_k;
+  }
+  const int64_t each = std::max<int64_t>(4 * kKT, ceil_div(keys, 2 * cus));
+  for (TermArgs* x : {&shared, &own}) {
+    x->splits = static_cast<int>(std::min<int64_t>(128, std::max<int64_t>(1, (x->len_k + each / 2) / each)));
+    p.blocks[x == &own] = static_cast<int64_t>(x->slots) * x->hk * x->splits;
   }
 }
 
 template <typename T, int DP>
-int launch_part(const TermArgs& a, hipStream_t stream) {
-  if (a.rows == 32) return launch_attend<T, DP, 1, 1, kAll>(a, stream, true);
-  return launch_attend<T, DP, 4, 1, kAll>(a, stream, true);
+int launch_halves(const Halves& p, hipStream_t stream) {
+  const bool z = p.of[0].mask != nullptr || p.of[1].mask != nullptr || p.of[0].dim < DP;
+  const int64_t blocks = p.blocks[0] + p.blocks[1];
+  HI3D_REQUIRE(blocks < (1ll << 31), "too many rows for one launch");
+  const size_t lds = 4 * kTile<DP> + (z ? kBiasBytes : 0) + term_bytes<kAll>(p.of[0]);
+  const int rc = z ? launch_tiles<&attend_shared_kernel<T, DP, true>>(p, blocks, 256, lds, stream)
+                   : launch_tiles<&attend_shared_kernel<T, DP, false>>(p, blocks, 256, lds, stream);
+  if (rc != HI3D_OK) return rc;
+  TermArgs all = p.of[0];
+  all.splits = p.of[0].splits + p.of[1].splits;
+  return launch_join<T>(all, stream);
 }
 
 template <typename T>
-int launch_shared(const TermArgs& shared, const TermArgs& own, hipStream_t stream) {
-  for (const TermArgs* a : {&shared, &own}) {
-    int rc = HI3D_OK;
-    switch ((a->dim + 31) / 32) {
-      case 1: rc = launch_part<T, 32>(*a, stream); break;
-      case 2: rc = launch_part<T, 64>(*a, stream); break;
-      case 3: rc = launch_part<T, 96>(*a, stream); break;
-      default: rc = launch_part<T, 128>(*a, stream);
-    }
-    if (rc != HI3D_OK) return rc;
+int launch_shared(const Halves& p, hipStream_t stream) {
+  switch ((p.of[0].dim + 31) / 32) {
+    case 1: return launch_halves<T, 32>(p, stream);
+    case 2: return launch_halves<T, 64>(p, stream);
+    case 3: return launch_halves<T, 96>(p, stream);
+    default: return launch_halves<T, 128>(p, stream);
   }
-  TermArgs all = shared;
-  all.splits = shared.splits + own.splits;
-  return launch_join<T>(all, stream);
 }
 
 int shared_args(const hi3d_attention_desc* d, const hi3d_attention_terms* t, const hi3d_attention_shared* s, TermArgs& a) {
@@ -158,21 +179,23 @@ int hi3d_attention_terms_forward(const hi3d_attention_desc* d, const hi3d_attent
 
 int hi3d_attention_shared_workspace(const hi3d_attention_desc* d, const hi3d_attention_terms* t,
                                     const hi3d_attention_shared* s, int64_t* bytes) {
-  TermArgs a, shared, own;
+  TermArgs a;
+  Halves p;
   const int rc = shared_args(d, t, s, a);
   if (rc != HI3D_OK) return rc;
   HI3D_REQUIRE(bytes != nullptr, "null pointer argument");
   *bytes = 0;
   if (a.total_q == 0 || a.batch == 0) return HI3D_OK;
   const int cus = compute_units();
-  choose_halves(a, s, shared, own, cus > 0 ? cus : 256);
-  *bytes = part_bytes(a, shared.splits + own.splits) + 256;
+  choose_halves(a, s, p, cus > 0 ? cus : 256);
+  *bytes = part_bytes(a, p.of[0].splits + p.of[1].splits) + 256;
   return HI3D_OK;
 }
 
 int hi3d_attention_shared_forward(const hi3d_attention_desc* d, const hi3d_attention_terms* t, const hi3d_attention_shared* s,
                                   void* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream_) {
-  TermArgs a, shared, own;
+  TermArgs a;
+  Halves p;
   const int rc = shared_args(d, t, s, a);
   if (rc != HI3D_OK) return rc;
   if (a.total_q == 0) return HI3D_OK;
@@ -180,7 +203,8 @@ int hi3d_attention_shared_forward(const hi3d_attention_desc* d, const hi3d_atten
   const int cus = compute_units();
   HI3D_REQUIRE(cus > 0, "cannot query the compute unit count");
   a.out = out, a.lse = lse;
-  choose_halves(a, s, shared, own, cus);
+  choose_halves(a, s, p, cus);
+  TermArgs &shared = p.of[0], &own = p.of[1];
   const int splits = shared.splits + own.splits;
   HI3D_REQUIRE(workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 &&
                    workspace_bytes >= part_bytes(a, splits),
@@ -191,7 +215,7 @@ int hi3d_attention_shared_forward(const hi3d_attention_desc* d, const hi3d_atten
   own.part = shared.part + shared.splits * rows * a.dim;
   own.part_ml = shared.part_ml + shared.splits * rows * 2;
   hipStream_t stream = as_stream(stream_);
-  return d->dtype == HI3D_F16 ? launch_shared<_Float16>(shared, own, stream) : launch_shared<__bf16>(shared, own, stream);
+  return d->dtype == HI3D_F16 ? launch_shared<_Float16>(p, stream) : launch_shared<__bf16>(p, stream);
 }
 
 }  // extern "C"

@@ -116,6 +116,8 @@ def _offsets_of(cu: torch.Tensor, what: str) -> torch.Tensor:
 class _Terms:
     """What scores carry besides: checked on their own, and with their problem by :meth:`of`."""
 
+    __slots__ = ("cap", "slopes", "bias", "buckets", "prefix")
+
     def __init__(self, cap, slopes, bias, buckets, prefix):
         if cap is not None:
             cap = float(cap)
@@ -147,12 +149,18 @@ class _Terms:
             self.prefix = prefix.to(torch.int32).contiguous()
 
     def desc(self) -> _TermsDesc:
-        bias, map_ = self.bias, self.buckets
-        d = _TermsDesc(_lib.ptr(self.slopes), _lib.ptr(bias), _lib.ptr(map_), _lib.ptr(self.prefix))
-        d.cap = self.cap or 0.0
-        if bias is not None:
-            d.bias_dtype, d.buckets, d.far = _lib.DTYPES[bias.dtype], bias.shape[0], map_.numel() // 2
-        return d
+        slopes, bias, prefix = _lib.ptr(self.slopes), self.bias, _lib.ptr(self.prefix)
+        if bias is None:
+            return _TermsDesc(slopes, None, None, prefix, 0, 0, 0, self.cap or 0.0)
+        return _TermsDesc(slopes, bias.data_ptr(), self.buckets.data_ptr(), prefix, _lib.DTYPES[bias.dtype], bias.shape[0],
+                          self.buckets.numel() // 2, self.cap or 0.0)
+
+    @classmethod
+    def again(cls, *values) -> _Terms:
+        """Terms that were checked before."""
+        t = cls.__new__(cls)
+        t.cap, t.slopes, t.bias, t.buckets, t.prefix = values
+        return t
 
 
 _BIAS = (torch.float32, torch.float16, torch.bfloat16)
@@ -223,10 +231,12 @@ class _Problem:
             if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.shape != key_shape[:-2]:
                 raise ValueError(f"key_mask must be bool {list(key_shape[:-2])}")
             key_mask = key_mask.contiguous()
-        self.device = _lib.require_gpu(q, k, v, cu_q, cu_k, lens_k, key_mask)
-        if terms is not None:
+        if terms is None:
+            self.device = _lib.require_gpu(q, k, v, cu_q, cu_k, lens_k, key_mask)
+        else:
             terms.of(hq, batch, causal)
-            _lib.require_gpu(q, terms.slopes, terms.bias, terms.buckets, terms.prefix)
+            self.device = _lib.require_gpu(q, k, v, cu_q, cu_k, lens_k, key_mask, terms.slopes, terms.bias, terms.buckets,
+                                           terms.prefix)
             self.use(terms)
         self.set((q, k, v, cu_q, cu_k, lens_k, key_mask),
                  (total_q, total_k, batch, len_q, len_k, hq, hk, dim, _lib.DTYPES[dtype], 1 if causal else 0, scale))
@@ -263,8 +273,8 @@ class _Problem:
             _lib.call("hi3d_attention_forward", ref, out.data_ptr(), _lib.ptr(lse), _lib.ptr(work), need,
                       _lib.stream(self.device))
             return out, lse
-        kept = ctypes.c_int32(0)
-        need = _lib.query("hi3d_attention_terms_workspace", ref, self.terms_ref, ctypes.byref(kept))
+        kept = ctypes.c_int32(0) if want_rest else None
+        need = _lib.query("hi3d_attention_terms_workspace", ref, self.terms_ref, kept if kept is None else ctypes.byref(kept))
         work = _lib.workspace(need, self.device) if need else None
         rest = torch.empty_like(out) if want_rest and kept.value else None
         _lib.call("hi3d_attention_terms_forward", ref, self.terms_ref, out.data_ptr(), _lib.ptr(rest), _lib.ptr(lse),
@@ -328,7 +338,7 @@ class _Attend(torch.autograd.Function):
         saved = ctx.saved_tensors
         tensors, out, lse, rest, terms = saved[:7], saved[7], saved[8], None, None
         if ctx.with_terms:
-            rest, terms = saved[9], _Terms(ctx.cap, *saved[10:])
+            rest, terms = saved[9], _Terms.again(ctx.cap, *saved[10:])
         dout = torch.zeros_like(out) if dout is None else dout
         p = _Problem.again(tensors, ctx.sizes, terms)
         with _lib.on(p.device):

@@ -38,6 +38,8 @@ RAGGED = [
     ([300, 20, 0, 77], [3, 0, 90, 400]),
     ([17] * 200, None),
     ([(7 * i) % 90 for i in range(150)], [(11 * i) % 70 for i in range(150)]),
+    ([17] * 100 + [900] + [5] * 100, None),
+    ([9] * 60 + [300], [5] * 60 + [1200]),
 ]
 
 
