@@ -483,47 +483,47 @@ __device__ __forceinline__ void stage_key_terms(const TermArgs& a, const Segment
   to[lane] = constant;
 }
 
-// Takes D from dp and adds the terms to scores sc of rows 32 n + 8 (e / 4) + 4 h + e % 4 of the tile and
-// the lane's key `key` of the workgroup. Scores in powers of two are then sc * mul + base; with a cap dp
-// takes its derivative, times -1/4. folded: distances are in the scores already.
+// Adds to scores sc of rows 32 n + 8 (e / 4) + 4 h + e % 4 of the tile and the lane's key `key` of the
+// workgroup what the loop over probabilities does not add by itself. Scores in powers of two are then sc *
+// mul + base (and, with one bias alone, the row's constant). folded: distances are in the scores
+// already. kAll: also takes D from dp, which takes the cap's derivative, times -1/4.
 template <int TERMS, int KEYS>
 __device__ __forceinline__ void add_key_terms(const TermArgs& a, f32x16& sc, f32x16& dp, const float* st, int key, int n,
                                               const float* table, const TileSides& side, bool folded, float& mul, float& base) {
   typedef int i32x4 __attribute__((ext_vector_type(4)));
   const int from = 32 * n + 4 * (fresh_lane() >> 5);
-#pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const f32x4 d4 = *reinterpret_cast<const f32x4*>(st + kKT + from + 8 * g);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) dp[4 * g + e] -= d4[e];
-    __builtin_amdgcn_sched_barrier(0);  // four numbers in flight: more would cost registers that are not there
-  }
-  // each term behind a branch of its own, also where it is the only one: in one straight line they are
-  // scheduled into registers that keys and values then have to leave
   mul = a.scale2, base = 0.0f;
-  if (has_cap<kAll>(a)) {
-    mul = 2.0f * a.cap2, base = a.cap2;
+  if constexpr (TERMS == kAll) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const float u = minus_u(a, sc[e]);
-      sc[e] = u;
-      dp[e] *= __builtin_fmaf(u, u, u);
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 d4 = *reinterpret_cast<const f32x4*>(st + kKT + from + 8 * g);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dp[4 * g + e] -= d4[e];
+      __builtin_amdgcn_sched_barrier(0);  // four numbers in flight: more would cost registers that are not there
+    }
+    if (a.cap2 > 0.0f) {
+      mul = 2.0f * a.cap2, base = a.cap2;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float u = minus_u(a, sc[e]);
+        sc[e] = u;
+        dp[e] *= __builtin_fmaf(u, u, u);
+      }
     }
   }
-  const bool slopes = has_slopes<kAll>(a) && !folded, bias = has_bias<kAll>(a);
-  if (bias && !slopes && !side.near && a.group == 1) {
-    base += table[side.left ? 0 : 2 * (a.far + kPadKeys)];
-    return;
-  }
-  if (!slopes && !bias) return;
+  const bool slopes = has_slopes<TERMS>(a) && !folded, look_up = has_bias<TERMS>(a) && side.near;
+  const bool constants = slopes || (TERMS == kAll && has_bias<TERMS>(a));
+  if (!constants && !look_up) return;
+  if (constants) {
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const f32x4 c4 = *reinterpret_cast<const f32x4*>(st + 2 * kKT + from + 8 * g);
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 c4 = *reinterpret_cast<const f32x4*>(st + 2 * kKT + from + 8 * g);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) sc[4 * g + e] = __builtin_fmaf(sc[4 * g + e], mul, c4[e]);
-    __builtin_amdgcn_sched_barrier(0);
+      for (int e = 0; e < 4; ++e) sc[4 * g + e] = __builtin_fmaf(sc[4 * g + e], mul, c4[e]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    mul = 1.0f;
   }
-  mul = 1.0f;
   if (slopes) {
     const float x = static_cast<float>(key);
     if (side.before || side.after) {
@@ -545,13 +545,14 @@ __device__ __forceinline__ void add_key_terms(const TermArgs& a, f32x16& sc, f32
       }
     }
   }
-  if (bias && side.near) {
+  if (look_up) {
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const i32x4 x4 = *reinterpret_cast<const i32x4*>(st + kBiasAt<TERMS> * kKT + from + 8 * g);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sc[4 * g + e] += table[x4[e] + key];
+      for (int e = 0; e < 4; ++e) sc[4 * g + e] = __builtin_fmaf(sc[4 * g + e], mul, table[x4[e] + key]);
     }
+    mul = 1.0f;
   }
   __builtin_amdgcn_sched_barrier(0);
 }
@@ -704,8 +705,11 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
       folds = !__any(most > 1000.0f);
     }
   }
-  if constexpr (TERMS != 0) by *= has_cap<TERMS>(a) ? -4.0f : 1.0f;  // add_key_terms has the derivative times -1/4
+  if constexpr (TERMS != 0) by *= has_cap<TERMS>(a) ? -4.0f : 1.0f;  // the cap's derivative comes times -1/4
   f32x16 dk[DB] = {}, dv[DB] = {};
+  // a hidden score; with a cap its derivative is formed of it, and stays finite (1e-6 * 1e9 are far more powers of
+  // two than there are)
+  constexpr float hidden = TERMS == kCap ? -1e9f : -INFINITY;
   // one tile; hide: some rows do not see some keys
   auto walk = [&](const char* qt, const float* st, int t, bool hide) {
     const TileLane place_of = tile_lane<DP>(DP == 128 || TERMS ? fresh_lane() : lane);
@@ -714,7 +718,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
     bool folded = false;
     int distance = 0;  // of the segment's first key to the tile's first row
     if constexpr (TERMS != 0) {
-      if (has_slopes<kAll>(a) || has_bias<kAll>(a)) side = tile_sides<KEYS>(a, s, key0, t, rows);
+      if (has_slopes<TERMS>(a) || has_bias<TERMS>(a)) side = tile_sides<KEYS>(a, s, key0, t, rows);
       if constexpr (FOLD) {
         distance = -(t * kKT / a.group + off);
         folded = folds && (side.before || side.after) && max(abs(distance + key0), abs(distance + key0 + KEYS)) <= SideProduct<T>::kFarthest;
@@ -735,7 +739,11 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
       }
       __builtin_amdgcn_sched_barrier(0);
       float mul = a.scale2, base = 0.0f;  // scores in powers of two are sc * mul + base
-      if constexpr (TERMS != 0)
+      if constexpr (TERMS == kCap) {
+        mul = 2.0f * a.cap2, base = a.cap2;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[e] = minus_u(a, sc[e]);
+      } else if constexpr (TERMS != 0)
         add_key_terms<TERMS, KEYS>(a, sc, dp, st, wkey - key0 + (fresh_lane() & 31), n, table, side, folded, mul, base);
       if (hide) {
         asm volatile("");  // a branch, not 16 selects for every tile
@@ -743,7 +751,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
         const int key = wkey + (l & 31), row = TERMS && key < seen_by_all ? 0 : max(0, key - off) * a.group;
         const int seen = row - t * kKT - 32 * n - 4 * (l >> 5);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) sc[e] = seen <= 8 * (e >> 2) + (e & 3) ? sc[e] : -INFINITY;
+        for (int e = 0; e < 16; ++e) sc[e] = seen <= 8 * (e >> 2) + (e & 3) ? sc[e] : hidden;
       }
       u32x4 p[2], ds[2];
 #pragma unroll
@@ -752,13 +760,20 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
           const f32x4 l4 = *reinterpret_cast<const f32x4*>(st + 32 * n + 16 * k + 8 * g + 4 * h);
-          f32x4 d4 = {0, 0, 0, 0};  // TERMS: already taken from dp
-          if constexpr (!TERMS) d4 = *reinterpret_cast<const f32x4*>(st + 64 + 32 * n + 16 * k + 8 * g + 4 * h);
+          f32x4 d4 = {0, 0, 0, 0}, c4 = {0, 0, 0, 0};
+          if constexpr (TERMS != kAll) d4 = *reinterpret_cast<const f32x4*>(st + 64 + 32 * n + 16 * k + 8 * g + 4 * h);
+          if constexpr (TERMS == kBias) c4 = *reinterpret_cast<const f32x4*>(st + 128 + 32 * n + 16 * k + 8 * g + 4 * h);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int at = 8 * k + 4 * g + e;
-            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[at], mul, TERMS ? base - l4[e] : -l4[e]));
-            ps[4 * g + e] = x, dss[4 * g + e] = (x * by) * (TERMS ? dp[at] : dp[at] - d4[e]);
+            const float score = sc[at];
+            float less = -l4[e], by_ds = dp[at];
+            if constexpr (TERMS == kBias) less = c4[e] - l4[e];
+            else if constexpr (TERMS != 0 && TERMS != kSlopes) less = base - l4[e];
+            if constexpr (TERMS != kAll) by_ds -= d4[e];
+            if constexpr (TERMS == kCap) by_ds *= __builtin_fmaf(score, score, score);  // -1/4 of the cap's derivative
+            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(score, mul, less));
+            ps[4 * g + e] = x, dss[4 * g + e] = (x * by) * by_ds;
           }
         }
         p[k] = pack8<T>(ps), ds[k] = pack8<T>(dss);
