@@ -124,6 +124,44 @@ def test_long(cuda, kind, nq, nk, hq, hk, d):
     check(q, k, v, [nq], [nk], dout=dout, **terms(kind, hq, far=128, count=32))
 
 
+@pytest.mark.parametrize("hq,hk", [(32, 8), (24, 8)])
+@pytest.mark.parametrize("causal,masked", [(False, False), (True, False), (True, True)])
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+@pytest.mark.parametrize("kind", KINDS)
+def test_wide_rows(cuda, kind, d, causal, masked, hq, hk):
+    """Enough rows that they are neither split nor a few waves' work: the kernels that are built for one term,
+    whose gradients take the output's digits past 16 bits; groups of heads that do and do not divide a tile."""
+    q, k, v, dout = tensors(440, 440, hq, hk, d, torch.float16 if d % 64 else torch.bfloat16, gain=2.0)
+    mask = (torch.rand(440, generator=torch.Generator().manual_seed(5)) < 0.7).cuda() if masked else None
+    kw = terms(kind + (" prefix" if causal else ""), hq, 2, far=50, count=16, causal=causal, longest=200)
+    check(q, k, v, [220, 220], dout=dout, causal=causal, mask=mask, **kw)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["cap", "slopes", "bias"])
+def test_sharp_rows_keep_their_digits(cuda, kind, dtype):
+    """Scores of standard deviation 4 over 400 keys leave a few keys to a row. Two roundings (of the score
+    gradients, and of the result) of u each, independent: sqrt 2 of a single one's error, and 6 % for
+    what is left of D's."""
+    from oracle import attention_terms as oterms
+    from terms_check import host, on_host
+
+    q, k, v, dout = tensors(1200, 400, 16, 16, 64, dtype, gain=4.0)
+    kw = terms(kind, 16, far=30, count=16)
+    _, _, grads = check(q, k, v, [1200], [400], dout=dout, **kw)
+    on = on_host(kw)
+    off, single = [0.0] * 2, [0.0] * 2
+    for h in range(16):
+        f = oterms.head(host(q[:, h]), host(k[:, h]), host(v[:, h]), h, **on)
+        r = oterms.head_grad(f, host(q[:, h]), host(dout[:, h]), 0.125, 0.0, 0.0, 0.0)
+        for i, n in enumerate(("dq", "dk")):
+            exact = torch.as_tensor(r[n])
+            off[i] += float((grads[i][:, h].double().cpu() - exact).square().sum())
+            single[i] += float((exact.to(dtype).double() - exact).square().sum())
+    for a, b in zip(off, single):
+        assert (a / b) ** 0.5 <= 1.5, (a / b) ** 0.5
+
+
 def test_many_parts_of_the_bias(cuda):
     lengths = [48] * 700 + [11]
     q, k, v, dout = tensors(sum(lengths), sum(lengths), 2, 2, 32, torch.float16)
