@@ -693,17 +693,18 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
   bool folds = false;
   u32x4* side_at = reinterpret_cast<u32x4*>(table);  // [2][64], no bias then
   if constexpr (FOLD) {
-    if (64 % a.group == 0) {
-      float most = 0.0f;
+    float most = 64 % a.group == 0 ? 0.0f : INFINITY;
+    u32x4 rows_of[2];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {  // every wave the same
-        const int r = 32 * n + c32, i = r / a.group;
-        const float t = a.slopes[head * a.group + r - i * a.group] * kLog2e * a.per_mul;
-        side_at[n * 64 + lane] = SideProduct<T>::of_row(t, i, h);
-        most = fmaxf(most, __builtin_fabsf(t));
-      }
-      folds = !__any(most > 1000.0f);
+    for (int n = 0; n < 2; ++n) {  // every wave the same
+      const int r = 32 * n + c32, i = r / a.group;
+      const float t = a.slopes[head * a.group + r - i * a.group] * kLog2e * a.per_mul;
+      rows_of[n] = SideProduct<T>::of_row(t, i, h);
+      most = fmaxf(most, __builtin_fabsf(t));
     }
+    folds = !__any(most > 1000.0f);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) side_at[n * 64 + lane] = folds ? rows_of[n] : u32x4{0, 0, 0, 0};  // zeros: infinity times zero is not
   }
   if constexpr (TERMS != 0) by *= has_cap<TERMS>(a) ? -4.0f : 1.0f;  // the cap's derivative comes times -1/4
   f32x16 dk[DB] = {}, dv[DB] = {};

@@ -256,3 +256,13 @@ def test_differentiable_once(cuda):
     out = attention.attend(q, k, v, bias=bias, buckets=terms("bias", 2)["buckets"])
     with pytest.raises(RuntimeError, match="once"):
         torch.autograd.grad(out, bias, dout, create_graph=True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("steep", [30.0, 1e5])
+def test_steep_slopes(cuda, steep, dtype):
+    """Slopes that the score product's step cannot hold (in fp16, or for keys): one key a row."""
+    q, k, v, dout = tensors(440, 440, 32, 8, 64, dtype)
+    slopes = torch.full((32,), steep).cuda()
+    slopes[::3] = 0.25
+    check(q, k, v, [220, 220], dout=dout, slopes=slopes)
