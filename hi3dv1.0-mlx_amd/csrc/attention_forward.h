@@ -191,12 +191,11 @@ __device__ __forceinline__ void attend_rows_of(const ArgsOf<TERMS>& a, int64_t b
       for (int b = 0; b < QW; ++b) m[b] = 0.0f;
   }
   constexpr bool FOLD = TERMS == kSlopes;
-  std::conditional_t<FOLD, SideProduct<T>, char> side[QW];
+  std::conditional_t<FOLD, SideProduct<T>, char> side;
   bool folds = false;
-  if constexpr (FOLD) {
-    folds = true;
-#pragma unroll
-    for (int b = 0; b < QW; ++b) side[b].set(terms.slope[b] * a.per_mul, h), folds = folds && side[b].on;
+  if constexpr (FOLD) {  // one for all blocks of a lane's rows, where these have the same head
+    side.set(terms.slope[0] * a.per_mul, h);
+    folds = side.on && (QW == 1 || 32 % a.group == 0);
   }
 
   if (Z && a.dim < DP) clear_tiles(smem, 2 * PAIR);
@@ -231,9 +230,10 @@ __device__ __forceinline__ void attend_rows_of(const ArgsOf<TERMS>& a, int64_t b
         const uint32_t turn = after ? 0x80008000u : 0u, keep = folded ? ~0u : 0u;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-          const u32x4 x = SideProduct<T>::keys(n, c32);
+          f32x16 from = {};
+          Mfma<T>::run(SideProduct<T>::keys(n, c32), (side.slope ^ turn) & keep, from);
 #pragma unroll
-          for (int b = 0; b < QW; ++b) Mfma<T>::run(x, (side[b].slope ^ turn) & keep, sc[n][b]);
+          for (int b = 0; b < QW; ++b) sc[n][b] = from;
         }
       }
 #pragma unroll
