@@ -234,3 +234,22 @@ def test_empty(cuda):
     assert not out.any() and bool(torch.isneginf(lse).all())
     assert attention.attend(q[:0], k[:0], v[:0], attention.offsets([]), **kw).shape == (0, 2, 64)
     assert np.array_equal(ends([]), [0])
+
+
+@pytest.mark.parametrize("nq,nk,hq,hk,d", [(16400, 130, 32, 32, 64), (5600, 200, 96, 32, 32)])
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("kind", KINDS)
+def test_rows_of_two_blocks_a_wave(cuda, kind, masked, nq, nk, hq, hk, d):
+    """256 rows to a workgroup, with heads that do and do not agree between a lane's two rows; some heads are
+    checked."""
+    from hi3d_amd import attention
+
+    q, k, v, _ = tensors(nq, nk, hq, hk, d, torch.float16, gain=2.0)
+    mask = (torch.rand(nk, generator=torch.Generator().manual_seed(7)) < 0.6).cuda() if masked else None
+    kw = terms(kind, hq, far=50, count=16)
+    out, lse = attention.attend(q, k, v, key_mask=mask, return_lse=True, **kw)
+    on, m = on_host(kw), None if mask is None else mask.cpu().numpy()
+    for h in (0, 1, 2, hq - 1):
+        g = h // (hq // hk)
+        f = oterms.head(host(q[:, h]), host(k[:, g]), host(v[:, g]), h, mask=m, **on)
+        check_rows(out[:, h], lse[:, h], f, torch.float16)
