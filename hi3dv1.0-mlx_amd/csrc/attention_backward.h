@@ -76,14 +76,14 @@ __device__ __forceinline__ float wave_max(float x) {
 // Scores with terms are sharp in rows of many keys too (a cap lets them be, slopes leave few keys). There
 // the forward also keeps what its rounding took from the output (TermArgs::rest), which gives D its
 // digits, and where it did not the walk is taken for every row: dq and dk of capped scores of
-// standard deviation 4 come from 2.0 times the error of a single rounding down to 1.2.
+// standard deviation 4 come from 2.0 times the error of a single rounding down to 1.4 (sqrt 2).
 constexpr int kExactTiles = 4;
 
 // The bias's gradient, one query head of a wave's 32 rows at consecutive places. ds of 8 keys at a time
 // (without the cap's derivative; `unscale` takes its scale out and is 0 for rows that are not there)
 // goes to LDS row by row, and each lane sums one relative position down its 8 keys (rows of zeros
 // stand in for those outside): rows of 9, so that neither side's accesses share banks. LDS float
-// atomics took 175 cycles each here (dq of 8,191 rows x 33 heads x 64: 838 us for TODO). Of the 63
+// atomics took 175 cycles each here (dq of 8,191 rows x 33 heads x 64: 838 us for 339). Of the 63
 // positions that 32 keys give the lower half is complete, and each is written once in a wave's life; the
 // upper half waits in `carry` for the next 32 keys. Keys of tiles past `far` only count by their side.
 struct BiasSums {

@@ -16,7 +16,8 @@ rotary positions and attention, as hand-written HIP kernels behind a C ABI
 * :mod:`hi3d_amd.w8a8` — ``signs``, ``quantize_activation``, ``linear``;
 * :mod:`hi3d_amd.kernels` — ``layer_norm_modulate``;
 * :mod:`hi3d_amd.rotary`, :mod:`hi3d_amd.attention`, :mod:`hi3d_amd.torso` — the torso's
-  token operators: rotary positions, attention over packed segments, windows and caches,
+  token operators: rotary positions, attention over packed segments, windows and caches
+  (with caps, distances and learned biases in its scores, and over keys that sequences share),
   their gradients, and the attention block made of them.
 
 Every operation runs on the GPU; there is no host fallback.
