@@ -673,6 +673,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a, int64_t ro
 template <typename T>
 int launch_join(const AttnArgs& a, hipStream_t stream) {
   const int64_t n = a.total_q * a.hq;
+  HI3D_REQUIRE(n < (1ll << 31), "too many rows for one launch");
   hipLaunchKernelGGL(attend_join_kernel<T>, dim3(static_cast<unsigned>(n)), dim3(256), 0, stream, a, n);
   HI3D_LAUNCH_CHECK();
   return HI3D_OK;

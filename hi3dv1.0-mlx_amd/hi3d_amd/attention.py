@@ -146,7 +146,9 @@ class _Terms:
                 raise ValueError("a prefix that all queries see belongs to causal segments")
             if prefix.shape != (segments,) or prefix.dtype not in (torch.int32, torch.int64):
                 raise ValueError(f"prefix must be int32 [{segments}]")
-            self.prefix = prefix.to(torch.int32).contiguous()
+            if prefix.dtype == torch.int64:  # numbers past 31 bits are as good as the largest one
+                prefix = prefix.clamp(0, (1 << 31) - 1).to(torch.int32)
+            self.prefix = prefix.contiguous()
 
     def desc(self) -> _TermsDesc:
         slopes, bias, prefix = _lib.ptr(self.slopes), self.bias, _lib.ptr(self.prefix)
@@ -484,6 +486,8 @@ def attend_shared(
     for name, x in (("shared_k", shared_k), ("shared_v", shared_v)):
         if x.dim() != 3 or x.shape[1:] != k.shape[2:] or x.dtype != q.dtype:
             raise ValueError(f"{name} must be [keys, {k.shape[2]}, {k.shape[3]}] of {q.dtype}")
+    if shared_k.shape[0] >= 1 << 31:
+        raise ValueError("at most 2^31 - 1 shared keys")
     if shared_k.shape != shared_v.shape:
         raise ValueError(f"keys {list(shared_k.shape)} and values {list(shared_v.shape)} differ")
     if shared_mask is not None:

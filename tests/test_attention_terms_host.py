@@ -89,6 +89,7 @@ def test_tangents_are_refused():
     (dict(shared_k=torch.zeros(5, 2, 64).bfloat16()), "shared_k"), (dict(shared_v=torch.zeros(6, 2, 64).half()), "differ"),
     (dict(shared_mask=torch.ones(6, dtype=torch.bool)), "shared_mask"), (dict(shared_mask=torch.ones(5)), "shared_mask"),
     (dict(cap=2000.0), "cap"), (dict(lens_k=torch.zeros(2, dtype=torch.int32)), "lens_k"),
+    (dict(shared_k=torch.zeros(1, 2, 64).half().expand(1 << 31, 2, 64)), "2\\^31"),
 ])
 def test_shared_refusals(kw, match, monkeypatch):
     from hi3d_amd import _lib, attention

@@ -142,7 +142,7 @@ def test_buckets_outside_the_table_count_as_the_nearest(cuda):
     check(q, k, v, [40], bias=bias, buckets=buckets)
 
 
-@pytest.mark.parametrize("prefix", [-3, 0, 1, 64, 65, 129, 200, 100000])
+@pytest.mark.parametrize("prefix", [-3, 0, 1, 64, 65, 129, 200, 100000, 1 << 32, -(1 << 33) + 7])
 def test_prefix(cuda, prefix):
     q, k, v, _ = tensors(260, 200, 4, 2, 64, torch.float16)
     check(q, k, v, [130, 130], [70, 130], causal=True, prefix=torch.tensor([prefix, prefix], dtype=torch.int64).cuda())
