@@ -125,14 +125,16 @@ class TokenAttention(nn.Module):
     def frequencies(self, device: torch.device) -> torch.Tensor:
         """The float64 frequencies on ``device`` (no buffer: a module's cast would round them)."""
         if device not in self._freqs:
-            self._freqs[device] = self._freqs[torch.device("cpu")].to(device)
+            with torch.inference_mode(False):  # kept past a first call in that mode, for gradients too
+                self._freqs[device] = self._freqs[torch.device("cpu")].to(device)
         return self._freqs[device]
 
     def terms(self, device: torch.device) -> dict:
         """What :func:`attention.attend` takes for the scores' terms."""
         if device not in self._fixed:
-            self._fixed[device] = {n: t.to(device) if torch.is_tensor(t) else t
-                                   for n, t in self._fixed[torch.device("cpu")].items()}
+            with torch.inference_mode(False):
+                self._fixed[device] = {n: t.to(device) if torch.is_tensor(t) else t
+                                       for n, t in self._fixed[torch.device("cpu")].items()}
         fixed = self._fixed[device]
         return fixed if self.relative_bias is None else dict(fixed, bias=self.relative_bias)
 

@@ -188,3 +188,16 @@ def test_captured_steps_over_a_shared_beginning(cuda):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, call())
+
+
+def test_gradients_after_a_first_call_in_inference_mode():
+    grads = []
+    for first in (True, False):
+        block = _block("all", torch.bfloat16)
+        x, positions = _tokens(70, block.heads * block.dim, torch.bfloat16)
+        if first:
+            with torch.inference_mode():
+                block(x, positions)
+        block(x, positions).float().square().sum().backward()
+        grads.append([p.grad for p in block.parameters()])
+    assert all(torch.equal(a, b) for a, b in zip(*grads))

@@ -146,3 +146,11 @@ def test_refusals(plain):
                   torso.KeyValueCache(1, 4, 1, 8, torch.float64, device="cpu")):
         with pytest.raises(ValueError, match="share"):
             torso.KeyValueCache(1, 4, 2, 8, torch.float64, device="cpu", shared=wrong)
+
+
+def test_terms_first_used_in_inference_mode_serve_gradients_later():
+    block = _block(slopes=True, buckets=8, far=20)
+    with torch.inference_mode():
+        terms, freqs = block.terms(torch.device("meta")), block.frequencies(torch.device("meta"))
+    assert not any(t.is_inference() for t in (freqs, terms["slopes"], terms["buckets"]))
+    assert block.terms(torch.device("meta"))["slopes"] is terms["slopes"]
