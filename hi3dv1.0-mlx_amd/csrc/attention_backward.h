@@ -294,12 +294,13 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(ArgsOf<TERMS> a) 
     table = reinterpret_cast<float*>(smem + 2 * PAIR + (Z ? kBiasBytes : 0));
     const int is[1] = {qi}, gs[1] = {0};
     row_terms<1>(a, s, terms, table, head, wrow, rows, is, gs);
-    if (has_bias<TERMS>(a)) {  // the barrier in front of the first tile is these loops' too
+    if (has_bias<TERMS>(a)) {  // the barrier in front of the first tile is this loop's too
       stage_bias<kPad>(a, table, a.stride, head, 1, 0, 2 * (a.far + kPad) + 1, threadIdx.x, 64 * NW);
       if (sums) {
         bias_sums = table + a.stride + wave * sum_stride(a.far);
         skew = table + a.stride + NW * sum_stride(a.far) + wave * kSkew;
         for (int x = threadIdx.x; x < NW * (sum_stride(a.far) + kSkew); x += 64 * NW) table[a.stride + x] = 0.0f;
+        __syncthreads();  // a wave adds to its sums and writes them also where there is no tile, and others zeroed them
       }
     }
   }
