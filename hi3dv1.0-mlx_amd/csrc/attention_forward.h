@@ -182,15 +182,6 @@ __device__ __forceinline__ void attend_rows_of(const ArgsOf<TERMS>& a, int64_t b
   // of standard deviation 4: 1.4 times the error of a single rounding, 1.5 with the forward's own factor of 256).
   float slack = 8.0f;
   if constexpr (TERMS != 0) slack = a.rest != nullptr ? 2.0f : 8.0f;
-  // Capped scores of bf16 need no maximum: from a reference of zero, probabilities of 2^-80 to 2^80 and their
-  // sums are far inside fp32's range and bf16's.
-  bool bounded = false;
-  if constexpr (TERMS == kCap && kBelow<T> == 0) {
-    bounded = a.cap2 <= 80.0f && a.rest == nullptr;
-    if (bounded)
-#pragma unroll
-      for (int b = 0; b < QW; ++b) m[b] = 0.0f;
-  }
   constexpr bool FOLD = TERMS == kSlopes;
   std::conditional_t<FOLD, SideProduct<T>, char> side;
   bool folds = false;
@@ -265,7 +256,6 @@ __device__ __forceinline__ void attend_rows_of(const ArgsOf<TERMS>& a, int64_t b
       }
       float top[QW];
       bool grow = false;
-      if (!bounded)
 #pragma unroll
       for (int b = 0; b < QW; ++b) {
         float x = larger(sc[0][b][0], sc[1][b][0]);
