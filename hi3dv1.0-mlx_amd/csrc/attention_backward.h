@@ -709,8 +709,8 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
   }
   if constexpr (TERMS != 0) by *= has_cap<TERMS>(a) ? -4.0f : 1.0f;  // the cap's derivative comes times -1/4
   f32x16 dk[DB] = {}, dv[DB] = {};
-  // a hidden score; with a cap its derivative is formed of it, and stays finite (1e-6 * 1e9 are far more powers of
-  // two than there are)
+  // a hidden score; with a cap a finite one, of which a derivative can be formed, whose exponential is zero all the same
+  // (1e-6 * 1e9 are far more powers of two than there are)
   constexpr float hidden = TERMS == kCap ? -1e9f : -INFINITY;
   // one tile; hide: some rows do not see some keys
   auto walk = [&](const char* qt, const float* st, int t, bool hide) {
@@ -754,6 +754,14 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
         const int seen = row - t * kKT - 32 * n - 4 * (l >> 5);
 #pragma unroll
         for (int e = 0; e < 16; ++e) sc[e] = seen <= 8 * (e >> 2) + (e & 3) ? sc[e] : hidden;
+        if constexpr (TERMS == kCap) {  // and dp is D there: (1e9)^2 times a difference can pass fp32's range
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const f32x4 d4 = *reinterpret_cast<const f32x4*>(st + kKT + 32 * n + 4 * (l >> 5) + 8 * g);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dp[4 * g + e] = seen <= 8 * g + e ? dp[4 * g + e] : d4[e];
+          }
+        }
       }
       u32x4 p[2], ds[2];
 #pragma unroll

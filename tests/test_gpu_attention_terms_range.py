@@ -23,3 +23,15 @@ def test_values_of_any_size_behind_capped_scores(cuda, cap, d, size):
     q, k = (sign.expand(q.shape)).to(q.dtype).contiguous(), at_the_bend.to(k.dtype)
     v = (v.float() * size).to(v.dtype)
     check(q, k, v, [220, 220], cap=cap)
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("cap", [1e-6, 1e-3, 3.0, 1024.0])
+@pytest.mark.parametrize("size", [1.0, 2.0 ** 40, 2.0 ** 55])
+def test_large_gradients_of_capped_scores(cuda, size, cap, masked):
+    """Pairs that a causal row does not see give nothing, however large dout v is: 2^110 and 64 of them are in
+    bf16's range."""
+    q, k, v, dout = tensors(440, 440, 32, 8, 64, torch.bfloat16)
+    v, dout = ((x.float() * size).to(x.dtype) for x in (v, dout))
+    mask = (torch.rand(440, generator=torch.Generator().manual_seed(5)) < 0.7).cuda() if masked else None
+    check(q, k, v, [220, 220], dout=dout, causal=True, mask=mask, cap=cap)
