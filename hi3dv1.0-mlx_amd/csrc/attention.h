@@ -339,16 +339,19 @@ __device__ __forceinline__ void store_row(T* to, int dim, int h, const f32x16* a
     }
 }
 
-// Launches kKernel, which may take more than 64 KB of LDS (asked for once a device).
+// Launches kKernel, which may take more than 64 KB of LDS: all that a compute unit has is asked for, once a
+// device, since the same kernel takes more or less of it from call to call (a bias in it).
+constexpr int kMostLds = 160 * 1024;
 template <auto kKernel, typename Args>
 int launch_tiles(const Args& a, int64_t blocks, int threads, size_t lds, hipStream_t stream) {
   static uint64_t asked = 0;
+  HI3D_REQUIRE(lds <= kMostLds, "a workgroup has %d bytes of LDS (%zu wanted)", kMostLds, lds);
   if (lds > 65536) {
     int dev = 0;
     HI3D_HIP_CHECK(hipGetDevice(&dev));
     if (dev >= 64 || !(__atomic_load_n(&asked, __ATOMIC_RELAXED) >> dev & 1)) {
       HI3D_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kKernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                         static_cast<int>(lds)));
+                                         kMostLds));
       if (dev < 64) __atomic_fetch_or(&asked, 1ull << dev, __ATOMIC_RELAXED);
     }
   }
