@@ -157,6 +157,12 @@ __device__ __forceinline__ float half_sum(float x) {
   return lo + hi;
 }
 
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) x = fmaxf(x, __shfl_xor(x, d));
+  return x;
+}
+
 struct Segment {
   int b, tile;          // segment and the workgroup's tile of it
   int lq, lk, room;     // queries, keys in use, keys there are

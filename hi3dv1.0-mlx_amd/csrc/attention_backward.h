@@ -62,12 +62,6 @@ __device__ __forceinline__ int ds_exponent(float bound) {
 }
 __device__ __forceinline__ float power_of_two(int e) { return __builtin_amdgcn_ldexpf(1.0f, e); }
 
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) x = fmaxf(x, __shfl_xor(x, d));
-  return x;
-}
-
 // D from the forward's output carries that output's rounding (p's and its own), which for a
 // row of few keys is as large as the rounding of ds: sum_j ds_ij, which is zero, misses by
 // just that. Rows that see at most 4 tiles of keys take one walk more to find and mend it:
@@ -324,7 +318,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_dq_kernel(ArgsOf<TERMS> a) 
         folded = side.on && (after || (t + 1) * kKT - 1 <= terms.first);
         // a product with zeros where it does not hold: a branch would copy the scores
         const u32x4 slope = (side.slope ^ (after ? 0x80008000u : 0u)) & (folded ? ~0u : 0u);
-        Mfma<T>::run(SideProduct<T>::keys(n, c32), slope, sc);
+        Mfma<T>::run(SideProduct<T>::keys(n, c32, side.down), slope, sc);
       }
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
@@ -692,20 +686,24 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
   };
   constexpr bool FOLD = TERMS == kSlopes;
   bool folds = false;
+  float down = 1.0f;
   u32x4* side_at = reinterpret_cast<u32x4*>(table);  // [2][64], no bias then
   if constexpr (FOLD) {
-    float most = 64 % a.group == 0 ? 0.0f : INFINITY;
-    u32x4 rows_of[2];
+    float t[2];
+    int i[2];
 #pragma unroll
     for (int n = 0; n < 2; ++n) {  // every wave the same
-      const int r = 32 * n + c32, i = r / a.group;
-      const float t = a.slopes[head * a.group + r - i * a.group] * kLog2e * a.per_mul;
-      rows_of[n] = SideProduct<T>::of_row(t, i, h);
-      most = fmaxf(most, __builtin_fabsf(t));
+      const int r = 32 * n + c32;
+      i[n] = r / a.group;
+      t[n] = a.slopes[head * a.group + r - i[n] * a.group] * kLog2e * a.per_mul;
     }
-    folds = !__any(most > 1000.0f);
+    const float most = wave_max(fmaxf(__builtin_fabsf(t[0]), __builtin_fabsf(t[1])));
+    folds = 64 % a.group == 0 && !(most > 1000.0f);
+    const float up = SideProduct<T>::upwards(most);
+    down = 1.0f / up;
 #pragma unroll
-    for (int n = 0; n < 2; ++n) side_at[n * 64 + lane] = folds ? rows_of[n] : u32x4{0, 0, 0, 0};  // zeros: infinity times zero is not
+    for (int n = 0; n < 2; ++n)  // zeros: infinity times zero is not
+      side_at[n * 64 + lane] = folds ? SideProduct<T>::of_row(t[n] * up, i[n], h) : u32x4{0, 0, 0, 0};
   }
   if constexpr (TERMS != 0) by *= has_cap<TERMS>(a) ? -4.0f : 1.0f;  // the cap's derivative comes times -1/4
   f32x16 dk[DB] = {}, dv[DB] = {};
@@ -731,7 +729,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(A
       f32x16 sc = {}, dp = {};
       if constexpr (FOLD) {  // a product with zeros where it does not hold: a branch would copy the scores
         const int l = fresh_lane();
-        const u32x4 far = SideProduct<T>::of_key(distance + wkey + (l & 31), l >> 5) ^ (side.after ? 0x80008000u : 0u);
+        const u32x4 far = SideProduct<T>::of_key(distance + wkey + (l & 31), l >> 5, down) ^ (side.after ? 0x80008000u : 0u);
         Mfma<T>::run(side_at[n * 64 + l], far & (folded ? ~0u : 0u), sc);
       }
 #pragma unroll

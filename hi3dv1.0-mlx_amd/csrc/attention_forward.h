@@ -223,7 +223,7 @@ __device__ __forceinline__ void attend_rows_of(const ArgsOf<TERMS>& a, int64_t b
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           f32x16 from = sc[n][0];  // zeros, or the masked keys' -infinity, the same in all blocks
-          Mfma<T>::run(SideProduct<T>::keys(n, c32), (side.slope ^ turn) & keep, from);
+          Mfma<T>::run(SideProduct<T>::keys(n, c32, side.down), (side.slope ^ turn) & keep, from);
 #pragma unroll
           for (int b = 0; b < QW; ++b) sc[n][b] = from;
         }

@@ -171,32 +171,44 @@ __device__ __forceinline__ void row_terms(const TermArgs& a, const Segment& s, R
 }
 
 // Distances to the keys of one side, as one more step of the score product: slope * (number of the key in
-// its tile), with the slope in three numbers of the inputs' type (22 bits and more) and the key's
-// number, which has one. It takes a matrix instruction a 32 x 32 block where a multiply-add a score takes
-// 16 vector ones, in loops that vector operations bound: slopes cost 20,011 rows x 33 heads x 64 6 % (17 % as
-// multiply-adds).
+// its tile), with the slope in three numbers of the inputs' type and the key's number, which has one. It
+// takes a matrix instruction a 32 x 32 block where a multiply-add a score takes 16 vector ones, in loops that
+// vector operations bound: slopes cost 20,011 rows x 33 heads x 64 6 % (17 % as multiply-adds).
+//
+// Three numbers of bf16 hold fp32's 24 bits. Those of fp16 end at 2^-24, which the second one of a slope
+// below 1/8 is already past: slopes are multiplied by a power of two, 1 to 2^14, that brings the wave's largest
+// up to 2^9, and the numbers of keys divided by it (2^-14 times a whole number of up to 11 bits is
+// exact). A slope is then off by at most 2^-34 of the largest, or 2^-39: over 65,504 keys, the
+// farthest that are taken this way, by 4e-6 of the largest slope, or 1.2e-7 scale, in a score.
 template <typename T>
 struct SideProduct {
   u32x4 slope;  // second operand: the lane's row (with the signs turned: keys behind it)
+  float down;   // of the keys' numbers
   bool on;      // within the type's range in all lanes
 
+  __device__ __forceinline__ static float upwards(float most) {
+    if constexpr (!std::is_same_v<T, _Float16>) return 1.0f;
+    const int e = min(max(10 - __builtin_amdgcn_frexp_expf(most), 0), 14);
+    return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane((127 + e) << 23));
+  }
   __device__ __forceinline__ static void split(float t, T (&x)[3]) {
     x[0] = static_cast<T>(t);
     const float r = t - static_cast<float>(x[0]);
     x[1] = static_cast<T>(r), x[2] = static_cast<T>(r - static_cast<float>(x[1]));
   }
   __device__ __forceinline__ void set(float t, int h) {
+    const float most = wave_max(__builtin_fabsf(t)), up = upwards(most);
+    on = !(most > 16384.0f), down = 1.0f / up;
     T x[3];
-    split(t, x);
+    split(t * up, x);
     const T zero = static_cast<T>(0.0f);
     const typename Vec8<T>::type v = {x[0], x[1], x[2], zero, zero, zero, zero, zero};
     slope = h == 0 ? __builtin_bit_cast(u32x4, v) : u32x4{0, 0, 0, 0};
-    on = !__any(__builtin_fabsf(t) > 16384.0f);
   }
   // Lanes that own keys: t * (key - place of the row) where the heads of a tile's 64 rows are the same in
   // every tile (the group divides 64). A row's slope in three numbers meets the key's distance to
   // the tile's first row in numbers of 8 (11) bits, and its own distance from there, slope times row /
-  // group in three numbers, meets -1: 12 of the 16 products of a step, all exact.
+  // group in three numbers, meets -1: 12 of the 16 products of a step. (t of up to 1024: 63 t is in fp16's range.)
   __device__ __forceinline__ static u32x4 of_row(float t, int row, int h) {
     T x[3], y[3];
     split(t, x), split(-t * static_cast<float>(row), y);
@@ -206,17 +218,17 @@ struct SideProduct {
   }
   static constexpr int kBits = std::is_same_v<T, _Float16> ? 11 : 8;
   static constexpr int kFarthest = std::is_same_v<T, _Float16> ? 65504 : (1 << 24) - 1;
-  __device__ __forceinline__ static u32x4 of_key(int distance, int h) {
+  __device__ __forceinline__ static u32x4 of_key(int distance, int h, float down) {
     const int far = distance < 0 ? -distance : distance, low = (1 << kBits) - 1;
-    auto number = [&](int x) { return static_cast<T>(static_cast<float>(distance < 0 ? -x : x)); };
+    auto number = [&](int x) { return static_cast<T>(static_cast<float>(distance < 0 ? -x : x) * down); };
     const T b0 = number(far & low), b1 = number(far & low << kBits), b2 = number(far & ~(low << kBits | low));
-    const T one = static_cast<T>(1.0f), zero = static_cast<T>(0.0f);
+    const T one = static_cast<T>(down), zero = static_cast<T>(0.0f);
     const typename Vec8<T>::type a = {b0, b0, b0, b1, b1, b1, b2, b2}, b = {b2, one, one, one, zero, zero, zero, zero};
     return h == 0 ? __builtin_bit_cast(u32x4, a) : __builtin_bit_cast(u32x4, b);
   }
   // first operand: keys 32 n + l % 32
-  __device__ __forceinline__ static u32x4 keys(int n, int c32) {
-    const T j = static_cast<T>(static_cast<float>(32 * n + c32)), zero = static_cast<T>(0.0f);
+  __device__ __forceinline__ static u32x4 keys(int n, int c32, float down) {
+    const T j = static_cast<T>(static_cast<float>(32 * n + c32) * down), zero = static_cast<T>(0.0f);
     const typename Vec8<T>::type v = {j, j, j, zero, zero, zero, zero, zero};
     return __builtin_bit_cast(u32x4, v);
   }

@@ -35,3 +35,18 @@ def test_large_gradients_of_capped_scores(cuda, size, cap, masked):
     v, dout = ((x.float() * size).to(x.dtype) for x in (v, dout))
     mask = (torch.rand(440, generator=torch.Generator().manual_seed(5)) < 0.7).cuda() if masked else None
     check(q, k, v, [220, 220], dout=dout, causal=True, mask=mask, cap=cap)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("parts", [0.4, 200.4])
+def test_small_slopes_keep_their_digits_over_long_distances(cuda, parts, dtype):
+    """Slopes / scale of `parts` 2^-24, subnormal in fp16, and keys some 64,000 places away, the only ones that a mask
+    leaves: 0.4 2^-24 of a slope lost would move each probability by 0.4 2^-24 64,000 scale = 2 %, all by as
+    much; the bound is u and 65,000 e = 0.4 % (and in bf16 u = 0.4 % itself)."""
+    scale, far, heads = 16.0, 64000, 4
+    q, k, v, dout = tensors(192, far + 192, heads, 1, 32, dtype, gain=0.05)
+    k = (k.float() * 0.05).to(dtype)
+    mask = torch.zeros(len(k), dtype=torch.bool, device="cuda")
+    mask[:300] = True
+    slopes = (scale * parts * 2.0 ** -24 * 0.7 ** torch.arange(heads, dtype=torch.float64)).float().cuda()
+    check(q, k, v, [192], [len(k)], dout=dout.abs(), mask=mask, slopes=slopes, scale=scale)
