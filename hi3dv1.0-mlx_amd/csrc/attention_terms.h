@@ -30,7 +30,11 @@
 
 namespace hi3d {
 
-constexpr float kHideBelow = -1e30f;  // a bias below hides its key (-infinity; the lowest numbers of a type too)
+// A bias below hides its key: -infinity, the lowest numbers of fp32 and bf16, and the -1e9 that stands for "not seen".
+// Beside any other key such a one has no part of a row in fp32; a row that sees nothing else would be left with
+// the rounding of its scores (1.4e9 in steps of 128), and lse with less. fp16's lowest, -65504, is a number:
+// scores keep steps of 2^-7 there.
+constexpr float kHideBelow = -1e5f;
 constexpr int kPad = kKT, kPadKeys = 128;  // what the rows' and the keys' kernels look up past `far`
 constexpr int kPadSums = 93;               // what a wave's 32 rows and a tile's 64 keys reach past it together
 constexpr int kMostTermBytes = 72 * 1024;

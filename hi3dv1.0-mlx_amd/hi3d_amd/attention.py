@@ -385,7 +385,7 @@ def attend(
     * ``slopes`` (float32 ``[hq]``, constants, as of :func:`head_slopes`): less ``slopes[h] * |r|``;
     * ``bias`` (``[count, hq]``, float32, fp16 or bf16) with ``buckets`` (int32 ``[2 far + 1]``, far at
       most 1024, as of :func:`relative_buckets`): plus ``bias[buckets[clamp(r, -far, far) + far], h]``.
-      Differentiable in ``bias``. A bias below -1e30 hides its keys; a bucket outside the table
+      Differentiable in ``bias``. A bias below -1e5 hides its keys; a bucket outside the table
       counts as the nearest one;
     * ``prefix`` (int32, one per segment), with ``causal``: keys ``j < prefix`` are seen by every query.
 

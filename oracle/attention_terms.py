@@ -13,6 +13,8 @@ from __future__ import annotations
 import numpy as np
 
 E = 2.0 ** -24
+HIDE_BELOW = -1e5
+"""A bias below hides its keys."""
 
 
 def positions(lq: int, lk: int) -> np.ndarray:
@@ -34,7 +36,7 @@ def _scores(q, k, head, scale, r, seen, cap, slopes, bias, buckets):
     if bias is not None:
         far = (len(buckets) - 1) // 2
         b = bias[np.clip(buckets, 0, len(bias) - 1)[np.clip(r, -far, far) + far], head]
-        seen = seen & ~(b < -1e30)
+        seen = seen & ~(b < HIDE_BELOW)
         b = np.where(seen, b, 0.0)
         x, off = x + b, off + 8 * E * np.abs(b)
     x = np.where(seen, x, -np.inf)

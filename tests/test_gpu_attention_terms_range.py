@@ -50,3 +50,20 @@ def test_small_slopes_keep_their_digits_over_long_distances(cuda, parts, dtype):
     mask[:300] = True
     slopes = (scale * parts * 2.0 ** -24 * 0.7 ** torch.arange(heads, dtype=torch.float64)).float().cuda()
     check(q, k, v, [192], [len(k)], dout=dout.abs(), mask=mask, slopes=slopes, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("low", [-65504.0, -1.1e5, -1e9, -1e12, -3e29])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("n,heads", [(440, 32), (300, 2), (48, 2)])
+def test_numbers_that_stand_for_not_seen(cuda, n, heads, causal, low, dtype):
+    """A window of seven tokens by a bias, and a padded sequence: rows that see no key inside their window. With
+    -65504 its keys share such a row, as in a softmax of 32 bits; below -1e5 it is a row without keys."""
+    q, k, v, dout = tensors(n, n, heads, heads // 2, 64, dtype, gain=6.0)
+    mask = torch.arange(n, device="cuda") < n // 3
+    dout[n // 3:] = 0  # nothing is asked of padding
+    bias = torch.tensor([[0.0], [low]]).expand(2, heads).cuda()
+    buckets = torch.tensor([1, 0, 0, 0, 0, 0, 0, 0, 1], dtype=torch.int32).cuda()
+    out, _, grads = check(q, k, v, [n], dout=dout, mask=mask, causal=causal, bias=bias, buckets=buckets)
+    if low < -1e5:
+        assert not out[n // 3 + 4:].any() and not grads[3][1].any()
