@@ -261,7 +261,7 @@ __device__ __forceinline__ void attend_rows_of(const ArgsOf<TERMS>& a, int64_t b
         float x = larger(sc[0][b][0], sc[1][b][0]);
 #pragma unroll
         for (int e = 1; e < 16; ++e) x = larger(larger(x, sc[0][b][e]), sc[1][b][e]);
-        if constexpr (TERMS != 0) top[b] = half_max(__builtin_fmaf(x, mul, add[b])) - kBelow<T>;
+        if constexpr (TERMS != 0) top[b] = kept_max(__builtin_fmaf(x, mul, add[b])) - kBelow<T>;
         else top[b] = half_max(x) * a.scale2 - kBelow<T>;
         grow = grow || top[b] > m[b] + slack;
       }
@@ -528,7 +528,7 @@ attend_short_kernel(ArgsOf<TERMS> a) {
 #pragma unroll
         for (int e = 8 * (k & 1); e < 8 * (k & 1) + 8; ++e) top = larger(top, sc[k >> 1][0][e]);
       }
-      if constexpr (TERMS != 0) top = half_max(__builtin_fmaf(top, mul, add[0]));
+      if constexpr (TERMS != 0) top = kept_max(__builtin_fmaf(top, mul, add[0]));
       else top = half_max(top) * a.scale2;
       const float to = fmaxf(m, top - kBelow<T>);
       if (k0 > start) {

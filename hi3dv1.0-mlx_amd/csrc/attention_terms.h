@@ -35,6 +35,15 @@ namespace hi3d {
 // the rounding of its scores (1.4e9 in steps of 128), and lse with less. fp16's lowest, -65504, is a number:
 // scores keep steps of 2^-7 there.
 constexpr float kHideBelow = -1e5f;
+// Keys of a tile whose scores are all below, in powers of two, are as good as hidden (from a reference of zero their
+// probabilities are), and so a row that sees no others counts as one that sees none: steep slopes and distant
+// keys alone get there. fp32 keeps half a power of two at that size, which fp16 probabilities of up to 2^15
+// have room for; where it keeps less, neither a reference nor lse says which power a row's probabilities have.
+constexpr float kLost = -4194304.0f;
+__device__ __forceinline__ float kept_max(float x) {
+  x = half_max(x);
+  return x < kLost ? -INFINITY : x;
+}
 constexpr int kPad = kKT, kPadKeys = 128;  // what the rows' and the keys' kernels look up past `far`
 constexpr int kPadSums = 93;               // what a wave's 32 rows and a tile's 64 keys reach past it together
 constexpr int kMostTermBytes = 72 * 1024;

@@ -382,7 +382,8 @@ def attend(
     key ``j`` relative to query ``i`` (the last of ``lq`` queries stands at the last of ``lk`` keys):
 
     * ``cap`` (at most 1024): ``cap * tanh(x / cap)`` in place of ``x``;
-    * ``slopes`` (float32 ``[hq]``, constants, as of :func:`head_slopes`): less ``slopes[h] * |r|``;
+    * ``slopes`` (float32 ``[hq]``, constants, as of :func:`head_slopes`): less ``slopes[h] * |r|``. A row whose
+      largest score is below -2.9e6, past which fp32 has no digits for it, counts as one that sees no key;
     * ``bias`` (``[count, hq]``, float32, fp16 or bf16) with ``buckets`` (int32 ``[2 far + 1]``, far at
       most 1024, as of :func:`relative_buckets`): plus ``bias[buckets[clamp(r, -far, far) + far], h]``.
       Differentiable in ``bias``. A bias below -1e5 hides its keys; a bucket outside the table

@@ -690,7 +690,8 @@ int hi3d_attention_backward(const hi3d_attention_desc* desc_host, const void* ou
  *     + bias[bucket_map[clamp(r, -far, far) + far], head]
  * slopes_dev: fp32 [heads_q]; bias: F32, F16 or BF16 [buckets, heads_q], with bucket_map int32 [2 far
  * + 1] (numbers outside 0 .. buckets - 1 count as the nearest), far <= 1024; either may be null. A
- * bias below -1e5 hides its keys, as -infinity does. prefix: int32 [batch] or null: in
+ * bias below -1e5 hides its keys, as -infinity does; a row whose largest score is below -2^22 ln 2 (2.9e6:
+ * distant keys and steep slopes) counts as one that sees no key. prefix: int32 [batch] or null: in
  * a causal segment keys j < prefix[b] are seen by all queries. cap is 0 or 1e-6 to 1024; with slopes the scale is
  * at least 1e-30; a bias takes LDS for the query heads of a key head: (heads_q / heads_k) * (2 far
  * + 257 and up to 63 more) * 4 bytes <= 72 KB. */

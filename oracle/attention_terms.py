@@ -15,6 +15,8 @@ import numpy as np
 E = 2.0 ** -24
 HIDE_BELOW = -1e5
 """A bias below hides its keys."""
+LOST_BELOW = -(2.0 ** 22) * np.log(2.0)
+"""A row whose largest score is below sees no key."""
 
 
 def positions(lq: int, lk: int) -> np.ndarray:
@@ -39,6 +41,8 @@ def _scores(q, k, head, scale, r, seen, cap, slopes, bias, buckets):
         seen = seen & ~(b < HIDE_BELOW)
         b = np.where(seen, b, 0.0)
         x, off = x + b, off + 8 * E * np.abs(b)
+    x = np.where(seen, x, -np.inf)
+    seen = seen & (x.max(1, initial=-np.inf) >= LOST_BELOW)[:, None]
     x = np.where(seen, x, -np.inf)
     return x, bend, np.where(seen, off, 0.0), seen
 

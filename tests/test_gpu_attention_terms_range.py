@@ -67,3 +67,34 @@ def test_numbers_that_stand_for_not_seen(cuda, n, heads, causal, low, dtype):
     out, _, grads = check(q, k, v, [n], dout=dout, mask=mask, causal=causal, bias=bias, buckets=buckets)
     if low < -1e5:
         assert not out[n // 3 + 4:].any() and not grads[3][1].any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("steep", [1e4, 1e6, 3e7, 1e12])
+@pytest.mark.parametrize("kind", ["", "cap"])
+@pytest.mark.parametrize("n,heads", [(440, 32), (300, 2), (48, 2), (2000, 1)])
+def test_rows_far_from_all_keys_they_see(cuda, n, heads, kind, steep, dtype):
+    """Steep slopes and a padded sequence, whose last rows see distant keys alone: a cost that fp32 keeps to half a
+    power of two is the row's score, one beyond leaves a row without keys."""
+    q, k, v, dout = tensors(n, n, heads, max(heads // 4, 1), 64, dtype, gain=6.0)
+    mask = torch.arange(n, device="cuda") < n // 3
+    dout[n // 3:] = 0  # nothing is asked of padding
+    slopes = torch.full((heads,), steep).cuda()
+    slopes[1::3] = 0.25
+    kw = dict(cap=20.0) if kind else {}
+    out, _, _ = check(q, k, v, [n], dout=dout, mask=mask, slopes=slopes, **kw)
+    if steep > 2.9e6:
+        assert not out[n // 3:, ::3].any()
+
+
+@pytest.mark.parametrize("steep", [1e4, 3e7])
+def test_single_tokens_far_from_all_keys_they_see(cuda, steep):
+    from hi3d_amd import attention
+
+    q, k, v, _ = tensors(2, 2 * 9000, 4, 1, 64, torch.float16, gain=6.0)
+    mask = (torch.arange(9000, device="cuda") < 5000).expand(2, -1)
+    slopes = torch.full((4,), steep).cuda()
+    out, lse = attention.attend(q[:, None], k.view(2, 9000, 1, 64), v.view(2, 9000, 1, 64), key_mask=mask, slopes=slopes, return_lse=True)
+    shared = attention.attend_shared(q[:, None], k[:4000], v[:4000], k.view(2, 9000, 1, 64)[:, 4000:], v.view(2, 9000, 1, 64)[:, 4000:],
+                                     key_mask=mask[:, 4000:], slopes=slopes)
+    assert not out.any() and bool(torch.isneginf(lse).all()) and not shared.any()
