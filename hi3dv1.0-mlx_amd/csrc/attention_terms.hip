@@ -119,6 +119,8 @@ int shared_args(const hi3d_attention_desc* d, const hi3d_attention_terms* t, con
   HI3D_REQUIRE(d->cu_q == nullptr && d->cu_k == nullptr, "shared keys stand in front of sequences of equal room, not of offsets");
   HI3D_REQUIRE(t->prefix == nullptr, "shared keys are seen by all queries as they are");
   HI3D_REQUIRE(s->len >= 0, "bad sizes");
+  HI3D_REQUIRE(static_cast<int64_t>(s->len) + d->len_k < (1ll << 31) - kKT,  // places count through both, and to a tile's end
+               "shared and own keys of a sequence must be fewer than 2^31 - %d", kKT);
   HI3D_REQUIRE(s->len == 0 || (s->k != nullptr && s->v != nullptr), "null pointer argument");
   HI3D_REQUIRE((reinterpret_cast<uintptr_t>(s->k) | reinterpret_cast<uintptr_t>(s->v)) % 16 == 0,
                "the shared keys and values must be 16-byte aligned");

@@ -487,8 +487,8 @@ def attend_shared(
     for name, x in (("shared_k", shared_k), ("shared_v", shared_v)):
         if x.dim() != 3 or x.shape[1:] != k.shape[2:] or x.dtype != q.dtype:
             raise ValueError(f"{name} must be [keys, {k.shape[2]}, {k.shape[3]}] of {q.dtype}")
-    if shared_k.shape[0] >= 1 << 31:
-        raise ValueError("at most 2^31 - 1 shared keys")
+    if shared_k.shape[0] + k.shape[1] >= (1 << 31) - 64:
+        raise ValueError("shared and own keys of a sequence must be fewer than 2^31 - 64")
     if shared_k.shape != shared_v.shape:
         raise ValueError(f"keys {list(shared_k.shape)} and values {list(shared_v.shape)} differ")
     if shared_mask is not None:

@@ -737,7 +737,7 @@ typedef struct hi3d_attention_shared {
 
 /* hi3d_attention_terms_forward of segments without offsets whose queries all see the shared keys
  * first, read once for the batch; relative positions count from a sequence's own keys on, so shared key j
- * stands at j - len. desc's lens_k, causal and key_mask belong to the sequences' own keys;
+ * stands at j - len. len + len_k < 2^31 - 64. desc's lens_k, causal and key_mask belong to the sequences' own keys;
  * terms_host->prefix is null. Forward only. */
 int hi3d_attention_shared_workspace(const hi3d_attention_desc* desc_host, const hi3d_attention_terms* terms_host,
                                     const hi3d_attention_shared* shared_host, int64_t* bytes_host);
