@@ -27,7 +27,10 @@ int term_args(const hi3d_attention_desc* d, const hi3d_attention_terms* t, TermA
                  "a bias that reaches %d keys takes at most %d query heads to a key head (got %d)", a.far,
                  kMostTermBytes / 4 / a.stride_keys, a.group);
   }
-  if (t->cap > 0.0f) a.cap2 = t->cap * kLog2e, a.cap_in = 2.0f * kLog2e * d->scale / t->cap;
+  if (t->cap > 0.0f) {
+    a.cap2 = t->cap * kLog2e, a.cap_in = 2.0f * kLog2e * d->scale / t->cap;
+    HI3D_REQUIRE(a.cap_in < INFINITY, "scale / cap must be a number of fp32 (scale %g, cap %g)", d->scale, t->cap);
+  }
   a.per_mul = 1.0f / (t->cap > 0.0f ? 2.0f * a.cap2 : a.scale2);
   a.slopes = t->slopes, a.prefix = t->prefix, a.share = 1;
   return HI3D_OK;

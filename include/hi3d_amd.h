@@ -692,8 +692,8 @@ int hi3d_attention_backward(const hi3d_attention_desc* desc_host, const void* ou
  * + 1] (numbers outside 0 .. buckets - 1 count as the nearest), far <= 1024; either may be null. A
  * bias below -1e5 hides its keys, as -infinity does; a row whose largest score is below -2^22 ln 2 (2.9e6:
  * distant keys and steep slopes) counts as one that sees no key. prefix: int32 [batch] or null: in
- * a causal segment keys j < prefix[b] are seen by all queries. cap is 0 or 1e-6 to 1024; with slopes the scale is
- * at least 1e-30; a bias takes LDS for the query heads of a key head: (heads_q / heads_k) * (2 far
+ * a causal segment keys j < prefix[b] are seen by all queries. cap is 0 or 1e-6 to 1024, and 3 scale / cap
+ * is finite; with slopes the scale is at least 1e-30; a bias takes LDS for the query heads of a key head: (heads_q / heads_k) * (2 far
  * + 257 and up to 63 more) * 4 bytes <= 72 KB. */
 typedef struct hi3d_attention_terms {
   const float* slopes;
