@@ -562,11 +562,13 @@ __device__ __forceinline__ void add_key_terms(const TermArgs& a, f32x16& sc, f32
 // register spilled into the loop waits, when it is read again, for the tile loads in flight
 // (48 of them: 1628 us for 1000; one: 545 for 532). So lse and D go straight to LDS, places are
 // formed anew from the lane, at 128 values those in LDS too, for every tile, and masked and
-// plain tiles share one path (two paths copied the sums): no register is spilled. The
-// same figures as above: 355 us (795 TFLOP/s of its 4 products) and 532 us (1035).
+// plain tiles share one path (two paths copied the sums): without terms no register is spilled
+// (with them: attention_terms.h). The same figures as above: 355 us (795 TFLOP/s of its 4 products)
+// and 532 us (1035).
 //
-// Causal: early keys see the most rows, so their blocks start first, and each block is split
-// at least in two, which levels the ends (1008 us to 623, with 25 for the join).
+// Causal: early keys see the most rows, so their blocks start first, and where blocks are few enough
+// that twice as many are still at most four to a compute unit, their rows are split, which levels the
+// ends (8,192 x 32/8 heads x 128, in two: 1008 us to 623, with 25 for the join).
 template <typename T, int DP, int NW, bool Z, bool SPLIT, int TERMS>
 __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attend_dkv_kernel(ArgsOf<TERMS> a) {
   constexpr int KEYS = NW * 32, KS = DP / 16, DB = DP / 32, PAIR = 2 * kTile<DP>, CH = DP / 8;

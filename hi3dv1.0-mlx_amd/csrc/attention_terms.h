@@ -18,10 +18,10 @@
 // the workgroup has its bias by relative position, extended on both sides by what a tile can reach
 // past `far`, so that a lane's places are one address with constant offsets.
 //
-// 20,011 rows x 33 heads x 64 fp16 in two objects: 2017 us without terms, 2069 with a bias of 128
-// keys to each side, 2145 with slopes, 2942 with a cap (its 24 cycles a score and wave are vector
-// operations in a loop that these bound); causal 8,192 x 32/8 heads x 128 bf16 in two: 279, 289, 311
-// and 324.
+// 20,011 rows x 33 heads x 64 fp16 in two objects: 1841 us without terms, 2000 with a bias of 128
+// keys to each side, 2121 with slopes, 2690 with a cap (its 24 cycles a score and wave are vector
+// operations in a loop that these bound); causal 8,192 x 32/8 heads x 128 bf16 in two: 273, 283, 307
+// and 323.
 #pragma once
 
 #include <type_traits>
@@ -186,7 +186,7 @@ __device__ __forceinline__ void row_terms(const TermArgs& a, const Segment& s, R
 // Distances to the keys of one side, as one more step of the score product: slope * (number of the key in
 // its tile), with the slope in three numbers of the inputs' type and the key's number, which has one. It
 // takes a matrix instruction a 32 x 32 block where a multiply-add a score takes 16 vector ones, in loops that
-// vector operations bound: slopes cost 20,011 rows x 33 heads x 64 6 % (17 % as multiply-adds).
+// vector operations bound: slopes cost 20,011 rows x 33 heads x 64 15 % (20 % as multiply-adds).
 //
 // Three numbers of bf16 hold fp32's 24 bits. Those of fp16 end at 2^-24, which the second one of a slope
 // below 1/8 is already past: slopes are multiplied by a power of two, 1 to 2^14, that brings the wave's largest
@@ -331,8 +331,9 @@ inline int one_term(const TermArgs& a) {
 }
 
 // Workgroups of four waves whose rows are not parts (attention_terms_one.hip), and the gradients over them
-// (attention_terms_grad_one.hip), built for one term each: with the others' registers gone they need
-// no spills.
+// (attention_terms_grad_one.hip), built for one term each: with the others' registers gone most need
+// no spills. (Left: dk and dv at 128 values a head, 8 registers in fp16 and 2 in bf16 with slopes, 4 and 8 with a
+// bias, and 4 at 64 values in fp16 with a bias; 3 of masked rows of two blocks a wave with a bias.)
 int launch_rows_of_one(const TermArgs& a, int dtype, int kind, hipStream_t stream);
 int launch_grad_of_one(const TermArgs& a, int dtype, int kind, hipStream_t stream);
 
